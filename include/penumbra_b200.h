@@ -221,6 +221,63 @@ int pnb_lwe_contract_gather_ld(const int8_t* W_dev, const int64_t* bias_dev, uin
                                const int32_t* index_dev, int groups, uint64_t* Y_dev, int ldy,
                                int lwe_len, void* stream);
 
+/* ---- weights that differ from request to request --------------------------------------------
+ * Ciphertext x cleartext sums need no key, so one call may hold the requests of many clients,
+ * each encrypted under its own key, each with its own weights.  Routing is in the clear.  All
+ * results are exact mod 2^64; rows are ciphertexts at explicit pitches as in the _ld calls above.
+ * Indices are checked on the device: a value outside its range counts as unused, never as an
+ * address.  Outputs must not overlap inputs.  Every call runs on the current device,
+ * asynchronously on `stream`; two calls at once need their own output buffers only.  The
+ * reference has one weight matrix per Linear node (runtime/src/ops/linear.rs:52-75). */
+#define PNB_MAX_EXPERTS 1024
+#define PNB_MAX_CHOICES (1 << 20) /* tokens * top_k of one call */
+#define PNB_MAX_RANK 64
+
+/* Rows sorted by expert.  ids int32 [tokens][top_k]; choice c = t*top_k + i is used when
+ * 0 <= ids[c] < experts.  The used choices, by expert and then in choice order, are the rows:
+ *   offsets [experts+1]: the first row of each expert, then the number of rows R;
+ *   row_choice, row_expert [tokens*top_k]: the choice and expert of each row, -1 from R on;
+ *   choice_row [tokens*top_k]: the row of each choice, -1 where unused. */
+int pnb_expert_route(const int32_t* ids_dev, int tokens, int top_k, int experts,
+                     int32_t* offsets_dev, int32_t* row_choice_dev, int32_t* row_expert_dev,
+                     int32_t* choice_row_dev, void* stream);
+/* out[choice_row[t][i]][f] = weights[t][i] * X[t][f] for every used choice: the tokens'
+ * ciphertexts (X [tokens][features][ldx]) in row order (out [tokens*top_k][features][ldo]);
+ * rows without a choice are left as they were.  weights int32 [tokens][top_k], NULL = all one.
+ * With a combine's weights this is that combine's gradient with respect to its rows. */
+int pnb_expert_dispatch(const int32_t* choice_row_dev, int tokens, int top_k,
+                        const int32_t* weights_dev, const uint64_t* X_dev, int features, int ldx,
+                        uint64_t* out_dev, int ldo, int lwe_len, void* stream);
+/* Y[r][j] = sum_i W[e][j][i] * X[src][i] (+ bias[e][j] * delta on the body), e = row_expert[r]:
+ * every row through its own expert's int8 matrix.  W [experts][M][K] (K <= 65536), bias int64
+ * [experts][M] (may be NULL).  sorted_rows = 0: X [tokens][K][ldx], src = the row's token
+ * (row_choice[r] / top_k), so no dispatch is needed; sorted_rows = 1: X [tokens*top_k][K][ldx],
+ * src = r.  Y [tokens*top_k][M][ldy]; rows from R on are left as they were. */
+int pnb_expert_contract(const int32_t* row_choice_dev, const int32_t* row_expert_dev, int tokens,
+                        int top_k, int experts, int sorted_rows, const int8_t* W_dev,
+                        const int64_t* bias_dev, uint64_t delta, int M, int K,
+                        const uint64_t* X_dev, int ldx, uint64_t* Y_dev, int ldy, int lwe_len,
+                        void* stream);
+/* out[t][f] = sum_i weights[t][i] * Y[choice_row[t][i]][f]: rows (Y [tokens*top_k][features][ldy])
+ * back in token order (out [tokens][features][ldo]).  Unused choices add nothing; a token without
+ * a used choice gets zero words.  weights as for pnb_expert_dispatch, whose gradient with respect
+ * to the tokens this is. */
+int pnb_expert_combine(const int32_t* choice_row_dev, int tokens, int top_k,
+                       const int32_t* weights_dev, const uint64_t* Y_dev, int features, int ldy,
+                       uint64_t* out_dev, int ldo, int lwe_len, void* stream);
+/* A shared projection with a low-rank adapter per request:
+ *   Y[b][j] = 2^base_shift * sum_i W[j][i] X[b][i] + sum_q B[a][j][q] (sum_i A[a][q][i] X[b][i])
+ *             (+ bias[j] * delta on the body),   a = adapter[b].
+ * W int8 [M][K], A int8 [adapters][rank][K], B int8 [adapters][M][rank], adapter int32 [batch]; a
+ * request whose adapter is outside [0, adapters) gets the shared projection alone.  base_shift
+ * (0..63) puts the shared weights on the grid of the adapters' products.  1 <= rank <=
+ * PNB_MAX_RANK, K <= 65536; X [batch][K][ldx], Y [batch][M][ldy]. */
+int pnb_adapter_contract(const int8_t* W_dev, const int64_t* bias_dev, uint64_t delta,
+                         int base_shift, int M, int K, const int8_t* A_dev, const int8_t* B_dev,
+                         int adapters, int rank, const int32_t* adapter_dev,
+                         const uint64_t* X_dev, int ldx, uint64_t* Y_dev, int ldy, int batch,
+                         int lwe_len, void* stream);
+
 /* Negacyclic products out[c] = a[c] * b[c] mod (X^N + 1) through the same f64 FFT the blind
  * rotation uses (a: small signed integers, |a| < 2^31; b: u64 torus), count polynomials.
  * Diagnostic entry point for the FFT's precision; no reference counterpart. */

@@ -25,7 +25,8 @@ __all__ = [
     "gather_shards", "evaluate_sharded", "op_bits", "wait_probe", "import_keys", "radix_merge",
     "TensorDesc", "KeyRing", "op_plan", "requant_batch", "argmax_batch", "add_batch",
     "radix_plan", "lwe_contract_ld", "lwe_contract_gather_ld", "deserialize_keys",
-    "serialize_lwe", "deserialize_lwe",
+    "serialize_lwe", "deserialize_lwe", "ExpertRoute", "expert_route", "expert_dispatch",
+    "expert_contract", "expert_combine", "adapter_contract",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -99,6 +100,22 @@ _SIGS = {
     "pnb_lwe_contract_gather_ld": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_int,
                                              C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
                                              C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "pnb_expert_route": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                   C.c_void_p, C.c_void_p, C.c_void_p]),
+    "pnb_expert_dispatch": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                      C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int,
+                                      C.c_void_p]),
+    "pnb_expert_contract": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
+                                      C.c_void_p, C.c_void_p, C.c_uint64, C.c_int, C.c_int,
+                                      C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int,
+                                      C.c_void_p]),
+    "pnb_expert_combine": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                     C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int,
+                                     C.c_void_p]),
+    "pnb_adapter_contract": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_int, C.c_int,
+                                       C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                       C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
+                                       C.c_int, C.c_int, C.c_void_p]),
     "pnb_keys_serialized_bytes": (C.c_size_t, [C.c_void_p, C.c_int]),
     "pnb_keys_serialize": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_size_t]),
     "pnb_keys_deserialize": (C.c_int, [C.c_int, C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p)]),
@@ -593,6 +610,186 @@ def lwe_contract_gather_ld(W: torch.Tensor, bias: torch.Tensor | None, delta: in
                                                 _ptr(_u64(X).contiguous()), ld,
                                                 _ptr(index.contiguous()), G, _ptr(out),
                                                 out.shape[-1], lwe_len, _stream(X.device)))
+    return out
+
+
+# ---- weights that differ from request to request ----------------------------------------------
+def _want(name: str, t, dtype, shape, device):
+    """``t`` on ``device`` with this dtype and shape (None = any size), contiguous."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if len(t.shape) != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
+                         f"{tuple('*' if w is None else w for w in shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    return t.contiguous()
+
+
+def _want_out(name: str, out, shape, device, lwe_len: int):
+    """The caller's buffer, checked, or a new one: zeros where the call leaves words behind
+    ``lwe_len``."""
+    if out is None:
+        make = torch.empty if shape[-1] == lwe_len else torch.zeros
+        return make(shape, dtype=torch.int64, device=device)
+    if _u64(out).shape != torch.Size(shape) or out.device != device or not out.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {tuple(shape)} tensor on {device}, got "
+                         f"{tuple(out.shape)} on {out.device}")
+    return out
+
+
+def _want_words(name: str, X, lwe_len):
+    """Ciphertext rows [*, *, ld] on a GPU and the words used of each."""
+    if _u64(X).dim() != 3 or not X.is_cuda:
+        raise ValueError(f"{name} must be a 3-dimensional CUDA tensor of ciphertext rows, got "
+                         f"{tuple(X.shape)} on {X.device}")
+    lwe_len = X.shape[2] if lwe_len is None else lwe_len
+    if not 1 <= lwe_len <= X.shape[2]:
+        raise ValueError(f"lwe_len {lwe_len} does not fit rows of {X.shape[2]} words")
+    return X.contiguous(), lwe_len
+
+
+class ExpertRoute:
+    """Where each choice of each token went (``pnb_expert_route``): ``offsets`` [experts+1],
+    ``row_choice`` and ``row_expert`` [tokens*top_k], ``choice_row`` [tokens, top_k], all int32.
+    The constructor makes the buffers; ``expert_route`` fills them."""
+
+    def __init__(self, tokens: int, top_k: int, experts: int, device):
+        self.tokens, self.top_k, self.experts = tokens, top_k, experts
+        self.device = torch.device(device)
+        n = tokens * top_k
+
+        def make(*shape):
+            return torch.empty(shape, dtype=torch.int32, device=self.device)
+
+        self.offsets, self.row_choice, self.row_expert = make(experts + 1), make(n), make(n)
+        self.choice_row = make(tokens, top_k)
+        self.device = self.offsets.device
+
+    @property
+    def rows(self) -> int:
+        """Rows the buffers hold: one per choice (the used ones come first)."""
+        return self.tokens * self.top_k
+
+
+def expert_route(ids: torch.Tensor, experts: int, out: ExpertRoute | None = None) -> ExpertRoute:
+    """Sort the choices ``ids`` [tokens, top_k] (int32) by expert, stably; a value outside
+    [0, experts) is an unused choice."""
+    if ids.dim() != 2 or not ids.is_cuda:
+        raise ValueError(f"ids must be a CUDA tensor [tokens, top_k], got {tuple(ids.shape)} on "
+                         f"{ids.device}")
+    T, k = ids.shape
+    ids = _want("ids", ids, torch.int32, (T, k), ids.device)
+    if out is None:
+        out = ExpertRoute(T, k, experts, ids.device)
+    elif (out.tokens, out.top_k, out.experts, out.device) != (T, k, experts, ids.device):
+        raise ValueError(f"out is a route of {out.tokens} x {out.top_k} choices of {out.experts} "
+                         f"experts on {out.device}, not {T} x {k} of {experts} on {ids.device}")
+    with torch.cuda.device(ids.device):
+        _check("pnb_expert_route",
+               lib().pnb_expert_route(_ptr(ids), T, k, experts, _ptr(out.offsets),
+                                      _ptr(out.row_choice), _ptr(out.row_expert),
+                                      _ptr(out.choice_row), _stream(ids.device)))
+    return out
+
+
+def _route_weights(route: ExpertRoute, weights):
+    return None if weights is None else _want("weights", weights, torch.int32,
+                                              (route.tokens, route.top_k), route.device)
+
+
+def expert_dispatch(route: ExpertRoute, X: torch.Tensor, lwe_len: int | None = None,
+                    weights: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """The tokens' ciphertexts ``X`` [tokens, features, ld] in row order, each times its choice's
+    weight (int32 [tokens, top_k], None = 1): [tokens*top_k, features, ld].  Rows without a choice
+    are left as they were (not set when ``out`` is made here), as are words behind ``lwe_len``."""
+    X, L = _want_words("X", X, lwe_len)
+    T, F, ld = X.shape
+    X = _want("X", X, X.dtype, (route.tokens, None, None), route.device)
+    w = _route_weights(route, weights)
+    out = _want_out("out", out, (route.rows, F, ld), X.device, L)
+    with torch.cuda.device(X.device):
+        _check("pnb_expert_dispatch",
+               lib().pnb_expert_dispatch(_ptr(route.choice_row), T, route.top_k, _ptr(w), _ptr(X),
+                                         F, ld, _ptr(out), ld, L, _stream(X.device)))
+    return out
+
+
+def expert_combine(route: ExpertRoute, Y: torch.Tensor, lwe_len: int | None = None,
+                   weights: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows ``Y`` [tokens*top_k, features, ld] back in token order, each times its choice's weight
+    (int32 [tokens, top_k], None = 1) and summed per token: [tokens, features, ld].  A token
+    without a used choice gets zero words."""
+    Y, L = _want_words("Y", Y, lwe_len)
+    Y = _want("Y", Y, Y.dtype, (route.rows, None, None), route.device)
+    F, ld = Y.shape[1:]
+    w = _route_weights(route, weights)
+    out = _want_out("out", out, (route.tokens, F, ld), Y.device, L)
+    with torch.cuda.device(Y.device):
+        _check("pnb_expert_combine",
+               lib().pnb_expert_combine(_ptr(route.choice_row), route.tokens, route.top_k, _ptr(w),
+                                        _ptr(Y), F, ld, _ptr(out), ld, L, _stream(Y.device)))
+    return out
+
+
+def expert_contract(route: ExpertRoute, W: torch.Tensor, bias: torch.Tensor | None, delta: int,
+                    X: torch.Tensor, lwe_len: int | None = None, sorted_rows: bool = False,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Every row through its own expert's matrix: ``W`` int8 [experts, M, K], ``bias`` int64
+    [experts, M] or None (times ``delta``, on the body).  ``X`` holds the tokens [tokens, K, ld]
+    (no dispatch needed), or with ``sorted_rows`` the rows [tokens*top_k, K, ld] of an earlier
+    call.  The result is [tokens*top_k, M, ld] in row order; rows without a choice are left as they
+    were (not set when ``out`` is made here), as are words behind ``lwe_len``."""
+    X, L = _want_words("X", X, lwe_len)
+    if W.dim() != 3:
+        raise ValueError(f"W must be [experts, M, K], got {tuple(W.shape)}")
+    M, K = W.shape[1:]
+    W = _want("W", W, torch.int8, (route.experts, M, K), route.device)
+    X = _want("X", X, X.dtype, (route.rows if sorted_rows else route.tokens, K, None),
+              route.device)
+    b = None if bias is None else _want("bias", bias, torch.int64, (route.experts, M),
+                                        route.device)
+    ld = X.shape[2]
+    out = _want_out("out", out, (route.rows, M, ld), X.device, L)
+    with torch.cuda.device(X.device):
+        _check("pnb_expert_contract",
+               lib().pnb_expert_contract(_ptr(route.row_choice), _ptr(route.row_expert),
+                                         route.tokens, route.top_k, route.experts,
+                                         int(sorted_rows), _ptr(W), _ptr(b), delta % (1 << 64), M,
+                                         K, _ptr(X), ld, _ptr(out), ld, L, _stream(X.device)))
+    return out
+
+
+def adapter_contract(W: torch.Tensor, bias: torch.Tensor | None, delta: int, A: torch.Tensor,
+                     B: torch.Tensor, adapter: torch.Tensor, X: torch.Tensor,
+                     lwe_len: int | None = None, base_shift: int = 0,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """A shared projection with a low-rank adapter per request (``pnb_adapter_contract``):
+    ``Y[b] = 2**base_shift * W X[b] + B[a] (A[a] X[b]) + bias * delta`` (on the body) with
+    ``a = adapter[b]``; a value outside [0, adapters) means the shared projection alone.
+    ``W`` int8 [M, K], ``A`` int8 [adapters, rank, K], ``B`` int8 [adapters, M, rank], ``bias``
+    int64 [M] or None, ``adapter`` int32 [batch], ``X`` [batch, K, ld] -> [batch, M, ld]."""
+    X, L = _want_words("X", X, lwe_len)
+    if W.dim() != 2 or A.dim() != 3:
+        raise ValueError(f"W must be [M, K] and A [adapters, rank, K], got {tuple(W.shape)} and "
+                         f"{tuple(A.shape)}")
+    (M, K), (n, rank) = W.shape, A.shape[:2]
+    batch, _, ld = X.shape
+    dev = X.device
+    W = _want("W", W, torch.int8, (M, K), dev)
+    A = _want("A", A, torch.int8, (n, rank, K), dev)
+    B = _want("B", B, torch.int8, (n, M, rank), dev)
+    adapter = _want("adapter", adapter, torch.int32, (batch,), dev)
+    X = _want("X", X, X.dtype, (None, K, None), dev)
+    b = None if bias is None else _want("bias", bias, torch.int64, (M,), dev)
+    out = _want_out("out", out, (batch, M, ld), dev, L)
+    with torch.cuda.device(dev):
+        _check("pnb_adapter_contract",
+               lib().pnb_adapter_contract(_ptr(W), _ptr(b), delta % (1 << 64), base_shift, M, K,
+                                          _ptr(A), _ptr(B), n, rank, _ptr(adapter), _ptr(X), ld,
+                                          _ptr(out), ld, batch, L, _stream(dev)))
     return out
 
 

@@ -468,6 +468,128 @@ int pnb_lwe_contract_gather_ld(const int8_t* W_dev, const int64_t* bias_dev, uin
                                     Y_dev, lwe_len, 0, (cudaStream_t)stream, ldx, ldy);
 }
 
+static int check_route(const char* fn, int tokens, int top_k) {
+  if (tokens < 0 || top_k < 1 || (long long)tokens * top_k > PNB_MAX_CHOICES) {
+    set_error("%s: bad shape tokens=%d top_k=%d (top_k >= 1, at most %d choices)", fn, tokens,
+              top_k, PNB_MAX_CHOICES);
+    return PNB_ERR_INVALID;
+  }
+  return PNB_OK;
+}
+
+// Rows of `features` ciphertexts at two pitches.
+static int check_rows(const char* fn, int features, int lwe_len, int ld_in, int ld_out) {
+  if (features < 1 || lwe_len < 1 || ld_in < lwe_len || ld_out < lwe_len) {
+    set_error("%s: bad rows: %d ciphertexts of %d words at pitches %d and %d", fn, features,
+              lwe_len, ld_in, ld_out);
+    return PNB_ERR_INVALID;
+  }
+  return PNB_OK;
+}
+
+static int check_weights(const char* fn, int M, int K) {
+  if (M < 1 || K < 1 || K > 65536) {
+    set_error("%s: bad weights M=%d K=%d (K <= 65536)", fn, M, K);
+    return PNB_ERR_INVALID;
+  }
+  return PNB_OK;
+}
+
+int pnb_expert_route(const int32_t* ids_dev, int tokens, int top_k, int experts,
+                     int32_t* offsets_dev, int32_t* row_choice_dev, int32_t* row_expert_dev,
+                     int32_t* choice_row_dev, void* stream) {
+  int rc = check_route("expert_route", tokens, top_k);
+  if (rc) return rc;
+  if (experts < 1 || experts > PNB_MAX_EXPERTS) {
+    set_error("expert_route: %d experts (1..%d)", experts, PNB_MAX_EXPERTS);
+    return PNB_ERR_INVALID;
+  }
+  if (!offsets_dev ||
+      (tokens > 0 && (!ids_dev || !row_choice_dev || !row_expert_dev || !choice_row_dev))) {
+    set_error("expert_route: NULL buffer");
+    return PNB_ERR_INVALID;
+  }
+  return expert_route(ids_dev, tokens * top_k, experts, offsets_dev, row_choice_dev,
+                      row_expert_dev, choice_row_dev, (cudaStream_t)stream);
+}
+
+int pnb_expert_dispatch(const int32_t* choice_row_dev, int tokens, int top_k,
+                        const int32_t* weights_dev, const uint64_t* X_dev, int features, int ldx,
+                        uint64_t* out_dev, int ldo, int lwe_len, void* stream) {
+  int rc = check_route("expert_dispatch", tokens, top_k);
+  if (!rc) rc = check_rows("expert_dispatch", features, lwe_len, ldx, ldo);
+  if (rc) return rc;
+  if (tokens == 0) return PNB_OK;
+  if (!choice_row_dev || !X_dev || !out_dev) {
+    set_error("expert_dispatch: NULL buffer");
+    return PNB_ERR_INVALID;
+  }
+  return expert_dispatch(choice_row_dev, tokens, top_k, weights_dev, X_dev, features, ldx, out_dev,
+                         ldo, lwe_len, (cudaStream_t)stream);
+}
+
+int pnb_expert_combine(const int32_t* choice_row_dev, int tokens, int top_k,
+                       const int32_t* weights_dev, const uint64_t* Y_dev, int features, int ldy,
+                       uint64_t* out_dev, int ldo, int lwe_len, void* stream) {
+  int rc = check_route("expert_combine", tokens, top_k);
+  if (!rc) rc = check_rows("expert_combine", features, lwe_len, ldy, ldo);
+  if (rc) return rc;
+  if (tokens == 0) return PNB_OK;
+  if (!choice_row_dev || !Y_dev || !out_dev) {
+    set_error("expert_combine: NULL buffer");
+    return PNB_ERR_INVALID;
+  }
+  return expert_combine(choice_row_dev, tokens, top_k, weights_dev, Y_dev, features, ldy, out_dev,
+                        ldo, lwe_len, (cudaStream_t)stream);
+}
+
+int pnb_expert_contract(const int32_t* row_choice_dev, const int32_t* row_expert_dev, int tokens,
+                        int top_k, int experts, int sorted_rows, const int8_t* W_dev,
+                        const int64_t* bias_dev, uint64_t delta, int M, int K,
+                        const uint64_t* X_dev, int ldx, uint64_t* Y_dev, int ldy, int lwe_len,
+                        void* stream) {
+  int rc = check_route("expert_contract", tokens, top_k);
+  if (!rc) rc = check_weights("expert_contract", M, K);
+  if (!rc) rc = check_rows("expert_contract", 1, lwe_len, ldx, ldy);
+  if (rc) return rc;
+  if (experts < 1 || experts > PNB_MAX_EXPERTS) {
+    set_error("expert_contract: %d experts (1..%d)", experts, PNB_MAX_EXPERTS);
+    return PNB_ERR_INVALID;
+  }
+  if (tokens == 0) return PNB_OK;
+  if (!row_choice_dev || !row_expert_dev || !W_dev || !X_dev || !Y_dev) {
+    set_error("expert_contract: NULL buffer");
+    return PNB_ERR_INVALID;
+  }
+  return expert_contract(row_choice_dev, row_expert_dev, tokens, top_k, experts, sorted_rows != 0,
+                         W_dev, bias_dev, delta, M, K, X_dev, ldx, Y_dev, ldy, lwe_len,
+                         (cudaStream_t)stream);
+}
+
+int pnb_adapter_contract(const int8_t* W_dev, const int64_t* bias_dev, uint64_t delta,
+                         int base_shift, int M, int K, const int8_t* A_dev, const int8_t* B_dev,
+                         int adapters, int rank, const int32_t* adapter_dev,
+                         const uint64_t* X_dev, int ldx, uint64_t* Y_dev, int ldy, int batch,
+                         int lwe_len, void* stream) {
+  int rc = check_weights("adapter_contract", M, K);
+  if (!rc) rc = check_rows("adapter_contract", 1, lwe_len, ldx, ldy);
+  if (rc) return rc;
+  if (batch < 0 || adapters < 1 || rank < 1 || rank > PNB_MAX_RANK || base_shift < 0 ||
+      base_shift > 63) {
+    set_error("adapter_contract: bad shape batch=%d adapters=%d rank=%d (1..%d) base_shift=%d "
+              "(0..63)", batch, adapters, rank, PNB_MAX_RANK, base_shift);
+    return PNB_ERR_INVALID;
+  }
+  if (batch == 0) return PNB_OK;
+  if (!W_dev || !A_dev || !B_dev || !adapter_dev || !X_dev || !Y_dev) {
+    set_error("adapter_contract: NULL buffer");
+    return PNB_ERR_INVALID;
+  }
+  return adapter_contract(W_dev, bias_dev, delta, base_shift, M, K, A_dev, B_dev, adapters, rank,
+                          adapter_dev, X_dev, ldx, Y_dev, ldy, batch, lwe_len,
+                          (cudaStream_t)stream);
+}
+
 int pnb_fft_negacyclic_mul(int device, int N, const int64_t* a_dev, const uint64_t* b_dev,
                            uint64_t* out_dev, int count, void* stream) {
   if (count < 0 || (count > 0 && (!a_dev || !b_dev || !out_dev))) {

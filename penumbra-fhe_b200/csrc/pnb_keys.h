@@ -71,6 +71,24 @@ int lwe_contract_gather_placed(const int8_t* W, const int64_t* bias, uint64_t de
 int lwe_contract_gather(const int8_t* W, const int64_t* bias, uint64_t delta, int M, int K,
                         const uint64_t* X, const int32_t* idx, int G, uint64_t* Y, int L,
                         cudaStream_t st);
+// Rows of tokens sorted by expert, moved there and back (expert.cu); contractions whose weights
+// differ from request to request (request.cu).  Arguments are checked by the C ABI.
+int expert_route(const int32_t* ids, int n, int experts, int32_t* offsets, int32_t* row_choice,
+                 int32_t* row_expert, int32_t* choice_row, cudaStream_t st);
+int expert_dispatch(const int32_t* choice_row, int tokens, int top_k, const int32_t* weights,
+                    const uint64_t* X, int features, int ldx, uint64_t* out, int ldo, int L,
+                    cudaStream_t st);
+int expert_combine(const int32_t* choice_row, int tokens, int top_k, const int32_t* weights,
+                   const uint64_t* Y, int features, int ldy, uint64_t* out, int ldo, int L,
+                   cudaStream_t st);
+int expert_contract(const int32_t* row_choice, const int32_t* row_expert, int tokens, int top_k,
+                    int experts, bool sorted_rows, const int8_t* W, const int64_t* bias,
+                    uint64_t delta, int M, int K, const uint64_t* X, int ldx, uint64_t* Y, int ldy,
+                    int L, cudaStream_t st);
+int adapter_contract(const int8_t* W, const int64_t* bias, uint64_t delta, int base_shift, int M,
+                     int K, const int8_t* A, const int8_t* B, int adapters, int rank,
+                     const int32_t* adapter, const uint64_t* X, int ldx, uint64_t* Y, int ldy,
+                     int batch, int L, cudaStream_t st);
 int keyswitch_tc(const pnb_keys* K, const uint64_t* in, uint64_t* out, int count, void* digits,
                  cudaStream_t st, int in_ld = 0);
 size_t ks_tc_workspace_bytes(const pnb_params& p, int count);
