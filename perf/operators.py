@@ -220,7 +220,7 @@ def _run_own(s):
     pnb, case, op = _pnb(), s["case"], s["op"]
     if op == "route":
         r = pnb.expert_route(s["ids"], case["experts"], out=s["route"])
-        return r.offsets, r.row_choice, r.choice_row
+        return r.offsets, r.row_choice, r.choice_row.view(-1)
     L = case["lwe_len"]
     if op == "dispatch":
         return pnb.expert_dispatch(s["route"], s["X"], L, weights=s["weights"], out=s["out"])
