@@ -286,7 +286,7 @@ int pnb_fft_negacyclic_mul(int device, int N, const int64_t* a_dev, const uint64
 
 /* Read and clear the device status words of the kernels with bounded waits: 0 when no wait ran
  * out since the last read; otherwise 1-3 keyswitch (producer, MMA, epilogue), 17 blind
- * rotation, 33 contraction.  No reference counterpart. */
+ * rotation, 33 contraction, 49 per-request contraction.  No reference counterpart. */
 int pnb_device_status(int device, int* status_out);
 
 /* Measure this device's FP64 FMA throughput (TFLOP/s) with a short register-only kernel; the

@@ -605,14 +605,16 @@ int pnb_device_status(int device, int* status_out) {
   if (!status_out) { set_error("status_out is NULL"); return PNB_ERR_INVALID; }
   DeviceGuard g(device);
   if (g.rc) return g.rc;
-  int a = 0, b = 0, c = 0;
+  int a = 0, b = 0, c = 0, d = 0;
   int rc = tc_status_read_and_clear(&a);
   if (rc) return rc;
   rc = br_status_read_and_clear(&b);
   if (rc) return rc;
   rc = ct_status_read_and_clear(&c);
   if (rc) return rc;
-  *status_out = a ? a : (b ? 16 + b : (c ? 32 + c : 0));
+  rc = rq_status_read_and_clear(&d);
+  if (rc) return rc;
+  *status_out = a ? a : (b ? 16 + b : (c ? 32 + c : (d ? 48 + d : 0)));
   return PNB_OK;
 }
 

@@ -99,4 +99,5 @@ int pbs_batch_noalloc(const pnb_keys* K, const uint64_t* tv, const uint64_t* in,
 int br_status_read_and_clear(int* out);
 int br8_status_read_and_clear(int* out);
 int ct_status_read_and_clear(int* out);
+int rq_status_read_and_clear(int* out);
 }  // namespace pnb
