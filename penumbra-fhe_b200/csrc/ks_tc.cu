@@ -39,7 +39,7 @@ int tc_status_read_and_clear(int* out) {
 // ------------------------------------------------------------------------------------------
 // Host: TMA descriptors through the driver entry point (no link-time libcuda dependency).
 // ------------------------------------------------------------------------------------------
-static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -56,7 +56,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 // 2-D u8 tensor [outer][inner] with a row pitch, tiles of box_inner x box_outer, 128B swizzle.
 int make_tmap_u8_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                     uint64_t pitch_bytes, uint32_t box_inner, uint32_t box_outer) {
-  auto fn = encode_fn();
+  auto fn = tmap_encoder();
   if (!fn) {
     set_error("cuTensorMapEncodeTiled is unavailable from the driver");
     return PNB_ERR_CUDA;

@@ -23,6 +23,11 @@
 // M = 128 operand would double it).  The epilogue warps add up the limbs of t = A X mod 2^64
 // across lanes, write t's bytes to shared memory as the next MN-major operand, and one short MMA
 // makes D = B t.  y = (C << s) + D.  X is read once; t never leaves the SM.
+//
+// Rows that start 16-byte aligned (an even pitch) move by TMA straight into the operand layout, and
+// results leave by TMA.  Other rows (contiguous [count][kN+1] ciphertexts) are off by one word
+// every other row, which no tiled load can shift: they land unshifted in a ring of raw slots, and
+// four warps copy them word by word into the operand layout.
 #include <algorithm>
 
 #include <cudaTypedefs.h>
@@ -45,36 +50,50 @@ int rq_status_read_and_clear(int* out) {
   return PNB_OK;
 }
 
-int make_tmap_u8_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
-                    uint64_t pitch_bytes, uint32_t box_inner, uint32_t box_outer);
+PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder();
 
 constexpr int RQ_BM = 128;      // output rows per tile
 constexpr int RQ_WORDS = 32;    // output words per tile
 constexpr int RQ_BN = 8 * RQ_WORDS;
 constexpr int RQ_BK = 128;      // K per stage
-constexpr int RQ_KBOX = 32;     // K per X box and MMA step: a ragged K costs at most 31 rows
+constexpr int RQ_KSTEP = 32;    // K per MMA; a ragged K costs at most 31 rows
 constexpr int RQ_W_BYTES = RQ_BM * RQ_BK;              // 16 KB
 constexpr int RQ_X_BYTES = RQ_BK * RQ_BN;              // 32 KB
 constexpr int RQ_A_BYTES = PNB_MAX_RANK * RQ_BK;       // 8 KB
 constexpr int RQ_T_BYTES = PNB_MAX_RANK * RQ_BN;       // 16 KB: t as bytes
-constexpr int RQ_B_BYTES = RQ_BM * 128;                // 16 KB: B rows, 128-byte pitch
+constexpr int RQ_B_BYTES = RQ_BM * PNB_MAX_RANK;       // 8 KB: B rows of 64 bytes
 constexpr int RQ_EPI_WARPS = 8;                        // two per TMEM lane quarter
-constexpr int RQ_EPI_BYTES = RQ_EPI_WARPS * 32 * 8 * 8;
+constexpr int RQ_COPY_WARPS = 4;
+constexpr int RQ_RAW_ROWS = 32;                        // rows per raw slot, half of each parity
+constexpr int RQ_RAW_PITCH = 8 * (RQ_WORDS + 2);       // one word of shift, to 16 bytes
+constexpr int RQ_RAW_BYTES = RQ_RAW_ROWS * RQ_RAW_PITCH;
 constexpr uint32_t RQ_WAIT_LIMIT = 1u << 24;
 
-// How X reaches shared memory: rows that start 16-byte aligned (an even pitch) by TMA; other rows
-// by 8-byte cp.async from 8 warps.
-enum : int { RQ_TMA = 0, RQ_COPY8 = 1 };
-
-template <int MODE, bool ADAPT>
+template <bool SHIFTED, bool ADAPT>
 struct RqShape {
-  static constexpr int STAGE = RQ_W_BYTES + (ADAPT ? RQ_A_BYTES : 0) + RQ_X_BYTES;
-  static constexpr int STAGES = ADAPT || MODE == RQ_COPY8 ? 3 : 4;
-  static constexpr int PW = MODE == RQ_TMA ? 1 : 8;  // producer warps
-  static constexpr int THREADS = 32 * (PW + 1 + RQ_EPI_WARPS);
-  static constexpr int T_AT = STAGES * STAGE;                  // t, then B (adapters only)
-  static constexpr int BARS_AT = T_AT + (ADAPT ? RQ_T_BYTES + RQ_B_BYTES : 0);
-  static constexpr int SMEM = 1024 + BARS_AT + 256 + RQ_EPI_BYTES;
+  static constexpr int STAGE = RQ_W_BYTES + RQ_X_BYTES + (ADAPT ? RQ_A_BYTES : 0);
+  // shifted rows wait in the raw ring, so two operand stages do
+  static constexpr int STAGES = SHIFTED ? 2 : ADAPT ? 3 : 4;
+  static constexpr int RAW = SHIFTED ? (ADAPT ? 8 : 12) : 0;  // raw slots
+  static constexpr int COPY = SHIFTED ? RQ_COPY_WARPS : 0;
+  static constexpr int MMA_WARP = 1 + COPY;  // warp 0 issues the loads
+  static constexpr int THREADS = 32 * (2 + COPY + RQ_EPI_WARPS);
+  // output staging of one epilogue warp: 32 rows x 16 words leaving by TMA, or x 8 by plain stores
+  static constexpr int OUT = SHIFTED ? 32 * 64 : 32 * 128;
+  static constexpr int RAW_AT = STAGES * STAGE;
+  static constexpr int T_AT = RAW_AT + RAW * RQ_RAW_BYTES;
+  static constexpr int B_AT = T_AT + (ADAPT ? RQ_T_BYTES : 0);
+  static constexpr int OUT_AT = B_AT + (ADAPT ? RQ_B_BYTES : 0);
+  static constexpr int BARS_AT = OUT_AT + RQ_EPI_WARPS * OUT;
+  static constexpr int SMEM = 1024 + BARS_AT + 512;
+  static_assert(SMEM <= 227 * 1024, "shared memory of one block");
+  static_assert(8 * (2 * STAGES + 8 + 2 * RAW) + 16 <= 512, "barriers");
+  static_assert(T_AT % 1024 == 0 && B_AT % 1024 == 0 && OUT_AT % 1024 == 0, "swizzle atoms");
+};
+
+struct RqMaps {
+  CUtensorMap W, A, B, Y;
+  CUtensorMap X[2];  // aligned: boxes of 128 and of 32 rows; shifted: rows 0, 2, .. and 1, 3, ..
 };
 
 struct RqArgs {
@@ -87,6 +106,7 @@ struct RqArgs {
   int rows, top_k, choices, n_which;
   int M, K, L, ldx, ldy;
   int shift, rank, rank16;    // adapters
+  int off0, off1;             // words by which rows 0, 2, .. / 1, 3, .. start past 16-byte alignment
   int m_tiles, n_tiles, k_blocks, w_rows;
 };
 
@@ -121,20 +141,32 @@ __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int m) {
   return (uint64_t)__shfl_xor_sync(0xffffffffu, (unsigned long long)v, m);
 }
 
-template <int MODE, bool ADAPT>
-__global__ void __launch_bounds__(RqShape<MODE, ADAPT>::THREADS, 1) request_kernel(
-    const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-    const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, RqArgs a) {
-  using S = RqShape<MODE, ADAPT>;
-  constexpr int STAGES = S::STAGES;
-  constexpr int MMA_WARP = S::PW;
+// v + sum_b c[b] << 8b mod 2^64: the low four limb sums reach into the high word (one multiply-add
+// of 32 x 32 + 64 bits each), the high four only live there.
+__device__ __forceinline__ uint64_t add_limbs(uint64_t v, const uint32_t* c) {
+  int64_t s = (int64_t)v;
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+    asm("mad.wide.s32 %0, %1, %2, %0;" : "+l"(s) : "r"((int)c[b]), "r"(1 << (8 * b)));
+  uint32_t hi = (uint32_t)((uint64_t)s >> 32);
+#pragma unroll
+  for (int b = 0; b < 4; ++b) hi += c[4 + b] << (8 * b);
+  return ((uint64_t)hi << 32) | (uint32_t)s;
+}
+
+template <bool SHIFTED, bool ADAPT>
+__global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
+    request_kernel(const __grid_constant__ RqMaps tm, RqArgs a) {
+  using S = RqShape<SHIFTED, ADAPT>;
+  constexpr int STAGES = S::STAGES, RAW = S::RAW;
   extern __shared__ unsigned char rq_raw[];
   const uint32_t raw = tc::smem_u32(rq_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   auto w_at = [&](int s) { return base + (uint32_t)(s * S::STAGE); };
   auto x_at = [&](int s) { return w_at(s) + RQ_W_BYTES; };
   auto a_at = [&](int s) { return x_at(s) + RQ_X_BYTES; };
-  const uint32_t t_at = base + S::T_AT, b_at = t_at + RQ_T_BYTES;
+  auto raw_at = [&](int r) { return base + (uint32_t)(S::RAW_AT + r * RQ_RAW_BYTES); };
+  const uint32_t t_at = base + S::T_AT, b_at = base + S::B_AT;
   const uint32_t bars = base + S::BARS_AT;
   auto full = [&](int s) { return bars + 8u * s; };
   auto empty = [&](int s) { return bars + 8u * (STAGES + s); };
@@ -142,13 +174,15 @@ __global__ void __launch_bounds__(RqShape<MODE, ADAPT>::THREADS, 1) request_kern
   auto acc_empty = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
   const uint32_t low_full = bars + 8u * (2 * STAGES + 4), t_full = low_full + 8,
                  b_full = low_full + 16, b_empty = low_full + 24;
-  const uint32_t holder = low_full + 32;
+  auto raw_full = [&](int r) { return low_full + 32 + 8u * r; };
+  auto raw_empty = [&](int r) { return low_full + 32 + 8u * (RAW + r); };
+  const uint32_t holder = low_full + 32 + 16u * RAW;
   volatile int* abort_s = reinterpret_cast<volatile int*>(rq_raw + (holder + 8 - raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      tc::mbar_init(full(s), MODE == RQ_TMA ? 1 : 32 * S::PW + 1);
+      tc::mbar_init(full(s), 1 + S::COPY);
       tc::mbar_init(empty(s), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -159,16 +193,22 @@ __global__ void __launch_bounds__(RqShape<MODE, ADAPT>::THREADS, 1) request_kern
     tc::mbar_init(t_full, 32 * RQ_EPI_WARPS);
     tc::mbar_init(b_full, 1);
     tc::mbar_init(b_empty, 1);
+    for (int r = 0; r < RAW; ++r) {
+      tc::mbar_init(raw_full(r), 1);
+      tc::mbar_init(raw_empty(r), RQ_COPY_WARPS);
+    }
     *abort_s = 0;
     tc::fence_mbar_init();
-    tc::prefetch_tmap(&tmW);
-    if (MODE == RQ_TMA) tc::prefetch_tmap(&tmX);
+    tc::prefetch_tmap(&tm.W);
+    tc::prefetch_tmap(&tm.X[0]);
+    tc::prefetch_tmap(&tm.X[1]);
     if (ADAPT) {
-      tc::prefetch_tmap(&tmA);
-      tc::prefetch_tmap(&tmB);
+      tc::prefetch_tmap(&tm.A);
+      tc::prefetch_tmap(&tm.B);
     }
+    if (!SHIFTED) tc::prefetch_tmap(&tm.Y);
   }
-  if (warp == MMA_WARP) tc::tmem_alloc(holder, 512);
+  if (warp == S::MMA_WARP) tc::tmem_alloc(holder, 512);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -183,18 +223,17 @@ __global__ void __launch_bounds__(RqShape<MODE, ADAPT>::THREADS, 1) request_kern
     mt = r / a.n_tiles;
     nt = r - mt * a.n_tiles;
   };
-  // K rows of block kb, rounded up to whole MMA steps
+  // K rows of block kb, rounded up to whole MMAs.  The rows past K belong to the next group (or lie
+  // past the tensor and read as zeros) and meet zero weights.
   auto k_rows = [&](int kb) {
-    return min(RQ_BK, ((a.K - kb * RQ_BK) + RQ_KBOX - 1) / RQ_KBOX * RQ_KBOX);
+    return min(RQ_BK, ((a.K - kb * RQ_BK) + RQ_KSTEP - 1) / RQ_KSTEP * RQ_KSTEP);
   };
-  const uint32_t w_bytes = (uint32_t)(a.w_rows * RQ_BK), a_bytes = (uint32_t)(a.rank16 * RQ_BK);
 
-  if (warp < S::PW) {
-    // ---------------- producers -----------------------------------------------------------------
-    constexpr int LAG = STAGES - 1;
-    int kbg = 0, released = 0, has_n = 0;
-    const bool lead = warp == 0 && lane == 0;
-    if (MODE != RQ_TMA || lead) {
+  if (warp == 0) {
+    // ---------------- loads (one lane) -----------------------------------------------------------
+    if (lane == 0) {
+      const uint32_t w_bytes = (uint32_t)(a.w_rows * RQ_BK), a_bytes = (uint32_t)(a.rank16 * RQ_BK);
+      int kbg = 0, rawg = 0, has_n = 0;
       for (long long t = blockIdx.x; t < total && !*abort_s; t += gridDim.x) {
         int n, mt, nt, src, w;
         decode(t, n, mt, nt);
@@ -203,76 +242,106 @@ __global__ void __launch_bounds__(RqShape<MODE, ADAPT>::THREADS, 1) request_kern
         const bool has = ADAPT && w >= 0;
         const int w_row = (ADAPT ? 0 : w * a.M) + mt * RQ_BM;
         bool ok = true;
-        for (int kb = 0; kb < a.k_blocks; ++kb, ++kbg) {
+        for (int kb = 0; kb < a.k_blocks && ok; ++kb, ++kbg) {
           const int s = kbg % STAGES;
+          const int kr = k_rows(kb);
+          const int row = src * a.K + kb * RQ_BK;
+          if (SHIFTED) {
+            for (int r = 0; r < kr; r += RQ_RAW_ROWS, ++rawg) {
+              const int slot = rawg % RAW;
+              const uint32_t use = (uint32_t)(rawg / RAW);
+              if (use > 0 && !rq_wait(raw_empty(slot), (use - 1) & 1u, abort_s)) { ok = false; break; }
+              tc::mbar_expect_tx(raw_full(slot), RQ_RAW_BYTES);
+              const int first = row + r;  // its rows of either parity, in order
+              tc::tma_load_2d(raw_at(slot), &tm.X[first & 1], nt * RQ_WORDS, first >> 1,
+                              raw_full(slot));
+              tc::tma_load_2d(raw_at(slot) + RQ_RAW_BYTES / 2, &tm.X[(first + 1) & 1],
+                              nt * RQ_WORDS, (first + 1) >> 1, raw_full(slot));
+            }
+            if (!ok) break;
+          }
           const uint32_t use = (uint32_t)(kbg / STAGES);
           if (use > 0 && !rq_wait(empty(s), (use - 1) & 1u, abort_s)) { ok = false; break; }
-          const int kr = k_rows(kb);
-          if (lead) {
-            tc::mbar_expect_tx(full(s), w_bytes + (has ? a_bytes : 0u) +
-                                            (MODE == RQ_TMA ? (uint32_t)(kr * RQ_BN) : 0u));
-            tc::tma_load_2d(w_at(s), &tmW, kb * RQ_BK, w_row, full(s));
-            if (has) tc::tma_load_2d(a_at(s), &tmA, kb * RQ_BK, w * a.rank, full(s));
-          }
-          if (MODE == RQ_TMA) {
-            // rows past K belong to the next group (or lie past the tensor and read as zeros)
-            // and meet zero weights
-            for (int r = 0; r < kr; r += RQ_KBOX) {
-              const int row = src * a.K + kb * RQ_BK + r;
-              tc::tma_load_2d(x_at(s) + r * 128, &tmX, nt * RQ_BN, row, full(s));
-              tc::tma_load_2d(x_at(s) + RQ_BK * 128 + r * 128, &tmX, nt * RQ_BN + 128, row,
+          tc::mbar_expect_tx(full(s), w_bytes + (has ? a_bytes : 0u) +
+                                          (SHIFTED ? 0u : (uint32_t)(kr * RQ_BN)));
+          tc::tma_load_2d(w_at(s), &tm.W, kb * RQ_BK, w_row, full(s));
+          if (has) tc::tma_load_2d(a_at(s), &tm.A, kb * RQ_BK, w * a.rank, full(s));
+          if (!SHIFTED) {
+            const CUtensorMap* mx = kr == RQ_BK ? &tm.X[0] : &tm.X[1];
+            const int step = kr == RQ_BK ? RQ_BK : RQ_KSTEP;
+            for (int r = 0; r < kr; r += step) {
+              tc::tma_load_2d(x_at(s) + r * 128, mx, nt * RQ_BN, row + r, full(s));
+              tc::tma_load_2d(x_at(s) + RQ_BK * 128 + r * 128, mx, nt * RQ_BN + 128, row + r,
                               full(s));
-            }
-          } else {
-            const int col = nt * RQ_WORDS + lane;
-            const int box = lane >> 4, ch = (lane & 15) >> 1, half = lane & 1;
-            const uint64_t* xp = a.X + ((size_t)src * a.K + kb * RQ_BK) * a.ldx + col;
-#pragma unroll 4
-            for (int r = warp; r < kr; r += S::PW) {
-              const bool in = col < a.L && kb * RQ_BK + r < a.K;
-              const uint32_t dst = x_at(s) + box * (RQ_BK * 128) + (r >> 3) * 1024 +
-                                   (r & 7) * 128 + ((ch ^ (r & 7)) << 4) + half * 8;
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst),
-                           "l"(in ? xp + (size_t)r * a.ldx : a.X), "r"(in ? 8u : 0u)
-                           : "memory");
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (kbg + 1 - released > LAG) {
-              asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              tc::mbar_arrive(full(released % STAGES));
-              ++released;
             }
           }
         }
         if (!ok) break;
-        if (has && lead) {
-          if (MODE != RQ_TMA) {  // the previous tile must not wait for copies that lag behind
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            for (; released < kbg; ++released) tc::mbar_arrive(full(released % STAGES));
-          }
+        if (has) {
           // after this tile's K blocks: the wait for the previous tile's last MMA is then short
           if (has_n > 0 && !rq_wait(b_empty, (uint32_t)(has_n - 1) & 1u, abort_s)) break;
           tc::mbar_expect_tx(b_full, RQ_B_BYTES);
-          tc::tma_load_2d(b_at, &tmB, 0, w * a.M + mt * RQ_BM, b_full);
+          tc::tma_load_2d(b_at, &tm.B, 0, w * a.M + mt * RQ_BM, b_full);
           ++has_n;
         }
       }
-      if (MODE != RQ_TMA) {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        for (; released < kbg; ++released) tc::mbar_arrive(full(released % STAGES));
-      }
-      // no copy may still be landing when the block exits: the last use of each slot completes
-      // when its copies have landed (bounded; immediate unless a wait ran out)
-      if (lead) {
-        for (int k = kbg > STAGES ? kbg - STAGES : 0; k < kbg; ++k)
-          (void)tc::mbar_wait(full(k % STAGES), (uint32_t)(k / STAGES) & 1u, RQ_WAIT_LIMIT);
-        if (has_n > 0) (void)tc::mbar_wait(b_full, (uint32_t)(has_n - 1) & 1u, RQ_WAIT_LIMIT);
-      }
+      // no load may still be landing when the block exits: the last use of each slot completes
+      // when it has landed (bounded; immediate unless a wait ran out)
+      for (int k = kbg > STAGES ? kbg - STAGES : 0; k < kbg; ++k)
+        (void)tc::mbar_wait(full(k % STAGES), (uint32_t)(k / STAGES) & 1u, RQ_WAIT_LIMIT);
+      if (SHIFTED)
+        for (int k = rawg > RAW ? rawg - RAW : 0; k < rawg; ++k)
+          (void)tc::mbar_wait(raw_full(k % RAW), (uint32_t)(k / RAW) & 1u, RQ_WAIT_LIMIT);
+      if (has_n > 0) (void)tc::mbar_wait(b_full, (uint32_t)(has_n - 1) & 1u, RQ_WAIT_LIMIT);
     }
-  } else if (warp == MMA_WARP) {
+  } else if (warp < S::MMA_WARP) {
+    // ---------------- raw rows -> operand layout (shifted rows only) -----------------------------
+    const int cw = warp - 1;
+    constexpr int ROWS = RQ_RAW_ROWS / RQ_COPY_WARPS;  // rows of each slot per warp
+    const int box = lane >> 4, ch = (lane & 15) >> 1, half = lane & 1;
+    int kbg = 0, rawg = 0;
+    for (long long t = blockIdx.x; t < total && !*abort_s; t += gridDim.x) {
+      int n, mt, nt, src, w;
+      decode(t, n, mt, nt);
+      rq_row<ADAPT>(a, n, src, w);
+      if (src < 0) continue;
+      bool ok = true;
+      for (int kb = 0; kb < a.k_blocks && ok; ++kb, ++kbg) {
+        const int s = kbg % STAGES;
+        const uint32_t use = (uint32_t)(kbg / STAGES);
+        if (use > 0 && !rq_wait(empty(s), (use - 1) & 1u, abort_s)) { ok = false; break; }
+        const int kr = k_rows(kb);
+        const int parity = (src * a.K + kb * RQ_BK) & 1;  // of the stage's first row
+        for (int r0 = 0; r0 < kr; r0 += RQ_RAW_ROWS, ++rawg) {
+          const int slot = rawg % RAW;
+          if (!rq_wait(raw_full(slot), (uint32_t)(rawg / RAW) & 1u, abort_s)) { ok = false; break; }
+          uint64_t v[ROWS];
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i) {
+            const int r = cw * ROWS + i;
+            const int off = ((parity + r) & 1) ? a.off1 : a.off0;
+            v[i] = *reinterpret_cast<const uint64_t*>(
+                rq_raw + (raw_at(slot) - raw) + (r & 1) * (RQ_RAW_BYTES / 2) +
+                (r >> 1) * RQ_RAW_PITCH + (lane + off) * 8);
+          }
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i) {
+            const int r = r0 + cw * ROWS + i;
+            *reinterpret_cast<uint64_t*>(rq_raw + (x_at(s) - raw) + box * (RQ_BK * 128) +
+                                         (r >> 3) * 1024 + (r & 7) * 128 +
+                                         ((ch ^ (r & 7)) << 4) + half * 8) = v[i];
+          }
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(raw_empty(slot));
+        }
+        if (!ok) break;
+        tc::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(full(s));
+      }
+      if (!ok) break;
+    }
+  } else if (warp == S::MMA_WARP) {
     // ---------------- MMA issue (one lane) -------------------------------------------------------
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, RQ_BN, true, false, false, true);
@@ -295,7 +364,7 @@ __global__ void __launch_bounds__(RqShape<MODE, ADAPT>::THREADS, 1) request_kern
           const int s = kbg % STAGES;
           if (!rq_wait(full(s), (uint32_t)(kbg / STAGES) & 1u, abort_s)) { ok = false; break; }
           tc::tc_fence_after();
-          const int steps = k_rows(kb) / RQ_KBOX;
+          const int steps = k_rows(kb) / RQ_KSTEP;
           for (int k = 0; k < steps; ++k) {
             const uint32_t acc = (kb | k) != 0 ? 1u : 0u;
             const uint64_t wd = tc::smem_desc_sw128(w_at(s) + 32u * k, 16u, 1024u);
@@ -319,7 +388,7 @@ __global__ void __launch_bounds__(RqShape<MODE, ADAPT>::THREADS, 1) request_kern
           tc::tc_fence_after();
           // columns of B past the rank are zero, so t's rows past it do not matter
           for (int k = 0; k < (a.rank + 31) / 32; ++k)
-            tc::mma_i8(tmem + 256u, tc::smem_desc_sw128(b_at + 32u * k, 16u, 1024u),
+            tc::mma_i8(tmem + 256u, tc::smem_desc_sw64(b_at + 32u * k, 16u, 512u),
                        tc::smem_desc_sw128(t_at + 4096u * k, PNB_MAX_RANK * 128u, 1024u), MAIN,
                        k != 0 ? 1u : 0u);
           tc::mma_commit(b_empty);
@@ -331,14 +400,14 @@ __global__ void __launch_bounds__(RqShape<MODE, ADAPT>::THREADS, 1) request_kern
     }
   } else {
     // ---------------- epilogue -------------------------------------------------------------------
-    // Warp w reads TMEM lane quarter w % 4 (32 output rows) and half eh of the tile's words, two
-    // chunks of 8 words; limbs become u64 words, staged in shared memory (32 rows x 8 words,
-    // XOR-swizzled) and written as 64-byte row segments.
-    const int e_w = warp - MMA_WARP - 1;
+    // Warp w reads TMEM lane quarter w % 4 (32 output rows, one per lane) and half eh of the tile's
+    // words.  Limb sums become u64 words, staged in shared memory with their 16-byte chunks XORed by
+    // the row, and leave as 32 rows x 16 words by TMA, or as 64-byte row segments by plain stores.
+    const int e_w = warp - S::MMA_WARP - 1;
     const int q = warp & 3, eh = e_w >> 2;
     constexpr int EW = RQ_WORDS / 2;
-    uint64_t* stage =
-        reinterpret_cast<uint64_t*>(rq_raw + (bars + 256 - raw)) + (size_t)e_w * 32 * 8;
+    const uint32_t out_at = base + S::OUT_AT + (uint32_t)(e_w * S::OUT);
+    unsigned char* out = rq_raw + (out_at - raw);
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
     int tt = 0, has_n = 0;
     for (long long t = blockIdx.x; t < total && !*abort_s; t += gridDim.x) {
@@ -378,7 +447,7 @@ __global__ void __launch_bounds__(RqShape<MODE, ADAPT>::THREADS, 1) request_kern
             *reinterpret_cast<uint64_t*>(rq_raw + (at - raw)) = v[j];
           }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc::fence_async_smem();
         tc::tc_fence_before();
         tc::mbar_arrive(t_full);
         ++has_n;
@@ -387,60 +456,87 @@ __global__ void __launch_bounds__(RqShape<MODE, ADAPT>::THREADS, 1) request_kern
       const int turn = ADAPT ? tt : tt >> 1;
       if (!rq_wait(acc_full(buf), (uint32_t)turn & 1u, abort_s)) break;
       tc::tc_fence_after();
+      if (!SHIFTED) {  // the staging rows of the previous tile have left
+        if (lane == 0) tc::tma_store_wait_read();
+        __syncwarp();
+      }
       const uint32_t c_tmem = tmem + (uint32_t)(buf * 256) + lanes + (uint32_t)(eh * EW * 8);
+      const int row0 = mt * RQ_BM + q * 32, col0 = nt * RQ_WORDS + eh * EW;
+      // the word of this half that is the body, and its bias
+      const int body = a.L - 1 - col0;
+      uint64_t bias = 0;
+      if (a.bias && body >= 0 && body < EW && row0 + lane < a.M)
+        bias = (uint64_t)__ldg(a.bias + (ADAPT ? (size_t)0 : (size_t)w * a.M) + row0 + lane) *
+               a.delta;
 #pragma unroll 1
       for (int cp = 0; cp < EW / 8; ++cp) {
         uint64_t y[8];
-        uint32_t r0[32];
+        const int bias_at = body - cp * 8;  // which of these 8 words is the body
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          tc::tmem_ld_32x32(c_tmem + (uint32_t)(cp * 64 + h * 32), r0);
+          uint32_t c[32], d[32];
+          tc::tmem_ld_32x32_nowait(c_tmem + (uint32_t)(cp * 64 + h * 32), c);
+          if (has) tc::tmem_ld_32x32_nowait(c_tmem + (uint32_t)(256 + cp * 64 + h * 32), d);
+          tc::tmem_ld_wait();
+          if (h == 1 && cp == EW / 8 - 1) {
+            tc::tc_fence_before();
+            tc::mbar_arrive(acc_empty(buf));
+          }
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            uint64_t v = 0;
-#pragma unroll
-            for (int b = 0; b < 8; ++b)
-              v += (uint64_t)(int64_t)(int32_t)r0[u * 8 + b] << (8 * b);
-            y[h * 4 + u] = ADAPT ? v << a.shift : v;
-          }
-          if (has) {
-            tc::tmem_ld_32x32(c_tmem + (uint32_t)(256 + cp * 64 + h * 32), r0);
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-              for (int b = 0; b < 8; ++b)
-                y[h * 4 + u] += (uint64_t)(int64_t)(int32_t)r0[u * 8 + b] << (8 * b);
+            uint64_t v = add_limbs(0, c + 8 * u);
+            if (ADAPT) v <<= a.shift;
+            if (has) v = add_limbs(v, d + 8 * u);
+            y[h * 4 + u] = v;
           }
         }
-        if (cp == EW / 8 - 1) {
-          tc::tc_fence_before();
-          tc::mbar_arrive(acc_empty(buf));
-        }
+        if (!SHIFTED) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) stage[lane * 8 + (u ^ (lane & 7))] = y[u];
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<ulonglong2*>(out + lane * 128 +
+                                           (((cp * 4 + u) ^ (lane & 7)) << 4)) =
+                make_ulonglong2(y[2 * u], y[2 * u + 1]);
+          if (bias_at >= 0 && bias_at < 8)
+            *reinterpret_cast<uint64_t*>(out + lane * 128 +
+                                         (((cp * 4 + (bias_at >> 1)) ^ (lane & 7)) << 4) +
+                                         (bias_at & 1) * 8) += bias;
+        } else {
+          uint64_t* stage = reinterpret_cast<uint64_t*>(out);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) stage[lane * 8 + (u ^ (lane & 7))] = y[u];
+          if (bias_at >= 0 && bias_at < 8) stage[lane * 8 + (bias_at ^ (lane & 7))] += bias;
+          __syncwarp();
+          // 4 rows per instruction, 8 lanes x 8 bytes = one 64-byte row segment each
+          const int wd = lane & 7;
+          const int col = col0 + cp * 8 + wd;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int rr = 4 * i + (lane >> 3);
+            if (row0 + rr < a.M && col < a.L)
+              a.Y[((size_t)n * a.M + row0 + rr) * a.ldy + col] = stage[rr * 8 + (wd ^ (rr & 7))];
+          }
+          __syncwarp();
+        }
+      }
+      if (!SHIFTED) {
+        // tiled stores end on 16-byte boundaries, so the last word of an odd count goes alone
+        if ((a.L & 1) && body >= 0 && body < EW && row0 + lane < a.M)
+          a.Y[((size_t)n * a.M + row0 + lane) * a.ldy + a.L - 1] =
+              *reinterpret_cast<const uint64_t*>(out + lane * 128 +
+                                                 (((body >> 1) ^ (lane & 7)) << 4) +
+                                                 (body & 1) * 8);
+        tc::fence_async_smem();
         __syncwarp();
-        // 4 rows per instruction, 8 lanes x 8 bytes = one 64-byte row segment each
-        const int wd = lane & 7;
-        const int col = nt * RQ_WORDS + eh * EW + cp * 8 + wd;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int rr = 4 * i + (lane >> 3);
-          const int row = mt * RQ_BM + q * 32 + rr;
-          uint64_t v = stage[rr * 8 + (wd ^ (rr & 7))];
-          if (row < a.M && col < a.L) {
-            if (col == a.L - 1 && a.bias)
-              v += (uint64_t)a.bias[(ADAPT ? (size_t)0 : (size_t)w * a.M) + row] * a.delta;
-            a.Y[((size_t)n * a.M + row) * a.ldy + col] = v;
-          }
-        }
-        __syncwarp();
+        if (lane == 0 && row0 < a.M && col0 < (a.L & ~1))
+          tc::tma_store_3d(&tm.Y, col0, row0, n, out_at);
       }
       ++tt;
     }
+    if (!SHIFTED && lane == 0) tc::tma_store_wait();
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == MMA_WARP) {
+  if (warp == S::MMA_WARP) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
@@ -477,29 +573,57 @@ static int rq_place(RqMatrix& m, int8_t*& ws, cudaStream_t st) {
   return PNB_OK;
 }
 
-static int rq_map(CUtensorMap* map, const RqMatrix& m, int box_rows) {
-  return make_tmap_u8_2d(map, m.p, (uint64_t)m.pitch(), (uint64_t)m.rows, (uint64_t)m.pitch(), 128,
-                         (uint32_t)box_rows);
+// A tiled map of `rank` dimensions (strides of all but the first, in bytes).
+static int rq_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank,
+                  const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                  CUtensorMapSwizzle swizzle) {
+  auto fn = tmap_encoder();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is unavailable from the driver");
+    return PNB_ERR_CUDA;
+  }
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return PNB_OK;
+  set_error("cuTensorMapEncodeTiled failed (%d): %llu x %llu, pitch %llu", (int)r,
+            (unsigned long long)dims[0], (unsigned long long)dims[1],
+            (unsigned long long)strides[0]);
+  return PNB_ERR_CUDA;
 }
 
-template <int MODE, bool ADAPT>
-static int rq_launch(int grid, const CUtensorMap (&tm)[4], const RqArgs& a, cudaStream_t st) {
-  using S = RqShape<MODE, ADAPT>;
-  static_assert(S::SMEM <= 227 * 1024, "shared memory of one block");
-  PNB_CUDA(cudaFuncSetAttribute(request_kernel<MODE, ADAPT>,
+// Byte matrix [rows][cols] at a pitch, in boxes of box_cols bytes (one swizzle span) x box_rows.
+static int rq_map_bytes(CUtensorMap* map, const void* p, uint64_t cols, uint64_t rows,
+                        uint64_t pitch, int box_cols, int box_rows) {
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  return rq_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, p, 2, dims, strides, box,
+                box_cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+static int rq_map_weights(CUtensorMap* map, const RqMatrix& m, int box_cols, int box_rows) {
+  return rq_map_bytes(map, m.p, (uint64_t)m.pitch(), (uint64_t)m.rows, (uint64_t)m.pitch(), box_cols,
+                      box_rows);
+}
+
+template <bool SHIFTED, bool ADAPT>
+static int rq_launch(int grid, const RqMaps& tm, const RqArgs& a, cudaStream_t st) {
+  using S = RqShape<SHIFTED, ADAPT>;
+  PNB_CUDA(cudaFuncSetAttribute(request_kernel<SHIFTED, ADAPT>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
-  request_kernel<MODE, ADAPT><<<grid, S::THREADS, S::SMEM, st>>>(tm[0], tm[1], tm[2], tm[3], a);
+  request_kernel<SHIFTED, ADAPT><<<grid, S::THREADS, S::SMEM, st>>>(tm, a);
   PNB_CHECK_LAUNCH("request_kernel");
   return PNB_OK;
 }
 
 template <bool ADAPT>
 static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, int x_groups, cudaStream_t st) {
+  const long long x_rows = (long long)x_groups * a.K;
   // TMA coordinates are 32-bit, and a tile reaches up to a stage past its first row
   constexpr long long MOST = 0x7fffffffLL - RQ_BK;
-  if ((long long)x_groups * a.K > MOST || W.rows > MOST || A.rows > MOST || B.rows > MOST) {
+  if (x_rows > MOST || W.rows > MOST || A.rows > MOST || B.rows > MOST) {
     set_error("%s: %lld ciphertexts or %lld weight rows exceed a 32-bit index",
-              ADAPT ? "adapter_contract" : "expert_contract", (long long)x_groups * a.K,
+              ADAPT ? "adapter_contract" : "expert_contract", x_rows,
               std::max(W.rows, std::max(A.rows, B.rows)));
     return PNB_ERR_INVALID;
   }
@@ -507,32 +631,63 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, int x_groups, cu
   a.n_tiles = (a.L + RQ_WORDS - 1) / RQ_WORDS;
   a.k_blocks = (a.K + RQ_BK - 1) / RQ_BK;
   a.w_rows = std::min(RQ_BM, (a.M + 7) & ~7);
+  const uintptr_t xw = (uintptr_t)a.X / 8;
+  a.off0 = (int)(xw & 1);
+  a.off1 = (int)((xw + (uintptr_t)a.ldx) & 1);
+  const bool shifted = a.off0 || a.off1 || a.ldy % 2 != 0 || ((uintptr_t)a.Y % 16) != 0;
+  RqMaps tm{};
+  int rc = PNB_OK;
+  if (!shifted) {
+    const uint64_t pitch = (uint64_t)a.ldx * 8;
+    rc = rq_map_bytes(&tm.X[0], a.X, pitch, (uint64_t)x_rows, pitch, 128, RQ_BK);
+    if (!rc) rc = rq_map_bytes(&tm.X[1], a.X, pitch, (uint64_t)x_rows, pitch, 128, RQ_KSTEP);
+    // writes end at word L (rounded down to 16 bytes) of row M of each ciphertext row
+    const cuuint64_t dims[3] = {(cuuint64_t)std::max(2, a.L & ~1), (cuuint64_t)a.M, (cuuint64_t)a.rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.ldy * 8, (cuuint64_t)a.M * a.ldy * 8};
+    const cuuint32_t box[3] = {RQ_WORDS / 2, 32, 1};
+    if (!rc)
+      rc = rq_map(&tm.Y, CU_TENSOR_MAP_DATA_TYPE_UINT64, a.Y, 3, dims, strides, box,
+                  CU_TENSOR_MAP_SWIZZLE_128B);
+  } else {
+    // rows p, p + 2, ..: from the 16-byte boundary at or before row p, at twice the pitch.  A row
+    // off by one word has that word's 16 bytes inside its allocation (allocations start aligned).
+    for (int p = 0; p < 2 && !rc; ++p) {
+      // (a single row has no row 1: both maps are its own, and the second meets zero weights)
+      const bool second = p && x_rows > 1;
+      const int off = second ? a.off1 : a.off0;
+      const cuuint64_t dims[2] = {(cuuint64_t)a.ldx + off,
+                                  (cuuint64_t)std::max<long long>(1, (x_rows + 1 - p) / 2)};
+      const cuuint64_t strides[1] = {(cuuint64_t)a.ldx * 16};
+      const cuuint32_t box[2] = {RQ_WORDS + 2, RQ_RAW_ROWS / 2};
+      const uint64_t* first = a.X + (second ? a.ldx : 0) - off;
+      rc = rq_map(&tm.X[p], CU_TENSOR_MAP_DATA_TYPE_UINT64, first, 2, dims, strides, box,
+                  CU_TENSOR_MAP_SWIZZLE_NONE);
+    }
+  }
+  if (rc) return rc;
   size_t need = W.in_place() ? 0 : W.copy_bytes();
   if (ADAPT) need += (A.in_place() ? 0 : A.copy_bytes()) + (B.in_place() ? 0 : B.copy_bytes());
   int8_t* own = nullptr;
   if (need) PNB_CUDA(cudaMallocAsync((void**)&own, need, st));
   int8_t* ws = own;
-  int rc = rq_place(W, ws, st);
+  rc = rq_place(W, ws, st);
   if (ADAPT && !rc) rc = rq_place(A, ws, st);
   if (ADAPT && !rc) rc = rq_place(B, ws, st);
-  const bool aligned = a.ldx % 2 == 0 && ((uintptr_t)a.X % 16) == 0;
-  CUtensorMap tm[4] = {};
-  if (!rc) rc = rq_map(&tm[0], W, a.w_rows);
-  if (!rc && aligned)
-    rc = make_tmap_u8_2d(&tm[1], a.X, (uint64_t)a.ldx * 8, (uint64_t)x_groups * a.K,
-                         (uint64_t)a.ldx * 8, 128, RQ_KBOX);
-  if (ADAPT && !rc) rc = rq_map(&tm[2], A, a.rank16);
-  if (ADAPT && !rc) rc = rq_map(&tm[3], B, RQ_BM);
+  if (!rc) rc = rq_map_weights(&tm.W, W, 128, a.w_rows);
+  if (ADAPT && !rc) rc = rq_map_weights(&tm.A, A, 128, a.rank16);
+  if (ADAPT && !rc) rc = rq_map_weights(&tm.B, B, PNB_MAX_RANK, RQ_BM);
+  int dev = 0, sms = 0;
   if (!rc) {
-    int dev = 0, sms = 148;
-    PNB_CUDA(cudaGetDevice(&dev));
-    PNB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) rc = cuda_status(e, "cudaDeviceGetAttribute");
+  }
+  if (!rc) {
     const int grid = (int)std::min<long long>((long long)a.rows * a.m_tiles * a.n_tiles, sms);
-    rc = aligned ? rq_launch<RQ_TMA, ADAPT>(grid, tm, a, st)
-                 : rq_launch<RQ_COPY8, ADAPT>(grid, tm, a, st);
+    rc = shifted ? rq_launch<true, ADAPT>(grid, tm, a, st) : rq_launch<false, ADAPT>(grid, tm, a, st);
   }
   if (own) {
-    cudaError_t e = cudaFreeAsync(own, st);
+    const cudaError_t e = cudaFreeAsync(own, st);
     if (!rc && e != cudaSuccess) rc = cuda_status(e, "cudaFreeAsync(padded weights)");
   }
   return rc;
