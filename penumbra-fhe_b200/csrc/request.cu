@@ -107,24 +107,51 @@ struct RqArgs {
   int M, K, L, ldx, ldy;
   int shift, rank, rank16;    // adapters
   int off0, off1;             // words by which rows 0, 2, .. / 1, 3, .. start past 16-byte alignment
-  int m_tiles, n_tiles, k_blocks, w_rows;
+  int n_tiles, k_blocks, w_rows;
+  int per_row;                // tiles of one row
+  int step_n, step_r;         // the grid as whole rows and tiles
 };
 
-// Row n's X group (-1: the row is skipped) and its weights (-1: no adapter).
+// A block's tiles (row n, 128 output rows, 32 words; words fastest), one grid apart.  What a row's
+// tables hold is fetched one tile ahead of its use.
 template <bool ADAPT>
-__device__ __forceinline__ void rq_row(const RqArgs& a, int n, int& src, int& w) {
-  w = __ldg(a.which + n);
-  if (w < 0 || w >= a.n_which) w = -1;
-  src = n;
-  if (!ADAPT) {
-    if (w < 0) { src = -1; return; }
-    const int c = __ldg(a.row_choice + n);
-    if (c < 0 || c >= a.choices)
-      src = -1;
-    else if (a.top_k > 0)
-      src = c / a.top_k;
+struct RqWalk {
+  int n, r, which, choice;
+  __device__ __forceinline__ void fetch(const RqArgs& a) {
+    which = choice = -1;
+    if (n < a.rows) {
+      which = __ldg(a.which + n);
+      if (!ADAPT) choice = __ldg(a.row_choice + n);
+    }
   }
-}
+  __device__ __forceinline__ void start(const RqArgs& a) {
+    n = (int)blockIdx.x / a.per_row;
+    r = (int)blockIdx.x - n * a.per_row;
+    fetch(a);
+  }
+  __device__ __forceinline__ RqWalk next(const RqArgs& a) const {
+    RqWalk o;
+    o.n = n + a.step_n;
+    o.r = r + a.step_r;
+    if (o.r >= a.per_row) {
+      o.r -= a.per_row;
+      ++o.n;
+    }
+    o.fetch(a);
+    return o;
+  }
+  __device__ __forceinline__ int mt(const RqArgs& a) const { return r / a.n_tiles; }
+  // the row's expert or adapter, -1 when it has none
+  __device__ __forceinline__ int weights(const RqArgs& a) const {
+    return which >= 0 && which < a.n_which ? which : -1;
+  }
+  // the row's X group, -1 when the row is skipped
+  __device__ __forceinline__ int source(const RqArgs& a) const {
+    if (ADAPT) return n;
+    if (weights(a) < 0 || choice < 0 || choice >= a.choices) return -1;
+    return a.top_k > 0 ? choice / a.top_k : n;
+  }
+};
 
 // Bounded wait that also gives up as soon as another role has flagged an abort.
 __device__ __forceinline__ bool rq_wait(uint32_t bar, uint32_t parity, volatile int* abort_s) {
@@ -214,33 +241,36 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   tc::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(rq_raw + (holder - raw));
 
-  const long long total = (long long)a.rows * a.m_tiles * a.n_tiles;
-  // tile -> (row n, 128 output rows mt, 32 words nt), nt fastest
-  auto decode = [&](long long t, int& n, int& mt, int& nt) {
-    const int per = a.m_tiles * a.n_tiles;
-    n = (int)(t / per);
-    const int r = (int)(t - (long long)n * per);
-    mt = r / a.n_tiles;
-    nt = r - mt * a.n_tiles;
-  };
   // K rows of block kb, rounded up to whole MMAs.  The rows past K belong to the next group (or lie
   // past the tensor and read as zeros) and meet zero weights.
   auto k_rows = [&](int kb) {
     return min(RQ_BK, ((a.K - kb * RQ_BK) + RQ_KSTEP - 1) / RQ_KSTEP * RQ_KSTEP);
   };
 
+  // the weights of K block kb into stage s, which takes x_bytes of X by TMA besides
+  auto load_weights = [&](int s, int kb, int mt, int w, uint32_t x_bytes) {
+    const bool has = ADAPT && w >= 0;
+    tc::mbar_expect_tx(full(s), (uint32_t)(a.w_rows + (has ? a.rank16 : 0)) * RQ_BK + x_bytes);
+    tc::tma_load_2d(w_at(s), &tm.W, kb * RQ_BK, (ADAPT ? 0 : w * a.M) + mt * RQ_BM, full(s));
+    if (has) tc::tma_load_2d(a_at(s), &tm.A, kb * RQ_BK, w * a.rank, full(s));
+  };
+  // no load may still be landing when the block exits: the last use of each stage completes when
+  // its loads have landed (bounded; immediate unless a wait ran out)
+  auto drain_stages = [&](int used) {
+    for (int k = used > STAGES ? used - STAGES : 0; k < used; ++k)
+      (void)tc::mbar_wait(full(k % STAGES), (uint32_t)(k / STAGES) & 1u, RQ_WAIT_LIMIT);
+  };
+
   if (warp == 0) {
     // ---------------- loads (one lane) -----------------------------------------------------------
     if (lane == 0) {
-      const uint32_t w_bytes = (uint32_t)(a.w_rows * RQ_BK), a_bytes = (uint32_t)(a.rank16 * RQ_BK);
-      int kbg = 0, rawg = 0, has_n = 0;
-      for (long long t = blockIdx.x; t < total && !*abort_s; t += gridDim.x) {
-        int n, mt, nt, src, w;
-        decode(t, n, mt, nt);
-        rq_row<ADAPT>(a, n, src, w);
+      int kbg = 0, rawg = 0;
+      RqWalk<ADAPT> at, ahead;
+      for (at.start(a); at.n < a.rows && !*abort_s; at = ahead) {
+        ahead = at.next(a);
+        const int src = at.source(a), w = at.weights(a);
         if (src < 0) continue;
-        const bool has = ADAPT && w >= 0;
-        const int w_row = (ADAPT ? 0 : w * a.M) + mt * RQ_BM;
+        const int mt = at.mt(a), nt = at.r - mt * a.n_tiles;
         bool ok = true;
         for (int kb = 0; kb < a.k_blocks && ok; ++kb, ++kbg) {
           const int s = kbg % STAGES;
@@ -260,13 +290,10 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
             }
             if (!ok) break;
           }
-          const uint32_t use = (uint32_t)(kbg / STAGES);
-          if (use > 0 && !rq_wait(empty(s), (use - 1) & 1u, abort_s)) { ok = false; break; }
-          tc::mbar_expect_tx(full(s), w_bytes + (has ? a_bytes : 0u) +
-                                          (SHIFTED ? 0u : (uint32_t)(kr * RQ_BN)));
-          tc::tma_load_2d(w_at(s), &tm.W, kb * RQ_BK, w_row, full(s));
-          if (has) tc::tma_load_2d(a_at(s), &tm.A, kb * RQ_BK, w * a.rank, full(s));
           if (!SHIFTED) {
+            const uint32_t use = (uint32_t)(kbg / STAGES);
+            if (use > 0 && !rq_wait(empty(s), (use - 1) & 1u, abort_s)) { ok = false; break; }
+            load_weights(s, kb, mt, w, (uint32_t)(kr * RQ_BN));
             const CUtensorMap* mx = kr == RQ_BK ? &tm.X[0] : &tm.X[1];
             const int step = kr == RQ_BK ? RQ_BK : RQ_KSTEP;
             for (int r = 0; r < kr; r += step) {
@@ -277,22 +304,13 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           }
         }
         if (!ok) break;
-        if (has) {
-          // after this tile's K blocks: the wait for the previous tile's last MMA is then short
-          if (has_n > 0 && !rq_wait(b_empty, (uint32_t)(has_n - 1) & 1u, abort_s)) break;
-          tc::mbar_expect_tx(b_full, RQ_B_BYTES);
-          tc::tma_load_2d(b_at, &tm.B, 0, w * a.M + mt * RQ_BM, b_full);
-          ++has_n;
-        }
       }
-      // no load may still be landing when the block exits: the last use of each slot completes
-      // when it has landed (bounded; immediate unless a wait ran out)
-      for (int k = kbg > STAGES ? kbg - STAGES : 0; k < kbg; ++k)
-        (void)tc::mbar_wait(full(k % STAGES), (uint32_t)(k / STAGES) & 1u, RQ_WAIT_LIMIT);
-      if (SHIFTED)
+      if (SHIFTED) {
         for (int k = rawg > RAW ? rawg - RAW : 0; k < rawg; ++k)
           (void)tc::mbar_wait(raw_full(k % RAW), (uint32_t)(k / RAW) & 1u, RQ_WAIT_LIMIT);
-      if (has_n > 0) (void)tc::mbar_wait(b_full, (uint32_t)(has_n - 1) & 1u, RQ_WAIT_LIMIT);
+      } else {
+        drain_stages(kbg);
+      }
     }
   } else if (warp < S::MMA_WARP) {
     // ---------------- raw rows -> operand layout (shifted rows only) -----------------------------
@@ -300,16 +318,18 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     constexpr int ROWS = RQ_RAW_ROWS / RQ_COPY_WARPS;  // rows of each slot per warp
     const int box = lane >> 4, ch = (lane & 15) >> 1, half = lane & 1;
     int kbg = 0, rawg = 0;
-    for (long long t = blockIdx.x; t < total && !*abort_s; t += gridDim.x) {
-      int n, mt, nt, src, w;
-      decode(t, n, mt, nt);
-      rq_row<ADAPT>(a, n, src, w);
+    RqWalk<ADAPT> at, ahead;
+    for (at.start(a); at.n < a.rows && !*abort_s; at = ahead) {
+      ahead = at.next(a);
+      const int src = at.source(a), w = at.weights(a);
       if (src < 0) continue;
+      const int mt = at.mt(a), nt = at.r - mt * a.n_tiles;
       bool ok = true;
       for (int kb = 0; kb < a.k_blocks && ok; ++kb, ++kbg) {
         const int s = kbg % STAGES;
         const uint32_t use = (uint32_t)(kbg / STAGES);
         if (use > 0 && !rq_wait(empty(s), (use - 1) & 1u, abort_s)) { ok = false; break; }
+        if (cw == 0 && lane == 0) load_weights(s, kb, mt, w, 0u);
         const int kr = k_rows(kb);
         const int parity = (src * a.K + kb * RQ_BK) & 1;  // of the stage's first row
         for (int r0 = 0; r0 < kr; r0 += RQ_RAW_ROWS, ++rawg) {
@@ -341,18 +361,24 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       }
       if (!ok) break;
     }
+    if (cw == 0 && lane == 0) drain_stages(kbg);
   } else if (warp == S::MMA_WARP) {
     // ---------------- MMA issue (one lane) -------------------------------------------------------
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, RQ_BN, true, false, false, true);
       const uint32_t LOW = tc::idesc_i8(128, a.rank16, false, true, true, false);
-      int kbg = 0, tt = 0, has_n = 0;
-      for (long long t = blockIdx.x; t < total && !*abort_s; t += gridDim.x) {
-        int n, mt, nt, src, w;
-        decode(t, n, mt, nt);
-        rq_row<ADAPT>(a, n, src, w);
-        if (src < 0) continue;
-        const bool has = ADAPT && w >= 0;
+      int kbg = 0, tt = 0, has_n = 0, b_n = 0;
+      auto load_b = [&](const RqWalk<ADAPT>& tile) {
+        tc::mbar_expect_tx(b_full, RQ_B_BYTES);
+        tc::tma_load_2d(b_at, &tm.B, 0, tile.weights(a) * a.M + tile.mt(a) * RQ_BM, b_full);
+        ++b_n;
+      };
+      RqWalk<ADAPT> at, ahead;
+      for (at.start(a); at.n < a.rows && !*abort_s; at = ahead) {
+        ahead = at.next(a);
+        if (at.source(a) < 0) continue;
+        const bool has = ADAPT && at.weights(a) >= 0;
+        if (has && b_n == has_n) load_b(at);
         // experts: two accumulators in turn; adapters: C in columns 0-255, L^T and then D in 256-511
         const int buf = ADAPT ? 0 : tt & 1;
         const int turn = ADAPT ? tt : tt >> 1;
@@ -396,7 +422,13 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         }
         tc::mma_commit(acc_full(buf));
         ++tt;
+        if (ADAPT && ahead.n < a.rows && ahead.weights(a) >= 0) {
+          // B of the next tile, once this one's has been read; the epilogue hides it
+          if (has && !rq_wait(b_empty, (uint32_t)(has_n - 1) & 1u, abort_s)) break;
+          load_b(ahead);
+        }
       }
+      if (b_n > 0) (void)tc::mbar_wait(b_full, (uint32_t)(b_n - 1) & 1u, RQ_WAIT_LIMIT);
     }
   } else {
     // ---------------- epilogue -------------------------------------------------------------------
@@ -410,11 +442,12 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     unsigned char* out = rq_raw + (out_at - raw);
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
     int tt = 0, has_n = 0;
-    for (long long t = blockIdx.x; t < total && !*abort_s; t += gridDim.x) {
-      int n, mt, nt, src, w;
-      decode(t, n, mt, nt);
-      rq_row<ADAPT>(a, n, src, w);
+    RqWalk<ADAPT> at, ahead;
+    for (at.start(a); at.n < a.rows && !*abort_s; at = ahead) {
+      ahead = at.next(a);
+      const int src = at.source(a), w = at.weights(a);
       if (src < 0) continue;
+      const int mt = at.mt(a), nt = at.r - mt * a.n_tiles;
       const bool has = ADAPT && w >= 0;
       if (has) {
         // t = A X: lane l of quarter q holds limb l % 8 of word eh*16 + q*4 + l/8 for every rank
@@ -425,7 +458,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         for (int r0 = 0; r0 < a.rank16; r0 += 16) {
           uint32_t c[16];
           tc::tmem_ld_32x32_x16(tmem + 256u + eh * PNB_MAX_RANK + lanes + r0, c);
-          tc::tmem_ld_wait();
+          tc::tmem_ld_wait_for(c);
           uint64_t v[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) v[j] = (uint64_t)(int64_t)(int32_t)c[j] << (8 * (lane & 7));
@@ -454,81 +487,105 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       }
       const int buf = ADAPT ? 0 : tt & 1;
       const int turn = ADAPT ? tt : tt >> 1;
-      if (!rq_wait(acc_full(buf), (uint32_t)turn & 1u, abort_s)) break;
-      tc::tc_fence_after();
-      if (!SHIFTED) {  // the staging rows of the previous tile have left
-        if (lane == 0) tc::tma_store_wait_read();
-        __syncwarp();
-      }
       const uint32_t c_tmem = tmem + (uint32_t)(buf * 256) + lanes + (uint32_t)(eh * EW * 8);
       const int row0 = mt * RQ_BM + q * 32, col0 = nt * RQ_WORDS + eh * EW;
+      // C is complete with the low product; only D is still to come
+      if (!has && !rq_wait(acc_full(buf), (uint32_t)turn & 1u, abort_s)) break;
+      tc::tc_fence_after();
+      if (row0 >= a.M || col0 >= a.L) {  // nothing of this warp's share is kept
+        if (has && !rq_wait(acc_full(buf), (uint32_t)turn & 1u, abort_s)) break;
+        tc::tc_fence_before();
+        tc::mbar_arrive(acc_empty(buf));
+        ++tt;
+        continue;
+      }
       // the word of this half that is the body, and its bias
       const int body = a.L - 1 - col0;
       uint64_t bias = 0;
-      if (a.bias && body >= 0 && body < EW && row0 + lane < a.M)
+      if (a.bias && body < EW && row0 + lane < a.M)
         bias = (uint64_t)__ldg(a.bias + (ADAPT ? (size_t)0 : (size_t)w * a.M) + row0 + lane) *
                a.delta;
-#pragma unroll 1
-      for (int cp = 0; cp < EW / 8; ++cp) {
-        uint64_t y[8];
-        const int bias_at = body - cp * 8;  // which of these 8 words is the body
+      // 4 words (32 columns) at a time, the next columns on their way while these are added up
+      constexpr int CHUNKS = EW / 4;
+      uint32_t c[2][32], d[32];
+      bool ok = true;
+      tc::tmem_ld_32x32_nowait(c_tmem, c[0]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t c[32], d[32];
-          tc::tmem_ld_32x32_nowait(c_tmem + (uint32_t)(cp * 64 + h * 32), c);
-          if (has) tc::tmem_ld_32x32_nowait(c_tmem + (uint32_t)(256 + cp * 64 + h * 32), d);
-          tc::tmem_ld_wait();
-          if (h == 1 && cp == EW / 8 - 1) {
-            tc::tc_fence_before();
-            tc::mbar_arrive(acc_empty(buf));
+      for (int i = 0; i < CHUNKS; ++i) {
+        uint32_t(&ci)[32] = c[i & 1];
+        tc::tmem_ld_wait_for(ci);
+        if (has) {
+          if (i == 0) {
+            ok = rq_wait(acc_full(buf), (uint32_t)turn & 1u, abort_s);
+            tc::tc_fence_after();
           }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint64_t v = add_limbs(0, c + 8 * u);
-            if (ADAPT) v <<= a.shift;
-            if (has) v = add_limbs(v, d + 8 * u);
-            y[h * 4 + u] = v;
-          }
+          tc::tmem_ld_32x32_nowait(c_tmem + (uint32_t)(256 + i * 32), d);
+        } else if (i + 1 < CHUNKS) {
+          tc::tmem_ld_32x32_nowait(c_tmem + (uint32_t)((i + 1) * 32), c[(i + 1) & 1]);
         }
-        if (!SHIFTED) {
+        uint64_t y[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            *reinterpret_cast<ulonglong2*>(out + lane * 128 +
-                                           (((cp * 4 + u) ^ (lane & 7)) << 4)) =
-                make_ulonglong2(y[2 * u], y[2 * u + 1]);
-          if (bias_at >= 0 && bias_at < 8)
-            *reinterpret_cast<uint64_t*>(out + lane * 128 +
-                                         (((cp * 4 + (bias_at >> 1)) ^ (lane & 7)) << 4) +
-                                         (bias_at & 1) * 8) += bias;
-        } else {
-          uint64_t* stage = reinterpret_cast<uint64_t*>(out);
+        for (int u = 0; u < 4; ++u) {
+          y[u] = add_limbs(0, ci + 8 * u);
+          if (ADAPT) y[u] <<= a.shift;
+        }
+        if (has) {
+          tc::tmem_ld_wait_for(d);
+          if (i + 1 < CHUNKS)
+            tc::tmem_ld_32x32_nowait(c_tmem + (uint32_t)((i + 1) * 32), c[(i + 1) & 1]);
+        }
+        if (i + 1 == CHUNKS) {
+          tc::tc_fence_before();
+          tc::mbar_arrive(acc_empty(buf));
+        }
+        if (has) {
 #pragma unroll
-          for (int u = 0; u < 8; ++u) stage[lane * 8 + (u ^ (lane & 7))] = y[u];
-          if (bias_at >= 0 && bias_at < 8) stage[lane * 8 + (bias_at ^ (lane & 7))] += bias;
+          for (int u = 0; u < 4; ++u) y[u] = add_limbs(y[u], d + 8 * u);
+        }
+        if (!SHIFTED && i == 0) {  // the staging rows of the previous tile have left
+          if (lane == 0) tc::tma_store_wait_read();
+          __syncwarp();
+        }
+        // lane's row, its 16-byte chunks XORed by the lane
+        constexpr int PITCH = S::OUT / 32, SPAN = PITCH / 32;  // SPAN chunks of 4 words per row
+        const int ch = (i % SPAN) * 2;
+        const int x = SHIFTED ? (lane >> 1) & 3 : lane & 7;
+        *reinterpret_cast<ulonglong2*>(out + lane * PITCH + ((ch ^ x) << 4)) =
+            make_ulonglong2(y[0], y[1]);
+        *reinterpret_cast<ulonglong2*>(out + lane * PITCH + (((ch + 1) ^ x) << 4)) =
+            make_ulonglong2(y[2], y[3]);
+        const int at_word = body - (i - i % SPAN) * 4;  // the body within the staged words
+        if (body >= i * 4 && body < i * 4 + 4)
+          *reinterpret_cast<uint64_t*>(out + lane * PITCH + (((at_word >> 1) ^ x) << 4) +
+                                       (at_word & 1) * 8) += bias;
+        if (SHIFTED && i % SPAN == SPAN - 1) {
           __syncwarp();
           // 4 rows per instruction, 8 lanes x 8 bytes = one 64-byte row segment each
           const int wd = lane & 7;
-          const int col = col0 + cp * 8 + wd;
+          const int col = col0 + (i - i % SPAN) * 4 + wd;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int rr = 4 * i + (lane >> 3);
+          for (int j = 0; j < 8; ++j) {
+            const int rr = 4 * j + (lane >> 3);
             if (row0 + rr < a.M && col < a.L)
-              a.Y[((size_t)n * a.M + row0 + rr) * a.ldy + col] = stage[rr * 8 + (wd ^ (rr & 7))];
+              a.Y[((size_t)at.n * a.M + row0 + rr) * a.ldy + col] =
+                  *reinterpret_cast<const uint64_t*>(
+                      out + rr * PITCH + (((wd >> 1) ^ ((rr >> 1) & 3)) << 4) + (wd & 1) * 8);
           }
           __syncwarp();
         }
       }
+      if (!ok) break;
       if (!SHIFTED) {
         // tiled stores end on 16-byte boundaries, so the last word of an odd count goes alone
-        if ((a.L & 1) && body >= 0 && body < EW && row0 + lane < a.M)
-          a.Y[((size_t)n * a.M + row0 + lane) * a.ldy + a.L - 1] =
+        if ((a.L & 1) && body < EW && row0 + lane < a.M)
+          a.Y[((size_t)at.n * a.M + row0 + lane) * a.ldy + a.L - 1] =
               *reinterpret_cast<const uint64_t*>(out + lane * 128 +
                                                  (((body >> 1) ^ (lane & 7)) << 4) +
                                                  (body & 1) * 8);
         tc::fence_async_smem();
         __syncwarp();
-        if (lane == 0 && row0 < a.M && col0 < (a.L & ~1))
-          tc::tma_store_3d(&tm.Y, col0, row0, n, out_at);
+        if (lane == 0 && col0 < (a.L & ~1))
+          tc::tma_store_3d(&tm.Y, col0, row0, at.n, out_at);
       }
       ++tt;
     }
@@ -627,8 +684,14 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, int x_groups, cu
               std::max(W.rows, std::max(A.rows, B.rows)));
     return PNB_ERR_INVALID;
   }
-  a.m_tiles = (a.M + RQ_BM - 1) / RQ_BM;
   a.n_tiles = (a.L + RQ_WORDS - 1) / RQ_WORDS;
+  const long long per_row = (long long)((a.M + RQ_BM - 1) / RQ_BM) * a.n_tiles;
+  if (per_row > 1 << 30 || a.rows > 1 << 30) {
+    set_error("%s: %d rows of %lld tiles exceed one launch",
+              ADAPT ? "adapter_contract" : "expert_contract", a.rows, per_row);
+    return PNB_ERR_INVALID;
+  }
+  a.per_row = (int)per_row;
   a.k_blocks = (a.K + RQ_BK - 1) / RQ_BK;
   a.w_rows = std::min(RQ_BM, (a.M + 7) & ~7);
   const uintptr_t xw = (uintptr_t)a.X / 8;
@@ -683,7 +746,9 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, int x_groups, cu
     if (e != cudaSuccess) rc = cuda_status(e, "cudaDeviceGetAttribute");
   }
   if (!rc) {
-    const int grid = (int)std::min<long long>((long long)a.rows * a.m_tiles * a.n_tiles, sms);
+    const int grid = (int)std::min<long long>(a.rows * per_row, sms);
+    a.step_n = grid / a.per_row;
+    a.step_r = grid % a.per_row;
     rc = shifted ? rq_launch<true, ADAPT>(grid, tm, a, st) : rq_launch<false, ADAPT>(grid, tm, a, st);
   }
   if (own) {
