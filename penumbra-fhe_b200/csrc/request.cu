@@ -67,7 +67,7 @@ constexpr int RQ_COPY_WARPS = 4;
 constexpr int RQ_RAW_ROWS = 32;                        // rows per raw slot, half of each parity
 constexpr int RQ_B_SLOTS = 2;
 constexpr int RQ_MAX_W = 13, RQ_MAX_X = 13, RQ_MAX_RAW = 16;  // most slots of each ring
-constexpr int RQ_BARS = 2 * (RQ_MAX_W + RQ_MAX_X + RQ_MAX_RAW + RQ_B_SLOTS) + 6;
+constexpr int RQ_BARS = 2 * (RQ_MAX_W + RQ_MAX_X + RQ_MAX_RAW + RQ_B_SLOTS) + 7;
 constexpr int RQ_BAR_BYTES = (8 * RQ_BARS + 16 + 127) / 128 * 128;
 constexpr int RQ_SMEM = 227 * 1024;                    // of one block
 constexpr uint32_t RQ_WAIT_LIMIT = 1u << 24;
@@ -85,7 +85,8 @@ struct RqShape {
   static constexpr int OUT = 32 * EW * 8;              // its staging: 32 rows
   static constexpr int COPY = SHIFTED ? RQ_COPY_WARPS : 0;
   static constexpr int MMA_WARP = 2 + COPY;            // warp 0 loads X, warp 1 the weights
-  static constexpr int THREADS = 32 * (3 + COPY + RQ_EPI_WARPS);
+  static constexpr int EPI_WARP = MMA_WARP + (ADAPT ? 2 : 1);  // the low product has its own warp
+  static constexpr int THREADS = 32 * (EPI_WARP + RQ_EPI_WARPS);
 };
 
 struct RqMaps {
@@ -177,8 +178,11 @@ struct RqRing {
   }
 };
 
-// Bounded wait that also gives up as soon as another role has flagged an abort.
+// Bounded wait that also gives up as soon as another role has flagged an abort.  A completed phase
+// is found by the plain test: a third of a suspending wait's time (51 against 165 cycles), which
+// the thread that issues the MMAs pays at every slot.
 __device__ __forceinline__ bool rq_wait(uint32_t bar, uint32_t parity, volatile int* abort_s) {
+  if (tc::mbar_test(bar, parity & 1u)) return true;
   for (uint32_t it = 0; it < RQ_WAIT_LIMIT; it += 1024) {
     if (tc::mbar_wait(bar, parity & 1u, 1024)) return true;
     if (*abort_s) return false;
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   const uint32_t r_full = bars + 8 * R0, r_empty = r_full + 8 * RQ_MAX_RAW;
   const uint32_t b_full = bars + 8 * B0, b_empty = b_full + 8 * RQ_B_SLOTS;
   const uint32_t acc_full = bars + 8 * C0, acc_empty = acc_full + 16;
-  const uint32_t low_full = acc_full + 32, t_full = acc_full + 40;
+  const uint32_t low_full = acc_full + 32, t_full = acc_full + 48;
   const uint32_t holder = bars + 8 * RQ_BARS;
   volatile int* abort_s = reinterpret_cast<volatile int*>(rq_raw + (holder + 8 - raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     }
     for (int s = 0; s < a.x_slots; ++s) {
       tc::mbar_init(x_full + 8 * s, SHIFTED ? RQ_COPY_WARPS + (ADAPT ? 1 : 0) : 1);
-      tc::mbar_init(x_empty + 8 * s, 1);
+      tc::mbar_init(x_empty + 8 * s, ADAPT ? 2 : 1);
     }
     for (int s = 0; s < a.raw_slots; ++s) {
       tc::mbar_init(r_full + 8 * s, 1);
@@ -258,11 +262,11 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(b_full + 8 * s, 1);
       tc::mbar_init(b_empty + 8 * s, 1);
-      tc::mbar_init(acc_full + 8 * s, 1);
-      tc::mbar_init(acc_empty + 8 * s, 32 * RQ_EPI_WARPS);
+      tc::mbar_init(acc_full + 8 * s, ADAPT ? 2 : 1);
+      tc::mbar_init(acc_empty + 8 * s, RQ_EPI_WARPS);
+      tc::mbar_init(low_full + 8 * s, 1);
     }
-    tc::mbar_init(low_full, 1);
-    tc::mbar_init(t_full, 32 * RQ_EPI_WARPS);
+    tc::mbar_init(t_full, RQ_EPI_WARPS);
     *abort_s = 0;
     tc::fence_mbar_init();
     tc::prefetch_tmap(&tm.W);
@@ -280,6 +284,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   tc::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(rq_raw + (holder - raw));
 
+  constexpr uint32_t D_AT = 256;               // adapters: TMEM columns of L^T and D
   const int kb_n = (a.K + RQ_WK - 1) / RQ_WK;  // weight slots of one tile
   const int kx_n = (a.K + S::XK - 1) / S::XK;  // X slots of one tile
   // rows of X slot kx, rounded up to whole MMAs.  Those past K belong to the next group (or lie past
@@ -436,14 +441,18 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     }
     if (ADAPT && cw == 0 && lane == 0) rq_drain(x_full, xr, x_wrap, a.x_slots);
   } else if (warp == S::MMA_WARP) {
-    // ---------------- MMA issue (one lane) -------------------------------------------------------
+    // ---------------- main products and D (one lane) --------------------------------------------
+    // Issuing one MMA takes a thread about as long as the tensor cores take to run it, so this loop
+    // is kept short and the low products have a thread of their own.
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, S::BN, true, false, false, true);
-      const uint32_t LOW = tc::idesc_i8(128, a.rank16, false, true, true, false);
       // accumulators in turn: experts C in 256 columns each; adapters C in 128 columns each, then L^T
       // and after it D in another 128 each
-      constexpr uint32_t C_COLS = S::BN, D_AT = 256;
-      RqRing xr, br;
+      constexpr uint32_t C_COLS = S::BN;
+      const uint64_t wd = tc::smem_desc_sw128(w_at(0), 16u, 1024u);
+      const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
+      const uint32_t w_hi = (uint32_t)(wd >> 32), x_hi = (uint32_t)(xd >> 32);
+      RqRing x, br;
       int tt = 0, low_n = 0, w_slot = 0;
       uint32_t w_par = 0;
       bool first = true;
@@ -473,9 +482,6 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         low_n += pend_first;
         pending = false;
       };
-      const uint64_t w_desc = tc::smem_desc_sw128(w_at(0), 16u, 1024u);
-      const uint64_t x_desc = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
-      const uint64_t a_desc = tc::smem_desc_sw128(a_at(0), 16u, 1024u);
       RqWalk<ADAPT> at, ahead, beyond, held;
       at.start(a);
       ahead = at.next(a);
@@ -492,25 +498,28 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         // weights are let go with their last use when the next group is known to need others
         const bool drop = !a.keep_w || (ahead.used(a) && !ahead.same_w(at));
         unreleased = drop ? 0 : m_n * kb_n;
-        for (int m = 0; m < m_n && ok; ++m) {
+        const RqRing x0 = x;
+        int keep_slot = 0;
+        for (int m = 0; m < m_n; ++m) {
           const int buf = tt & 1;
           const uint32_t c_tmem = tmem + (uint32_t)buf * C_COLS;
-          const uint32_t l_tmem = tmem + D_AT + (uint32_t)(buf * 128);
           ok = rq_wait(acc_empty + 8 * buf, (uint32_t)(tt >> 1) ^ 1u, abort_s);
           if (!ok) break;
-          RqRing x = xr;
-          const bool low = has && m == 0;
-          int left = (a.K + RQ_KSTEP - 1) / RQ_KSTEP;  // MMAs of K still to come
+          tc::tc_fence_after();  // (operands in shared memory need none: their mbarriers order them)
+          x = x0;
+          const bool last = m == m_n - 1;
+          int left = (a.K + RQ_KSTEP - 1) / RQ_KSTEP;  // MMAs still to come
           uint32_t acc = 0;
-          for (int kb = 0; kb < kb_n; ++kb) {
-            const int ws = a.keep_w ? m * kb_n + kb : w_slot;
+          while (left > 0) {  // 128 of K: one weight slot
+            const int ws = a.keep_w ? keep_slot++ : w_slot;
             if (load) {
               ok = rq_wait(w_full + 8 * ws, w_par >> ws, abort_s);
               if (!ok) break;
               w_par ^= 1u << ws;
               if (++w_slot == a.w_slots) w_slot = 0;
             }
-            const uint64_t wd = w_desc + (uint64_t)(ws * (RQ_W_SLOT / 16));
+            uint32_t w_lo = (uint32_t)wd + (uint32_t)(ws * (RQ_W_SLOT / 16));
+            constexpr int STEPS = S::XK / RQ_KSTEP;
 #pragma unroll
             for (int h = 0; h < RQ_WK / S::XK; ++h) {
               if (left <= 0) break;
@@ -518,35 +527,30 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
                 ok = rq_wait(x_full + 8 * x.slot, x.phase, abort_s);
                 if (!ok) break;
               }
-              tc::tc_fence_after();
-              const uint64_t xd = x_desc + (uint64_t)(x.slot * (S::X_SLOT / 16));
-              constexpr int STEPS = S::XK / RQ_KSTEP;
-#pragma unroll
-              for (int k = 0; k < STEPS; ++k)
-                if (k < left)
-                  tc::mma_i8(c_tmem, wd + (uint64_t)(2 * (h * STEPS + k)), xd + (uint64_t)(256 * k),
-                             MAIN, k > 0 ? 1u : acc);
-              if (low) {
-                const uint64_t ad = a_desc + (uint64_t)(x.slot * (a_slot / 16));
+              uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
+              if (left >= STEPS) {
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k)
-                  if (k < left)
-                    tc::mma_i8(l_tmem, xd + (uint64_t)(256 * k), ad + (uint64_t)(2 * k), LOW,
-                               k > 0 ? 1u : acc);
+                  tc::mma_i8_lo(c_tmem, w_lo + 2 * k, w_hi, x_lo + 256 * k, x_hi, MAIN,
+                                k > 0 ? 1u : acc);
+              } else {
+                for (int k = 0; k < left; ++k)
+                  tc::mma_i8_lo(c_tmem, w_lo + 2 * k, w_hi, x_lo + 256 * k, x_hi, MAIN,
+                                k > 0 ? 1u : acc);
               }
+              if (last) tc::mma_commit(x_empty + 8 * x.slot);
+              x.advance(a.x_slots);
               acc = 1;
               left -= STEPS;
-              if (m == m_n - 1) tc::mma_commit(x_empty + 8 * x.slot);
-              x.advance(a.x_slots);
+              w_lo += 2 * STEPS;
             }
             if (!ok) break;
             if (drop) tc::mma_commit(w_empty + 8 * ws);
-            if (pending) finish(false);
+            if (ADAPT && pending) finish(false);
           }
-          if (pending && ok) finish(true);
+          if (ADAPT && pending && ok) finish(true);
           if (!ok) break;
           if (has) {
-            if (m == 0) tc::mma_commit(low_full);
             pending = true;
             pend_first = m == 0;
             pend_buf = buf;
@@ -555,24 +559,74 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
             tc::mma_commit(acc_full + 8 * buf);
           }
           ++tt;
-          if (m == m_n - 1) xr = x;
         }
       }
-      if (pending && ok) finish(true);
+      if (ADAPT && pending && ok) finish(true);
+    }
+  } else if (ADAPT && warp == S::MMA_WARP + 1) {
+    // ---------------- low products L^T = X^T A^T (one lane) -------------------------------------
+    if (lane == 0) {
+      const uint32_t LOW = tc::idesc_i8(128, a.rank16, false, true, true, false);
+      const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
+      const uint64_t ad = tc::smem_desc_sw128(a_at(0), 16u, 1024u);
+      const uint32_t x_hi = (uint32_t)(xd >> 32), a_hi = (uint32_t)(ad >> 32);
+      RqRing x;
+      int tt = 0;
+      bool ok = true;
+      RqWalk<ADAPT> at, ahead;
+      for (at.start(a); at.n < a.rows && ok && !*abort_s; at = ahead) {
+        ahead = at.next(a);
+        const bool has = at.weights(a) >= 0;
+        const int buf = tt & 1;
+        const uint32_t l_tmem = tmem + D_AT + (uint32_t)(buf * 128);
+        // The columns are those of this buffer's last D.  Every tile's turn is waited for and answered,
+        // also where nothing is issued: a parity tells only neighbouring turns apart, so neither this
+        // thread nor the other roles may get two turns ahead.
+        auto turn = [&] {
+          ok = rq_wait(acc_empty + 8 * (tt & 1), (uint32_t)(tt >> 1) ^ 1u, abort_s);
+          if (ok) tc::mbar_arrive(acc_full + 8 * (tt & 1));
+          ++tt;
+        };
+        turn();
+        if (!ok) break;
+        tc::tc_fence_after();
+        uint32_t acc = 0;
+        for (int left = (a.K + RQ_KSTEP - 1) / RQ_KSTEP; left > 0; left -= S::XK / RQ_KSTEP) {
+          ok = rq_wait(x_full + 8 * x.slot, x.phase, abort_s);
+          if (!ok) break;
+          if (has) {
+            const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
+            const uint32_t a_lo = (uint32_t)ad + (uint32_t)(x.slot * (a_slot / 16));
+#pragma unroll
+            for (int k = 0; k < S::XK / RQ_KSTEP; ++k)
+              if (k < left)
+                tc::mma_i8_lo(l_tmem, x_lo + 256 * k, x_hi, a_lo + 2 * k, a_hi, LOW,
+                              k > 0 ? 1u : acc);
+            acc = 1;
+            tc::mma_commit(x_empty + 8 * x.slot);
+          } else {
+            tc::mbar_arrive(x_empty + 8 * x.slot);
+          }
+          x.advance(a.x_slots);
+        }
+        if (has && ok) tc::mma_commit(low_full + 8 * buf);
+        for (int m = tiles(at.mg); m > 1 && ok; --m) turn();
+      }
     }
   } else {
     // ---------------- epilogue -------------------------------------------------------------------
     // Warp w reads TMEM lane quarter w % 4 (32 output rows, one per lane) and half eh of the tile's
     // words.  Limb sums become u64 words, staged in shared memory with their 16-byte chunks XORed by
     // the row, and leave as 32 rows x EW words by TMA, or as row segments by plain stores.
-    const int e_w = warp - S::MMA_WARP - 1;
+    const int e_w = warp - S::EPI_WARP;
     const int q = warp & 3, eh = e_w >> 2;
     constexpr int EW = S::EW, PITCH = EW * 8, CHUNKS = EW / 4;
     const uint32_t out_at = base + (uint32_t)(a.out_at + e_w * S::OUT);
     unsigned char* out = rq_raw + (out_at - raw);
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
     auto xored = [](int row) { return PITCH == 128 ? row & 7 : (row >> 1) & 3; };
-    int tt = 0, low_n = 0;
+    int tt = 0;
+    uint32_t low_par = 0;  // a bit per accumulator
     bool ok = true;
     RqWalk<ADAPT> at, ahead;
     for (at.start(a); at.n < a.rows && ok && !*abort_s; at = ahead) {
@@ -583,12 +637,12 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       const int m_n = tiles(mg);
       for (int m = 0; m < m_n; ++m, ++tt) {
         const int buf = tt & 1;
-        const uint32_t d_tmem = tmem + 256u + (uint32_t)(buf * 128) + lanes;
+        const uint32_t d_tmem = tmem + D_AT + (uint32_t)(buf * 128) + lanes;
         const bool low = has && m == 0;
         if (low) {
           // t = A X: lane l of quarter q holds limb l % 8 of word 4q + l/8 for every rank row.  Eight
           // lanes add up 16 rows at a time, halving the rows they keep at each step.
-          ok = rq_wait(low_full, (uint32_t)low_n, abort_s);
+          ok = rq_wait(low_full + 8 * buf, low_par >> buf, abort_s);
           if (!ok) break;
           tc::tc_fence_after();
           const int word = q * 4 + (lane >> 3);
@@ -619,22 +673,20 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           }
           tc::fence_async_smem();
           tc::tc_fence_before();
-          tc::mbar_arrive(t_full);
-          ++low_n;
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(t_full);
+          low_par ^= 1u << buf;
         }
         const uint32_t c_tmem = tmem + (uint32_t)(buf * S::BN) + lanes + (uint32_t)(eh * EW * 8);
         const int row0 = (mg * a.m_group + m) * RQ_BM + q * 32, col0 = nt * S::WORDS + eh * EW;
-        // with the low product C is complete, too; only D is still to come
-        if (!low) ok = rq_wait(acc_full + 8 * buf, (uint32_t)(tt >> 1), abort_s);
+        ok = rq_wait(acc_full + 8 * buf, (uint32_t)(tt >> 1), abort_s);
+        if (!ok) break;
         tc::tc_fence_after();
         if (row0 >= a.M || col0 >= a.L) {  // nothing of this warp's share is kept
-          if (low) ok = rq_wait(acc_full + 8 * buf, (uint32_t)(tt >> 1), abort_s);
-          if (!ok) break;
           tc::tc_fence_before();
-          tc::mbar_arrive(acc_empty + 8 * buf);
+          if (lane == 0) tc::mbar_arrive(acc_empty + 8 * buf);
           continue;
         }
-        if (!ok) break;
         // the word of this half that is the body, and its bias
         const int body = a.L - 1 - col0;
         uint64_t bias = 0;
@@ -649,10 +701,6 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           uint32_t(&ci)[32] = c[i & 1];
           tc::tmem_ld_wait_for(ci);
           if (has) {
-            if (i == 0 && low) {
-              ok = rq_wait(acc_full + 8 * buf, (uint32_t)(tt >> 1), abort_s);
-              tc::tc_fence_after();
-            }
             tc::tmem_ld_32x32_nowait(d_tmem + (uint32_t)(eh * EW * 8 + i * 32), d);
           } else if (i + 1 < CHUNKS) {
             tc::tmem_ld_32x32_nowait(c_tmem + (uint32_t)((i + 1) * 32), c[(i + 1) & 1]);
@@ -670,7 +718,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           }
           if (i + 1 == CHUNKS) {
             tc::tc_fence_before();
-            tc::mbar_arrive(acc_empty + 8 * buf);
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(acc_empty + 8 * buf);
           }
           if (has) {
 #pragma unroll
@@ -685,7 +734,6 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           *reinterpret_cast<ulonglong2*>(out + lane * PITCH + (((2 * i + 1) ^ xored(lane)) << 4)) =
               make_ulonglong2(y[2], y[3]);
         }
-        if (!ok) break;
         if (body < EW) {
           uint64_t* p = reinterpret_cast<uint64_t*>(
               out + lane * PITCH + (((body >> 1) ^ xored(lane)) << 4) + (body & 1) * 8);
