@@ -26,8 +26,7 @@
 // C = W X it also accumulates the transposed low product  L^T = X^T A^T  (the X tile as the M = 128
 // operand and A's rows as N: rank/128 of the main product's work, where A as a padded M = 128
 // operand would double it).  The epilogue warps add up the limbs of t = A X mod 2^64 across lanes,
-// write t's bytes to shared memory as the next MN-major operand, and one short MMA, issued between
-// the next tile's, makes D = B t.  y = (C << s) + D.  X is read once; t never leaves the SM.
+// write t's bytes to shared memory as the next MN-major operand, and one short MMA makes D = B t.  y = (C << s) + D.  X is read once; t never leaves the SM.
 //
 // Rows that start 16-byte aligned (an even pitch) move by TMA straight into the operand layout, and
 // results leave by TMA.  Other rows (contiguous [count][kN+1] ciphertexts) are off by one word
@@ -67,7 +66,7 @@ constexpr int RQ_COPY_WARPS = 4;
 constexpr int RQ_RAW_ROWS = 32;                        // rows per raw slot, half of each parity
 constexpr int RQ_B_SLOTS = 2;
 constexpr int RQ_MAX_W = 13, RQ_MAX_X = 13, RQ_MAX_RAW = 16;  // most slots of each ring
-constexpr int RQ_BARS = 2 * (RQ_MAX_W + RQ_MAX_X + RQ_MAX_RAW + RQ_B_SLOTS) + 7;
+constexpr int RQ_BARS = 2 * (RQ_MAX_W + RQ_MAX_X + RQ_MAX_RAW + RQ_B_SLOTS) + 6;
 constexpr int RQ_BAR_BYTES = (8 * RQ_BARS + 16 + 127) / 128 * 128;
 constexpr int RQ_SMEM = 227 * 1024;                    // of one block
 constexpr uint32_t RQ_WAIT_LIMIT = 1u << 24;
@@ -241,7 +240,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   const uint32_t r_full = bars + 8 * R0, r_empty = r_full + 8 * RQ_MAX_RAW;
   const uint32_t b_full = bars + 8 * B0, b_empty = b_full + 8 * RQ_B_SLOTS;
   const uint32_t acc_full = bars + 8 * C0, acc_empty = acc_full + 16;
-  const uint32_t low_full = acc_full + 32, t_full = acc_full + 48;
+  const uint32_t low_full = acc_full + 32, t_full = acc_full + 40;
   const uint32_t holder = bars + 8 * RQ_BARS;
   volatile int* abort_s = reinterpret_cast<volatile int*>(rq_raw + (holder + 8 - raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -264,8 +263,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       tc::mbar_init(b_empty + 8 * s, 1);
       tc::mbar_init(acc_full + 8 * s, ADAPT ? 2 : 1);
       tc::mbar_init(acc_empty + 8 * s, RQ_EPI_WARPS);
-      tc::mbar_init(low_full + 8 * s, 1);
     }
+    tc::mbar_init(low_full, 1);
     tc::mbar_init(t_full, RQ_EPI_WARPS);
     *abort_s = 0;
     tc::fence_mbar_init();
@@ -441,58 +440,29 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     }
     if (ADAPT && cw == 0 && lane == 0) rq_drain(x_full, xr, x_wrap, a.x_slots);
   } else if (warp == S::MMA_WARP) {
-    // ---------------- main products and D (one lane) --------------------------------------------
+    // ---------------- main products (one lane issues) --------------------------------------------
     // Issuing one MMA takes a thread about as long as the tensor cores take to run it, so this loop
-    // is kept short and the low products have a thread of their own.
+    // is kept short, and the low products have a thread of their own.
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, S::BN, true, false, false, true);
-      // accumulators in turn: experts C in 256 columns each; adapters C in 128 columns each, then L^T
-      // and after it D in another 128 each
-      constexpr uint32_t C_COLS = S::BN;
       const uint64_t wd = tc::smem_desc_sw128(w_at(0), 16u, 1024u);
       const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
       const uint32_t w_hi = (uint32_t)(wd >> 32), x_hi = (uint32_t)(xd >> 32);
-      RqRing x, br;
-      int tt = 0, low_n = 0, w_slot = 0;
+      RqRing x;
+      int tt = 0, w_slot = 0;
       uint32_t w_par = 0;
-      bool first = true;
-      int unreleased = 0;    // weight slots kept for a group that has not come
-      bool pending = false;  // the previous tile's D is still to be issued
-      bool pend_first = false;
-      int pend_buf = 0;
-      bool ok = true;
-      auto finish = [&](bool block) {  // D = B t of the pending tile, when t is there
-        if (pend_first) {
-          if (block)
-            ok = ok && rq_wait(t_full, (uint32_t)low_n, abort_s);
-          else if (!tc::mbar_test(t_full, (uint32_t)low_n & 1u))
-            return;
-        }
-        ok = ok && rq_wait(b_full + 8 * br.slot, br.phase, abort_s);
-        if (!ok) return;
-        tc::tc_fence_after();
-        // columns of B past the rank are zero, so t's rows past it do not matter
-        for (int k = 0; k < (a.rank + 31) / 32; ++k)
-          tc::mma_i8(tmem + D_AT + (uint32_t)(pend_buf * 128),
-                     tc::smem_desc_sw64(b_at(br.slot) + 32u * k, 16u, 512u),
-                     tc::smem_desc_sw128(t_at + 4096u * k, 16u, 1024u), MAIN, k != 0 ? 1u : 0u);
-        tc::mma_commit(b_empty + 8 * br.slot);
-        tc::mma_commit(acc_full + 8 * pend_buf);
-        br.advance(RQ_B_SLOTS);
-        low_n += pend_first;
-        pending = false;
-      };
+      bool first = true, ok = true;
+      int unreleased = 0;  // weight slots kept for a group that has not come
       RqWalk<ADAPT> at, ahead, beyond, held;
       at.start(a);
       ahead = at.next(a);
       for (; at.n < a.rows && ok && !*abort_s; at = ahead, ahead = beyond) {
         beyond = ahead.next(a);
         if (!at.used(a)) continue;
-        const bool has = ADAPT && at.weights(a) >= 0;
         const bool load = !a.keep_w || first || !at.same_w(held);
         const int m_n = tiles(at.mg);
         if (load)
-          for (; unreleased > 0; --unreleased) tc::mma_commit(w_empty + 8 * (unreleased - 1));
+          for (int s = 0; s < unreleased; ++s) tc::mma_commit(w_empty + 8 * s);
         held = at;
         first = false;
         // weights are let go with their last use when the next group is known to need others
@@ -500,9 +470,10 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         unreleased = drop ? 0 : m_n * kb_n;
         const RqRing x0 = x;
         int keep_slot = 0;
-        for (int m = 0; m < m_n; ++m) {
+        for (int m = 0; m < m_n; ++m, ++tt) {
+          // accumulators in turn: experts C in 256 columns each; adapters C in 128 columns each
           const int buf = tt & 1;
-          const uint32_t c_tmem = tmem + (uint32_t)buf * C_COLS;
+          const uint32_t c_tmem = tmem + (uint32_t)(buf * S::BN);
           ok = rq_wait(acc_empty + 8 * buf, (uint32_t)(tt >> 1) ^ 1u, abort_s);
           if (!ok) break;
           tc::tc_fence_after();  // (operands in shared memory need none: their mbarriers order them)
@@ -527,7 +498,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
                 ok = rq_wait(x_full + 8 * x.slot, x.phase, abort_s);
                 if (!ok) break;
               }
-              uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
+              const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
               if (left >= STEPS) {
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k)
@@ -546,72 +517,99 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
             }
             if (!ok) break;
             if (drop) tc::mma_commit(w_empty + 8 * ws);
-            if (ADAPT && pending) finish(false);
           }
-          if (ADAPT && pending && ok) finish(true);
           if (!ok) break;
-          if (has) {
-            pending = true;
-            pend_first = m == 0;
-            pend_buf = buf;
-            if (m > 0) finish(true);  // t is there
-          } else {
-            tc::mma_commit(acc_full + 8 * buf);
-          }
-          ++tt;
+          tc::mma_commit(acc_full + 8 * buf);
         }
       }
-      if (ADAPT && pending && ok) finish(true);
     }
   } else if (ADAPT && warp == S::MMA_WARP + 1) {
-    // ---------------- low products L^T = X^T A^T (one lane) -------------------------------------
+    // ---------------- low products L^T = X^T A^T and D = B t (one lane) --------------------------
     if (lane == 0) {
+      constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, S::BN, true, false, false, true);
       const uint32_t LOW = tc::idesc_i8(128, a.rank16, false, true, true, false);
       const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
       const uint64_t ad = tc::smem_desc_sw128(a_at(0), 16u, 1024u);
       const uint32_t x_hi = (uint32_t)(xd >> 32), a_hi = (uint32_t)(ad >> 32);
-      RqRing x;
+      RqRing x, br;
       int tt = 0;
+      uint32_t t_par = 0;
+      int pending = -1;  // the accumulator whose D is still to come
       bool ok = true;
+      auto product = [&](int buf) {  // D = B t
+        ok = rq_wait(b_full + 8 * br.slot, br.phase, abort_s);
+        if (!ok) return;
+        tc::tc_fence_after();
+        // columns of B past the rank are zero, so t's rows past it do not matter
+        for (int k = 0; k < (a.rank + 31) / 32; ++k)
+          tc::mma_i8(tmem + D_AT + (uint32_t)(buf * 128),
+                     tc::smem_desc_sw64(b_at(br.slot) + 32u * k, 16u, 512u),
+                     tc::smem_desc_sw128(t_at + 4096u * k, 16u, 1024u), MAIN, k != 0 ? 1u : 0u);
+        tc::mma_commit(b_empty + 8 * br.slot);
+        tc::mma_commit(acc_full + 8 * buf);
+        br.advance(RQ_B_SLOTS);
+      };
+      auto finish = [&](bool block) {  // the pending D, once t is there
+        if (block)
+          ok = rq_wait(t_full, t_par, abort_s);
+        else if (!tc::mbar_test(t_full, t_par & 1u))
+          return;
+        if (!ok) return;
+        t_par ^= 1u;
+        product(pending);
+        pending = -1;
+      };
       RqWalk<ADAPT> at, ahead;
       for (at.start(a); at.n < a.rows && ok && !*abort_s; at = ahead) {
         ahead = at.next(a);
         const bool has = at.weights(a) >= 0;
-        const int buf = tt & 1;
-        const uint32_t l_tmem = tmem + D_AT + (uint32_t)(buf * 128);
-        // The columns are those of this buffer's last D.  Every tile's turn is waited for and answered,
-        // also where nothing is issued: a parity tells only neighbouring turns apart, so neither this
-        // thread nor the other roles may get two turns ahead.
-        auto turn = [&] {
-          ok = rq_wait(acc_empty + 8 * (tt & 1), (uint32_t)(tt >> 1) ^ 1u, abort_s);
-          if (ok) tc::mbar_arrive(acc_full + 8 * (tt & 1));
-          ++tt;
-        };
-        turn();
-        if (!ok) break;
-        tc::tc_fence_after();
-        uint32_t acc = 0;
-        for (int left = (a.K + RQ_KSTEP - 1) / RQ_KSTEP; left > 0; left -= S::XK / RQ_KSTEP) {
-          ok = rq_wait(x_full + 8 * x.slot, x.phase, abort_s);
+        const int m_n = tiles(at.mg);
+        for (int m = 0; m < m_n && ok; ++m, ++tt) {
+          // Every tile's turn is waited for and answered, also where nothing is issued: a parity
+          // tells only neighbouring turns apart, so no role may get two turns ahead of another.
+          const int buf = tt & 1;
+          ok = rq_wait(acc_empty + 8 * buf, (uint32_t)(tt >> 1) ^ 1u, abort_s);
           if (!ok) break;
-          if (has) {
-            const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
-            const uint32_t a_lo = (uint32_t)ad + (uint32_t)(x.slot * (a_slot / 16));
+          tc::tc_fence_after();
+          if (m == 0) {
+            const uint32_t l_tmem = tmem + D_AT + (uint32_t)(buf * 128);
+            uint32_t acc = 0;
+            for (int left = (a.K + RQ_KSTEP - 1) / RQ_KSTEP; left > 0; left -= S::XK / RQ_KSTEP) {
+              ok = rq_wait(x_full + 8 * x.slot, x.phase, abort_s);
+              if (!ok) break;
+              if (has) {
+                const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
+                const uint32_t a_lo = (uint32_t)ad + (uint32_t)(x.slot * (a_slot / 16));
 #pragma unroll
-            for (int k = 0; k < S::XK / RQ_KSTEP; ++k)
-              if (k < left)
-                tc::mma_i8_lo(l_tmem, x_lo + 256 * k, x_hi, a_lo + 2 * k, a_hi, LOW,
-                              k > 0 ? 1u : acc);
-            acc = 1;
-            tc::mma_commit(x_empty + 8 * x.slot);
-          } else {
-            tc::mbar_arrive(x_empty + 8 * x.slot);
+                for (int k = 0; k < S::XK / RQ_KSTEP; ++k)
+                  if (k < left)
+                    tc::mma_i8_lo(l_tmem, x_lo + 256 * k, x_hi, a_lo + 2 * k, a_hi, LOW,
+                                  k > 0 ? 1u : acc);
+                acc = 1;
+                tc::mma_commit(x_empty + 8 * x.slot);
+              } else {
+                tc::mbar_arrive(x_empty + 8 * x.slot);
+              }
+              x.advance(a.x_slots);
+              if (pending >= 0) finish(false);
+            }
+            if (ok && pending >= 0) finish(true);
+            if (!ok) break;
+            if (has) {
+              tc::mma_commit(low_full);
+              pending = buf;
+            }
+          } else if (pending >= 0) {
+            finish(true);
+            if (!ok) break;
           }
-          x.advance(a.x_slots);
+          if (!has)
+            tc::mbar_arrive(acc_full + 8 * buf);
+          else if (m > 0)
+            product(buf);
         }
-        if (has && ok) tc::mma_commit(low_full + 8 * buf);
-        for (int m = tiles(at.mg); m > 1 && ok; --m) turn();
       }
+      if (ok && pending >= 0) finish(true);
     }
   } else {
     // ---------------- epilogue -------------------------------------------------------------------
@@ -626,7 +624,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
     auto xored = [](int row) { return PITCH == 128 ? row & 7 : (row >> 1) & 3; };
     int tt = 0;
-    uint32_t low_par = 0;  // a bit per accumulator
+    uint32_t low_par = 0;
     bool ok = true;
     RqWalk<ADAPT> at, ahead;
     for (at.start(a); at.n < a.rows && ok && !*abort_s; at = ahead) {
@@ -642,7 +640,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         if (low) {
           // t = A X: lane l of quarter q holds limb l % 8 of word 4q + l/8 for every rank row.  Eight
           // lanes add up 16 rows at a time, halving the rows they keep at each step.
-          ok = rq_wait(low_full + 8 * buf, low_par >> buf, abort_s);
+          ok = rq_wait(low_full, low_par, abort_s);
           if (!ok) break;
           tc::tc_fence_after();
           const int word = q * 4 + (lane >> 3);
@@ -675,7 +673,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           tc::tc_fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(t_full);
-          low_par ^= 1u << buf;
+          low_par ^= 1u;
         }
         const uint32_t c_tmem = tmem + (uint32_t)(buf * S::BN) + lanes + (uint32_t)(eh * EW * 8);
         const int row0 = (mg * a.m_group + m) * RQ_BM + q * 32, col0 = nt * S::WORDS + eh * EW;
