@@ -62,7 +62,7 @@ constexpr int RQ_KSTEP = 32;    // K per MMA; a ragged K costs at most 31 rows
 constexpr int RQ_W_SLOT = RQ_BM * RQ_WK;               // 16 KB
 constexpr int RQ_B_SLOT = RQ_BM * PNB_MAX_RANK;        // 8 KB: B rows of 64 bytes
 constexpr int RQ_EPI_WARPS = 8;                        // two per TMEM lane quarter
-constexpr int RQ_COPY_WARPS = 4;
+constexpr int RQ_COPY_WARPS = 4;                       // each copies every fourth raw slot
 constexpr int RQ_RAW_ROWS = 32;                        // rows per raw slot, half of each parity
 constexpr int RQ_B_SLOTS = 2;
 constexpr int RQ_MAX_W = 13, RQ_MAX_X = 13, RQ_MAX_RAW = 16;  // most slots of each ring
@@ -80,6 +80,7 @@ struct RqShape {
   static constexpr int X_SLOT = XK * BN;               // 16 KB
   static constexpr int RAW_PITCH = BN + 16;            // one word of shift, to 16 bytes
   static constexpr int RAW_SLOT = RQ_RAW_ROWS * RAW_PITCH;
+  static constexpr int RAW_PER_X = XK / RQ_RAW_ROWS;
   static constexpr int EW = WORDS / 2;                 // words per epilogue warp
   static constexpr int OUT = 32 * EW * 8;              // its staging: 32 rows
   static constexpr int COPY = SHIFTED ? RQ_COPY_WARPS : 0;
@@ -251,12 +252,12 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       tc::mbar_init(w_empty + 8 * s, 1);
     }
     for (int s = 0; s < a.x_slots; ++s) {
-      tc::mbar_init(x_full + 8 * s, SHIFTED ? RQ_COPY_WARPS + (ADAPT ? 1 : 0) : 1);
+      tc::mbar_init(x_full + 8 * s, SHIFTED ? S::RAW_PER_X + (ADAPT ? 1 : 0) : 1);
       tc::mbar_init(x_empty + 8 * s, ADAPT ? 2 : 1);
     }
     for (int s = 0; s < a.raw_slots; ++s) {
       tc::mbar_init(r_full + 8 * s, 1);
-      tc::mbar_init(r_empty + 8 * s, RQ_COPY_WARPS);
+      tc::mbar_init(r_empty + 8 * s, 1);
     }
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(b_full + 8 * s, 1);
@@ -385,9 +386,11 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     }
   } else if (warp < S::MMA_WARP) {
     // ---------------- raw rows -> operand layout (shifted rows only) -----------------------------
+    // Raw slot r is always copied by warp r % 4 (their number is a multiple of 4), and every warp
+    // waits for every X slot's turn: a parity tells only neighbouring turns apart.
     const int cw = warp - 2;
-    constexpr int PER = 32 / S::WORDS;                    // rows per pass of a warp
-    constexpr int ROWS = RQ_RAW_ROWS / RQ_COPY_WARPS;     // rows of each slot per warp
+    constexpr int PER = 32 / S::WORDS;  // rows per pass of a warp
+    constexpr int BATCH = 16;           // passes whose words are on their way together
     const int word = lane % S::WORDS, sub = lane / S::WORDS;
     const int box = word >> 4, ch = (word & 15) >> 1, half = word & 1;
     RqRing xr, rr;
@@ -398,42 +401,50 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       if (!at.used(a)) continue;
       const int w = at.weights(a);
       const int parity = at.source(a) * a.K & 1;  // of the group's first row (slots hold an even number)
+      const int off_e = parity ? a.off1 : a.off0, off_o = parity ? a.off0 : a.off1;
       for (int kx = 0; kx < kx_n && ok; ++kx) {
         ok = rq_wait(x_empty + 8 * xr.slot, xr.phase ^ 1u, abort_s);
         if (!ok) break;
+        const uint32_t full = x_full + 8 * xr.slot;
         if (ADAPT && cw == 0 && lane == 0) {  // A's rows beside the slot
-          const uint32_t full = x_full + 8 * xr.slot;
           tc::mbar_expect_tx(full, w >= 0 ? (uint32_t)a_slot : 0u);
           if (w >= 0) tc::tma_load_2d(a_at(xr.slot), &tm.A, kx * S::XK, w * a.rank, full);
         }
-        unsigned char* xs = rq_raw + (x_at(xr.slot) - raw) + box * (S::XK * 128);
-        const int rows = x_rows(kx);
-        for (int r0 = 0; r0 < rows; r0 += RQ_RAW_ROWS) {
-          ok = rq_wait(r_full + 8 * rr.slot, rr.phase, abort_s);
-          if (!ok) break;
-          const unsigned char* from = rq_raw + (raw_at(rr.slot) - raw);
-          uint64_t v[ROWS / PER];
+        const int raws = x_rows(kx) / RQ_RAW_ROWS;
+        for (int i = 0; i < raws; ++i) {
+          if ((rr.slot & 3) == cw) {
+            ok = rq_wait(r_full + 8 * rr.slot, rr.phase, abort_s);
+            if (!ok) break;
+            // row r of the slot: its parity's half, r / 2; one word further where it is shifted
+            const unsigned char* from = rq_raw + (raw_at(rr.slot) - raw) + word * 8;
+            unsigned char* to = rq_raw + (x_at(xr.slot) - raw) + box * (S::XK * 128) +
+                                i * (RQ_RAW_ROWS * 128) + half * 8;
 #pragma unroll
-          for (int i = 0; i < ROWS / PER; ++i) {
-            const int r = cw * ROWS + i * PER + sub;
-            const int off = ((parity + r) & 1) ? a.off1 : a.off0;
-            v[i] = *reinterpret_cast<const uint64_t*>(from + (r & 1) * (S::RAW_SLOT / 2) +
-                                                      (r >> 1) * S::RAW_PITCH + (word + off) * 8);
-          }
+            for (int b = 0; b < RQ_RAW_ROWS / PER; b += BATCH) {
+              uint64_t v[BATCH];
 #pragma unroll
-          for (int i = 0; i < ROWS / PER; ++i) {
-            const int r = r0 + cw * ROWS + i * PER + sub;
-            *reinterpret_cast<uint64_t*>(xs + (r >> 3) * 1024 + (r & 7) * 128 +
-                                         ((ch ^ (r & 7)) << 4) + half * 8) = v[i];
+              for (int j = 0; j < BATCH; ++j) {
+                const int r = (b + j) * PER + sub;
+                v[j] = *reinterpret_cast<const uint64_t*>(
+                    from + (r & 1 ? S::RAW_SLOT / 2 + off_o * 8 : off_e * 8) +
+                    (r >> 1) * S::RAW_PITCH);
+              }
+#pragma unroll
+              for (int j = 0; j < BATCH; ++j) {
+                const int r = (b + j) * PER + sub;
+                *reinterpret_cast<uint64_t*>(to + r * 128 + ((ch ^ (r & 7)) << 4)) = v[j];
+              }
+            }
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tc::mbar_arrive(r_empty + 8 * rr.slot);
+              // the last one answers for those a ragged K leaves out
+              tc::mbar_arrive_n(full, i == raws - 1 ? (uint32_t)(S::RAW_PER_X - i) : 1u);
+            }
           }
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(r_empty + 8 * rr.slot);
           rr.advance(a.raw_slots);
         }
-        if (!ok) break;
-        tc::fence_async_smem();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(x_full + 8 * xr.slot);
         xr.advance(a.x_slots);
         x_wrap |= xr.slot == 0;
       }
@@ -863,7 +874,8 @@ static void rq_plan(RqArgs& a, int sms) {
   room -= a.w_slots * RQ_W_SLOT;
   if (SHIFTED) {
     a.x_slots = a.m_group > 1 ? std::max(3, kx + 1) : x_min;
-    a.raw_slots = std::min(RQ_MAX_RAW, (room - a.x_slots * (S::X_SLOT + a_slot)) / S::RAW_SLOT);
+    a.raw_slots =
+        std::min(RQ_MAX_RAW, (room - a.x_slots * (S::X_SLOT + a_slot)) / S::RAW_SLOT & ~3);
   } else {
     a.x_slots = std::min(RQ_MAX_X, room / (S::X_SLOT + a_slot));
     a.raw_slots = 0;
