@@ -180,16 +180,19 @@ struct RqRing {
 
 // Bounded wait that also gives up as soon as another role has flagged an abort.  A completed phase
 // is found by the plain test: a third of a suspending wait's time (51 against 165 cycles), which
-// the thread that issues the MMAs pays at every slot.
-__device__ __forceinline__ bool rq_wait(uint32_t bar, uint32_t parity, volatile int* abort_s) {
-  if (tc::mbar_test(bar, parity & 1u)) return true;
+// the thread that issues the MMAs pays at every slot.  The rest is out of line: the roles' loops
+// share the instruction cache, and a thread on its own runs at the pace of its fetches.
+__device__ __noinline__ bool rq_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_s) {
   for (uint32_t it = 0; it < RQ_WAIT_LIMIT; it += 1024) {
-    if (tc::mbar_wait(bar, parity & 1u, 1024)) return true;
+    if (tc::mbar_wait(bar, parity, 1024)) return true;
     if (*abort_s) return false;
   }
   *abort_s = 1;
   atomicExch(&g_rq_status, 1);
   return false;
+}
+__device__ __forceinline__ bool rq_wait(uint32_t bar, uint32_t parity, volatile int* abort_s) {
+  return tc::mbar_test(bar, parity & 1u) || rq_wait_slow(bar, parity & 1u, abort_s);
 }
 
 // No load may still be landing when the block exits: the last use of each slot completes when it has
