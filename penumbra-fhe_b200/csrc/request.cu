@@ -454,88 +454,82 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     }
     if (ADAPT && cw == 0 && lane == 0) rq_drain(x_full, xr, x_wrap, a.x_slots);
   } else if (warp == S::MMA_WARP) {
-    // ---------------- main products (one lane issues) --------------------------------------------
-    // Issuing one MMA takes a thread about as long as the tensor cores take to run it, so this loop
-    // is kept short, and the low products have a thread of their own.
+    // ---------------- main products (one lane) --------------------------------------------------
+    // Issuing one MMA takes a thread about as long as the tensor cores take to run it, and every
+    // branch between them counts, so this loop is kept short and the low products have a thread of
+    // their own.
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, S::BN, true, false, false, true);
+      constexpr int STEPS = S::XK / RQ_KSTEP;
       const uint64_t wd = tc::smem_desc_sw128(w_at(0), 16u, 1024u);
       const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
       const uint32_t w_hi = (uint32_t)(wd >> 32), x_hi = (uint32_t)(xd >> 32);
-      RqRing x;
-      int tt = 0, w_slot = 0;
-      uint32_t w_par = 0;
-      bool first = true, ok = true;
-      int unreleased = 0;  // weight slots kept for a group that has not come
-      RqWalk<ADAPT> at, ahead, beyond, held;
-      at.start(a);
-      ahead = at.next(a);
-      for (; at.n < a.rows && ok && !*abort_s; at = ahead, ahead = beyond) {
-        beyond = ahead.next(a);
-        if (!at.used(a)) continue;
-        const bool load = !a.keep_w || first || !at.same_w(held);
-        const int m_n = tiles(at.mg);
-        if (load)
-          for (int s = 0; s < unreleased; ++s) tc::mma_commit(w_empty + 8 * s);
-        held = at;
-        first = false;
-        // weights are let go with their last use when the next group is known to need others
-        const bool drop = !a.keep_w || (ahead.used(a) && !ahead.same_w(at));
-        unreleased = drop ? 0 : m_n * kb_n;
-        const RqRing x0 = x;
-        int keep_slot = 0;
-        for (int m = 0; m < m_n; ++m, ++tt) {
-          // accumulators in turn: experts C in 256 columns each; adapters C in 128 columns each
-          const int buf = tt & 1;
-          const uint32_t c_tmem = tmem + (uint32_t)(buf * S::BN);
-          ok = rq_wait(acc_empty + 8 * buf, (uint32_t)(tt >> 1) ^ 1u, abort_s);
-          if (!ok) break;
-          tc::tc_fence_after();  // (operands in shared memory need none: their mbarriers order them)
-          x = x0;
-          const bool last = m == m_n - 1;
-          int left = (a.K + RQ_KSTEP - 1) / RQ_KSTEP;  // MMAs still to come
-          uint32_t acc = 0;
-          while (left > 0) {  // 128 of K: one weight slot
-            const int ws = a.keep_w ? keep_slot++ : w_slot;
-            if (load) {
-              ok = rq_wait(w_full + 8 * ws, w_par >> ws, abort_s);
-              if (!ok) break;
-              w_par ^= 1u << ws;
+      const int steps = (a.K + RQ_KSTEP - 1) / RQ_KSTEP;  // MMAs of one tile
+      const int x_slots = a.x_slots;
+      const bool keep_w = a.keep_w != 0;
+      [&] {  // returns when a wait gives up
+        RqRing x;
+        int tt = 0, w_slot = 0;
+        uint32_t w_par = 0;
+        int unreleased = 0;  // weight slots kept for a group that has not come
+        RqWalk<ADAPT> at, ahead, beyond;
+        int held_mg = -1, held_w = -1;
+        at.start(a);
+        ahead = at.next(a);
+        for (; at.n < a.rows; at = ahead, ahead = beyond) {
+          beyond = ahead.next(a);
+          if (!at.used(a)) continue;
+          const bool load = !keep_w || at.mg != held_mg || (!ADAPT && at.which != held_w);
+          const int m_n = tiles(at.mg);
+          if (load)
+            for (int s = 0; s < unreleased; ++s) tc::mma_commit(w_empty + 8 * s);
+          held_mg = at.mg;
+          held_w = at.which;
+          // weights are let go with their last use when the next group is known to need others
+          const bool drop = !keep_w || (ahead.used(a) && !ahead.same_w(at));
+          unreleased = drop ? 0 : m_n * kb_n;
+          if (keep_w) w_slot = 0;
+          const RqRing x0 = x;
+          for (int m = 0; m < m_n; ++m, ++tt) {
+            // accumulators in turn: experts C in 256 columns each; adapters C in 128 columns each
+            const uint32_t turn = 8u * (uint32_t)(tt & 1);
+            const uint32_t c_tmem = tmem + (uint32_t)((tt & 1) * S::BN);
+            if (!rq_wait(acc_empty + turn, (uint32_t)(tt >> 1) ^ 1u, abort_s)) return;
+            tc::tc_fence_after();  // (operands in shared memory need none: their mbarriers order them)
+            x = x0;
+            const bool first = m == 0, last = m == m_n - 1;
+            uint32_t acc = 0;
+            for (int left = steps; left > 0;) {  // 128 of K: one weight slot
+              if (load) {
+                if (!rq_wait(w_full + 8 * w_slot, w_par >> w_slot, abort_s)) return;
+                w_par ^= 1u << w_slot;
+              }
+              uint32_t w_lo = (uint32_t)wd + (uint32_t)(w_slot * (RQ_W_SLOT / 16));
+#pragma unroll
+              for (int h = 0; h < RQ_WK / S::XK; ++h, left -= STEPS, w_lo += 2 * STEPS) {
+                if (h > 0 && left <= 0) break;
+                if (first && !rq_wait(x_full + 8 * x.slot, x.phase, abort_s)) return;
+                const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
+                tc::mma_i8_lo(c_tmem, w_lo, w_hi, x_lo, x_hi, MAIN, acc);
+                acc = 1;
+                if (left >= STEPS) {
+#pragma unroll
+                  for (int k = 1; k < STEPS; ++k)
+                    tc::mma_i8_lo(c_tmem, w_lo + 2 * k, w_hi, x_lo + 256 * k, x_hi, MAIN, 1u);
+                } else {
+                  for (int k = 1; k < left; ++k)
+                    tc::mma_i8_lo(c_tmem, w_lo + 2 * k, w_hi, x_lo + 256 * k, x_hi, MAIN, 1u);
+                }
+                if (last) tc::mma_commit(x_empty + 8 * x.slot);
+                x.advance(x_slots);
+              }
+              if (drop) tc::mma_commit(w_empty + 8 * w_slot);
               if (++w_slot == a.w_slots) w_slot = 0;
             }
-            uint32_t w_lo = (uint32_t)wd + (uint32_t)(ws * (RQ_W_SLOT / 16));
-            constexpr int STEPS = S::XK / RQ_KSTEP;
-#pragma unroll
-            for (int h = 0; h < RQ_WK / S::XK; ++h) {
-              if (left <= 0) break;
-              if (m == 0) {
-                ok = rq_wait(x_full + 8 * x.slot, x.phase, abort_s);
-                if (!ok) break;
-              }
-              const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
-              if (left >= STEPS) {
-#pragma unroll
-                for (int k = 0; k < STEPS; ++k)
-                  tc::mma_i8_lo(c_tmem, w_lo + 2 * k, w_hi, x_lo + 256 * k, x_hi, MAIN,
-                                k > 0 ? 1u : acc);
-              } else {
-                for (int k = 0; k < left; ++k)
-                  tc::mma_i8_lo(c_tmem, w_lo + 2 * k, w_hi, x_lo + 256 * k, x_hi, MAIN,
-                                k > 0 ? 1u : acc);
-              }
-              if (last) tc::mma_commit(x_empty + 8 * x.slot);
-              x.advance(a.x_slots);
-              acc = 1;
-              left -= STEPS;
-              w_lo += 2 * STEPS;
-            }
-            if (!ok) break;
-            if (drop) tc::mma_commit(w_empty + 8 * ws);
+            tc::mma_commit(acc_full + turn);
           }
-          if (!ok) break;
-          tc::mma_commit(acc_full + 8 * buf);
         }
-      }
+      }();
     }
   } else if (ADAPT && warp == S::MMA_WARP + 1) {
     // ---------------- low products L^T = X^T A^T and D = B t (one lane) --------------------------
