@@ -252,12 +252,16 @@ int pnb_expert_dispatch(const int32_t* choice_row_dev, int tokens, int top_k,
  * every row through its own expert's int8 matrix.  W [experts][M][K] (K <= 65536), bias int64
  * [experts][M] (may be NULL).  sorted_rows = 0: X [tokens][K][ldx], src = the row's token
  * (row_choice[r] / top_k), so no dispatch is needed; sorted_rows = 1: X [tokens*top_k][K][ldx],
- * src = r.  Y [tokens*top_k][M][ldy]; rows from R on are left as they were. */
+ * src = r.  Y [tokens*top_k][M][ldy]; rows from R on are left as they were.
+ * Weight rows that do not start 16-byte aligned (K not a multiple of 16) are first copied to
+ * rows that do, in `workspace` (16-byte aligned, pnb_expert_contract_workspace_bytes, 0 when none
+ * is needed; one per call in flight) or, when that is NULL, in memory allocated on `stream`. */
 int pnb_expert_contract(const int32_t* row_choice_dev, const int32_t* row_expert_dev, int tokens,
                         int top_k, int experts, int sorted_rows, const int8_t* W_dev,
                         const int64_t* bias_dev, uint64_t delta, int M, int K,
                         const uint64_t* X_dev, int ldx, uint64_t* Y_dev, int ldy, int lwe_len,
-                        void* stream);
+                        void* workspace, size_t workspace_bytes, void* stream);
+size_t pnb_expert_contract_workspace_bytes(const int8_t* W_dev, int experts, int M, int K);
 /* out[t][f] = sum_i weights[t][i] * Y[choice_row[t][i]][f]: rows (Y [tokens*top_k][features][ldy])
  * back in token order (out [tokens][features][ldo]).  Unused choices add nothing; a token without
  * a used choice gets zero words.  weights as for pnb_expert_dispatch, whose gradient with respect
@@ -271,12 +275,16 @@ int pnb_expert_combine(const int32_t* choice_row_dev, int tokens, int top_k,
  * W int8 [M][K], A int8 [adapters][rank][K], B int8 [adapters][M][rank], adapter int32 [batch]; a
  * request whose adapter is outside [0, adapters) gets the shared projection alone.  base_shift
  * (0..63) puts the shared weights on the grid of the adapters' products.  1 <= rank <=
- * PNB_MAX_RANK, K <= 65536; X [batch][K][ldx], Y [batch][M][ldy]. */
+ * PNB_MAX_RANK, K <= 65536; X [batch][K][ldx], Y [batch][M][ldy].  The workspace is as for
+ * pnb_expert_contract (rows of B are `rank` long). */
 int pnb_adapter_contract(const int8_t* W_dev, const int64_t* bias_dev, uint64_t delta,
                          int base_shift, int M, int K, const int8_t* A_dev, const int8_t* B_dev,
                          int adapters, int rank, const int32_t* adapter_dev,
                          const uint64_t* X_dev, int ldx, uint64_t* Y_dev, int ldy, int batch,
-                         int lwe_len, void* stream);
+                         int lwe_len, void* workspace, size_t workspace_bytes, void* stream);
+size_t pnb_adapter_contract_workspace_bytes(const int8_t* W_dev, int M, int K,
+                                            const int8_t* A_dev, const int8_t* B_dev,
+                                            int adapters, int rank);
 
 /* Negacyclic products out[c] = a[c] * b[c] mod (X^N + 1) through the same f64 FFT the blind
  * rotation uses (a: small signed integers, |a| < 2^31; b: u64 torus), count polynomials.

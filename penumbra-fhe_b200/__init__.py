@@ -108,14 +108,18 @@ _SIGS = {
     "pnb_expert_contract": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                       C.c_void_p, C.c_void_p, C.c_uint64, C.c_int, C.c_int,
                                       C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int,
-                                      C.c_void_p]),
+                                      C.c_void_p, C.c_size_t, C.c_void_p]),
+    "pnb_expert_contract_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
     "pnb_expert_combine": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
                                      C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int,
                                      C.c_void_p]),
     "pnb_adapter_contract": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_int, C.c_int,
                                        C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
                                        C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
-                                       C.c_int, C.c_int, C.c_void_p]),
+                                       C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "pnb_adapter_contract_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int,
+                                                          C.c_void_p, C.c_void_p, C.c_int,
+                                                          C.c_int]),
     "pnb_keys_serialized_bytes": (C.c_size_t, [C.c_void_p, C.c_int]),
     "pnb_keys_serialize": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_size_t]),
     "pnb_keys_deserialize": (C.c_int, [C.c_int, C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p)]),
@@ -614,39 +618,68 @@ def lwe_contract_gather_ld(W: torch.Tensor, bias: torch.Tensor | None, delta: in
 
 
 # ---- weights that differ from request to request ----------------------------------------------
-def _want(name: str, t, dtype, shape, device):
-    """``t`` on ``device`` with this dtype and shape (None = any size), contiguous."""
+# These calls may be a few microseconds of GPU work, so their host side is kept short: plain checks,
+# addresses as integers, and the device switched only when it is another one.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _want(name: str, t, dtype, shape, device) -> torch.Tensor:
+    """``t``, on ``device`` with this dtype and shape (None = any size), contiguous."""
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if len(t.shape) != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
+    got = t.shape
+    if got != shape and (len(got) != len(shape) or
+                         any(w is not None and w != g for w, g in zip(shape, got))):
+        raise ValueError(f"{name} has shape {tuple(got)}, expected "
                          f"{tuple('*' if w is None else w for w in shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _want_out(name: str, out, shape, device, lwe_len: int):
+def _want_words(name: str, X, lwe_len, device, shape):
+    """Ciphertext rows [*, *, ld], contiguous, their pitch and the words used of each."""
+    if X.dtype is not torch.int64 and X.dtype is not torch.uint64:
+        raise TypeError(f"expected a 64-bit tensor, got {X.dtype}")
+    if X.dim() != 3 or not X.is_cuda:
+        raise ValueError(f"{name} must be a 3-dimensional CUDA tensor of ciphertext rows, got "
+                         f"{tuple(X.shape)} on {X.device}")
+    ld = X.shape[2]
+    lwe_len = ld if lwe_len is None else lwe_len
+    if not 1 <= lwe_len <= ld:
+        raise ValueError(f"lwe_len {lwe_len} does not fit rows of {ld} words")
+    return _want(name, X, X.dtype, shape + (ld,), device), ld, lwe_len
+
+
+def _want_out(out, shape, device, lwe_len: int) -> torch.Tensor:
     """The caller's buffer, checked, or a new one: zeros where the call leaves words behind
     ``lwe_len``."""
     if out is None:
         make = torch.empty if shape[-1] == lwe_len else torch.zeros
         return make(shape, dtype=torch.int64, device=device)
-    if _u64(out).shape != torch.Size(shape) or out.device != device or not out.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {tuple(shape)} tensor on {device}, got "
+    if out.dtype is not torch.int64 and out.dtype is not torch.uint64:
+        raise TypeError(f"expected a 64-bit tensor, got {out.dtype}")
+    if out.shape != shape or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {tuple(shape)} tensor on {device}, got "
                          f"{tuple(out.shape)} on {out.device}")
     return out
 
 
-def _want_words(name: str, X, lwe_len):
-    """Ciphertext rows [*, *, ld] on a GPU and the words used of each."""
-    if _u64(X).dim() != 3 or not X.is_cuda:
-        raise ValueError(f"{name} must be a 3-dimensional CUDA tensor of ciphertext rows, got "
-                         f"{tuple(X.shape)} on {X.device}")
-    lwe_len = X.shape[2] if lwe_len is None else lwe_len
-    if not 1 <= lwe_len <= X.shape[2]:
-        raise ValueError(f"lwe_len {lwe_len} does not fit rows of {X.shape[2]} words")
-    return X.contiguous(), lwe_len
+def _at(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(name: str, device: torch.device, *args):
+    """Call ``name`` on ``device`` with its current stream behind the other arguments."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = getattr(_LIB or lib(), name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(_LIB or lib(), name)(*args, _raw_stream(index))
+    if rc != 0:
+        _check(name, rc)
 
 
 class ExpertRoute:
@@ -679,17 +712,15 @@ def expert_route(ids: torch.Tensor, experts: int, out: ExpertRoute | None = None
         raise ValueError(f"ids must be a CUDA tensor [tokens, top_k], got {tuple(ids.shape)} on "
                          f"{ids.device}")
     T, k = ids.shape
-    ids = _want("ids", ids, torch.int32, (T, k), ids.device)
+    device = ids.device
+    ids = _want("ids", ids, torch.int32, (T, k), device)
     if out is None:
-        out = ExpertRoute(T, k, experts, ids.device)
-    elif (out.tokens, out.top_k, out.experts, out.device) != (T, k, experts, ids.device):
+        out = ExpertRoute(T, k, experts, device)
+    elif (out.tokens, out.top_k, out.experts, out.device) != (T, k, experts, device):
         raise ValueError(f"out is a route of {out.tokens} x {out.top_k} choices of {out.experts} "
-                         f"experts on {out.device}, not {T} x {k} of {experts} on {ids.device}")
-    with torch.cuda.device(ids.device):
-        _check("pnb_expert_route",
-               lib().pnb_expert_route(_ptr(ids), T, k, experts, _ptr(out.offsets),
-                                      _ptr(out.row_choice), _ptr(out.row_expert),
-                                      _ptr(out.choice_row), _stream(ids.device)))
+                         f"experts on {out.device}, not {T} x {k} of {experts} on {device}")
+    _launch("pnb_expert_route", device, ids.data_ptr(), T, k, experts, out.offsets.data_ptr(),
+            out.row_choice.data_ptr(), out.row_expert.data_ptr(), out.choice_row.data_ptr())
     return out
 
 
@@ -704,15 +735,12 @@ def expert_dispatch(route: ExpertRoute, X: torch.Tensor, lwe_len: int | None = N
     """The tokens' ciphertexts ``X`` [tokens, features, ld] in row order, each times its choice's
     weight (int32 [tokens, top_k], None = 1): [tokens*top_k, features, ld].  Rows without a choice
     are left as they were (not set when ``out`` is made here), as are words behind ``lwe_len``."""
-    X, L = _want_words("X", X, lwe_len)
-    T, F, ld = X.shape
-    X = _want("X", X, X.dtype, (route.tokens, None, None), route.device)
+    X, ld, L = _want_words("X", X, lwe_len, route.device, (route.tokens, None))
+    F = X.shape[1]
     w = _route_weights(route, weights)
-    out = _want_out("out", out, (route.rows, F, ld), X.device, L)
-    with torch.cuda.device(X.device):
-        _check("pnb_expert_dispatch",
-               lib().pnb_expert_dispatch(_ptr(route.choice_row), T, route.top_k, _ptr(w), _ptr(X),
-                                         F, ld, _ptr(out), ld, L, _stream(X.device)))
+    out = _want_out(out, (route.rows, F, ld), route.device, L)
+    _launch("pnb_expert_dispatch", route.device, route.choice_row.data_ptr(), route.tokens,
+            route.top_k, _at(w), X.data_ptr(), F, ld, out.data_ptr(), ld, L)
     return out
 
 
@@ -722,15 +750,12 @@ def expert_combine(route: ExpertRoute, Y: torch.Tensor, lwe_len: int | None = No
     """Rows ``Y`` [tokens*top_k, features, ld] back in token order, each times its choice's weight
     (int32 [tokens, top_k], None = 1) and summed per token: [tokens, features, ld].  A token
     without a used choice gets zero words."""
-    Y, L = _want_words("Y", Y, lwe_len)
-    Y = _want("Y", Y, Y.dtype, (route.rows, None, None), route.device)
-    F, ld = Y.shape[1:]
+    Y, ld, L = _want_words("Y", Y, lwe_len, route.device, (route.rows, None))
+    F = Y.shape[1]
     w = _route_weights(route, weights)
-    out = _want_out("out", out, (route.tokens, F, ld), Y.device, L)
-    with torch.cuda.device(Y.device):
-        _check("pnb_expert_combine",
-               lib().pnb_expert_combine(_ptr(route.choice_row), route.tokens, route.top_k, _ptr(w),
-                                        _ptr(Y), F, ld, _ptr(out), ld, L, _stream(Y.device)))
+    out = _want_out(out, (route.tokens, F, ld), route.device, L)
+    _launch("pnb_expert_combine", route.device, route.choice_row.data_ptr(), route.tokens,
+            route.top_k, _at(w), Y.data_ptr(), F, ld, out.data_ptr(), ld, L)
     return out
 
 
@@ -742,23 +767,22 @@ def expert_contract(route: ExpertRoute, W: torch.Tensor, bias: torch.Tensor | No
     (no dispatch needed), or with ``sorted_rows`` the rows [tokens*top_k, K, ld] of an earlier
     call.  The result is [tokens*top_k, M, ld] in row order; rows without a choice are left as they
     were (not set when ``out`` is made here), as are words behind ``lwe_len``."""
-    X, L = _want_words("X", X, lwe_len)
     if W.dim() != 3:
         raise ValueError(f"W must be [experts, M, K], got {tuple(W.shape)}")
-    M, K = W.shape[1:]
-    W = _want("W", W, torch.int8, (route.experts, M, K), route.device)
-    X = _want("X", X, X.dtype, (route.rows if sorted_rows else route.tokens, K, None),
-              route.device)
-    b = None if bias is None else _want("bias", bias, torch.int64, (route.experts, M),
-                                        route.device)
-    ld = X.shape[2]
-    out = _want_out("out", out, (route.rows, M, ld), X.device, L)
-    with torch.cuda.device(X.device):
-        _check("pnb_expert_contract",
-               lib().pnb_expert_contract(_ptr(route.row_choice), _ptr(route.row_expert),
-                                         route.tokens, route.top_k, route.experts,
-                                         int(sorted_rows), _ptr(W), _ptr(b), delta % (1 << 64), M,
-                                         K, _ptr(X), ld, _ptr(out), ld, L, _stream(X.device)))
+    device = route.device
+    E, M, K = W.shape
+    X, ld, L = _want_words("X", X, lwe_len, device,
+                           (route.rows if sorted_rows else route.tokens, K))
+    W = _want("W", W, torch.int8, (route.experts, M, K), device)
+    b = None if bias is None else _want("bias", bias, torch.int64, (E, M), device)
+    out = _want_out(out, (route.rows, M, ld), device, L)
+    need = 0 if K % 16 == 0 and W.data_ptr() % 16 == 0 else \
+        lib().pnb_expert_contract_workspace_bytes(W.data_ptr(), E, M, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _launch("pnb_expert_contract", device, route.row_choice.data_ptr(),
+            route.row_expert.data_ptr(), route.tokens, route.top_k, E, 1 if sorted_rows else 0,
+            W.data_ptr(), _at(b), delta % (1 << 64), M, K, X.data_ptr(), ld, out.data_ptr(), ld, L,
+            _at(ws), need)
     return out
 
 
@@ -771,25 +795,26 @@ def adapter_contract(W: torch.Tensor, bias: torch.Tensor | None, delta: int, A: 
     ``a = adapter[b]``; a value outside [0, adapters) means the shared projection alone.
     ``W`` int8 [M, K], ``A`` int8 [adapters, rank, K], ``B`` int8 [adapters, M, rank], ``bias``
     int64 [M] or None, ``adapter`` int32 [batch], ``X`` [batch, K, ld] -> [batch, M, ld]."""
-    X, L = _want_words("X", X, lwe_len)
     if W.dim() != 2 or A.dim() != 3:
         raise ValueError(f"W must be [M, K] and A [adapters, rank, K], got {tuple(W.shape)} and "
                          f"{tuple(A.shape)}")
-    (M, K), (n, rank) = W.shape, A.shape[:2]
-    batch, _, ld = X.shape
-    dev = X.device
-    W = _want("W", W, torch.int8, (M, K), dev)
-    A = _want("A", A, torch.int8, (n, rank, K), dev)
-    B = _want("B", B, torch.int8, (n, M, rank), dev)
-    adapter = _want("adapter", adapter, torch.int32, (batch,), dev)
-    X = _want("X", X, X.dtype, (None, K, None), dev)
-    b = None if bias is None else _want("bias", bias, torch.int64, (M,), dev)
-    out = _want_out("out", out, (batch, M, ld), dev, L)
-    with torch.cuda.device(dev):
-        _check("pnb_adapter_contract",
-               lib().pnb_adapter_contract(_ptr(W), _ptr(b), delta % (1 << 64), base_shift, M, K,
-                                          _ptr(A), _ptr(B), n, rank, _ptr(adapter), _ptr(X), ld,
-                                          _ptr(out), ld, batch, L, _stream(dev)))
+    device = X.device
+    M, K = W.shape
+    n, rank, _ = A.shape
+    X, ld, L = _want_words("X", X, lwe_len, device, (None, K))
+    batch = X.shape[0]
+    W = _want("W", W, torch.int8, (M, K), device)
+    A = _want("A", A, torch.int8, (n, rank, K), device)
+    B = _want("B", B, torch.int8, (n, M, rank), device)
+    adapter = _want("adapter", adapter, torch.int32, (batch,), device)
+    b = None if bias is None else _want("bias", bias, torch.int64, (M,), device)
+    out = _want_out(out, (batch, M, ld), device, L)
+    need = lib().pnb_adapter_contract_workspace_bytes(W.data_ptr(), M, K, A.data_ptr(),
+                                                      B.data_ptr(), n, rank)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _launch("pnb_adapter_contract", device, W.data_ptr(), _at(b), delta % (1 << 64), base_shift, M, K,
+            A.data_ptr(), B.data_ptr(), n, rank, adapter.data_ptr(), X.data_ptr(), ld,
+            out.data_ptr(), ld, batch, L, _at(ws), need)
     return out
 
 

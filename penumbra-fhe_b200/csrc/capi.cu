@@ -547,7 +547,7 @@ int pnb_expert_contract(const int32_t* row_choice_dev, const int32_t* row_expert
                         int top_k, int experts, int sorted_rows, const int8_t* W_dev,
                         const int64_t* bias_dev, uint64_t delta, int M, int K,
                         const uint64_t* X_dev, int ldx, uint64_t* Y_dev, int ldy, int lwe_len,
-                        void* stream) {
+                        void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_route("expert_contract", tokens, top_k);
   if (!rc) rc = check_weights("expert_contract", M, K);
   if (!rc) rc = check_rows("expert_contract", 1, lwe_len, ldx, ldy);
@@ -562,15 +562,29 @@ int pnb_expert_contract(const int32_t* row_choice_dev, const int32_t* row_expert
     return PNB_ERR_INVALID;
   }
   return expert_contract(row_choice_dev, row_expert_dev, tokens, top_k, experts, sorted_rows != 0,
-                         W_dev, bias_dev, delta, M, K, X_dev, ldx, Y_dev, ldy, lwe_len,
-                         (cudaStream_t)stream);
+                         W_dev, bias_dev, delta, M, K, X_dev, ldx, Y_dev, ldy, lwe_len, workspace,
+                         workspace_bytes, (cudaStream_t)stream);
+}
+
+size_t pnb_expert_contract_workspace_bytes(const int8_t* W_dev, int experts, int M, int K) {
+  if (experts < 1 || M < 1 || K < 1) return 0;
+  return padded_weight_bytes(W_dev, (long long)experts * M, K);
+}
+
+size_t pnb_adapter_contract_workspace_bytes(const int8_t* W_dev, int M, int K,
+                                            const int8_t* A_dev, const int8_t* B_dev,
+                                            int adapters, int rank) {
+  if (M < 1 || K < 1 || adapters < 1 || rank < 1) return 0;
+  return padded_weight_bytes(W_dev, M, K) +
+         padded_weight_bytes(A_dev, (long long)adapters * rank, K) +
+         padded_weight_bytes(B_dev, (long long)adapters * M, rank);
 }
 
 int pnb_adapter_contract(const int8_t* W_dev, const int64_t* bias_dev, uint64_t delta,
                          int base_shift, int M, int K, const int8_t* A_dev, const int8_t* B_dev,
                          int adapters, int rank, const int32_t* adapter_dev,
                          const uint64_t* X_dev, int ldx, uint64_t* Y_dev, int ldy, int batch,
-                         int lwe_len, void* stream) {
+                         int lwe_len, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_weights("adapter_contract", M, K);
   if (!rc) rc = check_rows("adapter_contract", 1, lwe_len, ldx, ldy);
   if (rc) return rc;
@@ -586,8 +600,8 @@ int pnb_adapter_contract(const int8_t* W_dev, const int64_t* bias_dev, uint64_t 
     return PNB_ERR_INVALID;
   }
   return adapter_contract(W_dev, bias_dev, delta, base_shift, M, K, A_dev, B_dev, adapters, rank,
-                          adapter_dev, X_dev, ldx, Y_dev, ldy, batch, lwe_len,
-                          (cudaStream_t)stream);
+                          adapter_dev, X_dev, ldx, Y_dev, ldy, batch, lwe_len, workspace,
+                          workspace_bytes, (cudaStream_t)stream);
 }
 
 int pnb_fft_negacyclic_mul(int device, int N, const int64_t* a_dev, const uint64_t* b_dev,

@@ -18,10 +18,11 @@
 namespace pnb {
 
 // ---- route --------------------------------------------------------------------------------------
-// One block: a counting sort whose counters are per (warp, expert).  Warp w owns one run of
+// Latency, not traffic: 12 bytes a choice.  One block: a counting sort whose counters are per (warp, expert).  Warp w owns one run of
 // consecutive choices, so "warps in order, choices in order within a warp" is choice order and the
 // sort is stable without atomics whose order could matter.
 constexpr int RT_MAX_WARPS = 32;
+constexpr int RT_AHEAD = 8;  // loads of a lane on their way together
 
 __global__ void __launch_bounds__(32 * RT_MAX_WARPS) route_kernel(
     const int32_t* __restrict__ ids, int n, int experts, int32_t* __restrict__ offsets,
@@ -37,22 +38,30 @@ __global__ void __launch_bounds__(32 * RT_MAX_WARPS) route_kernel(
   const int per = ((n + warps - 1) / warps + 31) & ~31;  // choices per warp
   const int lo = min(n, warp * per), hi = min(n, lo + per);
   int* cnt = rt_cnt + warp * experts;
-  for (int i = lo + lane; i < hi; i += 32) {
-    const int e = ids[i];
-    if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1);
+  auto load = [&](int i0, int (&e)[RT_AHEAD]) {  // -1: unused or behind the end
+#pragma unroll
+    for (int j = 0; j < RT_AHEAD; ++j) {
+      const int i = i0 + 32 * j + lane;
+      e[j] = i < hi ? __ldg(ids + i) : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < RT_AHEAD; ++j)
+      if (e[j] < 0 || e[j] >= experts) e[j] = -1;
+  };
+  int e[RT_AHEAD];
+  for (int i0 = lo; i0 < hi; i0 += 32 * RT_AHEAD) {
+    load(i0, e);
+#pragma unroll
+    for (int j = 0; j < RT_AHEAD; ++j)
+      if (e[j] >= 0) atomicAdd(&cnt[e[j]], 1);
   }
   __syncthreads();
   // exclusive prefix over (expert, warp), blockDim.x experts at a time
   for (int e0 = 0; e0 < experts; e0 += blockDim.x) {
-    const int e = e0 + threadIdx.x;
+    const int x = e0 + threadIdx.x;
     int total = 0;
-    if (e < experts) {
-      for (int w = 0; w < warps; ++w) {
-        const int c = rt_cnt[w * experts + e];
-        rt_cnt[w * experts + e] = total;
-        total += c;
-      }
-    }
+    if (x < experts)
+      for (int w = 0; w < warps; ++w) total += rt_cnt[w * experts + x];
     int incl = total;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -66,10 +75,14 @@ __global__ void __launch_bounds__(32 * RT_MAX_WARPS) route_kernel(
       if (w < warp) before += warp_sum[w];
       all += warp_sum[w];
     }
-    const int first = before + incl - total;
-    if (e < experts) {
-      offsets[e] = first;
-      for (int w = 0; w < warps; ++w) rt_cnt[w * experts + e] += first;
+    int first = before + incl - total;
+    if (x < experts) {
+      offsets[x] = first;
+      for (int w = 0; w < warps; ++w) {
+        const int c = rt_cnt[w * experts + x];
+        rt_cnt[w * experts + x] = first;
+        first += c;
+      }
     }
     __syncthreads();
     if (threadIdx.x == 0) carry_s += all;
@@ -78,24 +91,23 @@ __global__ void __launch_bounds__(32 * RT_MAX_WARPS) route_kernel(
   const int rows = carry_s;
   if (threadIdx.x == 0) offsets[experts] = rows;
   // places: within 32 choices, the lanes of one expert rank by lane number
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane;
-    int e = -1;
-    if (i < hi) {
-      e = ids[i];
-      if (e >= experts || e < 0) e = -1;
-    }
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    int at = -1;
-    if (e >= 0) at = cnt[e] + rank;
-    __syncwarp();
-    if (e >= 0 && rank == 0) cnt[e] += __popc(same);
-    __syncwarp();
-    if (i < hi) choice_row[i] = at;
-    if (e >= 0) {
-      row_choice[at] = i;
-      row_expert[at] = e;
+  for (int i0 = lo; i0 < hi; i0 += 32 * RT_AHEAD) {
+    load(i0, e);
+#pragma unroll
+    for (int j = 0; j < RT_AHEAD; ++j) {
+      const unsigned same = __match_any_sync(0xffffffffu, e[j]);
+      const int rank = __popc(same & ((1u << lane) - 1u));
+      int at = -1;
+      if (e[j] >= 0) at = cnt[e[j]] + rank;
+      __syncwarp();
+      if (e[j] >= 0 && rank == 0) cnt[e[j]] += __popc(same);
+      __syncwarp();
+      const int i = i0 + 32 * j + lane;
+      if (i < hi) choice_row[i] = at;
+      if (at >= 0) {
+        row_choice[at] = i;
+        row_expert[at] = e[j];
+      }
     }
   }
   for (int r = rows + threadIdx.x; r < n; r += blockDim.x) {
@@ -108,8 +120,9 @@ int expert_route(const int32_t* ids, int n, int experts, int32_t* offsets, int32
                  int32_t* row_expert, int32_t* choice_row, cudaStream_t st) {
   const int warps = std::max(1, std::min(RT_MAX_WARPS, (n + 31) / 32));
   const int smem = warps * experts * (int)sizeof(int);
-  PNB_CUDA(cudaFuncSetAttribute(route_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                RT_MAX_WARPS * PNB_MAX_EXPERTS * (int)sizeof(int)));
+  if (smem > 48 * 1024)
+    PNB_CUDA(cudaFuncSetAttribute(route_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  RT_MAX_WARPS * PNB_MAX_EXPERTS * (int)sizeof(int)));
   route_kernel<<<1, 32 * warps, smem, st>>>(ids, n, experts, offsets, row_choice, row_expert,
                                             choice_row);
   PNB_CHECK_LAUNCH("route_kernel");
@@ -117,74 +130,159 @@ int expert_route(const int32_t* ids, int n, int experts, int32_t* offsets, int32
 }
 
 // ---- dispatch and combine -----------------------------------------------------------------------
+// Copies with at most one multiply per word: HBM bounds them.  A block takes a run of one token's
+// words, so that dispatch reads a token once however many rows it becomes, and combine writes it
+// once.  Rows at even pitches with aligned bases move 16 bytes at a time, others 8; every thread
+// has MV_AHEAD loads on their way.  Runs do not end with a ciphertext: 1025 units of 16 bytes would
+// leave every second round of a block to one thread (combining 96 x 2 tokens of 128 ciphertexts:
+// 190 us so, 162 with a word per thread, XX with these runs).
+constexpr int MV_THREADS = 256;
+constexpr int MV_AHEAD = 4;
+constexpr int MV_RUN = MV_THREADS * MV_AHEAD;  // units of a run
+
 struct MoveArgs {
   const int32_t* choice_row;  // [tokens][top_k]
   const int32_t* weights;     // [tokens][top_k] or null
   const uint64_t* in;
   uint64_t* out;
   int tokens, top_k, features, L, ldi, ldo;
+  int per_row;                // units (1 or 2 words) of one ciphertext
+  uint32_t magic;             // u / per_row = umulhi(u, magic) >> shift for u < 2^21; 0: per_row = 1
+  int shift;
 };
 
-__global__ void dispatch_kernel(MoveArgs a) {
-  const int t = blockIdx.x;
-  const long long words = (long long)a.features * a.L;
+template <int WORDS> struct MvUnit;
+template <> struct MvUnit<1> { using T = unsigned long long; };
+template <> struct MvUnit<2> { using T = ulonglong2; };
+
+__device__ __forceinline__ void mv_madd(unsigned long long& a, unsigned long long v,
+                                        unsigned long long w) { a += v * w; }
+__device__ __forceinline__ void mv_madd(ulonglong2& a, ulonglong2 v, unsigned long long w) {
+  a.x += v.x * w;
+  a.y += v.y * w;
+}
+
+template <int WORDS, bool COMBINE>
+__global__ void __launch_bounds__(MV_THREADS) move_kernel(const MoveArgs a) {
+  using T = typename MvUnit<WORDS>::T;
   const int choices = a.tokens * a.top_k;
-  for (long long i = (long long)blockIdx.y * blockDim.x + threadIdx.x; i < words;
-       i += (long long)gridDim.y * blockDim.x) {
-    const long long f = i / a.L;
-    const int c = (int)(i % a.L);
-    const uint64_t v = a.in[((size_t)t * a.features + f) * a.ldi + c];
-    for (int k = 0; k < a.top_k; ++k) {
-      const int r = a.choice_row[t * a.top_k + k];
-      if (r < 0 || r >= choices) continue;
-      const uint64_t w = a.weights ? (uint64_t)(int64_t)a.weights[t * a.top_k + k] : 1ull;
-      a.out[((size_t)r * a.features + f) * a.ldo + c] = w * v;
+  const long long units = (long long)a.features * a.per_row;
+  const long long first = (long long)blockIdx.x * MV_RUN;
+  for (int t = blockIdx.y; t < a.tokens; t += gridDim.y) {
+    const int32_t* row_of = a.choice_row + (size_t)t * a.top_k;
+    const int32_t* weight = a.weights ? a.weights + (size_t)t * a.top_k : nullptr;
+    const long long f0 = first / a.per_row;
+    const int u0 = (int)(first - f0 * a.per_row) + threadIdx.x;
+    const int left = (int)min((long long)MV_RUN, units - first);
+    size_t in_at[MV_AHEAD], out_at[MV_AHEAD];
+    bool live[MV_AHEAD], whole[MV_AHEAD];
+#pragma unroll
+    for (int j = 0; j < MV_AHEAD; ++j) {
+      const int u = u0 + j * MV_THREADS;
+      const int f = a.magic ? (int)(__umulhi((uint32_t)u, a.magic) >> a.shift) : u;
+      const int c = (u - f * a.per_row) * WORDS;
+      live[j] = (int)threadIdx.x + j * MV_THREADS < left;
+      whole[j] = c + WORDS <= a.L;  // else the last word of an odd count
+      in_at[j] = (size_t)(f0 + f) * a.ldi + c;
+      out_at[j] = (size_t)(f0 + f) * a.ldo + c;
+    }
+    // the row of choice k and its weight; -1 past the last and where unused
+    auto row = [&](int k, unsigned long long& w) {
+      w = 1;
+      if (k >= a.top_k) return -1;
+      if (weight) w = (unsigned long long)(long long)__ldg(weight + k);
+      const int r = __ldg(row_of + k);
+      return r < choices ? r : -1;
+    };
+    auto load = [&](long long token, T (&v)[MV_AHEAD]) {
+#pragma unroll
+      for (int j = 0; j < MV_AHEAD; ++j) {
+        v[j] = T{};
+        if (token >= 0 && live[j])
+          v[j] = __ldcs(
+              reinterpret_cast<const T*>(a.in + (size_t)token * a.features * a.ldi + in_at[j]));
+      }
+    };
+    auto store = [&](long long token, const T (&v)[MV_AHEAD]) {
+#pragma unroll
+      for (int j = 0; j < MV_AHEAD; ++j) {
+        if (token < 0 || !live[j]) continue;
+        uint64_t* to = a.out + (size_t)token * a.features * a.ldo + out_at[j];
+        if (whole[j])
+          __stcs(reinterpret_cast<T*>(to), v[j]);
+        else
+          *to = *reinterpret_cast<const uint64_t*>(&v[j]);
+      }
+    };
+    if (COMBINE) {
+      T sum[MV_AHEAD] = {};
+      for (int k = 0; k < a.top_k; k += 2) {  // two rows' loads at a time
+        unsigned long long w0, w1;
+        const int r0 = row(k, w0), r1 = row(k + 1, w1);
+        T v0[MV_AHEAD], v1[MV_AHEAD];
+        load(r0, v0);
+        load(r1, v1);
+#pragma unroll
+        for (int j = 0; j < MV_AHEAD; ++j) {
+          mv_madd(sum[j], v0[j], w0);
+          mv_madd(sum[j], v1[j], w1);
+        }
+      }
+      store(t, sum);
+    } else {
+      T v[MV_AHEAD];
+      load(t, v);
+      for (int k = 0; k < a.top_k; ++k) {
+        unsigned long long w;
+        const int r = row(k, w);
+        T p[MV_AHEAD] = {};
+#pragma unroll
+        for (int j = 0; j < MV_AHEAD; ++j) mv_madd(p[j], v[j], w);
+        store(r, p);
+      }
     }
   }
 }
 
-__global__ void combine_kernel(MoveArgs a) {
-  const int t = blockIdx.x;
-  const long long words = (long long)a.features * a.L;
-  const int choices = a.tokens * a.top_k;
-  for (long long i = (long long)blockIdx.y * blockDim.x + threadIdx.x; i < words;
-       i += (long long)gridDim.y * blockDim.x) {
-    const long long f = i / a.L;
-    const int c = (int)(i % a.L);
-    uint64_t v = 0;
-    for (int k = 0; k < a.top_k; ++k) {
-      const int r = a.choice_row[t * a.top_k + k];
-      if (r < 0 || r >= choices) continue;
-      const uint64_t w = a.weights ? (uint64_t)(int64_t)a.weights[t * a.top_k + k] : 1ull;
-      v += w * a.in[((size_t)r * a.features + f) * a.ldi + c];
-    }
-    a.out[((size_t)t * a.features + f) * a.ldo + c] = v;
+template <bool COMBINE>
+static int move_launch(MoveArgs a, cudaStream_t st) {
+  const bool wide = a.ldi % 2 == 0 && a.ldo % 2 == 0 && ((uintptr_t)a.in % 16) == 0 &&
+                    ((uintptr_t)a.out % 16) == 0;
+  a.per_row = wide ? (a.L + 1) / 2 : a.L;
+  if (a.per_row > 1 << 20) {
+    set_error("%s: ciphertexts of %d words", COMBINE ? "expert_combine" : "expert_dispatch", a.L);
+    return PNB_ERR_INVALID;
   }
-}
-
-static int move_launch(bool combine, const MoveArgs& a, cudaStream_t st) {
-  const long long words = (long long)a.features * a.L;
-  const dim3 grid((unsigned)a.tokens, (unsigned)std::min<long long>((words + 1023) / 1024, 4096));
-  if (combine)
-    combine_kernel<<<grid, 256, 0, st>>>(a);
+  // ceil(2^(32 + shift) / per_row) with 2^shift >= per_row / 2: exact for u < 2^21 (less than
+  // 2^20 into a ciphertext, and a run)
+  a.shift = 0;
+  while ((2 << a.shift) < a.per_row) ++a.shift;
+  a.magic = (uint32_t)((((uint64_t)1 << (32 + a.shift)) + a.per_row - 1) / a.per_row);
+  const long long runs = ((long long)a.features * a.per_row + MV_RUN - 1) / MV_RUN;
+  if (runs > 0x7fffffffLL) {
+    set_error("%s: tokens of %d ciphertexts of %d words exceed one launch",
+              COMBINE ? "expert_combine" : "expert_dispatch", a.features, a.L);
+    return PNB_ERR_INVALID;
+  }
+  const dim3 grid((unsigned)runs, (unsigned)std::min(65535, a.tokens));
+  if (wide)
+    move_kernel<2, COMBINE><<<grid, MV_THREADS, 0, st>>>(a);
   else
-    dispatch_kernel<<<grid, 256, 0, st>>>(a);
-  PNB_CHECK_LAUNCH(combine ? "combine_kernel" : "dispatch_kernel");
+    move_kernel<1, COMBINE><<<grid, MV_THREADS, 0, st>>>(a);
+  PNB_CHECK_LAUNCH("move_kernel");
   return PNB_OK;
 }
 
 int expert_dispatch(const int32_t* choice_row, int tokens, int top_k, const int32_t* weights,
                     const uint64_t* X, int features, int ldx, uint64_t* out, int ldo, int L,
                     cudaStream_t st) {
-  return move_launch(false, {choice_row, weights, X, out, tokens, top_k, features, L, ldx, ldo},
-                     st);
+  return move_launch<false>({choice_row, weights, X, out, tokens, top_k, features, L, ldx, ldo}, st);
 }
 
 int expert_combine(const int32_t* choice_row, int tokens, int top_k, const int32_t* weights,
                    const uint64_t* Y, int features, int ldy, uint64_t* out, int ldo, int L,
                    cudaStream_t st) {
-  return move_launch(true, {choice_row, weights, Y, out, tokens, top_k, features, L, ldy, ldo},
-                     st);
+  return move_launch<true>({choice_row, weights, Y, out, tokens, top_k, features, L, ldy, ldo}, st);
 }
 
 }  // namespace pnb

@@ -84,11 +84,13 @@ int expert_combine(const int32_t* choice_row, int tokens, int top_k, const int32
 int expert_contract(const int32_t* row_choice, const int32_t* row_expert, int tokens, int top_k,
                     int experts, bool sorted_rows, const int8_t* W, const int64_t* bias,
                     uint64_t delta, int M, int K, const uint64_t* X, int ldx, uint64_t* Y, int ldy,
-                    int L, cudaStream_t st);
+                    int L, void* ws, size_t ws_bytes, cudaStream_t st);
+// Bytes a matrix of weights takes in their workspace: none where it can be read in place.
+size_t padded_weight_bytes(const int8_t* W, long long rows, int cols);
 int adapter_contract(const int8_t* W, const int64_t* bias, uint64_t delta, int base_shift, int M,
                      int K, const int8_t* A, const int8_t* B, int adapters, int rank,
                      const int32_t* adapter, const uint64_t* X, int ldx, uint64_t* Y, int ldy,
-                     int batch, int L, cudaStream_t st);
+                     int batch, int L, void* ws, size_t ws_bytes, cudaStream_t st);
 int keyswitch_tc(const pnb_keys* K, const uint64_t* in, uint64_t* out, int count, void* digits,
                  cudaStream_t st, int in_ld = 0);
 size_t ks_tc_workspace_bytes(const pnb_params& p, int count);

@@ -33,6 +33,7 @@
 // every other row, which no tiled load can shift: they land unshifted in a ring of raw slots, and
 // four warps copy them word by word into the operand layout.
 #include <algorithm>
+#include <atomic>
 
 #include <cudaTypedefs.h>
 
@@ -785,27 +786,54 @@ struct RqMatrix {
   const int8_t* p;
   long long rows;
   int cols;
-  int pitch() const { return (cols + 15) & ~15; }
+  __host__ __device__ int pitch() const { return (cols + 15) & ~15; }
   bool in_place() const { return cols % 16 == 0 && ((uintptr_t)p % 16) == 0; }
   size_t copy_bytes() const { return (size_t)rows * pitch(); }
 };
 
-__global__ void rq_pad_kernel(const int8_t* __restrict__ in, long long rows, int cols, int pitch,
-                              int8_t* __restrict__ out) {
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= rows * pitch) return;
-  const long long r = i / pitch;
-  const int c = (int)(i - r * pitch);
-  out[i] = c < cols ? in[r * cols + c] : (int8_t)0;
+size_t padded_weight_bytes(const int8_t* W, long long rows, int cols) {
+  const RqMatrix m{W, rows, cols};
+  return m.in_place() ? 0 : m.copy_bytes();
 }
 
-static int rq_place(RqMatrix& m, int8_t*& ws, cudaStream_t st) {
-  if (m.in_place()) return PNB_OK;
-  const size_t n = m.copy_bytes();
-  rq_pad_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(m.p, m.rows, m.cols, m.pitch(), ws);
+struct RqCopy {
+  RqMatrix m[3];
+  int8_t* to[3];
+  size_t first[4];  // the bytes of copy i are first[i] .. first[i + 1]
+};
+
+// Up to three matrices in one launch, 16 bytes (of one row) per thread.
+__global__ void rq_pad_kernel(const __grid_constant__ RqCopy c) {
+  const size_t i = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * 16;
+  if (i >= c.first[3]) return;
+  const int w = i >= c.first[2] ? 2 : i >= c.first[1] ? 1 : 0;
+  const RqMatrix& m = c.m[w];
+  const size_t at = i - c.first[w];
+  const int pitch = m.pitch();
+  const size_t r = at / pitch;
+  const int col = (int)(at - r * pitch);
+  const int8_t* from = m.p + r * m.cols + col;
+  union { int8_t b[16]; uint4 v; } u;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) u.b[j] = col + j < m.cols ? from[j] : (int8_t)0;
+  *reinterpret_cast<uint4*>(c.to[w] + at) = u.v;
+}
+
+// Copies the matrices that TMA cannot read in place to ws, and points them there.
+static int rq_place(RqMatrix* (&m)[3], int8_t* ws, cudaStream_t st) {
+  RqCopy c{};
+  for (int i = 0; i < 3; ++i) {
+    c.first[i + 1] = c.first[i];
+    if (m[i]->rows == 0 || m[i]->in_place()) continue;
+    c.m[i] = *m[i];
+    c.to[i] = ws + c.first[i];
+    c.first[i + 1] += m[i]->copy_bytes();
+    m[i]->p = c.to[i];
+  }
+  const size_t threads = c.first[3] / 16;
+  if (threads == 0) return PNB_OK;
+  rq_pad_kernel<<<(unsigned)((threads + 127) / 128), 128, 0, st>>>(c);
   PNB_CHECK_LAUNCH("rq_pad_kernel");
-  m.p = ws;
-  ws += n;
   return PNB_OK;
 }
 
@@ -889,9 +917,17 @@ static void rq_plan(RqArgs& a, int sms) {
 template <bool SHIFTED, bool ADAPT>
 static int rq_launch(const RqMaps& tm, RqArgs a, cudaStream_t st) {
   using S = RqShape<SHIFTED, ADAPT>;
+  // what a device needs once: its number of SMs, and this kernel's shared-memory limit raised
+  static std::atomic<int> sm_count[64];
   int dev = 0, sms = 0;
   PNB_CUDA(cudaGetDevice(&dev));
-  PNB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64) sms = sm_count[dev].load(std::memory_order_acquire);
+  if (sms == 0) {
+    PNB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    PNB_CUDA(cudaFuncSetAttribute(request_kernel<SHIFTED, ADAPT>,
+                                  cudaFuncAttributeMaxDynamicSharedMemorySize, RQ_SMEM));
+    if (dev < 64) sm_count[dev].store(sms, std::memory_order_release);
+  }
   rq_plan<SHIFTED, ADAPT>(a, sms);
   a.groups = (a.m_tiles + a.m_group - 1) / a.m_group;
   if ((long long)a.groups * a.n_tiles > 1 << 30 || a.rows > 1 << 30) {
@@ -904,8 +940,6 @@ static int rq_launch(const RqMaps& tm, RqArgs a, cudaStream_t st) {
   a.step_n = grid / per_row;
   a.step_g = grid % per_row / a.n_tiles;
   a.step_t = grid % per_row % a.n_tiles;
-  PNB_CUDA(cudaFuncSetAttribute(request_kernel<SHIFTED, ADAPT>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, RQ_SMEM));
   request_kernel<SHIFTED, ADAPT>
       <<<grid, S::THREADS, 1024 + a.bars_at + RQ_BAR_BYTES, st>>>(tm, a);
   PNB_CHECK_LAUNCH("request_kernel");
@@ -914,7 +948,7 @@ static int rq_launch(const RqMaps& tm, RqArgs a, cudaStream_t st) {
 
 template <bool ADAPT>
 static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* X, int ldx,
-                  int x_groups, cudaStream_t st) {
+                  int x_groups, void* ws, size_t ws_bytes, cudaStream_t st) {
   using S = RqShape<false, ADAPT>;
   const long long x_rows = (long long)x_groups * a.K;
   // TMA coordinates are 32-bit, and a tile reaches up to a slot past its first row
@@ -965,11 +999,14 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
   size_t need = W.in_place() ? 0 : W.copy_bytes();
   if (ADAPT) need += (A.in_place() ? 0 : A.copy_bytes()) + (B.in_place() ? 0 : B.copy_bytes());
   int8_t* own = nullptr;
-  if (need) PNB_CUDA(cudaMallocAsync((void**)&own, need, st));
-  int8_t* ws = own;
-  rc = rq_place(W, ws, st);
-  if (ADAPT && !rc) rc = rq_place(A, ws, st);
-  if (ADAPT && !rc) rc = rq_place(B, ws, st);
+  if (need && ws && (ws_bytes < need || ((uintptr_t)ws % 16) != 0)) {
+    set_error("%s: workspace of %zu bytes at %p, %zu bytes 16-byte aligned are needed",
+              ADAPT ? "adapter_contract" : "expert_contract", ws_bytes, ws, need);
+    return PNB_ERR_INVALID;
+  }
+  if (need && !ws) PNB_CUDA(cudaMallocAsync((void**)&own, need, st));
+  RqMatrix* all[3] = {&W, &A, &B};
+  rc = rq_place(all, own ? own : (int8_t*)ws, st);
   if (!rc) rc = rq_map_weights(&tm.W, W, 128, a.w_rows);
   if (ADAPT && !rc) rc = rq_map_weights(&tm.A, A, 128, a.rank16);
   if (ADAPT && !rc) rc = rq_map_weights(&tm.B, B, PNB_MAX_RANK, RQ_BM);
@@ -984,7 +1021,7 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
 int expert_contract(const int32_t* row_choice, const int32_t* row_expert, int tokens, int top_k,
                     int experts, bool sorted_rows, const int8_t* W, const int64_t* bias,
                     uint64_t delta, int M, int K, const uint64_t* X, int ldx, uint64_t* Y, int ldy,
-                    int L, cudaStream_t st) {
+                    int L, void* ws, size_t ws_bytes, cudaStream_t st) {
   RqArgs a{};
   a.Y = Y; a.bias = bias; a.delta = delta;
   a.row_choice = row_choice; a.which = row_expert;
@@ -993,13 +1030,13 @@ int expert_contract(const int32_t* row_choice, const int32_t* row_expert, int to
   a.n_which = experts;
   a.M = M; a.K = K; a.L = L; a.ldy = ldy;
   return rq_run<false>({W, (long long)experts * M, K}, {}, {}, a, X, ldx,
-                       sorted_rows ? a.rows : tokens, st);
+                       sorted_rows ? a.rows : tokens, ws, ws_bytes, st);
 }
 
 int adapter_contract(const int8_t* W, const int64_t* bias, uint64_t delta, int base_shift, int M,
                      int K, const int8_t* A, const int8_t* B, int adapters, int rank,
                      const int32_t* adapter, const uint64_t* X, int ldx, uint64_t* Y, int ldy,
-                     int batch, int L, cudaStream_t st) {
+                     int batch, int L, void* ws, size_t ws_bytes, cudaStream_t st) {
   RqArgs a{};
   a.Y = Y; a.bias = bias; a.delta = delta;
   a.which = adapter; a.n_which = adapters;
@@ -1007,7 +1044,7 @@ int adapter_contract(const int8_t* W, const int64_t* bias, uint64_t delta, int b
   a.M = M; a.K = K; a.L = L; a.ldy = ldy;
   a.shift = base_shift; a.rank = rank; a.rank16 = (rank + 15) & ~15;
   return rq_run<true>({W, M, K}, {A, (long long)adapters * rank, K}, {B, (long long)adapters * M, rank},
-                      a, X, ldx, batch, st);
+                      a, X, ldx, batch, ws, ws_bytes, st);
 }
 
 }  // namespace pnb

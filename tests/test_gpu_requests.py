@@ -352,6 +352,51 @@ def test_adapter_extremes(pnb, oracle):
     assert np.array_equal(got, plain_adapter(oracle, W, None, 0, A, B, which, X, 0))
 
 
+def test_workspace_of_the_c_abi(pnb, oracle):
+    # rows of 13 and 5 bytes are copied first: to the caller's memory, or to the call's own
+    rng = np.random.default_rng(14)
+    n, rank, M, K, L = 2, 5, 6, 13, 40
+    W = rng.integers(-128, 128, (M, K)).astype(np.int8)
+    A = rng.integers(-128, 128, (n, rank, K)).astype(np.int8)
+    B = rng.integers(-128, 128, (n, M, rank)).astype(np.int8)
+    X, which = words(rng, 2, K, L), np.array([1, 0], np.int32)
+    want = plain_adapter(oracle, W, None, 0, A, B, which, X, 2)
+    Wd, Ad, Bd, wd, Xd = dev(W), dev(A), dev(B), dev(which), dev(X)
+    need = pnb.lib().pnb_adapter_contract_workspace_bytes(Wd.data_ptr(), M, K, Ad.data_ptr(),
+                                                          Bd.data_ptr(), n, rank)
+    assert need == (M + n * rank + n * M) * 16
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    for p, size, rc in ((ws.data_ptr(), need, 0), (None, 0, 0), (ws.data_ptr(), need - 1, 1),
+                        (ws.data_ptr() + 8, need, 1)):
+        out = marked(2, M, L)
+        got = pnb.lib().pnb_adapter_contract(
+            Wd.data_ptr(), None, 0, 2, M, K, Ad.data_ptr(), Bd.data_ptr(), n, rank, wd.data_ptr(),
+            Xd.data_ptr(), L, out.data_ptr(), L, 2, L, p, size, stream)
+        assert got == rc
+        if rc == 0:
+            assert np.array_equal(host(out), want)
+        else:
+            assert b"workspace" in pnb.lib().pnb_last_error()
+            assert np.all(host(out) == MARK)
+
+
+def test_strided_inputs(pnb):
+    # tensors that are not contiguous are used as the values they hold
+    rng = np.random.default_rng(15)
+    T, k, E, M, K, L = 4, 2, 3, 10, 12, 30
+    ids = dev(draw_ids(rng, T, 2 * k, E, 0.1))[:, ::2]
+    route = pnb.expert_route(ids, E)
+    assert torch.equal(route.row_choice, pnb.expert_route(ids.contiguous(), E).row_choice)
+    X = dev(words(rng, K, T, L)).transpose(0, 1)
+    W = dev(rng.integers(-128, 128, (E, K, M)).astype(np.int8)).mT
+    got = pnb.expert_contract(route, W, None, 0, X, out=marked(T * k, M, L))
+    assert torch.equal(got, pnb.expert_contract(route, W.contiguous(), None, 0, X.contiguous(),
+                                                out=marked(T * k, M, L)))
+    assert torch.equal(pnb.expert_dispatch(route, X, out=marked(T * k, K, L)),
+                       pnb.expert_dispatch(route, X.contiguous(), out=marked(T * k, K, L)))
+
+
 # ---- refusals of the binding --------------------------------------------------------------------
 def test_binding_refusals(pnb):
     i32, i8 = dict(dtype=torch.int32, device="cuda"), dict(dtype=torch.int8, device="cuda")

@@ -35,6 +35,7 @@ def test_route_refuses_null(pnb, hole):
     ({1: -1}, b"tokens=-1"), ({2: 0}, b"top_k=0"), ({5: 0}, b"0 ciphertexts"),
     ({9: 0}, b"0 words"), ({6: 9}, b"pitches 9"), ({8: 9}, b"and 9"), ({0: NUL}, b"NULL"),
     ({4: NUL}, b"NULL"), ({7: NUL}, b"NULL"),
+    ({6: 1 << 22, 8: 1 << 22, 9: (1 << 21) + 1}, b"2097153 words"),
 ])
 def test_moves_refuse(pnb, fn, change, text):
     args = [P, 4, 2, NUL, P, 3, 10, P, 10, 10, NUL]
@@ -50,7 +51,7 @@ def test_moves_refuse(pnb, fn, change, text):
     ({1: NUL}, b"NULL"), ({6: NUL}, b"NULL"), ({11: NUL}, b"NULL"), ({13: NUL}, b"NULL"),
 ])
 def test_contract_refuses(pnb, change, text):
-    args = [P, P, 4, 2, 4, 0, P, P, 1, 3, 5, P, 10, P, 10, 10, NUL]
+    args = [P, P, 4, 2, 4, 0, P, P, 1, 3, 5, P, 10, P, 10, 10, NUL, 0, NUL]
     for i, v in change.items():
         args[i] = v
     _refused(pnb, pnb.lib().pnb_expert_contract(*args), text)
@@ -64,10 +65,22 @@ def test_contract_refuses(pnb, change, text):
     ({11: NUL}, b"NULL"), ({13: NUL}, b"NULL"),
 ])
 def test_adapter_refuses(pnb, change, text):
-    args = [P, P, 1, 0, 3, 5, P, P, 2, 2, P, P, 10, P, 10, 4, 10, NUL]
+    args = [P, P, 1, 0, 3, 5, P, P, 2, 2, P, P, 10, P, 10, 4, 10, NUL, 0, NUL]
     for i, v in change.items():
         args[i] = v
     _refused(pnb, pnb.lib().pnb_adapter_contract(*args), text)
+
+
+def test_workspace_bytes(pnb):
+    L = pnb.lib()
+    at = [C.c_void_p(a) for a in (4096, 4104)]
+    assert L.pnb_expert_contract_workspace_bytes(at[0], 3, 5, 32) == 0  # read in place
+    assert L.pnb_expert_contract_workspace_bytes(at[1], 3, 5, 32) == 15 * 32
+    assert L.pnb_expert_contract_workspace_bytes(at[0], 3, 5, 33) == 15 * 48
+    assert L.pnb_adapter_contract_workspace_bytes(at[0], 5, 32, at[0], at[0], 2, 16) == 0
+    assert L.pnb_adapter_contract_workspace_bytes(at[0], 5, 33, at[0], at[0], 2, 7) == \
+        5 * 48 + 14 * 48 + 10 * 16
+    assert L.pnb_adapter_contract_workspace_bytes(at[0], 5, 32, at[0], at[1], 2, 16) == 10 * 16
 
 
 def test_empty_batches_run_nothing(pnb):
@@ -75,9 +88,9 @@ def test_empty_batches_run_nothing(pnb):
     assert L.pnb_expert_dispatch(NUL, 0, 2, NUL, NUL, 3, 10, NUL, 10, 10, NUL) == 0
     assert L.pnb_expert_combine(NUL, 0, 2, NUL, NUL, 3, 10, NUL, 10, 10, NUL) == 0
     assert L.pnb_expert_contract(NUL, NUL, 0, 2, 4, 0, NUL, NUL, 1, 3, 5, NUL, 10, NUL, 10, 10,
-                                 NUL) == 0
+                                 NUL, 0, NUL) == 0
     assert L.pnb_adapter_contract(NUL, NUL, 1, 0, 3, 5, NUL, NUL, 2, 2, NUL, NUL, 10, NUL, 10, 0,
-                                  10, NUL) == 0
+                                  10, NUL, 0, NUL) == 0
 
 
 def test_binding_refuses_host_tensors(pnb):
