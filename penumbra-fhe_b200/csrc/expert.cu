@@ -12,31 +12,43 @@
 // (runtime/src/ops/linear.rs:52-75) for networks whose weights differ from request to request.
 #include <algorithm>
 
+#include <cooperative_groups.h>
+
 #include "pnb_internal.cuh"
 #include "pnb_keys.h"
 
 namespace pnb {
 
+namespace cg = cooperative_groups;
+
 // ---- route --------------------------------------------------------------------------------------
-// Latency, not traffic: 12 bytes a choice.  One block: a counting sort whose counters are per (warp, expert).  Warp w owns one run of
-// consecutive choices, so "warps in order, choices in order within a warp" is choice order and the
-// sort is stable without atomics whose order could matter.
+// Latency, not traffic: 12 bytes a choice.  A counting sort whose counters are per (warp, expert).
+// Warp w of the launch owns one run of consecutive choices, so "warps in order, choices in order
+// within a warp" is choice order and the sort is stable without atomics whose order could matter.
+// Many choices are shared out over the blocks of one cluster, which read each other's totals: what
+// one block spends its time on is the scattered stores, one line after another (8191 x 4 choices of
+// 64 experts: 41 us with one block, 14 with a cluster; 8 x 2: 6 us).
 constexpr int RT_MAX_WARPS = 32;
-constexpr int RT_AHEAD = 8;  // loads of a lane on their way together
+constexpr int RT_CLUSTER = 8;
+constexpr int RT_AHEAD = 4;  // loads of a lane on their way together
+constexpr int RT_ONE_BLOCK = 32 * RT_MAX_WARPS;  // one choice per thread
 
 __global__ void __launch_bounds__(32 * RT_MAX_WARPS) route_kernel(
     const int32_t* __restrict__ ids, int n, int experts, int32_t* __restrict__ offsets,
     int32_t* __restrict__ row_choice, int32_t* __restrict__ row_expert,
     int32_t* __restrict__ choice_row) {
-  extern __shared__ int rt_cnt[];  // [warps][experts]
+  extern __shared__ int rt_cnt[];  // [warps][experts], then the block's totals [experts]
   __shared__ int warp_sum[RT_MAX_WARPS];
   __shared__ int carry_s;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = gridDim.x, rank = blockIdx.x;
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* totals = rt_cnt + warps * experts;
   for (int i = threadIdx.x; i < warps * experts; i += blockDim.x) rt_cnt[i] = 0;
   if (threadIdx.x == 0) carry_s = 0;
   __syncthreads();
-  const int per = ((n + warps - 1) / warps + 31) & ~31;  // choices per warp
-  const int lo = min(n, warp * per), hi = min(n, lo + per);
+  const int per = ((n + blocks * warps - 1) / (blocks * warps) + 31) & ~31;  // choices per warp
+  const int lo = min(n, (rank * warps + warp) * per), hi = min(n, lo + per);
   int* cnt = rt_cnt + warp * experts;
   auto load = [&](int i0, int (&e)[RT_AHEAD]) {  // -1: unused or behind the end
 #pragma unroll
@@ -56,12 +68,22 @@ __global__ void __launch_bounds__(32 * RT_MAX_WARPS) route_kernel(
       if (e[j] >= 0) atomicAdd(&cnt[e[j]], 1);
   }
   __syncthreads();
-  // exclusive prefix over (expert, warp), blockDim.x experts at a time
+  for (int x = threadIdx.x; x < experts; x += blockDim.x) {
+    int total = 0;
+    for (int w = 0; w < warps; ++w) total += rt_cnt[w * experts + x];
+    totals[x] = total;
+  }
+  if (blocks > 1) cluster.sync(); else __syncthreads();
+  // exclusive prefix over (expert, block, warp), blockDim.x experts at a time
   for (int e0 = 0; e0 < experts; e0 += blockDim.x) {
     const int x = e0 + threadIdx.x;
-    int total = 0;
+    int total = 0, mine = 0;  // of the expert, and in the blocks before this one
     if (x < experts)
-      for (int w = 0; w < warps; ++w) total += rt_cnt[w * experts + x];
+      for (int b = 0; b < blocks; ++b) {
+        const int t = blocks > 1 ? *cluster.map_shared_rank(totals + x, b) : totals[x];
+        if (b < rank) mine += t;
+        total += t;
+      }
     int incl = total;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -75,9 +97,10 @@ __global__ void __launch_bounds__(32 * RT_MAX_WARPS) route_kernel(
       if (w < warp) before += warp_sum[w];
       all += warp_sum[w];
     }
-    int first = before + incl - total;
     if (x < experts) {
-      offsets[x] = first;
+      int first = before + incl - total;
+      if (rank == 0) offsets[x] = first;
+      first += mine;
       for (int w = 0; w < warps; ++w) {
         const int c = rt_cnt[w * experts + x];
         rt_cnt[w * experts + x] = first;
@@ -89,18 +112,25 @@ __global__ void __launch_bounds__(32 * RT_MAX_WARPS) route_kernel(
     __syncthreads();
   }
   const int rows = carry_s;
-  if (threadIdx.x == 0) offsets[experts] = rows;
-  // places: within 32 choices, the lanes of one expert rank by lane number
+  const int bits = 32 - __clz(experts - 1);
+  if (rank == 0 && threadIdx.x == 0) offsets[experts] = rows;
+  // places: within 32 choices, the lanes of one expert (one ballot per bit of its number) rank by
+  // lane number
   for (int i0 = lo; i0 < hi; i0 += 32 * RT_AHEAD) {
-    load(i0, e);
+    if (hi - lo > 32 * RT_AHEAD) load(i0, e);  // else they are still here
 #pragma unroll
     for (int j = 0; j < RT_AHEAD; ++j) {
-      const unsigned same = __match_any_sync(0xffffffffu, e[j]);
-      const int rank = __popc(same & ((1u << lane) - 1u));
+      unsigned same = __ballot_sync(0xffffffffu, e[j] >= 0);
+      for (int b = 0; b < bits; ++b) {
+        const bool set = (e[j] >> b) & 1;
+        const unsigned with = __ballot_sync(0xffffffffu, set);
+        same &= set ? with : ~with;
+      }
+      const int place = __popc(same & ((1u << lane) - 1u));
       int at = -1;
-      if (e[j] >= 0) at = cnt[e[j]] + rank;
+      if (e[j] >= 0) at = cnt[e[j]] + place;
       __syncwarp();
-      if (e[j] >= 0 && rank == 0) cnt[e[j]] += __popc(same);
+      if (e[j] >= 0 && place == 0) cnt[e[j]] += __popc(same);
       __syncwarp();
       const int i = i0 + 32 * j + lane;
       if (i < hi) choice_row[i] = at;
@@ -110,35 +140,46 @@ __global__ void __launch_bounds__(32 * RT_MAX_WARPS) route_kernel(
       }
     }
   }
-  for (int r = rows + threadIdx.x; r < n; r += blockDim.x) {
+  for (int r = rows + rank * blockDim.x + threadIdx.x; r < n; r += blocks * blockDim.x) {
     row_choice[r] = -1;
     row_expert[r] = -1;
   }
+  if (blocks > 1) cluster.sync();  // the others may still be reading this block's totals
 }
 
 int expert_route(const int32_t* ids, int n, int experts, int32_t* offsets, int32_t* row_choice,
                  int32_t* row_expert, int32_t* choice_row, cudaStream_t st) {
-  const int warps = std::max(1, std::min(RT_MAX_WARPS, (n + 31) / 32));
-  const int smem = warps * experts * (int)sizeof(int);
+  const int blocks = n > RT_ONE_BLOCK ? RT_CLUSTER : 1;
+  const int warps = std::max(1, std::min(RT_MAX_WARPS, (n + 32 * blocks - 1) / (32 * blocks)));
+  const int smem = (warps + 1) * experts * (int)sizeof(int);
   if (smem > 48 * 1024)
     PNB_CUDA(cudaFuncSetAttribute(route_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  RT_MAX_WARPS * PNB_MAX_EXPERTS * (int)sizeof(int)));
-  route_kernel<<<1, 32 * warps, smem, st>>>(ids, n, experts, offsets, row_choice, row_expert,
-                                            choice_row);
-  PNB_CHECK_LAUNCH("route_kernel");
+                                  (RT_MAX_WARPS + 1) * PNB_MAX_EXPERTS * (int)sizeof(int)));
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim = {(unsigned)blocks, 1, 1};
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(32 * warps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  PNB_CUDA(cudaLaunchKernelEx(&cfg, route_kernel, ids, n, experts, offsets, row_choice, row_expert,
+                              choice_row));
   return PNB_OK;
 }
 
 // ---- dispatch and combine -----------------------------------------------------------------------
 // Copies with at most one multiply per word: HBM bounds them.  A block takes a run of one token's
 // words, so that dispatch reads a token once however many rows it becomes, and combine writes it
-// once.  Rows at even pitches with aligned bases move 16 bytes at a time, others 8; every thread
-// has MV_AHEAD loads on their way.  Runs do not end with a ciphertext: 1025 units of 16 bytes would
-// leave every second round of a block to one thread (combining 96 x 2 tokens of 128 ciphertexts:
-// 190 us so, 162 with a word per thread, XX with these runs).
+// once.  Rows at even pitches with aligned bases move 16 bytes at a time, others 8.  Runs do not end
+// with a ciphertext: 1025 units of 16 bytes would leave every second round of a block to one
+// thread.  Measured on 96 x 2 tokens of 128 ciphertexts (604 MB): dispatch 97 us with four loads of
+// a thread on their way (105 with one); combine, which has two rows' loads on their way for each of
+// them, 102 us with one (110 with two, 145 with four: fewer warps fit).
 constexpr int MV_THREADS = 256;
-constexpr int MV_AHEAD = 4;
-constexpr int MV_RUN = MV_THREADS * MV_AHEAD;  // units of a run
+template <bool COMBINE> constexpr int mv_ahead() { return COMBINE ? 1 : 4; }
 
 struct MoveArgs {
   const int32_t* choice_row;  // [tokens][top_k]
@@ -164,6 +205,7 @@ __device__ __forceinline__ void mv_madd(ulonglong2& a, ulonglong2 v, unsigned lo
 
 template <int WORDS, bool COMBINE>
 __global__ void __launch_bounds__(MV_THREADS) move_kernel(const MoveArgs a) {
+  constexpr int MV_AHEAD = mv_ahead<COMBINE>(), MV_RUN = MV_THREADS * MV_AHEAD;
   using T = typename MvUnit<WORDS>::T;
   const int choices = a.tokens * a.top_k;
   const long long units = (long long)a.features * a.per_row;
@@ -199,7 +241,7 @@ __global__ void __launch_bounds__(MV_THREADS) move_kernel(const MoveArgs a) {
       for (int j = 0; j < MV_AHEAD; ++j) {
         v[j] = T{};
         if (token >= 0 && live[j])
-          v[j] = __ldcs(
+          v[j] = __ldg(
               reinterpret_cast<const T*>(a.in + (size_t)token * a.features * a.ldi + in_at[j]));
       }
     };
@@ -258,6 +300,7 @@ static int move_launch(MoveArgs a, cudaStream_t st) {
   a.shift = 0;
   while ((2 << a.shift) < a.per_row) ++a.shift;
   a.magic = (uint32_t)((((uint64_t)1 << (32 + a.shift)) + a.per_row - 1) / a.per_row);
+  constexpr int MV_RUN = MV_THREADS * mv_ahead<COMBINE>();
   const long long runs = ((long long)a.features * a.per_row + MV_RUN - 1) / MV_RUN;
   if (runs > 0x7fffffffLL) {
     set_error("%s: tokens of %d ciphertexts of %d words exceed one launch",

@@ -96,7 +96,8 @@ def plain_adapter(oracle, W, bias, delta, A, B, which, X, shift):
 @pytest.mark.parametrize("T,k,E,unused", [
     (1, 1, 1, 0.0), (1, 4, 3, 0.5), (7, 3, 5, 0.2), (32, 1, 8, 0.0), (33, 1, 8, 0.0),
     (128, 8, 64, 0.1), (341, 3, 1024, 0.0), (1025, 1, 2, 0.3), (8191, 4, 64, 0.1),
-    (40000, 1, 200, 0.0), (64, 2, 8, 1.0), (513, 2, 1, 0.0),
+    (40000, 1, 200, 0.0), (64, 2, 8, 1.0), (513, 2, 1, 0.0), (1024, 1, 7, 0.1), (257, 4, 7, 0.1),
+    (2000, 1, 1000, 0.2),
 ])
 def test_route(pnb, T, k, E, unused):
     rng = np.random.default_rng(T * 31 + k * 7 + E)
