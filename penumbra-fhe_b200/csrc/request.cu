@@ -883,9 +883,12 @@ static void rq_plan(RqArgs& a, int sms) {
   const int a_slot = ADAPT ? a.rank16 * RQ_WK : 0;  // beside each X slot
   const int out_bytes = RQ_EPI_WARPS * S::OUT;
   int room = RQ_SMEM - 1024 - RQ_BAR_BYTES - t_bytes - b_bytes - out_bytes;
-  // what X wants at least: 64 KB in flight (shifted: three operand slots and 40 KB of raw rows)
-  const int raw_min = SHIFTED ? 40 * 1024 / S::RAW_SLOT : 0;
-  const int x_min = (SHIFTED ? 48 * 1024 : 64 * 1024) / S::X_SLOT;
+  // what X wants at least before weights may stay: four slots (shifted: three and 40 KB of raw
+  // rows); for adapters, whose weights would come twice as often, three (two and 32 KB).  256 rows
+  // of 784->128: one slot less costs experts at an odd pitch 928 -> 1065 us by letting the weights
+  // stay, and gains rank 64 1359 -> 1147 us, rank 16 at an odd pitch 1423 -> 1333 us.
+  const int raw_min = SHIFTED ? (ADAPT ? 32 : 40) * 1024 / S::RAW_SLOT : 0;
+  const int x_min = 4 - (SHIFTED ? 1 : 0) - (ADAPT ? 1 : 0);
   auto x_bytes = [&](int slots) { return slots * (S::X_SLOT + a_slot) + raw_min * S::RAW_SLOT; };
   const long long columns = (long long)a.rows * a.n_tiles;
   a.m_group = a.m_tiles;
