@@ -488,8 +488,8 @@ static int check_rows(const char* fn, int features, int lwe_len, int ld_in, int 
 }
 
 static int check_weights(const char* fn, int M, int K) {
-  if (M < 1 || K < 1 || K > 65536) {
-    set_error("%s: bad weights M=%d K=%d (K <= 65536)", fn, M, K);
+  if (M < 1 || M > PNB_MAX_REQUEST_ROWS || K < 1 || K > 65536) {
+    set_error("%s: bad weights M=%d K=%d (M <= %d, K <= 65536)", fn, M, K, PNB_MAX_REQUEST_ROWS);
     return PNB_ERR_INVALID;
   }
   return PNB_OK;

@@ -67,8 +67,12 @@ constexpr int RQ_COPY_WARPS = 4;                       // each copies every four
 constexpr int RQ_RAW_ROWS = 32;                        // rows per raw slot, half of each parity
 constexpr int RQ_B_SLOTS = 2;
 constexpr int RQ_MAX_W = 13, RQ_MAX_X = 13, RQ_MAX_RAW = 16;  // most slots of each ring
-constexpr int RQ_BARS = 2 * (RQ_MAX_W + RQ_MAX_X + RQ_MAX_RAW + RQ_B_SLOTS) + 6;
-constexpr int RQ_BAR_BYTES = (8 * RQ_BARS + 16 + 127) / 128 * 128;
+constexpr int RQ_LISTS = 2;                            // lists of groups, each
+constexpr int RQ_LIST = 32;                            // one round of a warp long
+constexpr int RQ_BARS = 2 * (RQ_MAX_W + RQ_MAX_X + RQ_MAX_RAW + RQ_B_SLOTS + RQ_LISTS) + 6;
+// the barriers, two words, the lists' lengths, the lists
+constexpr int RQ_LIST_AT = (8 * RQ_BARS + 16 + 4 * RQ_LISTS + 15) / 16 * 16;
+constexpr int RQ_BAR_BYTES = (RQ_LIST_AT + 16 * RQ_LISTS * RQ_LIST + 127) / 128 * 128;
 constexpr int RQ_SMEM = 227 * 1024;                    // of one block
 constexpr uint32_t RQ_WAIT_LIMIT = 1u << 24;
 
@@ -108,62 +112,90 @@ struct RqArgs {
   int w_rows;                 // weight rows per load
   int n_tiles, m_tiles, m_group;  // tiles of 128 rows that share one load of X
   int groups;                 // of m_group tiles in one row
-  int step_n, step_g, step_t; // the grid as rows, groups and tiles of words
   int w_slots, x_slots, raw_slots;
   int keep_w;                 // the group's weights stay for the next group that uses them
   int x_at, raw_at, a_at, b_at, t_at, out_at, bars_at;  // shared-memory offsets; weights at 0
 };
 
-// A block's groups (row n, m_group tiles of 128 output rows, one tile of words; words fastest), one
-// grid apart.  What a row's tables hold is fetched one group ahead of its use.
+// One group: row n, tiles mg * m_group .. of 128 output rows, tile nt of words.
+struct RqGroup {
+  int n, mg, nt;
+  int src;    // the row's X group
+  int w;      // its expert or adapter, -1 when it has no adapter
+  bool load;  // its weights are not those of the group before
+  bool drop;  // the next group is known to need others
+};
+// In a list a group is four words: n; src and mg (adapters: mg); w; nt and the two flags.
+constexpr int RQ_MG_BITS = 12, RQ_NT_BITS = 30;
+constexpr int RQ_LAST = 256;  // in a list's length: no list follows
+static_assert(PNB_MAX_CHOICES <= 1 << (32 - RQ_MG_BITS), "a row's token beside its group");
+
+// A block's groups, one grid apart, words fastest.  One warp works them out, a round of 32 at a time,
+// without those whose row is skipped; every role reads them from its lists, so that no role has to
+// follow the tables, whose loads and branches cost a thread on its own over a thousand cycles a
+// tile, more than the MMAs of a short K take.
 template <bool ADAPT>
-struct RqWalk {
-  int n, mg, nt, which, choice;
-  __device__ __forceinline__ void fetch(const RqArgs& a) {
-    which = choice = -1;
-    if (n < a.rows) {
-      which = __ldg(a.which + n);
-      if (!ADAPT) choice = __ldg(a.row_choice + n);
+struct RqLister {
+  int done = 0;                  // rounds
+  int last_w = -2, last_mg = -1;  // of the last group listed
+  // The next list: its groups go to `to`; returns its length, with RQ_LAST when it is the last.
+  __device__ __forceinline__ int fill(const RqArgs& a, int lane, uint4* to) {
+    const long long total = (long long)a.rows * a.groups * a.n_tiles;
+    const unsigned per_row = (unsigned)(a.groups * a.n_tiles);
+    for (;;) {
+      const long long t = blockIdx.x + ((long long)done * 32 + lane) * gridDim.x;
+      ++done;
+      const bool last = blockIdx.x + (long long)done * 32 * gridDim.x >= total;
+      int n = 0, mg = 0, nt = 0, w = -1, src = 0;
+      bool used = t < total;
+      if (used) {
+        // 32-bit divisions wherever the numbers allow
+        n = total <= 0xffffffffll ? (int)((unsigned)t / per_row) : (int)(t / per_row);
+        const unsigned r = (unsigned)(t - (long long)n * per_row);
+        mg = (int)(r / (unsigned)a.n_tiles);
+        nt = (int)(r - (unsigned)(mg * a.n_tiles));
+        w = __ldg(a.which + n);
+        if (w < 0 || w >= a.n_which) w = -1;
+        src = n;
+        if (!ADAPT) {
+          const int c = __ldg(a.row_choice + n);
+          used = w >= 0 && c >= 0 && c < a.choices;
+          if (a.top_k > 0) src = c / a.top_k;
+        }
+      }
+      const unsigned mask = __ballot_sync(0xffffffffu, used);
+      if (mask == 0 && !last) continue;
+      const unsigned below = mask & ((1u << lane) - 1u), above = mask & ~(2u * (1u << lane) - 1u);
+      const int before = below ? 31 - __clz(below) : lane, after = above ? __ffs(above) - 1 : lane;
+      const int w0 = __shfl_sync(0xffffffffu, w, before), mg0 = __shfl_sync(0xffffffffu, mg, before);
+      const int w1 = __shfl_sync(0xffffffffu, w, after), mg1 = __shfl_sync(0xffffffffu, mg, after);
+      // same weights: the tile rows, and for experts the expert, are the same
+      const bool load = !a.keep_w || (below ? mg0 != mg || (!ADAPT && w0 != w)
+                                            : last_mg != mg || (!ADAPT && last_w != w));
+      const bool drop = !a.keep_w || (above && (mg1 != mg || (!ADAPT && w1 != w)));
+      if (used)
+        to[__popc(below)] = make_uint4(
+            (unsigned)n, ADAPT ? (unsigned)mg : (unsigned)src << RQ_MG_BITS | (unsigned)mg, (unsigned)w,
+            (unsigned)nt | (load ? 1u << RQ_NT_BITS : 0u) | (drop ? 2u << RQ_NT_BITS : 0u));
+      if (mask) {
+        const int end = 31 - __clz(mask);
+        last_w = __shfl_sync(0xffffffffu, w, end);
+        last_mg = __shfl_sync(0xffffffffu, mg, end);
+      }
+      return __popc(mask) | (last ? RQ_LAST : 0);
     }
   }
-  __device__ __forceinline__ void start(const RqArgs& a) {
-    nt = (int)blockIdx.x % a.n_tiles;
-    mg = (int)blockIdx.x / a.n_tiles;
-    n = mg / a.groups;
-    mg -= n * a.groups;
-    fetch(a);
-  }
-  __device__ __forceinline__ RqWalk next(const RqArgs& a) const {
-    RqWalk o;
-    o.nt = nt + a.step_t;
-    o.mg = mg + a.step_g;
-    o.n = n + a.step_n;
-    if (o.nt >= a.n_tiles) {
-      o.nt -= a.n_tiles;
-      ++o.mg;
-    }
-    if (o.mg >= a.groups) {
-      o.mg -= a.groups;
-      ++o.n;
-    }
-    o.fetch(a);
-    return o;
-  }
-  // the row's expert or adapter, -1 when it has none
-  __device__ __forceinline__ int weights(const RqArgs& a) const {
-    return which >= 0 && which < a.n_which ? which : -1;
-  }
-  __device__ __forceinline__ bool used(const RqArgs& a) const {
-    return n < a.rows &&
-           (ADAPT || (which >= 0 && which < a.n_which && choice >= 0 && choice < a.choices));
-  }
-  // the X group of a used row
-  __device__ __forceinline__ int source(const RqArgs& a) const {
-    return !ADAPT && a.top_k > 0 ? choice / a.top_k : n;
-  }
-  // groups of one key use the same W
-  __device__ __forceinline__ bool same_w(const RqWalk& o) const {
-    return mg == o.mg && (ADAPT || which == o.which);
+  static __device__ __forceinline__ RqGroup read(const uint4* from) {
+    const uint4 e = *from;
+    RqGroup g;
+    g.n = (int)e.x;
+    g.src = ADAPT ? (int)e.x : (int)(e.y >> RQ_MG_BITS);
+    g.mg = ADAPT ? (int)e.y : (int)(e.y & ((1u << RQ_MG_BITS) - 1u));
+    g.w = (int)e.z;
+    g.nt = (int)(e.w & ((1u << RQ_NT_BITS) - 1u));
+    g.load = e.w >> RQ_NT_BITS & 1u;
+    g.drop = e.w >> RQ_NT_BITS & 2u;
+    return g;
   }
 };
 
@@ -239,15 +271,18 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   const uint32_t t_at = base + (uint32_t)a.t_at;
   const uint32_t bars = base + (uint32_t)a.bars_at;
   constexpr int W0 = 0, X0 = 2 * RQ_MAX_W, R0 = X0 + 2 * RQ_MAX_X, B0 = R0 + 2 * RQ_MAX_RAW,
-                C0 = B0 + 2 * RQ_B_SLOTS;
+                L0 = B0 + 2 * RQ_B_SLOTS, C0 = L0 + 2 * RQ_LISTS;
   const uint32_t w_full = bars + 8 * W0, w_empty = w_full + 8 * RQ_MAX_W;
   const uint32_t x_full = bars + 8 * X0, x_empty = x_full + 8 * RQ_MAX_X;
   const uint32_t r_full = bars + 8 * R0, r_empty = r_full + 8 * RQ_MAX_RAW;
   const uint32_t b_full = bars + 8 * B0, b_empty = b_full + 8 * RQ_B_SLOTS;
+  const uint32_t list_full = bars + 8 * L0, list_empty = list_full + 8 * RQ_LISTS;
   const uint32_t acc_full = bars + 8 * C0, acc_empty = acc_full + 16;
   const uint32_t low_full = acc_full + 32, t_full = acc_full + 40;
   const uint32_t holder = bars + 8 * RQ_BARS;
   volatile int* abort_s = reinterpret_cast<volatile int*>(rq_raw + (holder + 8 - raw));
+  volatile int* list_n = abort_s + 1;
+  uint4* lists = reinterpret_cast<uint4*>(rq_raw + (bars - raw) + RQ_LIST_AT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -268,6 +303,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       tc::mbar_init(b_empty + 8 * s, 1);
       tc::mbar_init(acc_full + 8 * s, ADAPT ? 2 : 1);
       tc::mbar_init(acc_empty + 8 * s, RQ_EPI_WARPS);
+      tc::mbar_init(list_full + 8 * s, 1);
+      tc::mbar_init(list_empty + 8 * s, S::THREADS / 32);
     }
     tc::mbar_init(low_full, 1);
     tc::mbar_init(t_full, RQ_EPI_WARPS);
@@ -297,32 +334,38 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     return min(S::XK, (a.K - kx * S::XK + RQ_KSTEP - 1) / RQ_KSTEP * RQ_KSTEP);
   };
   auto tiles = [&](int mg) { return min(a.m_group, a.m_tiles - mg * a.m_group); };
+  // body(group) for every group of the block, until it returns false; a lane on its own, or the first
+  // of a warp that goes together, says when a list has been read
+  auto each = [&](bool alone, auto&& body) {
+    for (int c = 0;; ++c) {
+      const int l = c % RQ_LISTS;
+      if (!rq_wait(list_full + 8 * l, (uint32_t)(c / RQ_LISTS), abort_s)) return;
+      const int n = list_n[l];
+      for (int j = 0; j < (n & (RQ_LAST - 1)); ++j)
+        if (!body(RqLister<ADAPT>::read(lists + l * RQ_LIST + j))) return;
+      if (n & RQ_LAST) return;
+      if (!alone) __syncwarp();
+      if (lane == 0) tc::mbar_arrive(list_empty + 8 * l);
+    }
+  };
 
   if (warp == 0) {
     // ---------------- X loads (one lane) ---------------------------------------------------------
     if (lane == 0) {
       RqRing ring;
-      bool wrapped = false, ok = true;
+      bool wrapped = false;
       const int slots = SHIFTED ? a.raw_slots : a.x_slots;
-      RqWalk<ADAPT> at, ahead;
-      for (at.start(a); at.n < a.rows && ok && !*abort_s; at = ahead) {
-        ahead = at.next(a);
-        if (!at.used(a)) continue;
-        const int src = at.source(a), nt = at.nt, w = at.weights(a);
-        const bool has = ADAPT && w >= 0;
-        const int step = SHIFTED ? RQ_RAW_ROWS : S::XK;
-        for (int k = 0; k < a.K; k += step) {
+      each(true, [&](const RqGroup& g) {
+        const bool has = ADAPT && g.w >= 0;
+        for (int k = 0; k < a.K; k += SHIFTED ? RQ_RAW_ROWS : S::XK) {
           const int s = ring.slot;
           const uint32_t full = (SHIFTED ? r_full : x_full) + 8 * s;
-          if (!rq_wait((SHIFTED ? r_empty : x_empty) + 8 * s, ring.phase ^ 1u, abort_s)) {
-            ok = false;
-            break;
-          }
-          const int row = src * a.K + k;
+          if (!rq_wait((SHIFTED ? r_empty : x_empty) + 8 * s, ring.phase ^ 1u, abort_s)) return false;
+          const int row = g.src * a.K + k;
           if (SHIFTED) {
             tc::mbar_expect_tx(full, S::RAW_SLOT);  // the rows of either parity, in order
-            tc::tma_load_2d(raw_at(s), &tm.X[row & 1], nt * S::WORDS, row >> 1, full);
-            tc::tma_load_2d(raw_at(s) + S::RAW_SLOT / 2, &tm.X[(row + 1) & 1], nt * S::WORDS,
+            tc::tma_load_2d(raw_at(s), &tm.X[row & 1], g.nt * S::WORDS, row >> 1, full);
+            tc::tma_load_2d(raw_at(s) + S::RAW_SLOT / 2, &tm.X[(row + 1) & 1], g.nt * S::WORDS,
                             (row + 1) >> 1, full);
           } else {
             const int rows = x_rows(k / S::XK);
@@ -332,57 +375,75 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
             for (int r = 0; r < rows; r += box)
 #pragma unroll
               for (int b = 0; b < S::BOXES; ++b)
-                tc::tma_load_2d(x_at(s) + (b * S::XK + r) * 128, map, nt * S::BN + b * 128, row + r,
+                tc::tma_load_2d(x_at(s) + (b * S::XK + r) * 128, map, g.nt * S::BN + b * 128, row + r,
                                 full);
-            if (has) tc::tma_load_2d(a_at(s), &tm.A, k, w * a.rank, full);
+            if (has) tc::tma_load_2d(a_at(s), &tm.A, k, g.w * a.rank, full);
           }
           ring.advance(slots);
           wrapped |= ring.slot == 0;
         }
-      }
+        return true;
+      });
       rq_drain(SHIFTED ? r_full : x_full, ring, wrapped, slots);
     }
   } else if (warp == 1) {
-    // ---------------- weight loads (one lane) ----------------------------------------------------
-    if (lane == 0) {
-      RqRing br;
-      bool b_wrap = false, first = true, ok = true;
-      int w_slot = 0;
-      uint32_t w_par = 0, w_used = 0;  // a bit per slot
-      RqWalk<ADAPT> at, ahead, held;   // held: whose weights are in shared memory
-      for (at.start(a); at.n < a.rows && ok && !*abort_s; at = ahead) {
-        ahead = at.next(a);
-        if (!at.used(a)) continue;
-        const int w = at.weights(a);
-        const bool has = ADAPT && w >= 0;
-        const bool load = !a.keep_w || first || !at.same_w(held);
-        held = at;
-        first = false;
-        const int m_n = tiles(at.mg);
-        for (int m = 0; m < m_n && ok; ++m) {
-          const int m_row = (at.mg * a.m_group + m) * RQ_BM;
-          for (int kb = 0; kb < kb_n && load; ++kb) {
-            const int s = a.keep_w ? m * kb_n + kb : w_slot;
-            ok = rq_wait(w_empty + 8 * s, (w_par >> s) ^ 1u, abort_s);
-            if (!ok) break;
-            tc::mbar_expect_tx(w_full + 8 * s, (uint32_t)(a.w_rows * RQ_WK));
-            tc::tma_load_2d(w_at(s), &tm.W, kb * RQ_WK, (ADAPT ? 0 : w * a.M) + m_row,
-                            w_full + 8 * s);
-            w_par ^= 1u << s;
-            w_used |= 1u << s;
-            if (++w_slot == a.w_slots) w_slot = 0;
-          }
-          if (has && ok) {
-            const int s = br.slot;
-            ok = rq_wait(b_empty + 8 * s, br.phase ^ 1u, abort_s);
-            if (!ok) break;
-            tc::mbar_expect_tx(b_full + 8 * s, RQ_B_SLOT);
-            tc::tma_load_2d(b_at(s), &tm.B, 0, w * a.M + m_row, b_full + 8 * s);
-            br.advance(RQ_B_SLOTS);
-            b_wrap |= br.slot == 0;
-          }
+    // ---------------- the lists (the warp) and weight loads (one lane) ---------------------------
+    RqRing br;
+    bool b_wrap = false, ok = true;
+    int w_slot = 0;
+    uint32_t w_par = 0, w_used = 0;  // a bit per slot
+    auto load = [&](const RqGroup& g) {
+      const bool has = ADAPT && g.w >= 0;
+      const int m_n = tiles(g.mg);
+      if (a.keep_w) w_slot = 0;
+      for (int m = 0; m < m_n; ++m) {
+        const int m_row = (g.mg * a.m_group + m) * RQ_BM;
+        for (int kb = 0; kb < kb_n && g.load; ++kb) {
+          const int s = w_slot;
+          if (!rq_wait(w_empty + 8 * s, (w_par >> s) ^ 1u, abort_s)) return false;
+          tc::mbar_expect_tx(w_full + 8 * s, (uint32_t)(a.w_rows * RQ_WK));
+          tc::tma_load_2d(w_at(s), &tm.W, kb * RQ_WK, (ADAPT ? 0 : g.w * a.M) + m_row,
+                          w_full + 8 * s);
+          w_par ^= 1u << s;
+          w_used |= 1u << s;
+          if (++w_slot == a.w_slots) w_slot = 0;
+        }
+        if (has) {
+          const int s = br.slot;
+          if (!rq_wait(b_empty + 8 * s, br.phase ^ 1u, abort_s)) return false;
+          tc::mbar_expect_tx(b_full + 8 * s, RQ_B_SLOT);
+          tc::tma_load_2d(b_at(s), &tm.B, 0, g.w * a.M + m_row, b_full + 8 * s);
+          br.advance(RQ_B_SLOTS);
+          b_wrap |= br.slot == 0;
         }
       }
+      return true;
+    };
+    RqLister<ADAPT> lister;
+    auto list = [&](int c) {  // list c, once its place has been read by every warp
+      const int l = c % RQ_LISTS;
+      if (!__all_sync(0xffffffffu,
+                      rq_wait(list_empty + 8 * l, (uint32_t)(c / RQ_LISTS) ^ 1u, abort_s)))
+        return 0;
+      const int n = lister.fill(a, lane, lists + l * RQ_LIST);
+      if (lane == 0) list_n[l] = n;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(list_full + 8 * l);
+      return n;
+    };
+    for (int c = 0, n = list(0), next = 0;; ++c, n = next) {
+      // the next list is made a few groups into this one, when the other warps have left the last
+      const int count = n & (RQ_LAST - 1), early = min(8, count);
+      const uint4* from = lists + c % RQ_LISTS * RQ_LIST;
+      if (lane == 0)
+        for (int j = 0; j < early && ok; ++j) ok = load(RqLister<ADAPT>::read(from + j));
+      if (!(n & RQ_LAST)) next = list(c + 1);
+      if (lane == 0)
+        for (int j = early; j < count && ok; ++j) ok = load(RqLister<ADAPT>::read(from + j));
+      if ((n & RQ_LAST) || !__all_sync(0xffffffffu, ok && !*abort_s)) break;
+      if (lane == 0) tc::mbar_arrive(list_empty + 8 * (c % RQ_LISTS));
+    }
+    if (lane == 0) {
       for (int s = 0; s < a.w_slots; ++s)
         if ((w_used >> s) & 1u)
           (void)tc::mbar_wait(w_full + 8 * s, ((w_par >> s) ^ 1u) & 1u, RQ_WAIT_LIMIT);
@@ -398,17 +459,13 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     const int word = lane % S::WORDS, sub = lane / S::WORDS;
     const int box = word >> 4, ch = (word & 15) >> 1, half = word & 1;
     RqRing xr, rr;
-    bool x_wrap = false, ok = true;
-    RqWalk<ADAPT> at, ahead;
-    for (at.start(a); at.n < a.rows && ok && !*abort_s; at = ahead) {
-      ahead = at.next(a);
-      if (!at.used(a)) continue;
-      const int w = at.weights(a);
-      const int parity = at.source(a) * a.K & 1;  // of the group's first row (slots hold an even number)
+    bool x_wrap = false;
+    each(false, [&](const RqGroup& g) {
+      const int w = g.w;
+      const int parity = g.src * a.K & 1;  // of the group's first row (slots hold an even number)
       const int off_e = parity ? a.off1 : a.off0, off_o = parity ? a.off0 : a.off1;
-      for (int kx = 0; kx < kx_n && ok; ++kx) {
-        ok = rq_wait(x_empty + 8 * xr.slot, xr.phase ^ 1u, abort_s);
-        if (!ok) break;
+      for (int kx = 0; kx < kx_n; ++kx) {
+        if (!rq_wait(x_empty + 8 * xr.slot, xr.phase ^ 1u, abort_s)) return false;
         const uint32_t full = x_full + 8 * xr.slot;
         if (ADAPT && cw == 0 && lane == 0) {  // A's rows beside the slot
           tc::mbar_expect_tx(full, w >= 0 ? (uint32_t)a_slot : 0u);
@@ -417,8 +474,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         const int raws = x_rows(kx) / RQ_RAW_ROWS;
         for (int i = 0; i < raws; ++i) {
           if ((rr.slot & 3) == cw) {
-            ok = rq_wait(r_full + 8 * rr.slot, rr.phase, abort_s);
-            if (!ok) break;
+            if (!rq_wait(r_full + 8 * rr.slot, rr.phase, abort_s)) return false;
             // row r of the slot: its parity's half, r / 2; one word further where it is shifted
             const unsigned char* from = rq_raw + (raw_at(rr.slot) - raw) + word * 8;
             unsigned char* to = rq_raw + (x_at(xr.slot) - raw) + box * (S::XK * 128) +
@@ -452,7 +508,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         xr.advance(a.x_slots);
         x_wrap |= xr.slot == 0;
       }
-    }
+      return true;
+    });
     if (ADAPT && cw == 0 && lane == 0) rq_drain(x_full, xr, x_wrap, a.x_slots);
   } else if (warp == S::MMA_WARP) {
     // ---------------- main products (one lane) --------------------------------------------------
@@ -468,26 +525,16 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       const int steps = (a.K + RQ_KSTEP - 1) / RQ_KSTEP;  // MMAs of one tile
       const int x_slots = a.x_slots;
       const bool keep_w = a.keep_w != 0;
-      [&] {  // returns when a wait gives up
-        RqRing x;
-        int tt = 0, w_slot = 0;
-        uint32_t w_par = 0;
-        int unreleased = 0;  // weight slots kept for a group that has not come
-        RqWalk<ADAPT> at, ahead, beyond;
-        int held_mg = -1, held_w = -1;
-        at.start(a);
-        ahead = at.next(a);
-        for (; at.n < a.rows; at = ahead, ahead = beyond) {
-          beyond = ahead.next(a);
-          if (!at.used(a)) continue;
-          const bool load = !keep_w || at.mg != held_mg || (!ADAPT && at.which != held_w);
-          const int m_n = tiles(at.mg);
+      RqRing x;
+      int tt = 0, w_slot = 0;
+      uint32_t w_par = 0;
+      int unreleased = 0;  // weight slots kept for a group that has not come
+      each(true, [&](const RqGroup& g) {
+          const int m_n = tiles(g.mg);
+          const bool load = g.load, drop = g.drop;
           if (load)
             for (int s = 0; s < unreleased; ++s) tc::mma_commit(w_empty + 8 * s);
-          held_mg = at.mg;
-          held_w = at.which;
           // weights are let go with their last use when the next group is known to need others
-          const bool drop = !keep_w || (ahead.used(a) && !ahead.same_w(at));
           unreleased = drop ? 0 : m_n * kb_n;
           if (keep_w) w_slot = 0;
           const RqRing x0 = x;
@@ -495,21 +542,21 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
             // accumulators in turn: experts C in 256 columns each; adapters C in 128 columns each
             const uint32_t turn = 8u * (uint32_t)(tt & 1);
             const uint32_t c_tmem = tmem + (uint32_t)((tt & 1) * S::BN);
-            if (!rq_wait(acc_empty + turn, (uint32_t)(tt >> 1) ^ 1u, abort_s)) return;
+            if (!rq_wait(acc_empty + turn, (uint32_t)(tt >> 1) ^ 1u, abort_s)) return false;
             tc::tc_fence_after();  // (operands in shared memory need none: their mbarriers order them)
             x = x0;
             const bool first = m == 0, last = m == m_n - 1;
             uint32_t acc = 0;
             for (int left = steps; left > 0;) {  // 128 of K: one weight slot
               if (load) {
-                if (!rq_wait(w_full + 8 * w_slot, w_par >> w_slot, abort_s)) return;
+                if (!rq_wait(w_full + 8 * w_slot, w_par >> w_slot, abort_s)) return false;
                 w_par ^= 1u << w_slot;
               }
               uint32_t w_lo = (uint32_t)wd + (uint32_t)(w_slot * (RQ_W_SLOT / 16));
 #pragma unroll
               for (int h = 0; h < RQ_WK / S::XK; ++h, left -= STEPS, w_lo += 2 * STEPS) {
                 if (h > 0 && left <= 0) break;
-                if (first && !rq_wait(x_full + 8 * x.slot, x.phase, abort_s)) return;
+                if (first && !rq_wait(x_full + 8 * x.slot, x.phase, abort_s)) return false;
                 const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
                 tc::mma_i8_lo(c_tmem, w_lo, w_hi, x_lo, x_hi, MAIN, acc);
                 acc = 1;
@@ -529,8 +576,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
             }
             tc::mma_commit(acc_full + turn);
           }
-        }
-      }();
+          return true;
+      });
     }
   } else if (ADAPT && warp == S::MMA_WARP + 1) {
     // ---------------- low products L^T = X^T A^T and D = B t (one lane) --------------------------
@@ -568,11 +615,9 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         product(pending);
         pending = -1;
       };
-      RqWalk<ADAPT> at, ahead;
-      for (at.start(a); at.n < a.rows && ok && !*abort_s; at = ahead) {
-        ahead = at.next(a);
-        const bool has = at.weights(a) >= 0;
-        const int m_n = tiles(at.mg);
+      each(true, [&](const RqGroup& g) {
+        const bool has = g.w >= 0;
+        const int m_n = tiles(g.mg);
         for (int m = 0; m < m_n && ok; ++m, ++tt) {
           // Every tile's turn is waited for and answered, also where nothing is issued: a parity
           // tells only neighbouring turns apart, so no role may get two turns ahead of another.
@@ -617,7 +662,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           else if (m > 0)
             product(buf);
         }
-      }
+        return ok;
+      });
       if (ok && pending >= 0) finish(true);
     }
   } else {
@@ -635,11 +681,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     int tt = 0;
     uint32_t low_par = 0;
     bool ok = true;
-    RqWalk<ADAPT> at, ahead;
-    for (at.start(a); at.n < a.rows && ok && !*abort_s; at = ahead) {
-      ahead = at.next(a);
-      if (!at.used(a)) continue;
-      const int w = at.weights(a), mg = at.mg, nt = at.nt;
+    each(false, [&](const RqGroup& g) {
+      const int w = g.w, mg = g.mg, nt = g.nt;
       const bool has = ADAPT && w >= 0;
       const int m_n = tiles(mg);
       for (int m = 0; m < m_n; ++m, ++tt) {
@@ -747,17 +790,17 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           *p += bias;
           // tiled stores end on 16-byte boundaries, so the last word of an odd count goes alone
           if (!SHIFTED && (a.L & 1) && row0 + lane < a.M)
-            a.Y[((size_t)at.n * a.M + row0 + lane) * a.ldy + a.L - 1] = *p;
+            a.Y[((size_t)g.n * a.M + row0 + lane) * a.ldy + a.L - 1] = *p;
         }
         if (!SHIFTED) {
           tc::fence_async_smem();
           __syncwarp();
-          if (lane == 0 && col0 < (a.L & ~1)) tc::tma_store_3d(&tm.Y, col0, row0, at.n, out_at);
+          if (lane == 0 && col0 < (a.L & ~1)) tc::tma_store_3d(&tm.Y, col0, row0, g.n, out_at);
         } else {
           __syncwarp();
           constexpr int PER = 32 / EW;  // rows per instruction
           const int wd = lane % EW;
-          uint64_t* y = a.Y + ((size_t)at.n * a.M + row0) * a.ldy + col0 + wd;
+          uint64_t* y = a.Y + ((size_t)g.n * a.M + row0) * a.ldy + col0 + wd;
 #pragma unroll 8
           for (int j = 0; j < 32 / PER; ++j) {
             const int r = j * PER + lane / EW;
@@ -768,7 +811,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           __syncwarp();
         }
       }
-    }
+      return ok;
+    });
     if (!SHIFTED && lane == 0) tc::tma_store_wait();
   }
   tc::tc_fence_before();
@@ -933,16 +977,12 @@ static int rq_launch(const RqMaps& tm, RqArgs a, cudaStream_t st) {
   }
   rq_plan<SHIFTED, ADAPT>(a, sms);
   a.groups = (a.m_tiles + a.m_group - 1) / a.m_group;
-  if ((long long)a.groups * a.n_tiles > 1 << 30 || a.rows > 1 << 30) {
-    set_error("%s: %d rows of %d x %d tiles exceed one launch",
-              ADAPT ? "adapter_contract" : "expert_contract", a.rows, a.groups, a.n_tiles);
+  if (a.groups >= 1 << RQ_MG_BITS || (long long)a.groups * a.n_tiles >= 1 << RQ_NT_BITS) {
+    set_error("%s: %d x %d tiles of one row exceed one launch",
+              ADAPT ? "adapter_contract" : "expert_contract", a.groups, a.n_tiles);
     return PNB_ERR_INVALID;
   }
-  const int per_row = a.groups * a.n_tiles;
-  const int grid = (int)std::min<long long>((long long)a.rows * per_row, sms);
-  a.step_n = grid / per_row;
-  a.step_g = grid % per_row / a.n_tiles;
-  a.step_t = grid % per_row % a.n_tiles;
+  const int grid = (int)std::min<long long>((long long)a.rows * a.groups * a.n_tiles, sms);
   request_kernel<SHIFTED, ADAPT>
       <<<grid, S::THREADS, 1024 + a.bars_at + RQ_BAR_BYTES, st>>>(tm, a);
   PNB_CHECK_LAUNCH("request_kernel");

@@ -46,7 +46,7 @@ def test_moves_refuse(pnb, fn, change, text):
 
 @pytest.mark.parametrize("change,text", [
     ({2: -1}, b"tokens=-1"), ({3: 0}, b"top_k=0"), ({4: 0}, b"0 experts"),
-    ({4: 2000}, b"2000 experts"), ({9: 0}, b"M=0"), ({10: 0}, b"K=0"), ({10: 65537}, b"K=65537"),
+    ({4: 2000}, b"2000 experts"), ({9: 0}, b"M=0"), ({9: 524161}, b"M=524161"), ({10: 0}, b"K=0"), ({10: 65537}, b"K=65537"),
     ({12: 9}, b"pitches 9"), ({14: 9}, b"and 9"), ({15: 0}, b"0 words"), ({0: NUL}, b"NULL"),
     ({1: NUL}, b"NULL"), ({6: NUL}, b"NULL"), ({11: NUL}, b"NULL"), ({13: NUL}, b"NULL"),
 ])
@@ -58,7 +58,8 @@ def test_contract_refuses(pnb, change, text):
 
 
 @pytest.mark.parametrize("change,text", [
-    ({3: -1}, b"base_shift=-1"), ({3: 64}, b"base_shift=64"), ({4: 0}, b"M=0"), ({5: 0}, b"K=0"),
+    ({3: -1}, b"base_shift=-1"), ({3: 64}, b"base_shift=64"), ({4: 0}, b"M=0"),
+    ({4: 524161}, b"M=524161"), ({5: 0}, b"K=0"),
     ({5: 65537}, b"K=65537"), ({8: 0}, b"adapters=0"), ({9: 0}, b"rank=0"), ({9: 65}, b"rank=65"),
     ({12: 9}, b"pitches 9"), ({14: 9}, b"and 9"), ({15: -1}, b"batch=-1"), ({16: 0}, b"0 words"),
     ({0: NUL}, b"NULL"), ({6: NUL}, b"NULL"), ({7: NUL}, b"NULL"), ({10: NUL}, b"NULL"),
