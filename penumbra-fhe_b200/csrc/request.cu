@@ -34,6 +34,7 @@
 // four warps copy them word by word into the operand layout.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include <cudaTypedefs.h>
 
@@ -523,60 +524,78 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
       const uint32_t w_hi = (uint32_t)(wd >> 32), x_hi = (uint32_t)(xd >> 32);
       const int steps = (a.K + RQ_KSTEP - 1) / RQ_KSTEP;  // MMAs of one tile
-      const int x_slots = a.x_slots;
+      const int x_slots = a.x_slots, w_slots = a.w_slots;
       const bool keep_w = a.keep_w != 0;
       RqRing x;
       int tt = 0, w_slot = 0;
       uint32_t w_par = 0;
       int unreleased = 0;  // weight slots kept for a group that has not come
-      each(true, [&](const RqGroup& g) {
-          const int m_n = tiles(g.mg);
-          const bool load = g.load, drop = g.drop;
-          if (load)
-            for (int s = 0; s < unreleased; ++s) tc::mma_commit(w_empty + 8 * s);
-          // weights are let go with their last use when the next group is known to need others
-          unreleased = drop ? 0 : m_n * kb_n;
-          if (keep_w) w_slot = 0;
-          const RqRing x0 = x;
-          for (int m = 0; m < m_n; ++m, ++tt) {
-            // accumulators in turn: experts C in 256 columns each; adapters C in 128 columns each
-            const uint32_t turn = 8u * (uint32_t)(tt & 1);
-            const uint32_t c_tmem = tmem + (uint32_t)((tt & 1) * S::BN);
-            if (!rq_wait(acc_empty + turn, (uint32_t)(tt >> 1) ^ 1u, abort_s)) return false;
-            tc::tc_fence_after();  // (operands in shared memory need none: their mbarriers order them)
-            x = x0;
-            const bool first = m == 0, last = m == m_n - 1;
-            uint32_t acc = 0;
-            for (int left = steps; left > 0;) {  // 128 of K: one weight slot
-              if (load) {
-                if (!rq_wait(w_full + 8 * w_slot, w_par >> w_slot, abort_s)) return false;
-                w_par ^= 1u << w_slot;
-              }
-              uint32_t w_lo = (uint32_t)wd + (uint32_t)(w_slot * (RQ_W_SLOT / 16));
+      // One tile.  Those whose weights are there and stay (kept), whose X nobody else uses (alone), and
+      // both, are compiled apart, without the branches that ask.
+      using yes = std::true_type;
+      using no = std::false_type;
+      auto tile = [&](auto kept, auto alone, bool load, bool drop, bool first, bool last) {
+        if (kept) load = drop = false;
+        if (alone) first = last = true;
+        // accumulators in turn: experts C in 256 columns each; adapters C in 128 columns each
+        const uint32_t turn = 8u * (uint32_t)(tt & 1);
+        const uint32_t c_tmem = tmem + (uint32_t)((tt & 1) * S::BN);
+        if (!rq_wait(acc_empty + turn, (uint32_t)(tt >> 1) ^ 1u, abort_s)) return false;
+        tc::tc_fence_after();  // (operands in shared memory need none: their mbarriers order them)
+        uint32_t acc = 0;
+        auto slot = [&](uint32_t w_lo, int n, bool whole) {  // n MMAs of one X slot
+          if (first && !rq_wait(x_full + 8 * x.slot, x.phase, abort_s)) return false;
+          const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
 #pragma unroll
-              for (int h = 0; h < RQ_WK / S::XK; ++h, left -= STEPS, w_lo += 2 * STEPS) {
-                if (h > 0 && left <= 0) break;
-                if (first && !rq_wait(x_full + 8 * x.slot, x.phase, abort_s)) return false;
-                const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
-                tc::mma_i8_lo(c_tmem, w_lo, w_hi, x_lo, x_hi, MAIN, acc);
-                acc = 1;
-                if (left >= STEPS) {
-#pragma unroll
-                  for (int k = 1; k < STEPS; ++k)
-                    tc::mma_i8_lo(c_tmem, w_lo + 2 * k, w_hi, x_lo + 256 * k, x_hi, MAIN, 1u);
-                } else {
-                  for (int k = 1; k < left; ++k)
-                    tc::mma_i8_lo(c_tmem, w_lo + 2 * k, w_hi, x_lo + 256 * k, x_hi, MAIN, 1u);
-                }
-                if (last) tc::mma_commit(x_empty + 8 * x.slot);
-                x.advance(x_slots);
-              }
-              if (drop) tc::mma_commit(w_empty + 8 * w_slot);
-              if (++w_slot == a.w_slots) w_slot = 0;
-            }
-            tc::mma_commit(acc_full + turn);
-          }
+          for (int k = 0; k < STEPS; ++k)
+            if (whole || k < n)
+              tc::mma_i8_lo(c_tmem, w_lo + 2 * k, w_hi, x_lo + 256 * k, x_hi, MAIN, k ? 1u : acc);
+          acc = 1;
+          if (last) tc::mma_commit(x_empty + 8 * x.slot);
+          x.advance(x_slots);
           return true;
+        };
+        constexpr int W_STEPS = RQ_WK / RQ_KSTEP;
+        for (int left = steps; left > 0; left -= W_STEPS) {  // one weight slot: 128 of K
+          if (load) {
+            if (!rq_wait(w_full + 8 * w_slot, w_par >> w_slot, abort_s)) return false;
+            w_par ^= 1u << w_slot;
+          }
+          const uint32_t w_lo = (uint32_t)wd + (uint32_t)(w_slot * (RQ_W_SLOT / 16));
+          if (left >= W_STEPS) {
+#pragma unroll
+            for (int h = 0; h < W_STEPS; h += STEPS)
+              if (!slot(w_lo + 2 * h, STEPS, true)) return false;
+          } else {
+            for (int h = 0; h < left; h += STEPS)
+              if (!slot(w_lo + 2 * h, left - h, false)) return false;
+          }
+          if (drop) tc::mma_commit(w_empty + 8 * w_slot);
+          if (++w_slot == w_slots) w_slot = 0;
+        }
+        tc::mma_commit(acc_full + turn);
+        ++tt;
+        return true;
+      };
+      each(true, [&](const RqGroup& g) {
+        const int m_n = tiles(g.mg);
+        if (g.load)
+          for (int s = 0; s < unreleased; ++s) tc::mma_commit(w_empty + 8 * s);
+        // weights are let go with their last use when the next group is known to need others
+        unreleased = g.drop ? 0 : m_n * kb_n;
+        if (keep_w) w_slot = 0;
+        const bool kept = !g.load && !g.drop;
+        if (m_n == 1)
+          return kept ? tile(yes{}, yes{}, false, false, true, true)
+                      : tile(no{}, yes{}, g.load, g.drop, true, true);
+        const RqRing x0 = x;
+        for (int m = 0; m < m_n; ++m) {
+          x = x0;
+          if (!(kept ? tile(yes{}, no{}, false, false, m == 0, m == m_n - 1)
+                     : tile(no{}, no{}, g.load, g.drop, m == 0, m == m_n - 1)))
+            return false;
+        }
+        return true;
       });
     }
   } else if (ADAPT && warp == S::MMA_WARP + 1) {
