@@ -670,6 +670,12 @@ def _at(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+def _padded(t: torch.Tensor, rows: int, cols: int) -> int:
+    """Workspace bytes of a matrix of weights (``pnb_*_contract_workspace_bytes``): none where its
+    rows start 16-byte aligned."""
+    return 0 if cols % 16 == 0 and t.data_ptr() % 16 == 0 else rows * ((cols + 15) & -16)
+
+
 def _launch(name: str, device: torch.device, *args):
     """Call ``name`` on ``device`` with its current stream behind the other arguments."""
     index = device.index
@@ -776,8 +782,7 @@ def expert_contract(route: ExpertRoute, W: torch.Tensor, bias: torch.Tensor | No
     W = _want("W", W, torch.int8, (route.experts, M, K), device)
     b = None if bias is None else _want("bias", bias, torch.int64, (E, M), device)
     out = _want_out(out, (route.rows, M, ld), device, L)
-    need = 0 if K % 16 == 0 and W.data_ptr() % 16 == 0 else \
-        lib().pnb_expert_contract_workspace_bytes(W.data_ptr(), E, M, K)
+    need = _padded(W, E * M, K)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch("pnb_expert_contract", device, route.row_choice.data_ptr(),
             route.row_expert.data_ptr(), route.tokens, route.top_k, E, 1 if sorted_rows else 0,
@@ -809,8 +814,7 @@ def adapter_contract(W: torch.Tensor, bias: torch.Tensor | None, delta: int, A: 
     adapter = _want("adapter", adapter, torch.int32, (batch,), device)
     b = None if bias is None else _want("bias", bias, torch.int64, (M,), device)
     out = _want_out(out, (batch, M, ld), device, L)
-    need = lib().pnb_adapter_contract_workspace_bytes(W.data_ptr(), M, K, A.data_ptr(),
-                                                      B.data_ptr(), n, rank)
+    need = _padded(W, M, K) + _padded(A, n * rank, K) + _padded(B, n * M, rank)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch("pnb_adapter_contract", device, W.data_ptr(), _at(b), delta % (1 << 64), base_shift, M, K,
             A.data_ptr(), B.data_ptr(), n, rank, adapter.data_ptr(), X.data_ptr(), ld,
