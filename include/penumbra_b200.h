@@ -232,7 +232,8 @@ int pnb_lwe_contract_gather_ld(const int8_t* W_dev, const int64_t* bias_dev, uin
 #define PNB_MAX_EXPERTS 1024
 #define PNB_MAX_CHOICES (1 << 20) /* tokens * top_k of one call */
 #define PNB_MAX_RANK 64
-#define PNB_MAX_REQUEST_ROWS 524160 /* M of one call */
+#define PNB_MAX_REQUEST_ROWS 524160    /* M of one call */
+#define PNB_MAX_REQUEST_WORDS (1 << 20) /* lwe_len of one call */
 
 /* Rows sorted by expert.  ids int32 [tokens][top_k]; choice c = t*top_k + i is used when
  * 0 <= ids[c] < experts.  The used choices, by expert and then in choice order, are the rows:

@@ -479,9 +479,10 @@ static int check_route(const char* fn, int tokens, int top_k) {
 
 // Rows of `features` ciphertexts at two pitches.
 static int check_rows(const char* fn, int features, int lwe_len, int ld_in, int ld_out) {
-  if (features < 1 || lwe_len < 1 || ld_in < lwe_len || ld_out < lwe_len) {
-    set_error("%s: bad rows: %d ciphertexts of %d words at pitches %d and %d", fn, features,
-              lwe_len, ld_in, ld_out);
+  if (features < 1 || lwe_len < 1 || lwe_len > PNB_MAX_REQUEST_WORDS || ld_in < lwe_len ||
+      ld_out < lwe_len) {
+    set_error("%s: bad rows: %d ciphertexts of %d words (1..%d) at pitches %d and %d", fn, features,
+              lwe_len, PNB_MAX_REQUEST_WORDS, ld_in, ld_out);
     return PNB_ERR_INVALID;
   }
   return PNB_OK;

@@ -291,12 +291,8 @@ static int move_launch(MoveArgs a, cudaStream_t st) {
   const bool wide = a.ldi % 2 == 0 && a.ldo % 2 == 0 && ((uintptr_t)a.in % 16) == 0 &&
                     ((uintptr_t)a.out % 16) == 0;
   a.per_row = wide ? (a.L + 1) / 2 : a.L;
-  if (a.per_row > 1 << 20) {
-    set_error("%s: ciphertexts of %d words", COMBINE ? "expert_combine" : "expert_dispatch", a.L);
-    return PNB_ERR_INVALID;
-  }
-  // ceil(2^(32 + shift) / per_row) with 2^shift >= per_row / 2: exact for u < 2^21 (less than
-  // 2^20 into a ciphertext, and a run)
+  // ceil(2^(32 + shift) / per_row) with 2^shift >= per_row / 2: exact for u < 2^21 (at most
+  // PNB_MAX_REQUEST_WORDS into a ciphertext, and a run)
   a.shift = 0;
   while ((2 << a.shift) < a.per_row) ++a.shift;
   a.magic = (uint32_t)((((uint64_t)1 << (32 + a.shift)) + a.per_row - 1) / a.per_row);

@@ -382,6 +382,73 @@ def test_workspace_of_the_c_abi(pnb, oracle):
             assert np.all(host(out) == MARK)
 
 
+@pytest.mark.parametrize("ld", [44, 45])
+@pytest.mark.parametrize("x_off,y_off", [(0, 1), (1, 0), (1, 1)])
+def test_every_alignment_of_rows(pnb, oracle, ld, x_off, y_off):
+    # inputs, outputs or both start at an address that is only 8-byte aligned, at either pitch
+    rng = np.random.default_rng(16)
+    n, rank, M, K, L, batch = 2, 16, 20, 96, 43, 3
+    at = lambda off, *shape: torch.zeros(int(np.prod(shape)) + off, dtype=torch.int64,  # noqa: E731
+                                         device="cuda")[off:].view(*shape)
+    W = rng.integers(-128, 128, (2, M, K)).astype(np.int8)
+    A = rng.integers(-128, 128, (n, rank, K)).astype(np.int8)
+    B = rng.integers(-128, 128, (n, M, rank)).astype(np.int8)
+    X = words(rng, batch, K, ld)
+    which, ids = np.array([1, -1, 0], np.int32), np.array([[1], [0], [1]], np.int32)
+    Xd = at(x_off, batch, K, ld).copy_(dev(X))
+    bytes_at = lambda a: torch.zeros(a.size + 3, dtype=torch.int8, device="cuda")[3:].view(  # noqa: E731
+        *a.shape).copy_(dev(a))
+    for place in (dev, bytes_at):  # weights 16-byte aligned, and at odd addresses
+        out = at(y_off, batch, M, ld).fill_(MARK)
+        got = host(pnb.adapter_contract(place(W[0]), None, 0, place(A), place(B), dev(which), Xd, L,
+                                        base_shift=3, out=out))
+        assert np.array_equal(got[:, :, :L], plain_adapter(oracle, W[0], None, 0, A, B, which,
+                                                           X[:, :, :L], 3))
+        assert np.all(got[:, :, L:] == MARK)
+        out = at(y_off, batch, M, ld).fill_(MARK)
+        route = pnb.expert_route(dev(ids), 2)
+        got = host(pnb.expert_contract(route, place(W), None, 0, Xd, L, out=out))
+        assert np.array_equal(got[:, :, :L], plain_contract(oracle, ids, 2, W, None, 0, X[:, :, :L],
+                                                            False, np.zeros((3, M, L), np.uint64)))
+        assert np.all(got[:, :, L:] == MARK)
+    out = at(y_off, batch, K, ld).fill_(MARK)
+    got = host(pnb.expert_dispatch(route, Xd, L, out=out))
+    assert np.array_equal(got[:, :, :L], X[[1, 0, 2], :, :L]) and np.all(got[:, :, L:] == MARK)
+    back = at(x_off, batch, K, ld).fill_(MARK)
+    got = host(pnb.expert_combine(route, out, L, out=back))
+    assert np.array_equal(got[:, :, :L], X[:, :, :L]) and np.all(got[:, :, L:] == MARK)
+    assert pnb.device_status(0) == 0
+
+
+@pytest.mark.parametrize("M,K,rank,ld", [(600, 700, 64, 34), (600, 700, 64, 33), (1100, 130, 20, 34),
+                                         (260, 1500, 40, 34), (260, 1500, 40, 33), (128, 5000, 3, 34)])
+def test_shapes_whose_operands_do_not_stay(pnb, oracle, M, K, rank, ld):
+    # every way of sharing out a block's memory: weights kept or streamed, X kept for several tiles of
+    # rows or read again
+    rng = np.random.default_rng(M + K)
+    L, batch, n = 33, 40, 5
+    W = rng.integers(-128, 128, (n, M, K)).astype(np.int8)
+    A = rng.integers(-128, 128, (n, rank, K)).astype(np.int8)
+    B = rng.integers(-128, 128, (n, M, rank)).astype(np.int8)
+    X = torch.randint(-(1 << 63), (1 << 63) - 1, (batch, K, ld), device="cuda")
+    which = rng.integers(-1, n, batch).astype(np.int32)
+    ids = rng.integers(-1, n, (batch, 1)).astype(np.int32)
+    got = pnb.adapter_contract(dev(W[0]), None, 0, dev(A), dev(B), dev(which), X, L, base_shift=9)
+    rows = [0, 1, batch // 2, batch - 1]
+    Xh = host(X[rows])[:, :, :L]
+    want = plain_adapter(oracle, W[0], None, 0, A, B, which[rows], Xh, 9)
+    assert np.array_equal(host(got[rows])[:, :, :L], want)
+    route = pnb.expert_route(dev(ids), n)
+    got = pnb.expert_contract(route, dev(W), None, 0, X, L)
+    choice_row = route.choice_row.cpu().numpy()[:, 0]
+    for i, t in enumerate(rows):
+        if ids[t, 0] >= 0:
+            want = oracle.contract(W[ids[t, 0]].astype(np.int64), None, 0,
+                                   np.ascontiguousarray(Xh[i])[None])[0]
+            assert np.array_equal(host(got[choice_row[t]])[:, :L], want), t
+    assert pnb.device_status(0) == 0
+
+
 def test_strided_inputs(pnb):
     # tensors that are not contiguous are used as the values they hold
     rng = np.random.default_rng(15)

@@ -33,9 +33,9 @@ def test_route_refuses_null(pnb, hole):
 @pytest.mark.parametrize("fn", ["pnb_expert_dispatch", "pnb_expert_combine"])
 @pytest.mark.parametrize("change,text", [
     ({1: -1}, b"tokens=-1"), ({2: 0}, b"top_k=0"), ({5: 0}, b"0 ciphertexts"),
-    ({9: 0}, b"0 words"), ({6: 9}, b"pitches 9"), ({8: 9}, b"and 9"), ({0: NUL}, b"NULL"),
+    ({9: 0}, b" 0 words"), ({6: 9}, b"at pitches 9"), ({8: 9}, b"and 9"), ({0: NUL}, b"NULL"),
     ({4: NUL}, b"NULL"), ({7: NUL}, b"NULL"),
-    ({6: 1 << 22, 8: 1 << 22, 9: (1 << 21) + 1}, b"2097153 words"),
+    ({6: 1 << 22, 8: 1 << 22, 9: (1 << 20) + 1}, b"1048577 words"),
 ])
 def test_moves_refuse(pnb, fn, change, text):
     args = [P, 4, 2, NUL, P, 3, 10, P, 10, 10, NUL]
@@ -47,7 +47,8 @@ def test_moves_refuse(pnb, fn, change, text):
 @pytest.mark.parametrize("change,text", [
     ({2: -1}, b"tokens=-1"), ({3: 0}, b"top_k=0"), ({4: 0}, b"0 experts"),
     ({4: 2000}, b"2000 experts"), ({9: 0}, b"M=0"), ({9: 524161}, b"M=524161"), ({10: 0}, b"K=0"), ({10: 65537}, b"K=65537"),
-    ({12: 9}, b"pitches 9"), ({14: 9}, b"and 9"), ({15: 0}, b"0 words"), ({0: NUL}, b"NULL"),
+    ({12: 9}, b"at pitches 9"), ({14: 9}, b"and 9"), ({15: 0}, b" 0 words"),
+    ({12: 1 << 21, 14: 1 << 21, 15: (1 << 20) + 1}, b"1048577 words"), ({0: NUL}, b"NULL"),
     ({1: NUL}, b"NULL"), ({6: NUL}, b"NULL"), ({11: NUL}, b"NULL"), ({13: NUL}, b"NULL"),
 ])
 def test_contract_refuses(pnb, change, text):
@@ -61,7 +62,7 @@ def test_contract_refuses(pnb, change, text):
     ({3: -1}, b"base_shift=-1"), ({3: 64}, b"base_shift=64"), ({4: 0}, b"M=0"),
     ({4: 524161}, b"M=524161"), ({5: 0}, b"K=0"),
     ({5: 65537}, b"K=65537"), ({8: 0}, b"adapters=0"), ({9: 0}, b"rank=0"), ({9: 65}, b"rank=65"),
-    ({12: 9}, b"pitches 9"), ({14: 9}, b"and 9"), ({15: -1}, b"batch=-1"), ({16: 0}, b"0 words"),
+    ({12: 9}, b"at pitches 9"), ({14: 9}, b"and 9"), ({15: -1}, b"batch=-1"), ({16: 0}, b" 0 words"),
     ({0: NUL}, b"NULL"), ({6: NUL}, b"NULL"), ({7: NUL}, b"NULL"), ({10: NUL}, b"NULL"),
     ({11: NUL}, b"NULL"), ({13: NUL}, b"NULL"),
 ])
