@@ -652,9 +652,9 @@ def _want_words(name: str, X, lwe_len, device, shape):
     return _want(name, X, X.dtype, shape + (ld,), device), ld, lwe_len
 
 
-def _want_out(out, shape, device, lwe_len: int) -> torch.Tensor:
-    """The caller's buffer, checked, or a new one: zeros where the call leaves words behind
-    ``lwe_len``."""
+def _want_out(out, shape, device, lwe_len: int, X: torch.Tensor) -> torch.Tensor:
+    """The caller's buffer, checked and apart from the input ``X``, or a new one: zeros where the
+    call leaves words behind ``lwe_len``."""
     if out is None:
         make = torch.empty if shape[-1] == lwe_len else torch.zeros
         return make(shape, dtype=torch.int64, device=device)
@@ -663,6 +663,9 @@ def _want_out(out, shape, device, lwe_len: int) -> torch.Tensor:
     if out.shape != shape or out.device != device or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {tuple(shape)} tensor on {device}, got "
                          f"{tuple(out.shape)} on {out.device}")
+    a, b = out.data_ptr(), X.data_ptr()
+    if a < b + 8 * X.numel() and b < a + 8 * out.numel():
+        raise ValueError("out overlaps the input's memory")
     return out
 
 
@@ -744,7 +747,7 @@ def expert_dispatch(route: ExpertRoute, X: torch.Tensor, lwe_len: int | None = N
     X, ld, L = _want_words("X", X, lwe_len, route.device, (route.tokens, None))
     F = X.shape[1]
     w = _route_weights(route, weights)
-    out = _want_out(out, (route.rows, F, ld), route.device, L)
+    out = _want_out(out, (route.rows, F, ld), route.device, L, X)
     _launch("pnb_expert_dispatch", route.device, route.choice_row.data_ptr(), route.tokens,
             route.top_k, _at(w), X.data_ptr(), F, ld, out.data_ptr(), ld, L)
     return out
@@ -759,7 +762,7 @@ def expert_combine(route: ExpertRoute, Y: torch.Tensor, lwe_len: int | None = No
     Y, ld, L = _want_words("Y", Y, lwe_len, route.device, (route.rows, None))
     F = Y.shape[1]
     w = _route_weights(route, weights)
-    out = _want_out(out, (route.tokens, F, ld), route.device, L)
+    out = _want_out(out, (route.tokens, F, ld), route.device, L, Y)
     _launch("pnb_expert_combine", route.device, route.choice_row.data_ptr(), route.tokens,
             route.top_k, _at(w), Y.data_ptr(), F, ld, out.data_ptr(), ld, L)
     return out
@@ -781,7 +784,7 @@ def expert_contract(route: ExpertRoute, W: torch.Tensor, bias: torch.Tensor | No
                            (route.rows if sorted_rows else route.tokens, K))
     W = _want("W", W, torch.int8, (route.experts, M, K), device)
     b = None if bias is None else _want("bias", bias, torch.int64, (E, M), device)
-    out = _want_out(out, (route.rows, M, ld), device, L)
+    out = _want_out(out, (route.rows, M, ld), device, L, X)
     need = _padded(W, E * M, K)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch("pnb_expert_contract", device, route.row_choice.data_ptr(),
@@ -813,7 +816,7 @@ def adapter_contract(W: torch.Tensor, bias: torch.Tensor | None, delta: int, A: 
     B = _want("B", B, torch.int8, (n, M, rank), device)
     adapter = _want("adapter", adapter, torch.int32, (batch,), device)
     b = None if bias is None else _want("bias", bias, torch.int64, (M,), device)
-    out = _want_out(out, (batch, M, ld), device, L)
+    out = _want_out(out, (batch, M, ld), device, L, X)
     need = _padded(W, M, K) + _padded(A, n * rank, K) + _padded(B, n * M, rank)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch("pnb_adapter_contract", device, W.data_ptr(), _at(b), delta % (1 << 64), base_shift, M, K,

@@ -1,4 +1,5 @@
 // capi.cu -- the extern "C" entry points declared in include/penumbra_b200.h.
+#include <initializer_list>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -496,6 +497,23 @@ static int check_weights(const char* fn, int M, int K) {
   return PNB_OK;
 }
 
+// Addresses of words and of 32-bit indices that those types cannot have: the tiled loads round
+// them down, so they must not get there.
+static int check_aligned(const char* fn, std::initializer_list<const void*> words,
+                         std::initializer_list<const void*> indices) {
+  for (const void* p : words)
+    if ((uintptr_t)p % 8) {
+      set_error("%s: 64-bit words at %p", fn, p);
+      return PNB_ERR_INVALID;
+    }
+  for (const void* p : indices)
+    if ((uintptr_t)p % 4) {
+      set_error("%s: 32-bit integers at %p", fn, p);
+      return PNB_ERR_INVALID;
+    }
+  return PNB_OK;
+}
+
 int pnb_expert_route(const int32_t* ids_dev, int tokens, int top_k, int experts,
                      int32_t* offsets_dev, int32_t* row_choice_dev, int32_t* row_expert_dev,
                      int32_t* choice_row_dev, void* stream) {
@@ -510,6 +528,9 @@ int pnb_expert_route(const int32_t* ids_dev, int tokens, int top_k, int experts,
     set_error("expert_route: NULL buffer");
     return PNB_ERR_INVALID;
   }
+  rc = check_aligned("expert_route", {},
+                     {ids_dev, offsets_dev, row_choice_dev, row_expert_dev, choice_row_dev});
+  if (rc) return rc;
   return expert_route(ids_dev, tokens * top_k, experts, offsets_dev, row_choice_dev,
                       row_expert_dev, choice_row_dev, (cudaStream_t)stream);
 }
@@ -525,6 +546,8 @@ int pnb_expert_dispatch(const int32_t* choice_row_dev, int tokens, int top_k,
     set_error("expert_dispatch: NULL buffer");
     return PNB_ERR_INVALID;
   }
+  rc = check_aligned("expert_dispatch", {X_dev, out_dev}, {choice_row_dev, weights_dev});
+  if (rc) return rc;
   return expert_dispatch(choice_row_dev, tokens, top_k, weights_dev, X_dev, features, ldx, out_dev,
                          ldo, lwe_len, (cudaStream_t)stream);
 }
@@ -540,6 +563,8 @@ int pnb_expert_combine(const int32_t* choice_row_dev, int tokens, int top_k,
     set_error("expert_combine: NULL buffer");
     return PNB_ERR_INVALID;
   }
+  rc = check_aligned("expert_combine", {Y_dev, out_dev}, {choice_row_dev, weights_dev});
+  if (rc) return rc;
   return expert_combine(choice_row_dev, tokens, top_k, weights_dev, Y_dev, features, ldy, out_dev,
                         ldo, lwe_len, (cudaStream_t)stream);
 }
@@ -562,6 +587,8 @@ int pnb_expert_contract(const int32_t* row_choice_dev, const int32_t* row_expert
     set_error("expert_contract: NULL buffer");
     return PNB_ERR_INVALID;
   }
+  rc = check_aligned("expert_contract", {bias_dev, X_dev, Y_dev}, {row_choice_dev, row_expert_dev});
+  if (rc) return rc;
   return expert_contract(row_choice_dev, row_expert_dev, tokens, top_k, experts, sorted_rows != 0,
                          W_dev, bias_dev, delta, M, K, X_dev, ldx, Y_dev, ldy, lwe_len, workspace,
                          workspace_bytes, (cudaStream_t)stream);
@@ -600,6 +627,8 @@ int pnb_adapter_contract(const int8_t* W_dev, const int64_t* bias_dev, uint64_t 
     set_error("adapter_contract: NULL buffer");
     return PNB_ERR_INVALID;
   }
+  rc = check_aligned("adapter_contract", {bias_dev, X_dev, Y_dev}, {adapter_dev});
+  if (rc) return rc;
   return adapter_contract(W_dev, bias_dev, delta, base_shift, M, K, A_dev, B_dev, adapters, rank,
                           adapter_dev, X_dev, ldx, Y_dev, ldy, batch, lwe_len, workspace,
                           workspace_bytes, (cudaStream_t)stream);

@@ -494,6 +494,16 @@ def test_binding_refusals(pnb):
                  lambda: pnb.adapter_contract(W[0], None, 0, W, W.mT, torch.zeros(3, **i32), X)):
         with pytest.raises(ValueError):
             call()
+    one = pnb.expert_route(torch.zeros(4, 1, **i32), 3)
+    buf = torch.zeros(5, 5, 10, dtype=torch.int64, device="cuda")
+    for call in (lambda: pnb.expert_dispatch(one, X, out=X),
+                 lambda: pnb.expert_combine(one, buf[:4], out=buf[1:]),
+                 lambda: pnb.expert_contract(one, torch.zeros(3, 5, 5, **i8), None, 0, buf[1:],
+                                             out=buf[:4]),
+                 lambda: pnb.adapter_contract(torch.zeros(5, 5, **i8), None, 0, W[:, :2], W[:, :5, :2],
+                                              torch.zeros(4, **i32), X, out=X)):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
     with pytest.raises(TypeError, match="int8"):
         pnb.expert_contract(route, W.int(), None, 0, X)
     with pytest.raises(pnb.LibraryError, match="rank"):
@@ -562,6 +572,106 @@ def test_captured_and_replayed(pnb):
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(outs[i][:, :, :301], want[i][1 if rep else 0]), (rep, i)
+
+
+def test_large_route_captured_and_replayed(pnb):  # several blocks, and more shared memory than usual
+    rng = np.random.default_rng(23)
+    T, k, E = 3000, 2, 700
+    ids = [draw_ids(rng, T, k, E, 0.2) for _ in range(2)]
+    at = dev(ids[0])
+    route = pnb.expert_route(at, E)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        pnb.expert_route(at, E, out=route)
+    for want in ids[::-1]:
+        at.copy_(dev(want))
+        g.replay()
+        torch.cuda.synchronize()
+        for name, w in zip(("offsets", "row_choice", "row_expert", "choice_row"),
+                           plain_route(want, E)):
+            assert np.array_equal(getattr(route, name).cpu().numpy(), w), name
+
+
+# ---- sizes past 32 bits -------------------------------------------------------------------------
+@pytest.fixture
+def room():
+    torch.cuda.empty_cache()
+    yield
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("ld", [1026, 1025])
+def test_inputs_past_32_bit_offsets(pnb, oracle, room, ld):
+    # 67 requests of the longest K: 4.5e9 words; the first, and the last two, hold something
+    rng = np.random.default_rng(41)
+    batch, K, M, L, rank = 67, 65536, 3, 1025, 2
+    X = torch.empty(batch, K, ld, dtype=torch.int64, device="cuda")
+    assert X.numel() > 1 << 32
+    rows = [0, batch - 2, batch - 1]
+    for b in rows:
+        X[b] = torch.randint(-(1 << 63), (1 << 63) - 1, (K, ld), device="cuda")
+    W = rng.integers(-128, 128, (2, M, K)).astype(np.int8)
+    A = rng.integers(-128, 128, (2, rank, K)).astype(np.int8)
+    B = rng.integers(-128, 128, (2, M, rank)).astype(np.int8)
+    ids = np.full((batch, 1), -1, np.int32)
+    which = np.full(batch, -1, np.int32)
+    ids[rows, 0], which[rows] = [1, 0, 1], [1, -1, 0]
+    route = pnb.expert_route(dev(ids), 2)
+    y = host(pnb.expert_contract(route, dev(W), None, 0, X, L)[:3])
+    z = host(pnb.adapter_contract(dev(W[0]), None, 0, dev(A), dev(B), dev(which), X, L)[rows])
+    for i, b in enumerate(rows):
+        x = np.ascontiguousarray(host(X[b])[:, :L])[None]
+        at = route.choice_row[b, 0].item()
+        assert np.array_equal(y[at, :, :L], oracle.contract(W[ids[b, 0]].astype(np.int64), None, 0,
+                                                            x)[0])
+        assert np.array_equal(z[i, :, :L], plain_adapter(oracle, W[0], None, 0, A, B, which[b:b + 1],
+                                                         x, 0)[0])
+    assert pnb.device_status(0) == 0
+
+
+@pytest.mark.parametrize("ld", [1026, 1025])
+def test_outputs_past_32_bit_offsets(pnb, oracle, room, ld):
+    rng = np.random.default_rng(42)
+    M, K, L, batch = 262144, 32, 1025, 17
+    W = rng.integers(-128, 128, (M, K)).astype(np.int8)
+    A, B = np.zeros((1, 1, K), np.int8), np.zeros((1, M, 1), np.int8)
+    which = np.full(batch, -1, np.int32)
+    X = words(rng, batch, K, ld)
+    y = pnb.adapter_contract(dev(W), None, 0, dev(A), dev(B), dev(which), dev(X), L)
+    assert y.numel() > 1 << 32
+    pick = np.array([0, 1, 131071, M - 129, M - 1])
+    got = host(y[-1][torch.tensor(pick, device="cuda")])[:, :L]
+    assert np.array_equal(got, oracle.contract(W[pick].astype(np.int64), None, 0,
+                                               np.ascontiguousarray(X[-1:, :, :L]))[0])
+    # the same rows moved: one token in, one row out, and back
+    route = pnb.expert_route(torch.zeros(1, 1, dtype=torch.int32, device="cuda"), 1)
+    whole = y.view(1, batch * M, ld)
+    moved = pnb.expert_dispatch(route, whole, L)
+    assert torch.equal(moved[0, -M:, :L], y[-1, :, :L])
+    assert torch.equal(moved[0, :M, :L], y[0, :, :L])
+    back = pnb.expert_combine(route, moved, L, out=whole.zero_())
+    assert torch.equal(back[0, -M:, :L], moved[0, -M:, :L])
+    assert pnb.device_status(0) == 0
+
+
+@pytest.mark.parametrize("K", [65536, 65535])  # read in place, and padded in the workspace
+def test_weights_past_32_bit_offsets(pnb, oracle, room, K):
+    rng = np.random.default_rng(43)
+    E, M, L = 1024, 65, 33
+    W = torch.empty(E, M, K, dtype=torch.int8, device="cuda")
+    assert W.numel() > 1 << 32
+    for e in (0, 511, E - 1):
+        W[e] = torch.randint(-128, 128, (M, K), device="cuda", dtype=torch.int8)
+    ids = np.array([[E - 1], [0], [511]], np.int32)
+    X = words(rng, 3, K, L + 1)
+    route = pnb.expert_route(dev(ids), E)
+    got = host(pnb.expert_contract(route, W, None, 0, dev(X), L))
+    for r, (t, e) in enumerate([(1, 0), (2, 511), (0, E - 1)]):
+        want = oracle.contract(W[e].cpu().numpy().astype(np.int64), None, 0,
+                               np.ascontiguousarray(X[t:t + 1, :, :L]))[0]
+        assert np.array_equal(got[r, :, :L], want), e
+    assert pnb.device_status(0) == 0
 
 
 # ---- the operators together, as they are used ----------------------------------------------------

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 P = C.c_void_p(4096)  # never dereferenced: every call here is refused on the host
+ODD4, ODD2 = C.c_void_p(4100), C.c_void_p(4098)
 NUL = C.c_void_p(0)
 
 
@@ -28,6 +29,22 @@ def test_route_refuses_null(pnb, hole):
     args = [P, 4, 2, 4, P, P, P, P, NUL]
     args[hole] = NUL
     _refused(pnb, pnb.lib().pnb_expert_route(*args), b"NULL")
+
+
+@pytest.mark.parametrize("fn,args,words,indices", [
+    ("pnb_expert_route", [P, 4, 2, 4, P, P, P, P, NUL], (), (0, 4, 5, 6, 7)),
+    ("pnb_expert_dispatch", [P, 4, 2, P, P, 3, 10, P, 10, 10, NUL], (4, 7), (0, 3)),
+    ("pnb_expert_combine", [P, 4, 2, P, P, 3, 10, P, 10, 10, NUL], (4, 7), (0, 3)),
+    ("pnb_expert_contract", [P, P, 4, 2, 4, 0, P, P, 1, 3, 5, P, 10, P, 10, 10, NUL, 0, NUL],
+     (7, 11, 13), (0, 1)),
+    ("pnb_adapter_contract", [P, P, 1, 0, 3, 5, P, P, 2, 2, P, P, 10, P, 10, 4, 10, NUL, 0, NUL],
+     (1, 11, 13), (10,)),
+])
+def test_misaligned_addresses_are_refused(pnb, fn, args, words, indices):
+    for i in words:
+        _refused(pnb, getattr(pnb.lib(), fn)(*args[:i], ODD4, *args[i + 1:]), b"64-bit words")
+    for i in indices:
+        _refused(pnb, getattr(pnb.lib(), fn)(*args[:i], ODD2, *args[i + 1:]), b"32-bit integers")
 
 
 @pytest.mark.parametrize("fn", ["pnb_expert_dispatch", "pnb_expert_combine"])
