@@ -89,9 +89,11 @@ struct RqShape {
   static constexpr int RAW_PER_X = XK / RQ_RAW_ROWS;
   static constexpr int EW = WORDS / 2;                 // words per epilogue warp
   static constexpr int OUT = 32 * EW * 8;              // its staging: 32 rows
+  static constexpr bool MAY_SPLIT = !SHIFTED && !ADAPT;  // which may be done in two parts
   static constexpr int COPY = SHIFTED ? RQ_COPY_WARPS : 0;
   static constexpr int MMA_WARP = 2 + COPY;            // warp 0 loads X, warp 1 the weights
-  static constexpr int EPI_WARP = MMA_WARP + (ADAPT ? 2 : 1);  // the low product has its own warp
+  static constexpr int MMA_WARPS = SHIFTED ? 1 : 2;    // two: one per accumulator
+  static constexpr int EPI_WARP = MMA_WARP + MMA_WARPS + (ADAPT ? 1 : 0);  // (the low product's)
   static constexpr int THREADS = 32 * (EPI_WARP + RQ_EPI_WARPS);
 };
 
@@ -114,6 +116,7 @@ struct RqArgs {
   int n_tiles, m_tiles, m_group;  // tiles of 128 rows that share one load of X
   int groups;                 // of m_group tiles in one row
   int w_slots, x_slots, raw_slots;
+  int out_split;              // results are staged, and leave, in two parts
   int keep_w;                 // the group's weights stay for the next group that uses them
   int x_at, raw_at, a_at, b_at, t_at, out_at, bars_at;  // shared-memory offsets; weights at 0
 };
@@ -256,13 +259,17 @@ __device__ __forceinline__ uint64_t add_limbs(uint64_t v, const uint32_t* c) {
   return ((uint64_t)hi << 32) | (uint32_t)s;
 }
 
-template <bool SHIFTED, bool ADAPT>
+template <bool SHIFTED, bool ADAPT, bool SPLIT>
 __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     request_kernel(const __grid_constant__ RqMaps tm, const __grid_constant__ RqArgs a) {
   using S = RqShape<SHIFTED, ADAPT>;
-  extern __shared__ unsigned char rq_raw[];
-  const uint32_t raw = tc::smem_u32(rq_raw);
-  const uint32_t base = (raw + 1023u) & ~1023u;
+  // the swizzles want 1024-byte boundaries; aligning by hand instead would cost 1 KB
+  extern __shared__ __align__(1024) unsigned char rq_raw[];
+  const uint32_t raw = tc::smem_u32(rq_raw), base = raw;
+  if (raw & 1023u) {
+    if (threadIdx.x == 0) atomicExch(&g_rq_status, 1);
+    return;
+  }
   const int a_slot = a.rank16 * RQ_WK;  // A's rows beside one X slot
   auto w_at = [&](int s) { return base + (uint32_t)(s * RQ_W_SLOT); };
   auto x_at = [&](int s) { return base + (uint32_t)(a.x_at + s * S::X_SLOT); };
@@ -286,14 +293,17 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   uint4* lists = reinterpret_cast<uint4*>(rq_raw + (bars - raw) + RQ_LIST_AT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  // adapters with one tile to a group: the second warp's answers cost what its share would gain
+  const int mma_warps = ADAPT && a.m_group == 1 ? 1 : S::MMA_WARPS;
+
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.w_slots; ++s) {
       tc::mbar_init(w_full + 8 * s, 1);
-      tc::mbar_init(w_empty + 8 * s, 1);
+      tc::mbar_init(w_empty + 8 * s, mma_warps);
     }
     for (int s = 0; s < a.x_slots; ++s) {
       tc::mbar_init(x_full + 8 * s, SHIFTED ? S::RAW_PER_X + (ADAPT ? 1 : 0) : 1);
-      tc::mbar_init(x_empty + 8 * s, ADAPT ? 2 : 1);
+      tc::mbar_init(x_empty + 8 * s, mma_warps + (ADAPT ? 1 : 0));
     }
     for (int s = 0; s < a.raw_slots; ++s) {
       tc::mbar_init(r_full + 8 * s, 1);
@@ -512,24 +522,31 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       return true;
     });
     if (ADAPT && cw == 0 && lane == 0) rq_drain(x_full, xr, x_wrap, a.x_slots);
-  } else if (warp == S::MMA_WARP) {
-    // ---------------- main products (one lane) --------------------------------------------------
-    // Issuing one MMA takes a thread about as long as the tensor cores take to run it, and every
-    // branch between them counts, so this loop is kept short and the low products have a thread of
-    // their own.
+  } else if (warp < S::MMA_WARP + S::MMA_WARPS) {
+    // ---------------- main products (one lane of each warp) --------------------------------------
+    // Tiles alternate between two warps, each with an accumulator of its own: waiting for a slot,
+    // issuing its MMAs and letting it go takes a thread longer than the tensor cores take to run
+    // them, the more so between tiles, so one thread's bookkeeping hides behind the other's MMAs.
+    // Either answers for every slot, also those of tiles that are not its own: a parity tells only
+    // neighbouring uses apart.
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, S::BN, true, false, false, true);
       constexpr int STEPS = S::XK / RQ_KSTEP;
+      constexpr int W_STEPS = RQ_WK / RQ_KSTEP;
       const uint64_t wd = tc::smem_desc_sw128(w_at(0), 16u, 1024u);
       const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
       const uint32_t w_hi = (uint32_t)(wd >> 32), x_hi = (uint32_t)(xd >> 32);
       const int steps = (a.K + RQ_KSTEP - 1) / RQ_KSTEP;  // MMAs of one tile
       const int x_slots = a.x_slots, w_slots = a.w_slots;
       const bool keep_w = a.keep_w != 0;
+      const int me = warp - S::MMA_WARP;
       RqRing x;
-      int tt = 0, w_slot = 0;
+      int w_slot = 0;
       uint32_t w_par = 0;
-      int unreleased = 0;  // weight slots kept for a group that has not come
+      int tt = 0;  // tiles of this warp
+      const bool turns = mma_warps == 2;
+      bool mine = me == 0;  // the next tile
+      int unreleased = 0;   // weight slots kept for a group that has not come
       // One tile.  Those whose weights are there and stay (kept), whose X nobody else uses (alone), and
       // both, are compiled apart, without the branches that ask.
       using yes = std::true_type;
@@ -537,10 +554,11 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       auto tile = [&](auto kept, auto alone, bool load, bool drop, bool first, bool last) {
         if (kept) load = drop = false;
         if (alone) first = last = true;
-        // accumulators in turn: experts C in 256 columns each; adapters C in 128 columns each
-        const uint32_t turn = 8u * (uint32_t)(tt & 1);
-        const uint32_t c_tmem = tmem + (uint32_t)((tt & 1) * S::BN);
-        if (!rq_wait(acc_empty + turn, (uint32_t)(tt >> 1) ^ 1u, abort_s)) return false;
+        const int buf = turns ? me : tt & 1;
+        const uint32_t c_tmem = tmem + (uint32_t)(buf * S::BN);
+        if (!rq_wait(acc_empty + 8 * buf, (uint32_t)(turns ? tt : tt >> 1) ^ 1u, abort_s))
+          return false;
+        ++tt;
         tc::tc_fence_after();  // (operands in shared memory need none: their mbarriers order them)
         uint32_t acc = 0;
         auto slot = [&](uint32_t w_lo, int n, bool whole) {  // n MMAs of one X slot
@@ -555,7 +573,6 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           x.advance(x_slots);
           return true;
         };
-        constexpr int W_STEPS = RQ_WK / RQ_KSTEP;
         for (int left = steps; left > 0; left -= W_STEPS) {  // one weight slot: 128 of K
           if (load) {
             if (!rq_wait(w_full + 8 * w_slot, w_par >> w_slot, abort_s)) return false;
@@ -573,11 +590,34 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           if (drop) tc::mma_commit(w_empty + 8 * w_slot);
           if (++w_slot == w_slots) w_slot = 0;
         }
-        tc::mma_commit(acc_full + turn);
-        ++tt;
+        tc::mma_commit(acc_full + 8 * buf);
+        return true;
+      };
+      // A tile of the other warp: its weight slots, and (alone) its X slots, in its order.
+      auto skip = [&](bool load, bool drop, bool alone) {
+        for (int left = steps; left > 0; left -= W_STEPS) {
+          if (load) {
+            if (!rq_wait(w_full + 8 * w_slot, w_par >> w_slot, abort_s)) return false;
+            w_par ^= 1u << w_slot;
+          }
+          if (drop) {
+            if (keep_w)
+              tc::mma_commit(w_empty + 8 * w_slot);  // earlier groups' MMAs may still read it
+            else
+              tc::mbar_arrive(w_empty + 8 * w_slot);
+          }
+          if (++w_slot == w_slots) w_slot = 0;
+          if (!alone) continue;
+          for (int h = 0; h < left && h < W_STEPS; h += STEPS) {
+            if (!rq_wait(x_full + 8 * x.slot, x.phase, abort_s)) return false;
+            tc::mbar_arrive(x_empty + 8 * x.slot);
+            x.advance(x_slots);
+          }
+        }
         return true;
       };
       each(true, [&](const RqGroup& g) {
+        if (me >= mma_warps) return true;
         const int m_n = tiles(g.mg);
         if (g.load)
           for (int s = 0; s < unreleased; ++s) tc::mma_commit(w_empty + 8 * s);
@@ -585,20 +625,29 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         unreleased = g.drop ? 0 : m_n * kb_n;
         if (keep_w) w_slot = 0;
         const bool kept = !g.load && !g.drop;
+        const bool own = mine;
+        if (turns && (m_n & 1)) mine = !mine;
         if (m_n == 1)
-          return kept ? tile(yes{}, yes{}, false, false, true, true)
-                      : tile(no{}, yes{}, g.load, g.drop, true, true);
+          return !own   ? skip(g.load, g.drop, true)
+                 : kept ? tile(yes{}, yes{}, false, false, true, true)
+                        : tile(no{}, yes{}, g.load, g.drop, true, true);
         const RqRing x0 = x;
+        const int m0 = own ? 0 : 1;
         for (int m = 0; m < m_n; ++m) {
+          if (turns && ((m ^ m0) & 1)) {
+            if (!skip(g.load, g.drop, false)) return false;
+            continue;
+          }
           x = x0;
-          if (!(kept ? tile(yes{}, no{}, false, false, m == 0, m == m_n - 1)
-                     : tile(no{}, no{}, g.load, g.drop, m == 0, m == m_n - 1)))
+          const bool first = m == m0, last = m + mma_warps >= m_n;
+          if (!(kept ? tile(yes{}, no{}, false, false, first, last)
+                     : tile(no{}, no{}, g.load, g.drop, first, last)))
             return false;
         }
         return true;
       });
     }
-  } else if (ADAPT && warp == S::MMA_WARP + 1) {
+  } else if (ADAPT && warp == S::MMA_WARP + S::MMA_WARPS) {
     // ---------------- low products L^T = X^T A^T and D = B t (one lane) --------------------------
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, S::BN, true, false, false, true);
@@ -692,11 +741,14 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     // the row, and leave as 32 rows x EW words by TMA, or as row segments by plain stores.
     const int e_w = warp - S::EPI_WARP;
     const int q = warp & 3, eh = e_w >> 2;
-    constexpr int EW = S::EW, PITCH = EW * 8, CHUNKS = EW / 4;
-    const uint32_t out_at = base + (uint32_t)(a.out_at + e_w * S::OUT);
+    constexpr int EW = S::EW, CHUNKS = EW / 4;
+    constexpr int PARTS = SPLIT ? 2 : 1, PITCH = EW * 8 / PARTS;  // staged one after the other
+    const uint32_t out_at = base + (uint32_t)(a.out_at + e_w * (S::OUT / PARTS));
     unsigned char* out = rq_raw + (out_at - raw);
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
-    auto xored = [](int row) { return PITCH == 128 ? row & 7 : (row >> 1) & 3; };
+    auto xored = [](int row) { return PITCH == 128 ? row & 7 : (row >> 1) & 3; };  // its swizzle
+    unsigned char* out_row = out + lane * PITCH;
+    const int out_x = xored(lane);
     int tt = 0;
     uint32_t low_par = 0;
     bool ok = true;
@@ -794,28 +846,33 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
 #pragma unroll
             for (int u = 0; u < 4; ++u) y[u] = add_limbs(y[u], d + 8 * u);
           }
-          if (!SHIFTED && i == 0) {  // the staging rows of the previous tile have left
+          constexpr int STAGED = CHUNKS / PARTS;
+          const int c2 = 2 * (i % STAGED);
+          if (!SHIFTED && c2 == 0) {  // what was staged before has left
             if (lane == 0) tc::tma_store_wait_read();
             __syncwarp();
           }
-          *reinterpret_cast<ulonglong2*>(out + lane * PITCH + (((2 * i) ^ xored(lane)) << 4)) =
-              make_ulonglong2(y[0], y[1]);
-          *reinterpret_cast<ulonglong2*>(out + lane * PITCH + (((2 * i + 1) ^ xored(lane)) << 4)) =
+          *reinterpret_cast<ulonglong2*>(out_row + ((c2 ^ out_x) << 4)) = make_ulonglong2(y[0], y[1]);
+          *reinterpret_cast<ulonglong2*>(out_row + (((c2 + 1) ^ out_x) << 4)) =
               make_ulonglong2(y[2], y[3]);
+          if ((i + 1) % STAGED != 0) continue;
+          const int w0 = (i + 1 - STAGED) * 4;  // the first staged word
+          if (body >= w0 && body < (i + 1) * 4) {
+            uint64_t* p = reinterpret_cast<uint64_t*>(
+                out_row + ((((body - w0) >> 1) ^ out_x) << 4) + (body & 1) * 8);
+            *p += bias;
+            // tiled stores end on 16-byte boundaries, so the last word of an odd count goes alone
+            if (!SHIFTED && (a.L & 1) && row0 + lane < a.M)
+              a.Y[((size_t)g.n * a.M + row0 + lane) * a.ldy + a.L - 1] = *p;
+          }
+          if (!SHIFTED) {
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && col0 + w0 < (a.L & ~1))
+              tc::tma_store_3d(&tm.Y, col0 + w0, row0, g.n, out_at);
+          }
         }
-        if (body < EW) {
-          uint64_t* p = reinterpret_cast<uint64_t*>(
-              out + lane * PITCH + (((body >> 1) ^ xored(lane)) << 4) + (body & 1) * 8);
-          *p += bias;
-          // tiled stores end on 16-byte boundaries, so the last word of an odd count goes alone
-          if (!SHIFTED && (a.L & 1) && row0 + lane < a.M)
-            a.Y[((size_t)g.n * a.M + row0 + lane) * a.ldy + a.L - 1] = *p;
-        }
-        if (!SHIFTED) {
-          tc::fence_async_smem();
-          __syncwarp();
-          if (lane == 0 && col0 < (a.L & ~1)) tc::tma_store_3d(&tm.Y, col0, row0, g.n, out_at);
-        } else {
+        if (SHIFTED) {
           __syncwarp();
           constexpr int PER = 32 / EW;  // rows per instruction
           const int wd = lane % EW;
@@ -944,8 +1001,8 @@ static void rq_plan(RqArgs& a, int sms) {
   const int t_bytes = ADAPT ? rank32 * S::BN : 0;
   const int b_bytes = ADAPT ? RQ_B_SLOTS * RQ_B_SLOT : 0;
   const int a_slot = ADAPT ? a.rank16 * RQ_WK : 0;  // beside each X slot
-  const int out_bytes = RQ_EPI_WARPS * S::OUT;
-  int room = RQ_SMEM - 1024 - RQ_BAR_BYTES - t_bytes - b_bytes - out_bytes;
+  int out_bytes = RQ_EPI_WARPS * S::OUT;
+  int room = RQ_SMEM - RQ_BAR_BYTES - t_bytes - b_bytes - out_bytes;
   // what X wants at least before weights may stay: four slots (shifted: three and 40 KB of raw
   // rows); for adapters, whose weights would come twice as often, three (two and 32 KB).  256 rows
   // of 784->128: one slot less costs experts at an odd pitch 928 -> 1065 us by letting the weights
@@ -969,6 +1026,11 @@ static void rq_plan(RqArgs& a, int sms) {
         std::min(RQ_MAX_RAW, (room - a.x_slots * (S::X_SLOT + a_slot)) / S::RAW_SLOT & ~3);
   } else {
     a.x_slots = std::min(RQ_MAX_X, room / (S::X_SLOT + a_slot));
+    if (S::MAY_SPLIT && a.x_slots < 6) {
+      a.out_split = 1;
+      out_bytes /= 2;
+      a.x_slots = (room + out_bytes) / S::X_SLOT;
+    }
     a.raw_slots = 0;
   }
   a.x_at = a.w_slots * RQ_W_SLOT;
@@ -980,30 +1042,42 @@ static void rq_plan(RqArgs& a, int sms) {
   a.bars_at = a.raw_at + a.raw_slots * S::RAW_SLOT;
 }
 
+// What the device needs once (its number of SMs read, the kernel's shared-memory limit raised), and
+// the plan.
 template <bool SHIFTED, bool ADAPT>
-static int rq_launch(const RqMaps& tm, RqArgs a, cudaStream_t st) {
-  using S = RqShape<SHIFTED, ADAPT>;
-  // what a device needs once: its number of SMs, and this kernel's shared-memory limit raised
+static int rq_prepare(RqArgs& a, int& sms) {
   static std::atomic<int> sm_count[64];
-  int dev = 0, sms = 0;
+  int dev = 0;
   PNB_CUDA(cudaGetDevice(&dev));
-  if (dev < 64) sms = sm_count[dev].load(std::memory_order_acquire);
+  sms = dev < 64 ? sm_count[dev].load(std::memory_order_acquire) : 0;
   if (sms == 0) {
     PNB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    PNB_CUDA(cudaFuncSetAttribute(request_kernel<SHIFTED, ADAPT>,
+    PNB_CUDA(cudaFuncSetAttribute(request_kernel<SHIFTED, ADAPT, false>,
                                   cudaFuncAttributeMaxDynamicSharedMemorySize, RQ_SMEM));
+    if (RqShape<SHIFTED, ADAPT>::MAY_SPLIT)
+      PNB_CUDA(cudaFuncSetAttribute(
+          request_kernel<SHIFTED, ADAPT, RqShape<SHIFTED, ADAPT>::MAY_SPLIT>,
+          cudaFuncAttributeMaxDynamicSharedMemorySize, RQ_SMEM));
     if (dev < 64) sm_count[dev].store(sms, std::memory_order_release);
   }
   rq_plan<SHIFTED, ADAPT>(a, sms);
   a.groups = (a.m_tiles + a.m_group - 1) / a.m_group;
-  if (a.groups >= 1 << RQ_MG_BITS || (long long)a.groups * a.n_tiles >= 1 << RQ_NT_BITS) {
-    set_error("%s: %d x %d tiles of one row exceed one launch",
-              ADAPT ? "adapter_contract" : "expert_contract", a.groups, a.n_tiles);
-    return PNB_ERR_INVALID;
-  }
+  if (a.groups < 1 << RQ_MG_BITS && (long long)a.groups * a.n_tiles < 1 << RQ_NT_BITS) return PNB_OK;
+  set_error("%s: %d x %d tiles of one row exceed one launch",
+            ADAPT ? "adapter_contract" : "expert_contract", a.groups, a.n_tiles);
+  return PNB_ERR_INVALID;
+}
+
+template <bool SHIFTED, bool ADAPT>
+static int rq_launch(const RqMaps& tm, const RqArgs& a, int sms, cudaStream_t st) {
+  using S = RqShape<SHIFTED, ADAPT>;
   const int grid = (int)std::min<long long>((long long)a.rows * a.groups * a.n_tiles, sms);
-  request_kernel<SHIFTED, ADAPT>
-      <<<grid, S::THREADS, 1024 + a.bars_at + RQ_BAR_BYTES, st>>>(tm, a);
+  if (a.out_split)
+    request_kernel<SHIFTED, ADAPT, S::MAY_SPLIT>
+        <<<grid, S::THREADS, a.bars_at + RQ_BAR_BYTES, st>>>(tm, a);
+  else
+    request_kernel<SHIFTED, ADAPT, false>
+        <<<grid, S::THREADS, a.bars_at + RQ_BAR_BYTES, st>>>(tm, a);
   PNB_CHECK_LAUNCH("request_kernel");
   return PNB_OK;
 }
@@ -1029,7 +1103,9 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
   a.off1 = (int)((xw + (uintptr_t)ldx) & 1);
   const bool shifted = a.off0 || a.off1 || a.ldy % 2 != 0 || ((uintptr_t)a.Y % 16) != 0;
   RqMaps tm{};
-  int rc = PNB_OK;
+  int sms = 0;
+  int rc = shifted ? rq_prepare<true, ADAPT>(a, sms) : rq_prepare<false, ADAPT>(a, sms);
+  if (rc) return rc;
   if (!shifted) {
     const uint64_t pitch = (uint64_t)ldx * 8;
     rc = rq_map_bytes(&tm.X[0], X, pitch, (uint64_t)x_rows, pitch, 128, S::XK);
@@ -1038,10 +1114,11 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
     const cuuint64_t dims[3] = {(cuuint64_t)std::max(2, a.L & ~1), (cuuint64_t)a.M,
                                 (cuuint64_t)a.rows};
     const cuuint64_t strides[2] = {(cuuint64_t)a.ldy * 8, (cuuint64_t)a.M * a.ldy * 8};
-    const cuuint32_t box[3] = {S::EW, 32, 1};
+    const int words = a.out_split ? S::EW / 2 : S::EW;
+    const cuuint32_t box[3] = {(cuuint32_t)words, 32, 1};
     if (!rc)
       rc = rq_map(&tm.Y, CU_TENSOR_MAP_DATA_TYPE_UINT64, a.Y, 3, dims, strides, box,
-                  S::EW == 16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+                  words == 16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
   } else {
     // rows p, p + 2, ..: from the 16-byte boundary at or before row p, at twice the pitch.  A row
     // off by one word has that word's 16 bytes inside its allocation (allocations start aligned).
@@ -1072,7 +1149,8 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
   if (!rc) rc = rq_map_weights(&tm.W, W, 128, a.w_rows);
   if (ADAPT && !rc) rc = rq_map_weights(&tm.A, A, 128, a.rank16);
   if (ADAPT && !rc) rc = rq_map_weights(&tm.B, B, PNB_MAX_RANK, RQ_BM);
-  if (!rc) rc = shifted ? rq_launch<true, ADAPT>(tm, a, st) : rq_launch<false, ADAPT>(tm, a, st);
+  if (!rc)
+    rc = shifted ? rq_launch<true, ADAPT>(tm, a, sms, st) : rq_launch<false, ADAPT>(tm, a, sms, st);
   if (own) {
     const cudaError_t e = cudaFreeAsync(own, st);
     if (!rc && e != cudaSuccess) rc = cuda_status(e, "cudaFreeAsync(padded weights)");
