@@ -70,7 +70,7 @@ constexpr int RQ_B_SLOTS = 2;
 constexpr int RQ_MAX_W = 13, RQ_MAX_X = 13, RQ_MAX_RAW = 16;  // most slots of each ring
 constexpr int RQ_LISTS = 2;                            // lists of groups, each
 constexpr int RQ_LIST = 32;                            // one round of a warp long
-constexpr int RQ_BARS = 2 * (RQ_MAX_W + RQ_MAX_X + RQ_MAX_RAW + RQ_B_SLOTS + RQ_LISTS) + 6;
+constexpr int RQ_BARS = 2 * (RQ_MAX_W + RQ_MAX_X + RQ_MAX_RAW + RQ_B_SLOTS + RQ_LISTS) + 7;
 // the barriers, two words, the lists' lengths, the lists
 constexpr int RQ_LIST_AT = (8 * RQ_BARS + 16 + 4 * RQ_LISTS + 15) / 16 * 16;
 constexpr int RQ_BAR_BYTES = (RQ_LIST_AT + 16 * RQ_LISTS * RQ_LIST + 127) / 128 * 128;
@@ -93,7 +93,9 @@ struct RqShape {
   static constexpr int COPY = SHIFTED ? RQ_COPY_WARPS : 0;
   static constexpr int MMA_WARP = 2 + COPY;            // warp 0 loads X, warp 1 the weights
   static constexpr int MMA_WARPS = SHIFTED ? 1 : 2;    // two: one per accumulator
-  static constexpr int EPI_WARP = MMA_WARP + MMA_WARPS + (ADAPT ? 1 : 0);  // (the low product's)
+  static constexpr int LOW_WARP = MMA_WARP + MMA_WARPS;       // adapters: L^T = X^T A^T and D = B t
+  static constexpr int LOW_WARPS = !ADAPT ? 0 : SHIFTED ? 1 : 2;  // (16 warps are all that fit)
+  static constexpr int EPI_WARP = LOW_WARP + LOW_WARPS;
   static constexpr int THREADS = 32 * (EPI_WARP + RQ_EPI_WARPS);
 };
 
@@ -286,7 +288,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   const uint32_t b_full = bars + 8 * B0, b_empty = b_full + 8 * RQ_B_SLOTS;
   const uint32_t list_full = bars + 8 * L0, list_empty = list_full + 8 * RQ_LISTS;
   const uint32_t acc_full = bars + 8 * C0, acc_empty = acc_full + 16;
-  const uint32_t low_full = acc_full + 32, t_full = acc_full + 40;
+  const uint32_t low_full = acc_full + 32, t_full = acc_full + 48;
   const uint32_t holder = bars + 8 * RQ_BARS;
   volatile int* abort_s = reinterpret_cast<volatile int*>(rq_raw + (holder + 8 - raw));
   volatile int* list_n = abort_s + 1;
@@ -314,10 +316,10 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       tc::mbar_init(b_empty + 8 * s, 1);
       tc::mbar_init(acc_full + 8 * s, ADAPT ? 2 : 1);
       tc::mbar_init(acc_empty + 8 * s, RQ_EPI_WARPS);
+      tc::mbar_init(low_full + 8 * s, 1);
       tc::mbar_init(list_full + 8 * s, 1);
       tc::mbar_init(list_empty + 8 * s, S::THREADS / 32);
     }
-    tc::mbar_init(low_full, 1);
     tc::mbar_init(t_full, RQ_EPI_WARPS);
     *abort_s = 0;
     tc::fence_mbar_init();
@@ -647,22 +649,24 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         return true;
       });
     }
-  } else if (ADAPT && warp == S::MMA_WARP + S::MMA_WARPS) {
-    // ---------------- low products L^T = X^T A^T and D = B t (one lane) --------------------------
+  } else if (ADAPT && warp < S::LOW_WARP + S::LOW_WARPS) {
+    // ---------------- low products L^T = X^T A^T and D = B t (one lane of each warp) --------------
+    // Two warps, or one that does both and looks for t between its slots: D waits for the epilogue's
+    // t, and a thread that waits for it issues no L^T for the next group.
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, S::BN, true, false, false, true);
+      const bool low = warp == S::LOW_WARP, d = warp == S::LOW_WARP + S::LOW_WARPS - 1;
       const uint32_t LOW = tc::idesc_i8(128, a.rank16, false, true, true, false);
       const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
       const uint64_t ad = tc::smem_desc_sw128(a_at(0), 16u, 1024u);
       const uint32_t x_hi = (uint32_t)(xd >> 32), a_hi = (uint32_t)(ad >> 32);
+      const int steps = (a.K + RQ_KSTEP - 1) / RQ_KSTEP;
       RqRing x, br;
       int tt = 0;
       uint32_t t_par = 0;
-      int pending = -1;  // the accumulator whose D is still to come
-      bool ok = true;
+      int pending = -1;  // the accumulator whose t and D are still to come
       auto product = [&](int buf) {  // D = B t
-        ok = rq_wait(b_full + 8 * br.slot, br.phase, abort_s);
-        if (!ok) return;
+        if (!rq_wait(b_full + 8 * br.slot, br.phase, abort_s)) return false;
         tc::tc_fence_after();
         // columns of B past the rank are zero, so t's rows past it do not matter
         for (int k = 0; k < (a.rank + 31) / 32; ++k)
@@ -672,33 +676,35 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         tc::mma_commit(b_empty + 8 * br.slot);
         tc::mma_commit(acc_full + 8 * buf);
         br.advance(RQ_B_SLOTS);
+        return true;
       };
       auto finish = [&](bool block) {  // the pending D, once t is there
-        if (block)
-          ok = rq_wait(t_full, t_par, abort_s);
-        else if (!tc::mbar_test(t_full, t_par & 1u))
-          return;
-        if (!ok) return;
+        if (pending < 0) return true;
+        if (block) {
+          if (!rq_wait(t_full, t_par, abort_s)) return false;
+        } else if (!tc::mbar_test(t_full, t_par & 1u)) {
+          return true;
+        }
         t_par ^= 1u;
-        product(pending);
+        const int buf = pending;
         pending = -1;
+        return product(buf);
       };
       each(true, [&](const RqGroup& g) {
         const bool has = g.w >= 0;
         const int m_n = tiles(g.mg);
-        for (int m = 0; m < m_n && ok; ++m, ++tt) {
+        for (int m = 0; m < m_n; ++m, ++tt) {
           // Every tile's turn is waited for and answered, also where nothing is issued: a parity
           // tells only neighbouring turns apart, so no role may get two turns ahead of another.
           const int buf = tt & 1;
-          ok = rq_wait(acc_empty + 8 * buf, (uint32_t)(tt >> 1) ^ 1u, abort_s);
-          if (!ok) break;
+          if (!rq_wait(acc_empty + 8 * buf, (uint32_t)(tt >> 1) ^ 1u, abort_s)) return false;
           tc::tc_fence_after();
-          if (m == 0) {
+          if (m > 0 && !finish(true)) return false;
+          if (low && m == 0) {
             const uint32_t l_tmem = tmem + D_AT + (uint32_t)(buf * 128);
             uint32_t acc = 0;
-            for (int left = (a.K + RQ_KSTEP - 1) / RQ_KSTEP; left > 0; left -= S::XK / RQ_KSTEP) {
-              ok = rq_wait(x_full + 8 * x.slot, x.phase, abort_s);
-              if (!ok) break;
+            for (int left = steps; left > 0; left -= S::XK / RQ_KSTEP) {
+              if (!rq_wait(x_full + 8 * x.slot, x.phase, abort_s)) return false;
               if (has) {
                 const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (S::X_SLOT / 16));
                 const uint32_t a_lo = (uint32_t)ad + (uint32_t)(x.slot * (a_slot / 16));
@@ -713,26 +719,24 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
                 tc::mbar_arrive(x_empty + 8 * x.slot);
               }
               x.advance(a.x_slots);
-              if (pending >= 0) finish(false);
+              if (!finish(false)) return false;
             }
-            if (ok && pending >= 0) finish(true);
-            if (!ok) break;
-            if (has) {
-              tc::mma_commit(low_full);
-              pending = buf;
-            }
-          } else if (pending >= 0) {
-            finish(true);
-            if (!ok) break;
+            if (!finish(true)) return false;
+            if (has) tc::mma_commit(low_full + 8 * buf);
           }
-          if (!has)
+          if (!d) continue;
+          if (!has) {
             tc::mbar_arrive(acc_full + 8 * buf);
-          else if (m > 0)
-            product(buf);
+          } else if (m > 0) {
+            if (!product(buf)) return false;
+          } else {
+            pending = buf;
+            if (!low && !finish(true)) return false;
+          }
         }
-        return ok;
+        return true;
       });
-      if (ok && pending >= 0) finish(true);
+      (void)finish(true);
     }
   } else {
     // ---------------- epilogue -------------------------------------------------------------------
@@ -750,7 +754,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     unsigned char* out_row = out + lane * PITCH;
     const int out_x = xored(lane);
     int tt = 0;
-    uint32_t low_par = 0;
+    uint32_t low_par = 0;  // a bit per accumulator
     bool ok = true;
     each(false, [&](const RqGroup& g) {
       const int w = g.w, mg = g.mg, nt = g.nt;
@@ -763,7 +767,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         if (low) {
           // t = A X: lane l of quarter q holds limb l % 8 of word 4q + l/8 for every rank row.  Eight
           // lanes add up 16 rows at a time, halving the rows they keep at each step.
-          ok = rq_wait(low_full, low_par, abort_s);
+          ok = rq_wait(low_full + 8 * buf, low_par >> buf, abort_s);
           if (!ok) break;
           tc::tc_fence_after();
           const int word = q * 4 + (lane >> 3);
@@ -796,7 +800,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           tc::tc_fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(t_full);
-          low_par ^= 1u;
+          low_par ^= 1u << buf;
         }
         const uint32_t c_tmem = tmem + (uint32_t)(buf * S::BN) + lanes + (uint32_t)(eh * EW * 8);
         const int row0 = (mg * a.m_group + m) * RQ_BM + q * 32, col0 = nt * S::WORDS + eh * EW;
