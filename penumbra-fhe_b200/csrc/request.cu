@@ -65,7 +65,6 @@ constexpr int RQ_W_SLOT = RQ_BM * RQ_WK;               // 16 KB
 constexpr int RQ_B_SLOT = RQ_BM * PNB_MAX_RANK;        // 8 KB: B rows of 64 bytes
 constexpr int RQ_EPI_WARPS = 8;                        // two per TMEM lane quarter
 constexpr int RQ_COPY_WARPS = 4;                       // each copies every fourth raw slot
-constexpr int RQ_RAW_ROWS = 32;                        // rows per raw slot, half of each parity
 constexpr int RQ_B_SLOTS = 2;
 constexpr int RQ_MAX_W = 13, RQ_MAX_X = 13, RQ_MAX_RAW = 16;  // most slots of each ring
 constexpr int RQ_LISTS = 2;                            // lists of groups, each
@@ -85,8 +84,9 @@ struct RqShape {
   static constexpr int XK = ADAPT ? 128 : 64;          // K per X slot
   static constexpr int X_SLOT = XK * BN;               // 16 KB
   static constexpr int RAW_PITCH = BN + 16;            // one word of shift, to 16 bytes
-  static constexpr int RAW_SLOT = RQ_RAW_ROWS * RAW_PITCH;
-  static constexpr int RAW_PER_X = XK / RQ_RAW_ROWS;
+  static constexpr int RAW_ROWS = ADAPT ? 64 : 32;     // rows per raw slot, half of each parity
+  static constexpr int RAW_SLOT = RAW_ROWS * RAW_PITCH;
+  static constexpr int RAW_PER_X = XK / RAW_ROWS;
   static constexpr int EW = WORDS / 2;                 // words per epilogue warp
   static constexpr int OUT = 32 * EW * 8;              // its staging: 32 rows
   static constexpr bool MAY_SPLIT = !SHIFTED && !ADAPT;  // which may be done in two parts
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       const int slots = SHIFTED ? a.raw_slots : a.x_slots;
       each(true, [&](const RqGroup& g) {
         const bool has = ADAPT && g.w >= 0;
-        for (int k = 0; k < a.K; k += SHIFTED ? RQ_RAW_ROWS : S::XK) {
+        for (int k = 0; k < a.K; k += SHIFTED ? S::RAW_ROWS : S::XK) {
           const int s = ring.slot;
           const uint32_t full = (SHIFTED ? r_full : x_full) + 8 * s;
           if (!rq_wait((SHIFTED ? r_empty : x_empty) + 8 * s, ring.phase ^ 1u, abort_s)) return false;
@@ -484,16 +484,16 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           tc::mbar_expect_tx(full, w >= 0 ? (uint32_t)a_slot : 0u);
           if (w >= 0) tc::tma_load_2d(a_at(xr.slot), &tm.A, kx * S::XK, w * a.rank, full);
         }
-        const int raws = x_rows(kx) / RQ_RAW_ROWS;
+        const int raws = (x_rows(kx) + S::RAW_ROWS - 1) / S::RAW_ROWS;
         for (int i = 0; i < raws; ++i) {
           if ((rr.slot & 3) == cw) {
             if (!rq_wait(r_full + 8 * rr.slot, rr.phase, abort_s)) return false;
             // row r of the slot: its parity's half, r / 2; one word further where it is shifted
             const unsigned char* from = rq_raw + (raw_at(rr.slot) - raw) + word * 8;
             unsigned char* to = rq_raw + (x_at(xr.slot) - raw) + box * (S::XK * 128) +
-                                i * (RQ_RAW_ROWS * 128) + half * 8;
+                                i * (S::RAW_ROWS * 128) + half * 8;
 #pragma unroll
-            for (int b = 0; b < RQ_RAW_ROWS / PER; b += BATCH) {
+            for (int b = 0; b < S::RAW_ROWS / PER; b += BATCH) {
               uint64_t v[BATCH];
 #pragma unroll
               for (int j = 0; j < BATCH; ++j) {
@@ -1007,11 +1007,11 @@ static void rq_plan(RqArgs& a, int sms) {
   const int a_slot = ADAPT ? a.rank16 * RQ_WK : 0;  // beside each X slot
   int out_bytes = RQ_EPI_WARPS * S::OUT;
   int room = RQ_SMEM - RQ_BAR_BYTES - t_bytes - b_bytes - out_bytes;
-  // what X wants at least before weights may stay: four slots (shifted: three and 40 KB of raw
-  // rows); for adapters, whose weights would come twice as often, three (two and 32 KB).  256 rows
+  // what X wants at least before weights may stay: four slots (shifted: three, and 40 KB of raw rows);
+  // for adapters, whose weights would come twice as often, one less.  256 rows
   // of 784->128: one slot less costs experts at an odd pitch 928 -> 1065 us by letting the weights
   // stay, and gains rank 64 1359 -> 1147 us, rank 16 at an odd pitch 1423 -> 1333 us.
-  const int raw_min = SHIFTED ? (ADAPT ? 32 : 40) * 1024 / S::RAW_SLOT : 0;
+  const int raw_min = SHIFTED ? 40 * 1024 / S::RAW_SLOT : 0;
   const int x_min = 4 - (SHIFTED ? 1 : 0) - (ADAPT ? 1 : 0);
   auto x_bytes = [&](int slots) { return slots * (S::X_SLOT + a_slot) + raw_min * S::RAW_SLOT; };
   const long long columns = (long long)a.rows * a.n_tiles;
@@ -1133,7 +1133,7 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
       const cuuint64_t dims[2] = {(cuuint64_t)ldx + off,
                                   (cuuint64_t)std::max<long long>(1, (x_rows + 1 - p) / 2)};
       const cuuint64_t strides[1] = {(cuuint64_t)ldx * 16};
-      const cuuint32_t box[2] = {S::WORDS + 2, RQ_RAW_ROWS / 2};
+      const cuuint32_t box[2] = {S::WORDS + 2, S::RAW_ROWS / 2};
       rc = rq_map(&tm.X[p], CU_TENSOR_MAP_DATA_TYPE_UINT64, X + (second ? ldx : 0) - off, 2, dims,
                   strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
     }
