@@ -62,7 +62,6 @@ constexpr int RQ_BM = 128;      // output rows per tile
 constexpr int RQ_WK = 128;      // K per weight slot
 constexpr int RQ_KSTEP = 32;    // K per MMA; a ragged K costs at most 31 rows
 constexpr int RQ_W_SLOT = RQ_BM * RQ_WK;               // 16 KB
-constexpr int RQ_B_SLOT = RQ_BM * PNB_MAX_RANK;        // 8 KB: B rows of 64 bytes
 constexpr int RQ_EPI_WARPS = 8;                        // two per TMEM lane quarter
 constexpr int RQ_COPY_WARPS = 4;                       // each copies every fourth raw slot
 constexpr int RQ_B_SLOTS = 2;
@@ -89,7 +88,7 @@ struct RqShape {
   static constexpr int RAW_PER_X = XK / RAW_ROWS;
   static constexpr int EW = WORDS / 2;                 // words per epilogue warp
   static constexpr int OUT = 32 * EW * 8;              // its staging: 32 rows
-  static constexpr bool MAY_SPLIT = !SHIFTED && !ADAPT;  // which may be done in two parts
+  static constexpr bool MAY_SPLIT = !SHIFTED;          // which may be done in two parts
   static constexpr int COPY = SHIFTED ? RQ_COPY_WARPS : 0;
   static constexpr int MMA_WARP = 2 + COPY;            // warp 0 loads X, warp 1 the weights
   static constexpr int MMA_WARPS = SHIFTED ? 1 : 2;    // two: one per accumulator
@@ -113,6 +112,7 @@ struct RqArgs {
   int rows, top_k, choices, n_which;  // top_k = 0: row n reads X row group n
   int M, K, L, ldy;
   int shift, rank, rank16;    // adapters
+  int b_row;                  // bytes of B's rows in shared memory: one swizzle span, 32 or 64
   int off0, off1;             // words by which rows 0, 2, .. / 1, 3, .. start past 16-byte alignment
   int w_rows;                 // weight rows per load
   int n_tiles, m_tiles, m_group;  // tiles of 128 rows that share one load of X
@@ -273,11 +273,12 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     return;
   }
   const int a_slot = a.rank16 * RQ_WK;  // A's rows beside one X slot
+  const int b_slot = RQ_BM * a.b_row;
   auto w_at = [&](int s) { return base + (uint32_t)(s * RQ_W_SLOT); };
   auto x_at = [&](int s) { return base + (uint32_t)(a.x_at + s * S::X_SLOT); };
   auto raw_at = [&](int s) { return base + (uint32_t)(a.raw_at + s * S::RAW_SLOT); };
   auto a_at = [&](int s) { return base + (uint32_t)(a.a_at + s * a_slot); };
-  auto b_at = [&](int s) { return base + (uint32_t)(a.b_at + s * RQ_B_SLOT); };
+  auto b_at = [&](int s) { return base + (uint32_t)(a.b_at + s * b_slot); };
   const uint32_t t_at = base + (uint32_t)a.t_at;
   const uint32_t bars = base + (uint32_t)a.bars_at;
   constexpr int W0 = 0, X0 = 2 * RQ_MAX_W, R0 = X0 + 2 * RQ_MAX_X, B0 = R0 + 2 * RQ_MAX_RAW,
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         if (has) {
           const int s = br.slot;
           if (!rq_wait(b_empty + 8 * s, br.phase ^ 1u, abort_s)) return false;
-          tc::mbar_expect_tx(b_full + 8 * s, RQ_B_SLOT);
+          tc::mbar_expect_tx(b_full + 8 * s, (uint32_t)b_slot);
           tc::tma_load_2d(b_at(s), &tm.B, 0, g.w * a.M + m_row, b_full + 8 * s);
           br.advance(RQ_B_SLOTS);
           b_wrap |= br.slot == 0;
@@ -671,7 +672,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         // columns of B past the rank are zero, so t's rows past it do not matter
         for (int k = 0; k < (a.rank + 31) / 32; ++k)
           tc::mma_i8(tmem + D_AT + (uint32_t)(buf * 128),
-                     tc::smem_desc_sw64(b_at(br.slot) + 32u * k, 16u, 512u),
+                     a.b_row == 32 ? tc::smem_desc_sw32(b_at(br.slot), 16u, 256u)
+                                   : tc::smem_desc_sw64(b_at(br.slot) + 32u * k, 16u, 512u),
                      tc::smem_desc_sw128(t_at + 4096u * k, 16u, 1024u), MAIN, k != 0 ? 1u : 0u);
         tc::mma_commit(b_empty + 8 * br.slot);
         tc::mma_commit(acc_full + 8 * buf);
@@ -750,7 +752,9 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     const uint32_t out_at = base + (uint32_t)(a.out_at + e_w * (S::OUT / PARTS));
     unsigned char* out = rq_raw + (out_at - raw);
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
-    auto xored = [](int row) { return PITCH == 128 ? row & 7 : (row >> 1) & 3; };  // its swizzle
+    auto xored = [](int row) {  // its swizzle
+      return PITCH == 128 ? row & 7 : PITCH == 64 ? (row >> 1) & 3 : (row >> 2) & 1;
+    };
     unsigned char* out_row = out + lane * PITCH;
     const int out_x = xored(lane);
     int tt = 0;
@@ -981,13 +985,20 @@ static int rq_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, 
   return PNB_ERR_CUDA;
 }
 
+// The swizzle whose span is a box row of these bytes.
+static CUtensorMapSwizzle rq_swizzle(int bytes) {
+  return bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+         : bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                       : CU_TENSOR_MAP_SWIZZLE_32B;
+}
+
 // Byte matrix [rows][cols] at a pitch, in boxes of box_cols bytes (one swizzle span) x box_rows.
 static int rq_map_bytes(CUtensorMap* map, const void* p, uint64_t cols, uint64_t rows,
                         uint64_t pitch, int box_cols, int box_rows) {
   const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
   const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   return rq_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, p, 2, dims, strides, box,
-                box_cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+                rq_swizzle(box_cols));
 }
 static int rq_map_weights(CUtensorMap* map, const RqMatrix& m, int box_cols, int box_rows) {
   return rq_map_bytes(map, m.p, (uint64_t)m.pitch(), (uint64_t)m.rows, (uint64_t)m.pitch(), box_cols,
@@ -1003,7 +1014,7 @@ static void rq_plan(RqArgs& a, int sms) {
   const int kb = (a.K + RQ_WK - 1) / RQ_WK, kx = (a.K + S::XK - 1) / S::XK;
   const int rank32 = (a.rank + 31) & ~31;
   const int t_bytes = ADAPT ? rank32 * S::BN : 0;
-  const int b_bytes = ADAPT ? RQ_B_SLOTS * RQ_B_SLOT : 0;
+  const int b_bytes = ADAPT ? RQ_B_SLOTS * RQ_BM * a.b_row : 0;
   const int a_slot = ADAPT ? a.rank16 * RQ_WK : 0;  // beside each X slot
   int out_bytes = RQ_EPI_WARPS * S::OUT;
   int room = RQ_SMEM - RQ_BAR_BYTES - t_bytes - b_bytes - out_bytes;
@@ -1030,10 +1041,10 @@ static void rq_plan(RqArgs& a, int sms) {
         std::min(RQ_MAX_RAW, (room - a.x_slots * (S::X_SLOT + a_slot)) / S::RAW_SLOT & ~3);
   } else {
     a.x_slots = std::min(RQ_MAX_X, room / (S::X_SLOT + a_slot));
-    if (S::MAY_SPLIT && a.x_slots < 6) {
+    if (S::MAY_SPLIT && a.x_slots < (ADAPT ? 5 : 6)) {
       a.out_split = 1;
       out_bytes /= 2;
-      a.x_slots = (room + out_bytes) / S::X_SLOT;
+      a.x_slots = (room + out_bytes) / (S::X_SLOT + a_slot);
     }
     a.raw_slots = 0;
   }
@@ -1122,7 +1133,7 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
     const cuuint32_t box[3] = {(cuuint32_t)words, 32, 1};
     if (!rc)
       rc = rq_map(&tm.Y, CU_TENSOR_MAP_DATA_TYPE_UINT64, a.Y, 3, dims, strides, box,
-                  words == 16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+                  rq_swizzle(8 * words));
   } else {
     // rows p, p + 2, ..: from the 16-byte boundary at or before row p, at twice the pitch.  A row
     // off by one word has that word's 16 bytes inside its allocation (allocations start aligned).
@@ -1152,7 +1163,7 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
   rc = rq_place(all, own ? own : (int8_t*)ws, st);
   if (!rc) rc = rq_map_weights(&tm.W, W, 128, a.w_rows);
   if (ADAPT && !rc) rc = rq_map_weights(&tm.A, A, 128, a.rank16);
-  if (ADAPT && !rc) rc = rq_map_weights(&tm.B, B, PNB_MAX_RANK, RQ_BM);
+  if (ADAPT && !rc) rc = rq_map_weights(&tm.B, B, a.b_row, RQ_BM);
   if (!rc)
     rc = shifted ? rq_launch<true, ADAPT>(tm, a, sms, st) : rq_launch<false, ADAPT>(tm, a, sms, st);
   if (own) {
@@ -1187,6 +1198,7 @@ int adapter_contract(const int8_t* W, const int64_t* bias, uint64_t delta, int b
   a.rows = batch;
   a.M = M; a.K = K; a.L = L; a.ldy = ldy;
   a.shift = base_shift; a.rank = rank; a.rank16 = (rank + 15) & ~15;
+  a.b_row = rank <= 32 ? 32 : 64;
   return rq_run<true>({W, M, K}, {A, (long long)adapters * rank, K}, {B, (long long)adapters * M, rank},
                       a, X, ldx, batch, ws, ws_bytes, st);
 }

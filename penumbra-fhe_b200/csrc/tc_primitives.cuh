@@ -271,6 +271,13 @@ __device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t addr, uint32_t lbo_b
   return (d & ~((uint64_t)7 << 61)) | ((uint64_t)4 << 61);
 }
 
+// K-major operand whose rows are 32 bytes (SWIZZLE_32B): 8-row groups of 256 bytes.
+__device__ __forceinline__ uint64_t smem_desc_sw32(uint32_t addr, uint32_t lbo_bytes,
+                                                   uint32_t sbo_bytes) {
+  uint64_t d = smem_desc_sw128(addr, lbo_bytes, sbo_bytes);
+  return (d & ~((uint64_t)7 << 61)) | ((uint64_t)6 << 61);
+}
+
 // Instruction descriptor of kind::i8 with s32 accumulation.
 __host__ __device__ constexpr uint32_t idesc_i8(int M, int N, bool a_signed, bool b_signed,
                                                 bool a_mn_major, bool b_mn_major) {
