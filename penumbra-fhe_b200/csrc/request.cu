@@ -337,6 +337,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
+  // what came before in the stream is done from here on (rq_pad_kernel lets this one start early)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(rq_raw + (holder - raw));
 
   constexpr uint32_t D_AT = 256;               // adapters: TMEM columns of L^T and D
@@ -932,6 +934,7 @@ struct RqCopy {
 
 // Up to three matrices in one launch, 16 bytes (of one row) per thread.
 __global__ void rq_pad_kernel(const __grid_constant__ RqCopy c) {
+  asm volatile("griddepcontrol.launch_dependents;");
   const size_t i = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * 16;
   if (i >= c.first[3]) return;
   const int w = i >= c.first[2] ? 2 : i >= c.first[1] ? 1 : 0;
@@ -948,7 +951,7 @@ __global__ void rq_pad_kernel(const __grid_constant__ RqCopy c) {
 }
 
 // Copies the matrices that TMA cannot read in place to ws, and points them there.
-static int rq_place(RqMatrix* (&m)[3], int8_t* ws, cudaStream_t st) {
+static int rq_place(RqMatrix* (&m)[3], int8_t* ws, cudaStream_t st, bool& placed) {
   RqCopy c{};
   for (int i = 0; i < 3; ++i) {
     c.first[i + 1] = c.first[i];
@@ -959,7 +962,8 @@ static int rq_place(RqMatrix* (&m)[3], int8_t* ws, cudaStream_t st) {
     m[i]->p = c.to[i];
   }
   const size_t threads = c.first[3] / 16;
-  if (threads == 0) return PNB_OK;
+  placed = threads != 0;
+  if (!placed) return PNB_OK;
   rq_pad_kernel<<<(unsigned)((threads + 127) / 128), 128, 0, st>>>(c);
   PNB_CHECK_LAUNCH("rq_pad_kernel");
   return PNB_OK;
@@ -1083,17 +1087,24 @@ static int rq_prepare(RqArgs& a, int& sms) {
   return PNB_ERR_INVALID;
 }
 
+// `early`: behind rq_pad_kernel, whose launch and whose run the set-up of this one then hides.
 template <bool SHIFTED, bool ADAPT>
-static int rq_launch(const RqMaps& tm, const RqArgs& a, int sms, cudaStream_t st) {
+static int rq_launch(const RqMaps& tm, const RqArgs& a, int sms, bool early, cudaStream_t st) {
   using S = RqShape<SHIFTED, ADAPT>;
-  const int grid = (int)std::min<long long>((long long)a.rows * a.groups * a.n_tiles, sms);
-  if (a.out_split)
-    request_kernel<SHIFTED, ADAPT, S::MAY_SPLIT>
-        <<<grid, S::THREADS, a.bars_at + RQ_BAR_BYTES, st>>>(tm, a);
-  else
-    request_kernel<SHIFTED, ADAPT, false>
-        <<<grid, S::THREADS, a.bars_at + RQ_BAR_BYTES, st>>>(tm, a);
-  PNB_CHECK_LAUNCH("request_kernel");
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(
+      (unsigned)std::min<long long>((long long)a.rows * a.groups * a.n_tiles, sms));
+  cfg.blockDim = dim3(S::THREADS);
+  cfg.dynamicSmemBytes = (size_t)(a.bars_at + RQ_BAR_BYTES);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = early ? 1 : 0;
+  auto kernel = a.out_split ? request_kernel<SHIFTED, ADAPT, S::MAY_SPLIT>
+                            : request_kernel<SHIFTED, ADAPT, false>;
+  PNB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tm, a));
   return PNB_OK;
 }
 
@@ -1160,12 +1171,14 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
   }
   if (need && !ws) PNB_CUDA(cudaMallocAsync((void**)&own, need, st));
   RqMatrix* all[3] = {&W, &A, &B};
-  rc = rq_place(all, own ? own : (int8_t*)ws, st);
+  bool placed = false;
+  rc = rq_place(all, own ? own : (int8_t*)ws, st, placed);
   if (!rc) rc = rq_map_weights(&tm.W, W, 128, a.w_rows);
   if (ADAPT && !rc) rc = rq_map_weights(&tm.A, A, 128, a.rank16);
   if (ADAPT && !rc) rc = rq_map_weights(&tm.B, B, a.b_row, RQ_BM);
   if (!rc)
-    rc = shifted ? rq_launch<true, ADAPT>(tm, a, sms, st) : rq_launch<false, ADAPT>(tm, a, sms, st);
+    rc = shifted ? rq_launch<true, ADAPT>(tm, a, sms, placed, st)
+                 : rq_launch<false, ADAPT>(tm, a, sms, placed, st);
   if (own) {
     const cudaError_t e = cudaFreeAsync(own, st);
     if (!rc && e != cudaSuccess) rc = cuda_status(e, "cudaFreeAsync(padded weights)");
