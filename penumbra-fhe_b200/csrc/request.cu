@@ -17,21 +17,37 @@
 // groups of tiles that share their X.  Weights are picked per tile by the TMA coordinate, so rows of
 // different experts share a launch.
 //
-// What bounds it is first the path from L2 to the SM, then HBM: a tile reads K x 256 bytes of X
-// once, and as many weight rows again unless they stay.  So weights stay in shared memory while
-// consecutive tiles of a block use the same ones (rows sorted by expert see to that), and where the
-// output has several tiles of 128 rows, X stays while they take turns.
+// The floor is HBM: X read once and Y written once (256 requests 784->128: 3.83 GB, 586 us at the
+// measured copy bandwidth, where the MMAs need 251 us at twice the measured bf16 rate).  What stands
+// between is the path from L2 to the SM: a tile reads K x 256 bytes of X, and as many weight rows
+// again unless they stay.  So weights stay in shared memory while consecutive tiles of a block use
+// the same ones (rows sorted by expert see to that), and where the output has several tiles of 128
+// rows, X stays while they take turns (122 rows 130->200: one tile at a time 181 -> 237 us).
+// Groups are dealt out to the blocks in turn, so that the blocks work on one ciphertext row at a
+// time and its lines are still in L2 for all of them; consecutive runs for each block keep weights
+// longer but cost more (45 x 257->384: 263 -> 295 us).
+//
+// Measured (sustained, SM clock falling to 1.2-1.7 GHz under the power cap; in brackets the best
+// launch): 256 x 784->128 of 16 experts 670-710 us (606) = 5.4-5.7 TB/s (6.3); with adapters of rank
+// 16 857 us (743) = 4.5 TB/s (5.2); one request 13 us, 15 with an adapter of rank 8.  At an odd pitch 256 x
+// 784->128 760-880 us, 122 x 130->200 166-180 us, 45 x 257->384 of rank 33 264 us.  DRAM is busy
+// 74% of a short run of 64 x 784->128 (its bytes are the algorithm's), the tensor pipe 34%.
 //
 // Adapters: the low-rank pair rides on the same pass over X.  While the K loop accumulates
 // C = W X it also accumulates the transposed low product  L^T = X^T A^T  (the X tile as the M = 128
-// operand and A's rows as N: rank/128 of the main product's work, where A as a padded M = 128
-// operand would double it).  The epilogue warps add up the limbs of t = A X mod 2^64 across lanes,
-// write t's bytes to shared memory as the next MN-major operand, and one short MMA makes D = B t.  y = (C << s) + D.  X is read once; t never leaves the SM.
+// operand, A's rows as N: 46 cycles a step of 32 against 64 for the main product; A as a padded M
+// operand would take 64 for any rank).  The epilogue warps add up the limbs of t = A X mod 2^64
+// across lanes, write t's bytes to shared memory as the next MN-major operand, and a short MMA makes
+// D = B t.  y = (C << s) + D.  X is read once; t never leaves the SM.  C, L^T and D of two tiles
+// fill the 512 TMEM columns at 16 words; MMAs that narrow (N = 128) read 8 KB of shared memory in
+// their 64 cycles, all that it delivers, which is what keeps adapters from the bytes' floor.  (32
+// words with one accumulator: 45 x 257->384 263 -> 388 us.)
 //
 // Rows that start 16-byte aligned (an even pitch) move by TMA straight into the operand layout, and
 // results leave by TMA.  Other rows (contiguous [count][kN+1] ciphertexts) are off by one word
 // every other row, which no tiled load can shift: they land unshifted in a ring of raw slots, and
-// four warps copy them word by word into the operand layout.
+// four warps copy them word by word into the operand layout.  (8-byte cp.async into place, without
+// the ring and the copy, is slower: 256 x 784->128 760 -> 1024 us.)
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -218,8 +234,8 @@ struct RqRing {
 };
 
 // Bounded wait that also gives up as soon as another role has flagged an abort.  A completed phase
-// is found by the plain test: a third of a suspending wait's time (51 against 165 cycles), which
-// the thread that issues the MMAs pays at every slot.  The rest is out of line: the roles' loops
+// is found by the plain test: 145 cycles against a suspending wait's 186, which the thread that
+// issues the MMAs pays at every slot.  The rest is out of line: the roles' loops
 // share the instruction cache, and a thread on its own runs at the pace of its fetches.
 __device__ __noinline__ bool rq_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_s) {
   for (uint32_t it = 0; it < RQ_WAIT_LIMIT; it += 1024) {
@@ -296,7 +312,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   uint4* lists = reinterpret_cast<uint4*>(rq_raw + (bars - raw) + RQ_LIST_AT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // adapters with one tile to a group: the second warp's answers cost what its share would gain
+  // adapters with one tile to a group: the second warp's answers cost more than its share gains
+  // (256 x 784->128 of rank 16: 937 -> 957 us; with four tiles, 64 x 512->512, it is 512 -> 484)
   const int mma_warps = ADAPT && a.m_group == 1 ? 1 : S::MMA_WARPS;
 
   if (threadIdx.x == 0) {
@@ -531,9 +548,10 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     // ---------------- main products (one lane of each warp) --------------------------------------
     // Tiles alternate between two warps, each with an accumulator of its own: waiting for a slot,
     // issuing its MMAs and letting it go takes a thread longer than the tensor cores take to run
-    // them, the more so between tiles, so one thread's bookkeeping hides behind the other's MMAs.
-    // Either answers for every slot, also those of tiles that are not its own: a parity tells only
-    // neighbouring uses apart.
+    // them, the more so between tiles, so one thread's bookkeeping hides behind the other's MMAs
+    // (64 x 512->512 350 -> 335 us, 122 x 130->200 154 -> 144).  Either answers for every slot, also
+    // those of tiles that are not its own: a parity tells only neighbouring uses apart.  At odd
+    // pitches the copies bound the tiles and one warp does it (183 us either way for 122 x 130->200).
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, S::BN, true, false, false, true);
       constexpr int STEPS = S::XK / RQ_KSTEP;
@@ -655,7 +673,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   } else if (ADAPT && warp < S::LOW_WARP + S::LOW_WARPS) {
     // ---------------- low products L^T = X^T A^T and D = B t (one lane of each warp) --------------
     // Two warps, or one that does both and looks for t between its slots: D waits for the epilogue's
-    // t, and a thread that waits for it issues no L^T for the next group.
+    // t, and a thread that waits for it issues no L^T for the next group (256 x 784->128 of rank 16:
+    // 943 us with one, 908 with two).
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, S::BN, true, false, false, true);
       const bool low = warp == S::LOW_WARP, d = warp == S::LOW_WARP + S::LOW_WARPS - 1;
@@ -969,7 +988,9 @@ static int rq_place(RqMatrix* (&m)[3], int8_t* ws, cudaStream_t st, bool& placed
   return PNB_OK;
 }
 
-// A tiled map of `rank` dimensions (strides of all but the first, in bytes).
+// A tiled map of `rank` dimensions (strides of all but the first, in bytes).  No promotion to larger
+// L2 reads: rows at an odd pitch would bring their neighbours' lines again (880 -> 790 us for 256 x
+// 784->128 without it; even pitches show no difference).
 static int rq_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank,
                   const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
                   CUtensorMapSwizzle swizzle) {
@@ -1011,7 +1032,11 @@ static int rq_map_weights(CUtensorMap* map, const RqMatrix& m, int box_cols, int
 
 // How one block's shared memory is shared out.  Weights stay (keep_w) when the slots of a group's
 // weights leave X enough; X stays for all tiles of 128 rows (m_group) when it fits beside a ring of
-// weights and the batch fills the machine without splitting them.
+// weights and the batch fills the machine without splitting them.  Beyond that, slots of X in flight
+// are what hides memory's latency: with weights kept, 256 x 784->128 takes 848, 713, 664 and 606 us
+// (best launches) with 3, 4, 5 and 6 of them, adapters of 640->128 713, 646, 609 and 600.  So where X
+// has fewer than six (five), results are staged in two halves, which costs short K something (256 x
+// 128->10: 110 -> 119 us) and pays for a slot.
 template <bool SHIFTED, bool ADAPT>
 static void rq_plan(RqArgs& a, int sms) {
   using S = RqShape<SHIFTED, ADAPT>;
@@ -1023,9 +1048,10 @@ static void rq_plan(RqArgs& a, int sms) {
   int out_bytes = RQ_EPI_WARPS * S::OUT;
   int room = RQ_SMEM - RQ_BAR_BYTES - t_bytes - b_bytes - out_bytes;
   // what X wants at least before weights may stay: four slots (shifted: three, and 40 KB of raw rows);
-  // for adapters, whose weights would come twice as often, one less.  256 rows
-  // of 784->128: one slot less costs experts at an odd pitch 928 -> 1065 us by letting the weights
-  // stay, and gains rank 64 1359 -> 1147 us, rank 16 at an odd pitch 1423 -> 1333 us.
+  // for adapters, whose weights would come twice as often, one less.  256 rows of 784->128: one slot
+  // less costs experts at an odd pitch 928 -> 1065 us by letting the weights stay, and gains rank 64
+  // 1359 -> 1147 us, rank 16 at an odd pitch 1423 -> 1333 us.  (Shifted rows are in flight in the raw
+  // ring: with four slots of it and more of X, 256 x 784->128 takes 1042 us instead of 760.)
   const int raw_min = SHIFTED ? 40 * 1024 / S::RAW_SLOT : 0;
   const int x_min = 4 - (SHIFTED ? 1 : 0) - (ADAPT ? 1 : 0);
   auto x_bytes = [&](int slots) { return slots * (S::X_SLOT + a_slot) + raw_min * S::RAW_SLOT; };
@@ -1040,7 +1066,7 @@ static void rq_plan(RqArgs& a, int sms) {
                        : std::max(3, std::min(4, (room - x_bytes(x_need)) / RQ_W_SLOT));
   room -= a.w_slots * RQ_W_SLOT;
   if (SHIFTED) {
-    a.x_slots = a.m_group > 1 ? std::max(3, kx + 1) : x_min;
+    a.x_slots = x_need;
     a.raw_slots =
         std::min(RQ_MAX_RAW, (room - a.x_slots * (S::X_SLOT + a_slot)) / S::RAW_SLOT & ~3);
   } else {
@@ -1080,6 +1106,12 @@ static int rq_prepare(RqArgs& a, int& sms) {
     if (dev < 64) sm_count[dev].store(sms, std::memory_order_release);
   }
   rq_plan<SHIFTED, ADAPT>(a, sms);
+  if (a.x_slots < 2 || a.w_slots < 1 || (SHIFTED && a.raw_slots < RQ_COPY_WARPS) ||
+      a.bars_at + RQ_BAR_BYTES > RQ_SMEM) {
+    set_error("%s: no plan for M=%d K=%d rank=%d", ADAPT ? "adapter_contract" : "expert_contract",
+              a.M, a.K, a.rank);
+    return PNB_ERR_INVALID;
+  }
   a.groups = (a.m_tiles + a.m_group - 1) / a.m_group;
   if (a.groups < 1 << RQ_MG_BITS && (long long)a.groups * a.n_tiles < 1 << RQ_NT_BITS) return PNB_OK;
   set_error("%s: %d x %d tiles of one row exceed one launch",

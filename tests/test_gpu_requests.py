@@ -449,6 +449,35 @@ def test_shapes_whose_operands_do_not_stay(pnb, oracle, M, K, rank, ld):
     assert pnb.device_status(0) == 0
 
 
+@pytest.mark.parametrize("ld", [33, 34])
+@pytest.mark.parametrize("M,K,rank", [(896, 128, 16), (800, 97, 16), (769, 128, 33), (640, 128, 64),
+                                      (1537, 128, 8), (1664, 64, 1), (256, 256, 48)])
+def test_short_k_of_many_tiles(pnb, oracle, M, K, rank, ld):
+    # all tiles' weights stay, and take the memory that X is left with
+    rng = np.random.default_rng(M + K + rank)
+    L, batch, n = 33, 80, 3
+    W = rng.integers(-128, 128, (n, M, K)).astype(np.int8)
+    A = rng.integers(-128, 128, (n, rank, K)).astype(np.int8)
+    B = rng.integers(-128, 128, (n, M, rank)).astype(np.int8)
+    X = words(rng, batch, K, ld)
+    which = rng.integers(-1, n, batch).astype(np.int32)
+    ids = rng.integers(-1, n, (batch, 1)).astype(np.int32)
+    rows = [0, 7, batch - 1]
+    got = pnb.adapter_contract(dev(W[0]), None, 0, dev(A), dev(B), dev(which), dev(X), L,
+                               base_shift=2)
+    assert np.array_equal(host(got[rows])[:, :, :L],
+                          plain_adapter(oracle, W[0], None, 0, A, B, which[rows], X[rows][:, :, :L], 2))
+    route = pnb.expert_route(dev(ids), n)
+    got = pnb.expert_contract(route, dev(W), None, 0, dev(X), L)
+    for t in rows:
+        if ids[t, 0] >= 0:
+            want = oracle.contract(W[ids[t, 0]].astype(np.int64), None, 0,
+                                   np.ascontiguousarray(X[t, :, :L])[None])[0]
+            at = route.choice_row[t, 0].item()
+            assert np.array_equal(host(got[at])[:, :L], want), t
+    assert pnb.device_status(0) == 0
+
+
 def test_strided_inputs(pnb):
     # tensors that are not contiguous are used as the values they hold
     rng = np.random.default_rng(15)
