@@ -107,7 +107,7 @@ struct RqShape {
   static constexpr bool MAY_SPLIT = !SHIFTED;          // which may be done in two parts
   static constexpr int COPY = SHIFTED ? RQ_COPY_WARPS : 0;
   static constexpr int MMA_WARP = 2 + COPY;            // warp 0 loads X, warp 1 the weights
-  static constexpr int MMA_WARPS = SHIFTED ? 1 : 2;    // two: one per accumulator
+  static constexpr int MMA_WARPS = SHIFTED && ADAPT ? 1 : 2;  // two: one per accumulator
   static constexpr int LOW_WARP = MMA_WARP + MMA_WARPS;       // adapters: L^T = X^T A^T and D = B t
   static constexpr int LOW_WARPS = !ADAPT ? 0 : SHIFTED ? 1 : 2;  // (16 warps are all that fit)
   static constexpr int EPI_WARP = LOW_WARP + LOW_WARPS;
@@ -550,8 +550,8 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     // issuing its MMAs and letting it go takes a thread longer than the tensor cores take to run
     // them, the more so between tiles, so one thread's bookkeeping hides behind the other's MMAs
     // (64 x 512->512 350 -> 335 us, 122 x 130->200 154 -> 144).  Either answers for every slot, also
-    // those of tiles that are not its own: a parity tells only neighbouring uses apart.  At odd
-    // pitches the copies bound the tiles and one warp does it (183 us either way for 122 x 130->200).
+    // those of tiles that are not its own: a parity tells only neighbouring uses apart.  (Adapters
+    // at odd pitches have no warp left for it: 16 are all that get 128 registers a thread.)
     if (lane == 0) {
       constexpr uint32_t MAIN = tc::idesc_i8(RQ_BM, S::BN, true, false, false, true);
       constexpr int STEPS = S::XK / RQ_KSTEP;
@@ -904,14 +904,28 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         if (SHIFTED) {
           __syncwarp();
           constexpr int PER = 32 / EW;  // rows per instruction
-          const int wd = lane % EW;
-          uint64_t* y = a.Y + ((size_t)g.n * a.M + row0) * a.ldy + col0 + wd;
-#pragma unroll 8
-          for (int j = 0; j < 32 / PER; ++j) {
-            const int r = j * PER + lane / EW;
-            if (row0 + r < a.M && col0 + wd < a.L)
-              y[(size_t)r * a.ldy] = *reinterpret_cast<const uint64_t*>(
-                  out + r * PITCH + (((wd >> 1) ^ xored(r)) << 4) + (wd & 1) * 8);
+          const int wd = lane % EW, sub = lane / EW;
+          const unsigned char* from = out + sub * PITCH + (wd & 1) * 8;
+          const int ch = (wd >> 1) ^ xored(sub);  // (the rows' other bits join below)
+          const int left = col0 + wd < a.L ? a.M - row0 - sub : 0;
+          uint64_t* y = a.Y + ((size_t)g.n * a.M + row0 + sub) * a.ldy + col0 + wd;
+          // Eight rows' words are read before the first is stored: the compiler keeps the order of loads
+          // and stores, and one at a time costs their latency each.  122 x 130->200: 179 -> 167 us,
+          // adapters 45 x 257->384: 276 -> 262, 256 x 128->10: 177 -> 153; where the epilogue has time
+          // (256 x 784->128: 900 -> 930, 64 x 512->512: 537 -> 555) the bursts hold up the copies of X.
+          constexpr int BATCH = 8;
+#pragma unroll 1
+          for (int b = 0; b < 32; b += BATCH * PER, from += BATCH * PER * PITCH) {
+            uint64_t v[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j)
+              v[j] = *reinterpret_cast<const uint64_t*>(from + j * PER * PITCH +
+                                                        ((ch ^ xored(j * PER)) << 4));
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+              if (b + j * PER < left) *y = v[j];
+              y += (size_t)PER * a.ldy;
+            }
           }
           __syncwarp();
         }
