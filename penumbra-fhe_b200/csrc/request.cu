@@ -768,7 +768,16 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     // the row, and leave as 32 rows x EW words by TMA, or as row segments by plain stores.
     const int e_w = warp - S::EPI_WARP;
     const int q = warp & 3, eh = e_w >> 2;
-    constexpr int EW = S::EW, CHUNKS = EW / 4;
+    // Adapters read two accumulators, so half the words of each at a time: both are then on their way
+    // together, and nothing spills (256 x 784->128 of rank 16 892 -> 879 us, 45 x 257->384 267 -> 259;
+    // several tiles to a group at an even pitch lose 3%).
+    constexpr int EW = S::EW, CW = ADAPT ? 2 : 4, CHUNKS = EW / CW, COLS = 8 * CW;
+    auto tmem_ld = [](uint32_t at, uint32_t (&r)[COLS]) {
+      if constexpr (COLS == 16)
+        tc::tmem_ld_32x32_x16(at, r);
+      else
+        tc::tmem_ld_32x32_nowait(at, r);
+    };
     constexpr int PARTS = SPLIT ? 2 : 1, PITCH = EW * 8 / PARTS;  // staged one after the other
     const uint32_t out_at = base + (uint32_t)(a.out_at + e_w * (S::OUT / PARTS));
     unsigned char* out = rq_raw + (out_at - raw);
@@ -843,50 +852,47 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         if (a.bias && body < EW && row0 + lane < a.M)
           bias = (uint64_t)__ldg(a.bias + (ADAPT ? (size_t)0 : (size_t)w * a.M) + row0 + lane) *
                  a.delta;
-        // 4 words (32 columns) at a time, the next columns on their way while these are added up
-        uint32_t c[2][32], d[32];
-        tc::tmem_ld_32x32_nowait(c_tmem, c[0]);
+        // CW words at a time, the next ones' columns on their way while these are added up
+        uint32_t c[2][COLS], d[2][COLS];
+        auto fetch = [&](int i) {
+          tmem_ld(c_tmem + (uint32_t)(i * COLS), c[i & 1]);
+          if (has) tmem_ld(d_tmem + (uint32_t)(eh * EW * 8 + i * COLS), d[i & 1]);
+        };
+        fetch(0);
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) {
-          uint32_t(&ci)[32] = c[i & 1];
-          tc::tmem_ld_wait_for(ci);
-          if (has) {
-            tc::tmem_ld_32x32_nowait(d_tmem + (uint32_t)(eh * EW * 8 + i * 32), d);
-          } else if (i + 1 < CHUNKS) {
-            tc::tmem_ld_32x32_nowait(c_tmem + (uint32_t)((i + 1) * 32), c[(i + 1) & 1]);
-          }
-          uint64_t y[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            y[u] = add_limbs(0, ci + 8 * u);
-            if (ADAPT) y[u] <<= a.shift;
-          }
-          if (has) {
-            tc::tmem_ld_wait_for(d);
-            if (i + 1 < CHUNKS)
-              tc::tmem_ld_32x32_nowait(c_tmem + (uint32_t)((i + 1) * 32), c[(i + 1) & 1]);
-          }
-          if (i + 1 == CHUNKS) {
+          tc::tmem_ld_wait_for(c[i & 1]);
+          if (has) tc::tmem_ld_wait_for(d[i & 1]);
+          if (i + 1 < CHUNKS) {
+            fetch(i + 1);
+          } else {
             tc::tc_fence_before();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(acc_empty + 8 * buf);
           }
+          uint64_t y[CW];
+#pragma unroll
+          for (int u = 0; u < CW; ++u) {
+            y[u] = add_limbs(0, c[i & 1] + 8 * u);
+            if (ADAPT) y[u] <<= a.shift;
+          }
           if (has) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) y[u] = add_limbs(y[u], d + 8 * u);
+            for (int u = 0; u < CW; ++u) y[u] = add_limbs(y[u], d[i & 1] + 8 * u);
           }
           constexpr int STAGED = CHUNKS / PARTS;
-          const int c2 = 2 * (i % STAGED);
+          const int c2 = CW / 2 * (i % STAGED);
           if (!SHIFTED && c2 == 0) {  // what was staged before has left
             if (lane == 0) tc::tma_store_wait_read();
             __syncwarp();
           }
-          *reinterpret_cast<ulonglong2*>(out_row + ((c2 ^ out_x) << 4)) = make_ulonglong2(y[0], y[1]);
-          *reinterpret_cast<ulonglong2*>(out_row + (((c2 + 1) ^ out_x) << 4)) =
-              make_ulonglong2(y[2], y[3]);
+#pragma unroll
+          for (int u = 0; u < CW; u += 2)
+            *reinterpret_cast<ulonglong2*>(out_row + (((c2 + u / 2) ^ out_x) << 4)) =
+                make_ulonglong2(y[u], y[u + 1]);
           if ((i + 1) % STAGED != 0) continue;
-          const int w0 = (i + 1 - STAGED) * 4;  // the first staged word
-          if (body >= w0 && body < (i + 1) * 4) {
+          const int w0 = (i + 1 - STAGED) * CW;  // the first staged word
+          if (body >= w0 && body < (i + 1) * CW) {
             uint64_t* p = reinterpret_cast<uint64_t*>(
                 out_row + ((((body - w0) >> 1) ^ out_x) << 4) + (body & 1) * 8);
             *p += bias;
