@@ -175,11 +175,16 @@ int expert_route(const int32_t* ids, int n, int experts, int32_t* offsets, int32
 // words, so that dispatch reads a token once however many rows it becomes, and combine writes it
 // once.  Rows at even pitches with aligned bases move 16 bytes at a time, others 8.  Runs do not end
 // with a ciphertext: 1025 units of 16 bytes would leave every second round of a block to one
-// thread.  Measured on 96 x 2 tokens of 128 ciphertexts (604 MB): dispatch 97 us with four loads of
-// a thread on their way (105 with one); combine, which has two rows' loads on their way for each of
-// them, 102 us with one (110 with two, 145 with four: fewer warps fit).
-constexpr int MV_THREADS = 256;
-template <bool COMBINE> constexpr int mv_ahead() { return COMBINE ? 1 : 4; }
+// thread.  What is left is to have enough loads on their way: units per thread times the threads
+// that fit, four blocks a multiprocessor.  Measured on 96 x 2 tokens of 128 ciphertexts (604 MB, floor
+// 92 us): combine, which holds two rows' words beside the sums, 94 us with three units of 16 bytes (106
+// with one in eight blocks, 104 with three in three, 129 with three in five, which leave 48
+// registers), dispatch 98 us with four (105 with one); at an odd pitch combine 113 us with four of 8
+// bytes (162 with one), dispatch 107 us with five (115 with four).
+constexpr int MV_THREADS = 256, MV_BLOCKS = 4;
+template <int WORDS, bool COMBINE> constexpr int mv_ahead() {
+  return (COMBINE ? 3 : 4) + (WORDS == 1 ? 1 : 0);
+}
 
 struct MoveArgs {
   const int32_t* choice_row;  // [tokens][top_k]
@@ -204,8 +209,8 @@ __device__ __forceinline__ void mv_madd(ulonglong2& a, ulonglong2 v, unsigned lo
 }
 
 template <int WORDS, bool COMBINE>
-__global__ void __launch_bounds__(MV_THREADS) move_kernel(const MoveArgs a) {
-  constexpr int MV_AHEAD = mv_ahead<COMBINE>(), MV_RUN = MV_THREADS * MV_AHEAD;
+__global__ void __launch_bounds__(MV_THREADS, MV_BLOCKS) move_kernel(const MoveArgs a) {
+  constexpr int MV_AHEAD = mv_ahead<WORDS, COMBINE>(), MV_RUN = MV_THREADS * MV_AHEAD;
   using T = typename MvUnit<WORDS>::T;
   const int choices = a.tokens * a.top_k;
   const long long units = (long long)a.features * a.per_row;
@@ -296,8 +301,8 @@ static int move_launch(MoveArgs a, cudaStream_t st) {
   a.shift = 0;
   while ((2 << a.shift) < a.per_row) ++a.shift;
   a.magic = (uint32_t)((((uint64_t)1 << (32 + a.shift)) + a.per_row - 1) / a.per_row);
-  constexpr int MV_RUN = MV_THREADS * mv_ahead<COMBINE>();
-  const long long runs = ((long long)a.features * a.per_row + MV_RUN - 1) / MV_RUN;
+  const int run = MV_THREADS * (wide ? mv_ahead<2, COMBINE>() : mv_ahead<1, COMBINE>());
+  const long long runs = ((long long)a.features * a.per_row + run - 1) / run;
   if (runs > 0x7fffffffLL) {
     set_error("%s: tokens of %d ciphertexts of %d words exceed one launch",
               COMBINE ? "expert_combine" : "expert_dispatch", a.features, a.L);
