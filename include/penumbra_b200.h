@@ -226,7 +226,7 @@ int pnb_lwe_contract_gather_ld(const int8_t* W_dev, const int64_t* bias_dev, uin
  * each encrypted under its own key, each with its own weights.  Routing is in the clear.  All
  * results are exact mod 2^64; rows are ciphertexts at explicit pitches as in the _ld calls above.
  * Rows at an even pitch from a 16-byte aligned base move as tiles; others are copied word by word
- * on the way, which takes up to 1.6 times as long.
+ * on the way, which takes up to 1.8 times as long.
  * Indices are checked on the device: a value outside its range counts as unused, never as an
  * address.  Outputs must not overlap inputs.  Every call runs on the current device,
  * asynchronously on `stream`; two calls at once need their own output buffers only.  The

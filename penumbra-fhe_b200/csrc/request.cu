@@ -28,10 +28,11 @@
 // longer but cost more (45 x 257->384: 263 -> 295 us).
 //
 // Measured (sustained, SM clock falling to 1.2-1.7 GHz under the power cap; in brackets the best
-// launch): 256 x 784->128 of 16 experts 670-710 us (606) = 5.4-5.7 TB/s (6.3); with adapters of rank
-// 16 857 us (743) = 4.5 TB/s (5.2); one request 13 us, 15 with an adapter of rank 8.  At an odd pitch 256 x
-// 784->128 760-880 us, 122 x 130->200 166-180 us, 45 x 257->384 of rank 33 264 us.  DRAM is busy
-// 74% of a short run of 64 x 784->128 (its bytes are the algorithm's), the tensor pipe 34%.
+// launch): 256 x 784->128 of 16 experts 737 us (605) = 5.2 TB/s (6.3); with adapters of rank 16 895 us
+// (743) = 4.3 TB/s (5.2); one request 13 us, 15 with an adapter of rank 8.  122 x 130->200 140 us
+// (117), 45 x 257->384 of rank 33 231 us (216).  At an odd pitch 256 x 784->128 920 us (799), 122 x 130->200
+// 163 us (146), 45 x 257->384 of rank 33 263 us (249).  DRAM is busy 74% of a short run of 64 x
+// 784->128 (its bytes are the algorithm's), the tensor pipe 34%.
 //
 // Adapters: the low-rank pair rides on the same pass over X.  While the K loop accumulates
 // C = W X it also accumulates the transposed low product  L^T = X^T A^T  (the X tile as the M = 128
@@ -47,7 +48,7 @@
 // results leave by TMA.  Other rows (contiguous [count][kN+1] ciphertexts) are off by one word
 // every other row, which no tiled load can shift: they land unshifted in a ring of raw slots, and
 // four warps copy them word by word into the operand layout.  (8-byte cp.async into place, without
-// the ring and the copy, is slower: 256 x 784->128 760 -> 1024 us.)
+// the ring and the copy, is slower: 256 x 784->128 760 -> 1024 us at its best.)
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
