@@ -1108,6 +1108,144 @@ static void rq_plan(RqArgs& a, int sms) {
   a.bars_at = a.raw_at + a.raw_slots * S::RAW_SLOT;
 }
 
+// ---- few products -------------------------------------------------------------------------------
+// A tile of the tensor cores costs its block about 2000 cycles however small K and M are (lists, waits
+// and one warp's limb sums), so calls of few products take plain 64-bit multiply-adds instead: one
+// thread per word, 16 output rows at a time, weights in shared memory.  Weights are stored as
+// w + 128 >= 0, so that a product is one 32 x 32 + 64 and one 32 x 32 + 32 bit multiply-add, and
+// sum w x = sum (w + 128) x - 128 sum x.
+constexpr int FEW_ROWS = 16;      // per pass, and the largest rank
+constexpr int FEW_THREADS = 256;
+// Most weights (rows padded to 16) that go this way.  2049-word rows at an even pitch (odd in brackets):
+// 256 of experts 10->4 take 110 us (132) on the tensor cores and 54 here with 160 weights, 110 (135)
+// and 230 with 1024; 128 with adapters of rank 8 234 us (308) and 57 with 576, 230 (306) and 208 with
+// 2304, 230 (304) and 322 with 3584.
+template <bool ADAPT> constexpr int few_weights() { return ADAPT ? 2048 : 384; }
+
+struct FewArgs {
+  RqArgs a;
+  const int8_t *W, *A, *B;
+  const uint64_t* X;
+  int ldx, per_row, words;  // blocks of a row, and their words
+};
+
+__device__ __forceinline__ void few_madd(uint64_t& acc, uint64_t x, uint32_t w) {
+  const uint64_t lo = acc + (uint64_t)(uint32_t)x * w;
+  acc = lo + ((uint64_t)((uint32_t)(x >> 32) * w) << 32);
+}
+
+// acc[u] += sum_k (w[k][u] + 128) x_k;  returns sum_k x_k.  w: rows of `pitch` 32-bit weights.
+template <typename Load>
+__device__ __forceinline__ uint64_t few_rows(uint64_t (&acc)[FEW_ROWS], const uint32_t* w, int pitch,
+                                             int K, Load load) {
+  uint64_t sum = 0;
+#pragma unroll 4
+  for (int k = 0; k < K; ++k) {
+    const uint64_t x = load(k);
+    sum += x;
+    const uint4* wk = reinterpret_cast<const uint4*>(w + k * pitch);
+#pragma unroll
+    for (int u = 0; u < FEW_ROWS / 4; ++u) {
+      const uint4 v = wk[u];
+      few_madd(acc[4 * u], x, v.x);
+      few_madd(acc[4 * u + 1], x, v.y);
+      few_madd(acc[4 * u + 2], x, v.z);
+      few_madd(acc[4 * u + 3], x, v.w);
+    }
+  }
+  return sum;
+}
+
+template <bool ADAPT>
+__global__ void __launch_bounds__(FEW_THREADS) few_kernel(const __grid_constant__ FewArgs f) {
+  extern __shared__ __align__(16) uint32_t few_w[];  // [K][M16]; adapters: [K][16] of A, [16][M16] of B
+  const RqArgs& a = f.a;
+  const int n = (int)(blockIdx.x / (unsigned)f.per_row);
+  const int c = (int)(blockIdx.x - (unsigned)n * f.per_row) * f.words + (int)threadIdx.x;
+  int w = __ldg(a.which + n), src = n;
+  if (w < 0 || w >= a.n_which) w = -1;
+  if (!ADAPT) {
+    const int choice = __ldg(a.row_choice + n);
+    if (w < 0 || choice < 0 || choice >= a.choices) return;
+    if (a.top_k > 0) src = choice / a.top_k;
+  }
+  const bool has = ADAPT && w >= 0;
+  const int m16 = (a.M + FEW_ROWS - 1) / FEW_ROWS * FEW_ROWS;
+  uint32_t *wa = few_w + a.K * m16, *wb = wa + a.K * FEW_ROWS;
+  // weights [rows][cols] transposed to `to` [cols][pitch]; padding is w = 0
+  auto stage = [&](uint32_t* to, const int8_t* from, int rows, int cols, int pitch, int lines) {
+    for (int i = threadIdx.x; i < lines * pitch; i += FEW_THREADS) {
+      const int col = i / pitch, row = i - col * pitch;
+      to[i] = 128u + (uint32_t)(row < rows && col < cols ? (int)__ldg(from + (size_t)row * cols + col) : 0);
+    }
+  };
+  stage(few_w, f.W + (ADAPT ? (size_t)0 : (size_t)w * a.M * a.K), a.M, a.K, m16, a.K);
+  if (has) {
+    stage(wa, f.A + (size_t)w * a.rank * a.K, a.rank, a.K, FEW_ROWS, a.K);
+    stage(wb, f.B + (size_t)w * a.M * a.rank, a.M, a.rank, m16, FEW_ROWS);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x >= f.words || c >= a.L) return;
+  const uint64_t* x = f.X + (size_t)src * a.K * f.ldx + c;
+  auto load = [&](int k) { return __ldg(x + (size_t)k * f.ldx); };
+  uint64_t t[FEW_ROWS] = {}, t_sum = 0;
+  if (has) {
+    const uint64_t sum = few_rows(t, wa, FEW_ROWS, a.K, load);
+#pragma unroll
+    for (int q = 0; q < FEW_ROWS; ++q) {  // rows past the rank are zero: 128 sum - 128 sum
+      t[q] -= 128 * sum;
+      t_sum += t[q];
+    }
+  }
+  uint64_t* y = a.Y + (size_t)n * a.M * a.ldy + c;
+  for (int j0 = 0; j0 < a.M; j0 += FEW_ROWS) {
+    uint64_t acc[FEW_ROWS] = {}, low[FEW_ROWS] = {};
+    const uint64_t sum = few_rows(acc, few_w + j0, m16, a.K, load);
+    if (has) {
+#pragma unroll
+      for (int q = 0; q < FEW_ROWS; ++q) {
+        const uint4* wq = reinterpret_cast<const uint4*>(wb + q * m16 + j0);
+#pragma unroll
+        for (int u = 0; u < FEW_ROWS / 4; ++u) {
+          const uint4 v = wq[u];
+          few_madd(low[4 * u], t[q], v.x);
+          few_madd(low[4 * u + 1], t[q], v.y);
+          few_madd(low[4 * u + 2], t[q], v.z);
+          few_madd(low[4 * u + 3], t[q], v.w);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < FEW_ROWS; ++u) {
+      if (j0 + u >= a.M) break;
+      uint64_t v = acc[u] - 128 * sum;
+      if (ADAPT) v <<= a.shift;
+      if (has) v += low[u] - 128 * t_sum;
+      if (a.bias && c == a.L - 1)
+        v += (uint64_t)__ldg(a.bias + (ADAPT ? (size_t)0 : (size_t)w * a.M) + j0 + u) * a.delta;
+      y[(size_t)(j0 + u) * a.ldy] = v;
+    }
+  }
+}
+
+// Launches it when it is the faster one, and says so.
+template <bool ADAPT>
+static int few_run(const RqArgs& a, const int8_t* W, const int8_t* A, const int8_t* B,
+                   const uint64_t* X, int ldx, bool& done, cudaStream_t st) {
+  done = false;
+  const long long m16 = (a.M + FEW_ROWS - 1) / FEW_ROWS * FEW_ROWS;
+  if (ADAPT && a.rank > FEW_ROWS) return PNB_OK;
+  const long long weights = a.K * m16 + (ADAPT ? FEW_ROWS * (a.K + m16) : 0);
+  FewArgs f{a, W, A, B, X, ldx};
+  f.per_row = (a.L + FEW_THREADS - 1) / FEW_THREADS;
+  f.words = (a.L + f.per_row - 1) / f.per_row;
+  if (weights > few_weights<ADAPT>() || (long long)a.rows * f.per_row > 0x7fffffffLL) return PNB_OK;
+  done = true;
+  few_kernel<ADAPT><<<(unsigned)(a.rows * f.per_row), FEW_THREADS, (size_t)weights * 4, st>>>(f);
+  PNB_CHECK_LAUNCH("few_kernel");
+  return PNB_OK;
+}
+
 // What the device needs once (its number of SMs read, the kernel's shared-memory limit raised), and
 // the plan.
 template <bool SHIFTED, bool ADAPT>
@@ -1164,7 +1302,17 @@ static int rq_launch(const RqMaps& tm, const RqArgs& a, int sms, bool early, cud
 template <bool ADAPT>
 static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* X, int ldx,
                   int x_groups, void* ws, size_t ws_bytes, cudaStream_t st) {
+  size_t need = W.in_place() ? 0 : W.copy_bytes();
+  if (ADAPT) need += (A.in_place() ? 0 : A.copy_bytes()) + (B.in_place() ? 0 : B.copy_bytes());
+  if (need && ws && (ws_bytes < need || ((uintptr_t)ws % 16) != 0)) {
+    set_error("%s: workspace of %zu bytes at %p, %zu bytes 16-byte aligned are needed",
+              ADAPT ? "adapter_contract" : "expert_contract", ws_bytes, ws, need);
+    return PNB_ERR_INVALID;
+  }
   using S = RqShape<false, ADAPT>;
+  bool done;
+  const int few = few_run<ADAPT>(a, W.p, A.p, B.p, X, ldx, done, st);
+  if (few || done) return few;
   const long long x_rows = (long long)x_groups * a.K;
   // TMA coordinates are 32-bit, and a tile reaches up to a slot past its first row
   constexpr long long MOST = 0x7fffffffLL - RQ_BM;
@@ -1214,14 +1362,7 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
     }
   }
   if (rc) return rc;
-  size_t need = W.in_place() ? 0 : W.copy_bytes();
-  if (ADAPT) need += (A.in_place() ? 0 : A.copy_bytes()) + (B.in_place() ? 0 : B.copy_bytes());
   int8_t* own = nullptr;
-  if (need && ws && (ws_bytes < need || ((uintptr_t)ws % 16) != 0)) {
-    set_error("%s: workspace of %zu bytes at %p, %zu bytes 16-byte aligned are needed",
-              ADAPT ? "adapter_contract" : "expert_contract", ws_bytes, ws, need);
-    return PNB_ERR_INVALID;
-  }
   if (need && !ws) PNB_CUDA(cudaMallocAsync((void**)&own, need, st));
   RqMatrix* all[3] = {&W, &A, &B};
   bool placed = false;

@@ -478,6 +478,35 @@ def test_short_k_of_many_tiles(pnb, oracle, M, K, rank, ld):
     assert pnb.device_status(0) == 0
 
 
+@pytest.mark.parametrize("K,M,rank,L,ld", [(1, 1, 1, 1, 1), (24, 16, 16, 257, 257), (12, 32, 3, 256, 258),
+                                           (25, 16, 17, 300, 301), (8, 48, 1, 835, 835),
+                                           (57, 3, 9, 70, 72), (3, 65, 5, 40, 41)])
+def test_few_products(pnb, oracle, K, M, rank, L, ld):
+    # both sides of the change to plain multiply-adds, with extreme weights, bias and unused rows
+    rng = np.random.default_rng(K * 100 + M)
+    T, k, E = 5, 2, 3
+    ids = draw_ids(rng, T, k, E, 0.3)
+    W = rng.choice([-128, 127, 0, 5], (E, M, K)).astype(np.int8)
+    bias = rng.integers(-9, 9, (E, M))
+    X = words(rng, T, K, ld)
+    X[0] = np.uint64(2**64 - 1)
+    route = pnb.expert_route(dev(ids), E)
+    got = host(pnb.expert_contract(route, dev(W), dev(bias), 1 << 40, dev(X), L,
+                                   out=marked(T * k, M, ld)))
+    want = host(marked(T * k, M, ld))
+    want[:, :, :L] = plain_contract(oracle, ids, E, W, bias, 1 << 40, X[:, :, :L], False,
+                                    want[:, :, :L].copy())
+    assert np.array_equal(got, want)
+    A = rng.choice([-128, 127], (E, rank, K)).astype(np.int8)
+    B = rng.choice([-128, 127, 1], (E, M, rank)).astype(np.int8)
+    which = np.array([0, -1, 2, 3, 1], np.int32)
+    got = host(pnb.adapter_contract(dev(W[0]), dev(bias[0]), 3, dev(A), dev(B), dev(which), dev(X), L,
+                                    base_shift=11, out=marked(T, M, ld)))
+    assert np.array_equal(got[:, :, :L], plain_adapter(oracle, W[0], bias[0], 3, A, B, which,
+                                                       X[:, :, :L], 11))
+    assert np.all(got[:, :, L:] == MARK)
+
+
 def test_strided_inputs(pnb):
     # tensors that are not contiguous are used as the values they hold
     rng = np.random.default_rng(15)
