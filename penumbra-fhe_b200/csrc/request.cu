@@ -9,9 +9,9 @@
 // requests of one call may be encrypted under different clients' keys.  The reference has one W
 // per Linear node (runtime/src/ops/linear.rs:52-75).
 //
-// One kernel for both, on the tensor cores.  A u64 word is 8 little-endian byte limbs, so the K
-// ciphertexts of a row are a u8 matrix [K][8 ld], N-contiguous: kind::i8 reads it as an MN-major
-// operand and the epilogue puts the limb sums together,
+// One kernel for both, on the tensor cores (calls of few products take plain multiply-adds, below).
+// A u64 word is 8 little-endian byte limbs, so the K ciphertexts of a row are a u8 matrix [K][8 ld],
+// N-contiguous: kind::i8 reads it as an MN-major operand and the epilogue puts the limb sums together,
 //     y = sum_b C[.][8c + b] << 8b  (mod 2^64),  |C| <= 128 * 255 * K < 2^31 for K < 65794.
 // A tile is 128 output rows x 32 words (adapters: 16) of one ciphertext row; persistent blocks walk
 // groups of tiles that share their X.  Weights are picked per tile by the TMA coordinate, so rows of
