@@ -102,7 +102,6 @@ struct RqShape {
   static constexpr int RAW_PITCH = BN + 16;            // one word of shift, to 16 bytes
   static constexpr int RAW_ROWS = ADAPT ? 64 : 32;     // rows per raw slot, half of each parity
   static constexpr int RAW_SLOT = RAW_ROWS * RAW_PITCH;
-  static constexpr int RAW_PER_X = XK / RAW_ROWS;
   static constexpr int EW = WORDS / 2;                 // words per epilogue warp
   static constexpr int OUT = 32 * EW * 8;              // its staging: 32 rows
   static constexpr bool MAY_SPLIT = !SHIFTED;          // which may be done in two parts
@@ -323,7 +322,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       tc::mbar_init(w_empty + 8 * s, mma_warps);
     }
     for (int s = 0; s < a.x_slots; ++s) {
-      tc::mbar_init(x_full + 8 * s, SHIFTED ? S::RAW_PER_X + (ADAPT ? 1 : 0) : 1);
+      tc::mbar_init(x_full + 8 * s, SHIFTED ? S::COPY + (ADAPT ? 1 : 0) : 1);
       tc::mbar_init(x_empty + 8 * s, mma_warps + (ADAPT ? 1 : 0));
     }
     for (int s = 0; s < a.raw_slots; ++s) {
@@ -485,8 +484,11 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     }
   } else if (warp < S::MMA_WARP) {
     // ---------------- raw rows -> operand layout (shifted rows only) -----------------------------
-    // Raw slot r is always copied by warp r % 4 (their number is a multiple of 4), and every warp
-    // waits for every X slot's turn: a parity tells only neighbouring turns apart.
+    // Raw slot r is always copied by warp r % 4 (their number is a multiple of 4).  Every warp waits
+    // for every X slot's turn and answers it, also where it copies nothing: a parity tells only
+    // neighbouring turns apart, so the slot must not be filled and used again before a warp has seen
+    // its turn.  (An idle warp answers early, so this costs nothing that shows: 122 x 130->200 163 us
+    // either way, 45 x 257->384 of rank 33 262.)
     const int cw = warp - 2;
     constexpr int PER = 32 / S::WORDS;  // rows per pass of a warp
     constexpr int BATCH = 16;           // passes whose words are on their way together
@@ -531,14 +533,11 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
             }
             tc::fence_async_smem();
             __syncwarp();
-            if (lane == 0) {
-              tc::mbar_arrive(r_empty + 8 * rr.slot);
-              // the last one answers for those a ragged K leaves out
-              tc::mbar_arrive_n(full, i == raws - 1 ? (uint32_t)(S::RAW_PER_X - i) : 1u);
-            }
+            if (lane == 0) tc::mbar_arrive(r_empty + 8 * rr.slot);
           }
           rr.advance(a.raw_slots);
         }
+        if (lane == 0) tc::mbar_arrive(full);  // its words are in place, if it had any
         xr.advance(a.x_slots);
         x_wrap |= xr.slot == 0;
       }
