@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(b_full + 8 * s, 1);
       tc::mbar_init(b_empty + 8 * s, 1);
-      tc::mbar_init(acc_full + 8 * s, ADAPT ? 2 : 1);
+      tc::mbar_init(acc_full + 8 * s, 1 + S::LOW_WARPS);
       tc::mbar_init(acc_empty + 8 * s, RQ_EPI_WARPS);
       tc::mbar_init(low_full + 8 * s, 1);
       tc::mbar_init(list_full + 8 * s, 1);
@@ -718,10 +718,13 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         const int m_n = tiles(g.mg);
         for (int m = 0; m < m_n; ++m, ++tt) {
           // Every tile's turn is waited for and answered, also where nothing is issued: a parity
-          // tells only neighbouring turns apart, so no role may get two turns ahead of another.
+          // tells only neighbouring turns apart, so no role may get two turns ahead of another.  The
+          // warp of D answers when D is there; that of L^T, whose products have a barrier of their
+          // own, at once.
           const int buf = tt & 1;
           if (!rq_wait(acc_empty + 8 * buf, (uint32_t)(tt >> 1) ^ 1u, abort_s)) return false;
           tc::tc_fence_after();
+          if (!d) tc::mbar_arrive(acc_full + 8 * buf);
           if (m > 0 && !finish(true)) return false;
           if (low && m == 0) {
             const uint32_t l_tmem = tmem + D_AT + (uint32_t)(buf * 128);

@@ -114,3 +114,16 @@ def test_adapters_at_an_odd_pitch(pnb, K, without, M, rank, L, batch):
     check_adapters(pnb, weights(g, M, K), bias_of(g, M), (1 << 45) + 3,
                    weights(g, n, rank, K), weights(g, n, M, rank), which_of(g, batch, n, without),
                    words(g, batch, K, ld), L, 6)
+
+
+# ---- requests without an adapter, and several tiles to a group ------------------------------------
+# The warps that issue a tile's products must stay in step also over tiles for which one of them
+# issues nothing: those of requests without an adapter, and a group's second and later tiles.
+@pytest.mark.parametrize("K,M", [(128, 33), (48, 130), (200, 128), (64, 300), (128, 700)])
+@pytest.mark.parametrize("without", ["no", "runs", "all"])
+@pytest.mark.parametrize("rank,L", [(17, 258), (64, 70)])
+def test_adapters_here_and_there(pnb, K, M, without, rank, L):
+    g = source(K + M + rank)
+    n, batch, ld = 4, 250, L + 2
+    check_adapters(pnb, weights(g, M, K), bias_of(g, M), (1 << 45) + 3, weights(g, n, rank, K),
+                   weights(g, n, M, rank), which_of(g, batch, n, without), words(g, batch, K, ld), L, 6)
