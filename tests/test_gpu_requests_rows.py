@@ -3,6 +3,8 @@ block walks through many groups, slots and turns.  The plain form runs on the GP
 words as doubles, whose products with int8 weights stay below 2^53 and so are whole numbers."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -127,3 +129,154 @@ def test_adapters_here_and_there(pnb, K, M, without, rank, L):
     n, batch, ld = 4, 250, L + 2
     check_adapters(pnb, weights(g, M, K), bias_of(g, M), (1 << 45) + 3, weights(g, n, rank, K),
                    weights(g, n, M, rank), which_of(g, batch, n, without), words(g, batch, K, ld), L, 6)
+
+
+# ---- what small calls no longer reach --------------------------------------------------------------
+# Calls of few products take plain multiply-adds; these are above that: the tiles' own range checks of
+# indices, their padded copies of weights, and whole blocks that decrypt.
+@pytest.mark.parametrize("sorted_rows", [False, True])
+@pytest.mark.parametrize("ld", [40, 41])
+def test_damaged_route_in_tiles(pnb, ld, sorted_rows):
+    g = source(50 + ld)
+    T, k, E, M, K, L = 6, 2, 3, 33, 65, 40
+    ids = torch.randint(0, E, (T, k), dtype=torch.int32, device="cuda", generator=g)
+    W, X = weights(g, E, M, K), words(g, T * k if sorted_rows else T, K, ld)
+    route = pnb.expert_route(ids, E)
+    big, low = 2147483647, -2147483648
+    choice = torch.tensor([T * k, -3, big, low, 4, 5, 6, 7, 8, 9, 10, 11], dtype=torch.int32)
+    expert = torch.tensor([0, 1, 2, 0, E, -1, big, low, 2, 1, 0, 2], dtype=torch.int32)
+    route.row_choice.copy_(choice)
+    route.row_expert.copy_(expert)
+    out = torch.full((T * k, M, ld), MARK, dtype=torch.int64, device="cuda")
+    pnb.expert_contract(route, W, None, 0, X, L, sorted_rows=sorted_rows, out=out)
+    assert bool((out[:8] == MARK).all())
+    for r in range(8, 12):
+        x = X[r if sorted_rows else r // k, :, :L]
+        assert torch.equal(out[r, :, :L], times(W[int(expert[r])], x)), r
+    assert pnb.device_status(0) == 0
+
+
+@pytest.mark.parametrize("ld", [40, 41])
+@pytest.mark.parametrize("off", [0, 3])  # weights at an aligned address, and at an odd one
+def test_padded_weights_of_the_c_abi(pnb, ld, off):
+    # rows of 65 and 17 bytes are copied to the caller's memory or, without it, to the call's own
+    g = source(60 + ld)
+    E, M, K, rank, L, batch = 3, 33, 65, 17, 40, 5
+    place = lambda t: torch.zeros(t.numel() + off, dtype=torch.int8, device="cuda")[off:].view(  # noqa: E731
+        t.shape).copy_(t)
+    W, A, B = (place(weights(g, *s)) for s in ((E, M, K), (E, rank, K), (E, M, rank)))
+    X, lib = words(g, batch, K, ld), pnb.lib()
+    a = torch.tensor([2, -1, 0, 1, 1], dtype=torch.int32, device="cuda")
+    route = pnb.expert_route(a.view(-1, 1), E)
+    x = X[:, :, :L]
+    low = torch.stack([times(B[i], times(A[i], x[b])) if i >= 0 else torch.zeros_like(x[0, :M])
+                       for b, i in enumerate(a.tolist())])
+    choice = rows_of(a, E)
+    want = {"adapter": (times(W[0], x) << 2) + low, "expert": times(W[a[choice].long()], x[choice])}
+    p = lambda t: t.data_ptr()  # noqa: E731
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def call(op, out, ws, size, at):
+        if op == "adapter":
+            return lib.pnb_adapter_contract(p(W), None, 0, 2, M, K, p(A), p(B), E, rank, p(a), p(X), ld,
+                                            p(out), ld, batch, L, ws, size, at)
+        return lib.pnb_expert_contract(p(route.row_choice), p(route.row_expert), batch, 1, E, 0, p(W),
+                                       None, 0, M, K, p(X), ld, p(out), ld, L, ws, size, at)
+
+    need = {"adapter": lib.pnb_adapter_contract_workspace_bytes(p(W), M, K, p(A), p(B), E, rank),
+            "expert": lib.pnb_expert_contract_workspace_bytes(p(W), E, M, K)}
+    assert need == {"adapter": (M + E * rank) * 80 + E * M * 32, "expert": E * M * 80}
+    new = lambda: torch.full((batch, M, ld), MARK, dtype=torch.int64, device="cuda")  # noqa: E731
+    for op in ("adapter", "expert"):
+        n, y = need[op], want[op]
+        ws = torch.full((n + 256,), 7, dtype=torch.uint8, device="cuda")
+        for at, size in ((p(ws), n), (None, 0), (p(ws), n + 256), (None, 0)):
+            out = new()
+            assert call(op, out, at, size, stream) == 0, pnb.lib().pnb_last_error()
+            assert torch.equal(out[:len(y), :, :L], y)
+            assert bool((out[len(y):] == MARK).all()) and bool((out[:, :, L:] == MARK).all())
+        assert bool((ws[n:] == 7).all())  # nothing behind the bytes asked for
+        for at, size in ((p(ws), n - 1), (p(ws) + 8, n)):
+            out = new()
+            assert call(op, out, at, size, stream) == 1
+            assert b"workspace" in lib.pnb_last_error()
+            assert bool((out == MARK).all())
+        # the call's own memory inside a graph
+        out = new()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            rc = call(op, out, None, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        for _ in range(2):
+            out.fill_(MARK)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[:len(y), :, :L], y)
+            assert bool((out[len(y):] == MARK).all())
+    assert pnb.device_status(0) == 0
+
+
+@pytest.mark.parametrize("ld", [2049, 2050])
+def test_routed_block_of_tiles_decrypts(pnb, ld):
+    """route -> expert layer -> Requant -> expert layer on the sorted rows -> weighted combine, each
+    layer above the few products: the decrypted outputs are the integer block's."""
+    ring = pnb.KeyRing(seed=78)
+    g = torch.Generator().manual_seed(33)
+    T, k, E, K, H, M, scale, L = 6, 2, 3, 40, 20, 20, 50, 2049
+    draw = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=g)  # noqa: E731
+    ids = draw(0, E, T, k)
+    ids[1, 1] = -1
+    x, W1, b1 = draw(0, 4, T, K), draw(-1, 2, E, H, K), draw(-5, 6, E, H)
+    W2, w = draw(-1, 2, E, M, H), draw(1, 4, T, k)
+
+    def at_pitch(rows):
+        out = torch.zeros(*rows.shape[:2], ld, dtype=torch.int64, device="cuda")
+        out[:, :, :L] = rows
+        return out
+
+    X = at_pitch(ring.encrypt(x.reshape(-1), scale, seed=5).reshape(T, K, L))
+    route = pnb.expert_route(ids.int().cuda(), E)
+    R = int(route.offsets[-1])
+    h = pnb.expert_contract(route, W1.to(torch.int8).cuda(), b1.cuda(), 1 << scale, X, L)[:R, :, :L]
+    reach = int(W1.abs().sum(2).max() * 3 + 5)
+    fresh = math.log2(ring.params.glwe_std) + 64
+    sigma = fresh + 0.5 * math.log2(float((W1 ** 2).sum(2).max()))
+    hd = pnb.TensorDesc.make(H, -reach, reach, scale, sigma)
+    q, _ = pnb.requant_batch(ring, h.contiguous(), hd, shift=2, mult=1, round_bias=2, out_scale=52,
+                             out_sigma=43.0)
+    # noise of the outputs: 2^43 * sqrt(sum W2^2) * sqrt(sum w^2) <= 2^43 * 4.5 * 4.3 < 2^47.3, thirteen
+    # of them below half a step of 2^52
+    rows = torch.zeros(T * k, H, ld, dtype=torch.int64, device="cuda")
+    rows[:R] = at_pitch(q.reshape(R, H, L))
+    y = pnb.expert_contract(route, W2.to(torch.int8).cuda(), None, 0, rows, L, sorted_rows=True)
+    out = pnb.expert_combine(route, y, L, weights=w.int().cuda())
+    got = ring.decrypt(out[:, :, :L].contiguous(), 52).cpu()
+    want = torch.zeros(T, M, dtype=torch.int64)
+    for t in range(T):
+        for i in range(k):
+            if ids[t, i] >= 0:
+                a = W1[ids[t, i]] @ x[t] + b1[ids[t, i]]
+                a = ((a.clamp(min=0) + 2) >> 2).clamp(0, 3)
+                want[t] += w[t, i] * (W2[ids[t, i]] @ a)
+    assert int(want.abs().max()) < 1 << 10  # what a scale of 2^52 holds with the padding bit
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("ld", [2049, 2050])
+def test_adapters_in_tiles_of_clients_with_different_keys(pnb, ld):
+    keys = [pnb.keygen(seed=s, device=0) for s in (43, 44)]
+    g = torch.Generator().manual_seed(34)
+    K, M, rank, delta, shift, L = 70, 40, 20, 1 << 40, 4, 2049
+    draw = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=g)  # noqa: E731
+    W, A, B, x = draw(-8, 9, M, K), draw(-3, 4, 2, rank, K), draw(-3, 4, 2, M, rank), draw(0, 4, 2, K)
+    X = torch.zeros(2, K, ld, dtype=torch.int64, device="cuda")
+    for i in range(2):
+        X[i, :, :L] = pnb.encrypt(keys[i], x[i], seed=60 + i, delta=delta)
+    Y = pnb.adapter_contract(W.to(torch.int8).cuda(), None, 0, A.to(torch.int8).cuda(),
+                             B.to(torch.int8).cuda(),
+                             torch.tensor([1, 0], dtype=torch.int32, device="cuda"), X, L,
+                             base_shift=shift)
+    for i in range(2):
+        ph = pnb.phase(keys[i], Y[i, :, :L].contiguous()).cpu().double()
+        want = ((W @ x[i]) << shift) + B[1 - i] @ (A[1 - i] @ x[i])
+        assert torch.equal(torch.round(ph / delta).long(), want)
