@@ -280,3 +280,34 @@ def test_adapters_in_tiles_of_clients_with_different_keys(pnb, ld):
         ph = pnb.phase(keys[i], Y[i, :, :L].contiguous()).cpu().double()
         want = ((W @ x[i]) << shift) + B[1 - i] @ (A[1 - i] @ x[i])
         assert torch.equal(torch.round(ph / delta).long(), want)
+
+
+# ---- every way of sharing out a block's memory, every row ------------------------------------------
+# Weights kept or streamed, X kept for several tiles of rows or read again: a slot let go too early, or
+# weights kept over a change of expert, shows in a few rows and tiles, and in no status.
+PLANS = [(600, 700, 64, 34), (600, 700, 64, 33), (1100, 130, 20, 34), (260, 1500, 40, 34),
+         (260, 1500, 40, 33), (128, 5000, 3, 34), (128, 784, 16, 33), (128, 784, 64, 34)] + [
+    (M, K, rank, ld) for M, K, rank in ((896, 128, 16), (800, 97, 16), (769, 128, 33), (640, 128, 64),
+                                        (1537, 128, 8), (1664, 64, 1), (256, 256, 48)) for ld in (33, 34)]
+
+
+@pytest.mark.parametrize("M,K,rank,ld", PLANS)
+def test_every_row_of_every_plan(pnb, M, K, rank, ld):
+    g = source(M + K + rank)
+    n, batch, L = 3, 170, 33
+    W, X = weights(g, n, M, K), words(g, batch, K, ld)
+    check_adapters(pnb, W[0], None, 0, weights(g, n, rank, K), weights(g, n, M, rank),
+                   which_of(g, batch, n, "runs"), X, L, 9, step=16)
+    ids = torch.randint(-1, n, (batch, 1), dtype=torch.int32, device="cuda", generator=g)
+    check_experts(pnb, ids, W, None, 0, X, L, step=16)
+
+
+# Words across the tiles of 32 (16 beside adapters), among them a last one of a single word.
+@pytest.mark.parametrize("L,ld", [(2049, 2050), (2049, 2049), (835, 838), (97, 98), (1, 1), (16, 18)])
+def test_every_row_of_a_wide_call(pnb, L, ld):
+    g = source(L + ld)
+    E, T, k, K, M, rank = 7, 90, 2, 130, 200, 24
+    ids = torch.randint(-1, E, (T, k), dtype=torch.int32, device="cuda", generator=g)
+    check_experts(pnb, ids, weights(g, E, M, K), bias_of(g, E, M), 12345, words(g, T, K, ld), L, step=16)
+    check_adapters(pnb, weights(g, M, K), bias_of(g, M), 12345, weights(g, E, rank, K),
+                   weights(g, E, M, rank), which_of(g, T, E, "runs"), words(g, T, K, ld), L, 4, step=16)
