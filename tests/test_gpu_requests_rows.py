@@ -311,3 +311,24 @@ def test_every_row_of_a_wide_call(pnb, L, ld):
     check_experts(pnb, ids, weights(g, E, M, K), bias_of(g, E, M), 12345, words(g, T, K, ld), L, step=16)
     check_adapters(pnb, weights(g, M, K), bias_of(g, M), 12345, weights(g, E, rank, K),
                    weights(g, E, M, rank), which_of(g, T, E, "runs"), words(g, T, K, ld), L, 4, step=16)
+
+
+# ---- the largest limb sums --------------------------------------------------------------------------
+# 65536 weights of -128 against bytes of 255 reach -2139095040, 0.4% from the end of 32 bits; both for
+# the contraction and for the low product of an adapter.
+@pytest.mark.parametrize("L,ld", [(33, 34), (33, 33)])
+@pytest.mark.parametrize("value", [-128, 127])
+def test_largest_limb_sums(pnb, L, ld, value):
+    E, T, M, K, rank = 2, 3, 20, 65536, 17
+    W = torch.full((E, M, K), value, dtype=torch.int8, device="cuda")
+    X = torch.full((T, K, ld), -1, dtype=torch.int64, device="cuda")  # words of all ones
+    ids = torch.tensor([[1], [0], [1]], dtype=torch.int32, device="cuda")
+    check_experts(pnb, ids, W, None, 0, X, L)
+    A = torch.full((E, rank, K), value, dtype=torch.int8, device="cuda")
+    B = torch.full((E, M, rank), -128, dtype=torch.int8, device="cuda")
+    B[1] = 127
+    which = torch.tensor([1, -1, 0], dtype=torch.int32, device="cuda")
+    check_adapters(pnb, W[0], None, 0, A, B, which, X, L, 3)
+    if value == -128:  # -128 * 65536 * (2^64 - 1) = 2^23 mod 2^64
+        out = pnb.expert_contract(pnb.expert_route(ids, E), W, None, 0, X, L)
+        assert bool((out[:, :, :L] == 1 << 23).all())
