@@ -332,3 +332,51 @@ def test_largest_limb_sums(pnb, L, ld, value):
     if value == -128:  # -128 * 65536 * (2^64 - 1) = 2^23 mod 2^64
         out = pnb.expert_contract(pnb.expert_route(ids, E), W, None, 0, X, L)
         assert bool((out[:, :, :L] == 1 << 23).all())
+
+
+# ---- inputs and outputs at different pitches, through the C ABI ------------------------------------
+@pytest.mark.parametrize("L", [33, 34, 257])
+@pytest.mark.parametrize("dx,dy", [(0, 1), (1, 0), (0, 3), (3, 1), (1, 2), (2, 0)])
+@pytest.mark.parametrize("K,M,rank", [(3, 4, 2), (70, 40, 20), (65, 200, 33)])  # few products, tiles
+def test_pitches_apart(pnb, L, dx, dy, K, M, rank):
+    g = source(L + 10 * dx + dy)
+    lib, E, T, k = pnb.lib(), 3, 9, 2
+    ldx, ldy, n = L + dx, L + dy, T * k
+    stream = torch.cuda.current_stream().cuda_stream
+    p = lambda t: t.data_ptr()  # noqa: E731
+    ids = torch.randint(-1, E, (T, k), dtype=torch.int32, device="cuda", generator=g)
+    w = torch.randint(-99, 99, (T, k), dtype=torch.int32, device="cuda", generator=g)
+    route = pnb.expert_route(ids, E)
+    choice = rows_of(ids, E)
+    R = len(choice)
+    W, X, Y = weights(g, E, M, K), words(g, T, K, ldx), words(g, n, K, ldx)
+    A, B = weights(g, E, rank, K), weights(g, E, M, rank)
+    a = which_of(g, T, E, "runs")
+
+    def same(out, rows, want):
+        assert torch.equal(out[:rows, :, :L], want)
+        assert bool((out[rows:] == MARK).all()) and bool((out[:, :, L:] == MARK).all())
+
+    new = lambda *s: torch.full((*s, ldy), MARK, dtype=torch.int64, device="cuda")  # noqa: E731
+    out = new(n, M)
+    assert lib.pnb_expert_contract(p(route.row_choice), p(route.row_expert), T, k, E, 0, p(W), None, 0, M,
+                                   K, p(X), ldx, p(out), ldy, L, None, 0, stream) == 0
+    same(out, R, times(W[ids.reshape(-1)[choice].long()], X[choice // k, :, :L]))
+    out = new(T, M)
+    assert lib.pnb_adapter_contract(p(W), None, 0, 5, M, K, p(A), p(B), E, rank, p(a), p(X), ldx, p(out),
+                                    ldy, T, L, None, 0, stream) == 0
+    x, i = X[:, :, :L], a.long().clamp(min=0)
+    same(out, T, (times(W[0], x) << 5) +
+         torch.where((a >= 0).view(-1, 1, 1), times(B[i], times(A[i], x)), 0))
+    out = new(n, K)
+    assert lib.pnb_expert_dispatch(p(route.choice_row), T, k, p(w), p(X), K, ldx, p(out), ldy, L,
+                                   stream) == 0
+    same(out, R, X[choice // k, :, :L] * w.reshape(-1)[choice].long().view(-1, 1, 1))
+    out = new(T, K)
+    assert lib.pnb_expert_combine(p(route.choice_row), T, k, p(w), p(Y), K, ldx, p(out), ldy, L,
+                                  stream) == 0
+    want = torch.zeros(T, K, L, dtype=torch.int64, device="cuda")
+    want.index_add_(0, choice // k, Y[:R, :, :L] * w.reshape(-1)[choice].long().view(-1, 1, 1))
+    same(out, T, want)
+    torch.cuda.synchronize()
+    assert pnb.device_status(0) == 0
