@@ -229,8 +229,9 @@ int pnb_lwe_contract_gather_ld(const int8_t* W_dev, const int64_t* bias_dev, uin
  * on the way, which takes up to 1.8 times as long.
  * Indices are checked on the device: a value outside its range counts as unused, never as an
  * address.  Outputs must not overlap inputs.  Every call runs on the current device,
- * asynchronously on `stream`; two calls at once need their own output buffers only.  The
- * reference has one weight matrix per Linear node (runtime/src/ops/linear.rs:52-75). */
+ * asynchronously on `stream`; two calls at once need output buffers of their own, and workspaces
+ * where they are given any.  The reference has one weight matrix per Linear node
+ * (runtime/src/ops/linear.rs:52-75). */
 #define PNB_MAX_EXPERTS 1024
 #define PNB_MAX_CHOICES (1 << 20) /* tokens * top_k of one call */
 #define PNB_MAX_RANK 64
@@ -259,7 +260,9 @@ int pnb_expert_dispatch(const int32_t* choice_row_dev, int tokens, int top_k,
  * src = r.  Y [tokens*top_k][M][ldy]; rows from R on are left as they were.
  * Weight rows that do not start 16-byte aligned (K not a multiple of 16) are first copied to
  * rows that do, in `workspace` (16-byte aligned, pnb_expert_contract_workspace_bytes, 0 when none
- * is needed; one per call in flight) or, when that is NULL, in memory allocated on `stream`. */
+ * is needed; one per call in flight) or, when that is NULL, in memory allocated on `stream`.
+ * Calls of few products read such rows in place, but a workspace that is given is checked there
+ * too. */
 int pnb_expert_contract(const int32_t* row_choice_dev, const int32_t* row_expert_dev, int tokens,
                         int top_k, int experts, int sorted_rows, const int8_t* W_dev,
                         const int64_t* bias_dev, uint64_t delta, int M, int K,

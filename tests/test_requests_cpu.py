@@ -129,3 +129,18 @@ def test_binding_refuses_host_tensors(pnb):
         pnb.adapter_contract(W[0], None, 0, W, W, ids[:, 0], X)
     with pytest.raises(TypeError, match="64-bit"):
         pnb.expert_dispatch(route, X.to(torch.int32))
+
+
+@pytest.mark.parametrize("off", [0, 1, 8, 16])
+@pytest.mark.parametrize("rows,cols", [(3, 16), (3, 17), (1, 1), (7, 32), (5, 784), (5, 785), (2, 33)])
+def test_binding_and_library_agree_on_workspaces(pnb, off, rows, cols):
+    # the binding works them out by itself, and the library refuses one that is too small
+    base = torch.zeros(rows * cols + 64, dtype=torch.int8)
+    t = base[-base.data_ptr() % 16 + off:][:rows * cols].view(rows, cols)
+    at, L = C.c_void_p(t.data_ptr()), pnb.lib()
+    one = pnb._padded(t, rows, cols)
+    assert one == L.pnb_expert_contract_workspace_bytes(at, 1, rows, cols)
+    assert one == L.pnb_expert_contract_workspace_bytes(at, rows, 1, cols)
+    if cols <= 64:  # W [rows][cols], two adapters of rank cols over cols inputs
+        three = one + pnb._padded(t, 2 * cols, cols) + pnb._padded(t, 2 * rows, cols)
+        assert three == L.pnb_adapter_contract_workspace_bytes(at, rows, cols, at, at, 2, cols)
