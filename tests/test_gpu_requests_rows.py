@@ -380,3 +380,38 @@ def test_pitches_apart(pnb, L, dx, dy, K, M, rank):
     same(out, T, want)
     torch.cuda.synchronize()
     assert pnb.device_status(0) == 0
+
+
+# ---- two host threads at once -----------------------------------------------------------------------
+def test_two_threads_at_once(pnb):
+    # each on a stream of its own, through tiles with padded weights, few products and both pitches
+    import threading
+
+    def work(seed, ld, errors):
+        try:
+            torch.cuda.set_device(0)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                g = source(seed)
+                E, T, L = 4, 60, 130
+                for K, M, rank in ((70, 40, 20), (3, 4, 2), (130, 200, 33)) * 3:
+                    ids = torch.randint(-1, E, (T, 2), dtype=torch.int32, device="cuda", generator=g)
+                    route = pnb.expert_route(ids, E)
+                    W, X = weights(g, E, M, K), words(g, T, K, ld)
+                    A, B, a = weights(g, E, rank, K), weights(g, E, M, rank), which_of(g, T, E, "runs")
+                    y = pnb.expert_contract(route, W, None, 0, X, L)
+                    z = pnb.adapter_contract(W[0], None, 0, A, B, a, X, L)
+                    c, x, i = rows_of(ids, E), X[:, :, :L], a.long().clamp(min=0)
+                    assert torch.equal(y[:len(c), :, :L], times(W[ids.reshape(-1)[c].long()], x[c // 2]))
+                    assert torch.equal(z[:, :, :L], times(W[0], x) + torch.where(
+                        (a >= 0).view(-1, 1, 1), times(B[i], times(A[i], x)), 0))
+        except BaseException as e:  # handed to the test's own thread
+            errors.append(e)
+
+    errors = []
+    threads = [threading.Thread(target=work, args=(90 + ld, ld, errors)) for ld in (131, 132)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    assert pnb.device_status(0) == 0
