@@ -281,7 +281,8 @@ int pnb_expert_combine(const int32_t* choice_row_dev, int tokens, int top_k,
  *             (+ bias[j] * delta on the body),   a = adapter[b].
  * W int8 [M][K], A int8 [adapters][rank][K], B int8 [adapters][M][rank], adapter int32 [batch]; a
  * request whose adapter is outside [0, adapters) gets the shared projection alone.  base_shift
- * (0..63) puts the shared weights on the grid of the adapters' products.  1 <= rank <=
+ * (0..63) puts the shared weights on the grid of the adapters' products, one for all requests of a
+ * call.  1 <= rank <=
  * PNB_MAX_RANK, K <= 65536; X [batch][K][ldx], Y [batch][M][ldy].  The workspace is as for
  * pnb_expert_contract (rows of B are `rank` long). */
 int pnb_adapter_contract(const int8_t* W_dev, const int64_t* bias_dev, uint64_t delta,

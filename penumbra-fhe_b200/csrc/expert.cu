@@ -27,7 +27,7 @@ namespace cg = cooperative_groups;
 // within a warp" is choice order and the sort is stable without atomics whose order could matter.
 // Many choices are shared out over the blocks of one cluster, which read each other's totals: what
 // one block spends its time on is the scattered stores, one line after another (8191 x 4 choices of
-// 64 experts: 41 us with one block, 14 with a cluster; 8 x 2: 6 us).
+// 64 experts: 41 us with one block, 12 with a cluster; 8 x 2: 7 us a call, 3 replayed in a graph).
 constexpr int RT_MAX_WARPS = 32;
 constexpr int RT_CLUSTER = 8;
 constexpr int RT_AHEAD = 4;  // loads of a lane on their way together

@@ -28,11 +28,13 @@
 // longer but cost more (45 x 257->384: 263 -> 295 us).
 //
 // Measured (sustained, SM clock falling to 1.2-1.7 GHz under the power cap; in brackets the best
-// launch): 256 x 784->128 of 16 experts 737 us (605) = 5.2 TB/s (6.3); with adapters of rank 16 895 us
-// (743) = 4.3 TB/s (5.2); one request 13 us, 15 with an adapter of rank 8.  122 x 130->200 140 us
-// (117), 45 x 257->384 of rank 33 231 us (216).  At an odd pitch 256 x 784->128 920 us (799), 122 x 130->200
-// 163 us (146), 45 x 257->384 of rank 33 263 us (249).  DRAM is busy 74% of a short run of 64 x
-// 784->128 (its bytes are the algorithm's), the tensor pipe 34%.
+// launch): 256 x 784->128 of 16 experts 736 us (616) = 5.2 TB/s (6.2); with adapters of rank 16 888 us
+// (755) = 4.3 TB/s (5.1); one request 10.4 us a call and 9.4 replayed in a graph, 16.9 and 11.5 with an
+// adapter of rank 8.  122 x 130->200 144 us (120), 45 x 257->384 of rank 33 240 us (220).  At an odd pitch
+// 256 x 784->128 946 us (788), 122 x 130->200 163-171 us (145), 45 x 257->384 of rank 33 262 us (251).
+// Where weights stream (large K times M) every tile reads them again: 32 x 2048->1024 1207 us, 1760
+// at an odd pitch, 1726 with adapters of rank 16; 64 x 256->2048 683.  DRAM is busy 73% of a short run of
+// 64 x 784->128 (its bytes are the algorithm's), the tensor pipe 34%.
 //
 // Adapters: the low-rank pair rides on the same pass over X.  While the K loop accumulates
 // C = W X it also accumulates the transposed low product  L^T = X^T A^T  (the X tile as the M = 128
@@ -40,9 +42,10 @@
 // operand would take 64 for any rank).  The epilogue warps add up the limbs of t = A X mod 2^64
 // across lanes, write t's bytes to shared memory as the next MN-major operand, and a short MMA makes
 // D = B t.  y = (C << s) + D.  X is read once; t never leaves the SM.  C, L^T and D of two tiles
-// fill the 512 TMEM columns at 16 words; MMAs that narrow (N = 128) read 8 KB of shared memory in
-// their 64 cycles, all that it delivers, which is what keeps adapters from the bytes' floor.  (32
-// words with one accumulator: 45 x 257->384 263 -> 388 us.)
+// fill the 512 TMEM columns at 16 words (32 words with one accumulator: 45 x 257->384 263 -> 388 us).
+// MMAs that narrow (N = 128) read 8 KB of shared memory in their 64 cycles, and a step of 32 also has 46
+// of L^T and about 36 of writing X and A, which makes shared memory busy for half the time of 64 x
+// 784->128 (202 us: DRAM 57%, tensor pipe 31%); the rest is waiting, for X or for t.
 //
 // Rows that start 16-byte aligned (an even pitch) move by TMA straight into the operand layout, and
 // results leave by TMA.  Other rows (contiguous [count][kN+1] ciphertexts) are off by one word
@@ -1059,7 +1062,8 @@ static int rq_map_weights(CUtensorMap* map, const RqMatrix& m, int box_cols, int
 // are what hides memory's latency: with weights kept, 256 x 784->128 takes 848, 713, 664 and 606 us
 // (best launches) with 3, 4, 5 and 6 of them, adapters of 640->128 713, 646, 609 and 600.  So where X
 // has fewer than six (five), results are staged in two halves, which costs short K something (256 x
-// 128->10: 110 -> 119 us) and pays for a slot.
+// 128->10: 110 -> 119 us) and pays for a slot.  (These rules were weighed at K up to 1024 and M up to
+// 512; beyond that the weights stream, and only the times above are known.)
 template <bool SHIFTED, bool ADAPT>
 static void rq_plan(RqArgs& a, int sms) {
   using S = RqShape<SHIFTED, ADAPT>;
