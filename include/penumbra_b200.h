@@ -294,6 +294,55 @@ size_t pnb_adapter_contract_workspace_bytes(const int8_t* W_dev, int M, int K,
                                             const int8_t* A_dev, const int8_t* B_dev,
                                             int adapters, int rank);
 
+/* ---- ciphertexts in fewer bits, weights in four ----------------------------------------------
+ * The conventions of the calls above: exact mod 2^64, rows at explicit pitches, indices checked on
+ * the device, asynchronous on `stream`, outputs apart from inputs.
+ *
+ * A cache keeps the ciphertexts of up to cache_slots tokens between calls, every word rounded to its
+ * top `bits` bits (16, 24 or 32): q = floor((x + 2^(63-bits)) / 2^(64-bits)) mod 2^bits.  It is
+ * [cache_slots][features] rows of lwe_len little-endian words of bits / 8 bytes, each row padded to
+ * pnb_cache_row_bytes (a multiple of 16; the padding holds nothing), 16-byte aligned, in memory of
+ * the caller.  Rounding moves a phase under a binary key of D words by a standard deviation of about
+ * 2^(64-bits) * sqrt((D / 2 + 1) / 12): 2^35.2, 2^43.2 and 2^51.2 for D = 2048.  No reference
+ * counterpart (it holds SignedRadixCiphertext in full, runtime/src/ops/mod.rs:58). */
+#define PNB_MAX_CACHE_TOKENS 65536
+size_t pnb_cache_row_bytes(int lwe_len, int bits);
+/* Token t's ciphertexts X [tokens][features][ldx] into slot slots[t].  Tokens whose slot is outside
+ * [0, cache_slots) are skipped; of two tokens that name the same slot the later one stays. */
+int pnb_cache_write(const int32_t* slots_dev, int tokens, const uint64_t* X_dev, int features,
+                    int ldx, int lwe_len, void* cache_dev, int cache_slots, int bits,
+                    void* stream);
+/* out[t][f] = the words of slot slots[t] times 2^(64-bits) (out [tokens][features][ldo]); tokens
+ * whose slot is outside [0, cache_slots) are left as they were. */
+int pnb_cache_read(const int32_t* slots_dev, int tokens, const void* cache_dev, int cache_slots,
+                   int bits, int features, uint64_t* out_dev, int ldo, int lwe_len, void* stream);
+/* A projection with 4-bit weights, a scale and a zero point per group of `group` inputs:
+ *   w[j][i] = scales[j][i/group] * (q[j][i] - zeros[j][i/group]),
+ *   Y[b][j] = sum_i w[j][i] X[b][i] (+ bias[j] * delta on the body).
+ * q: [M][ceil(K/2)] bytes, input 2i in the low nibble of byte i, values 0..15; scales int8 and zeros
+ * uint8 (their low four bits) [M][ceil(K/group)]; zeros may be NULL: 8 everywhere.  So |w| <= 1920.
+ * X [batch][K][ldx], Y [batch][M][ldy].  transposed = 1: Y[b][i] = sum_j w[j][i] X[b][j] with X
+ * [batch][M][ldx], Y [batch][K][ldy] and no bias, the gradient with respect to the inputs.  At most
+ * 65536 inputs and PNB_MAX_REQUEST_ROWS outputs.  The workspace (16-byte aligned,
+ * pnb_group_contract_workspace_bytes, one per call in flight) holds the weights as bytes; when it is
+ * NULL, memory is allocated on `stream`.
+ * Replaces: the scalar_mul / add loops of Linear::eval (runtime/src/ops/linear.rs:52-75). */
+int pnb_group_contract(const uint8_t* W_dev, const int8_t* scales_dev, const uint8_t* zeros_dev,
+                       int group, const int64_t* bias_dev, uint64_t delta, int M, int K,
+                       int transposed, const uint64_t* X_dev, int ldx, uint64_t* Y_dev, int ldy,
+                       int batch, int lwe_len, void* workspace, size_t workspace_bytes,
+                       void* stream);
+size_t pnb_group_contract_workspace_bytes(int M, int K, int transposed);
+/* The same over a cache of K ciphertexts a token, in place: request b's inputs are the words of slot
+ * slots[b].  The result is that of pnb_cache_read and pnb_group_contract.  Requests whose slot is
+ * outside [0, cache_slots) are left as they were. */
+int pnb_group_contract_cached(const uint8_t* W_dev, const int8_t* scales_dev,
+                              const uint8_t* zeros_dev, int group, const int64_t* bias_dev,
+                              uint64_t delta, int M, int K, const int32_t* slots_dev,
+                              const void* cache_dev, int cache_slots, int bits, uint64_t* Y_dev,
+                              int ldy, int batch, int lwe_len, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 /* Negacyclic products out[c] = a[c] * b[c] mod (X^N + 1) through the same f64 FFT the blind
  * rotation uses (a: small signed integers, |a| < 2^31; b: u64 torus), count polynomials.
  * Diagnostic entry point for the FFT's precision; no reference counterpart. */

@@ -26,7 +26,8 @@ __all__ = [
     "TensorDesc", "KeyRing", "op_plan", "requant_batch", "argmax_batch", "add_batch",
     "radix_plan", "lwe_contract_ld", "lwe_contract_gather_ld", "deserialize_keys",
     "serialize_lwe", "deserialize_lwe", "ExpertRoute", "expert_route", "expert_dispatch",
-    "expert_contract", "expert_combine", "adapter_contract",
+    "expert_contract", "expert_combine", "adapter_contract", "CiphertextCache", "cache_write",
+    "cache_read", "GroupWeights", "pack_int4", "group_contract", "group_contract_cached",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -120,6 +121,21 @@ _SIGS = {
     "pnb_adapter_contract_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int,
                                                           C.c_void_p, C.c_void_p, C.c_int,
                                                           C.c_int]),
+    "pnb_cache_row_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "pnb_cache_write": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int,
+                                  C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "pnb_cache_read": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int,
+                                 C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "pnb_group_contract": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                     C.c_uint64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int,
+                                     C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p,
+                                     C.c_size_t, C.c_void_p]),
+    "pnb_group_contract_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "pnb_group_contract_cached": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
+                                            C.c_void_p, C.c_uint64, C.c_int, C.c_int, C.c_void_p,
+                                            C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int,
+                                            C.c_int, C.c_int, C.c_void_p, C.c_size_t,
+                                            C.c_void_p]),
     "pnb_keys_serialized_bytes": (C.c_size_t, [C.c_void_p, C.c_int]),
     "pnb_keys_serialize": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_size_t]),
     "pnb_keys_deserialize": (C.c_int, [C.c_int, C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p)]),
@@ -620,6 +636,7 @@ def lwe_contract_gather_ld(W: torch.Tensor, bias: torch.Tensor | None, delta: in
 # ---- weights that differ from request to request ----------------------------------------------
 # These calls may be a few microseconds of GPU work, so their host side is kept short: plain checks,
 # addresses as integers, and the device switched only when it is another one.
+_MAX_WORDS = 1 << 20  # PNB_MAX_REQUEST_WORDS
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -663,10 +680,14 @@ def _want_out(out, shape, device, lwe_len: int, X: torch.Tensor) -> torch.Tensor
     if out.shape != shape or out.device != device or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {tuple(shape)} tensor on {device}, got "
                          f"{tuple(out.shape)} on {out.device}")
-    a, b = out.data_ptr(), X.data_ptr()
-    if a < b + 8 * X.numel() and b < a + 8 * out.numel():
-        raise ValueError("out overlaps the input's memory")
+    _apart("out", out, X)
     return out
+
+
+def _apart(name: str, out: torch.Tensor, X: torch.Tensor):
+    a, b = out.data_ptr(), X.data_ptr()
+    if a < b + X.numel() * X.element_size() and b < a + out.numel() * out.element_size():
+        raise ValueError(f"{name} overlaps the input's memory")
 
 
 def _at(t: torch.Tensor | None):
@@ -823,6 +844,156 @@ def adapter_contract(W: torch.Tensor, bias: torch.Tensor | None, delta: int, A: 
             A.data_ptr(), B.data_ptr(), n, rank, adapter.data_ptr(), X.data_ptr(), ld,
             out.data_ptr(), ld, batch, L, _at(ws), need)
     return out
+
+
+# ---- ciphertexts in fewer bits, weights in four -------------------------------------------------
+class CiphertextCache:
+    """``slots`` tokens of ``features`` ciphertexts, every word rounded to its top ``bits`` bits (16,
+    24 or 32; ``pnb_cache_write``).  ``data`` is uint8 [slots, features, row_bytes], made empty here
+    or given (contiguous, 16-byte aligned)."""
+
+    def __init__(self, slots: int, features: int, lwe_len: int, bits: int = 32, device="cuda",
+                 data: torch.Tensor | None = None):
+        if bits not in (16, 24, 32):
+            raise ValueError(f"words of {bits} bits, expected 16, 24 or 32")
+        if slots < 1 or features < 1 or not 1 <= lwe_len <= _MAX_WORDS:
+            raise ValueError(f"a cache of {slots} tokens of {features} ciphertexts of {lwe_len} "
+                             f"words (1..{_MAX_WORDS})")
+        self.slots, self.features, self.lwe_len, self.bits = slots, features, lwe_len, bits
+        self.row_bytes = (lwe_len * (bits // 8) + 15) // 16 * 16
+        shape = (slots, features, self.row_bytes)
+        if data is None:
+            data = torch.zeros(shape, dtype=torch.uint8, device=device)
+        elif data.dtype is not torch.uint8:
+            raise TypeError(f"data must be torch.uint8, got {data.dtype}")
+        elif data.shape != shape or not data.is_contiguous() or data.data_ptr() % 16:
+            raise ValueError(f"data must be a contiguous {shape} tensor, 16-byte aligned, got "
+                             f"{tuple(data.shape)}")
+        self.data, self.device = data, data.device
+
+    def _slots(self, slots: torch.Tensor, n=None) -> torch.Tensor:
+        if not self.data.is_cuda:
+            raise ValueError(f"the cache must be a CUDA tensor, it is on {self.device}")
+        return _want("slots", slots, torch.int32, (n,), self.device)
+
+
+def cache_write(cache: CiphertextCache, X: torch.Tensor, slots: torch.Tensor) -> CiphertextCache:
+    """Token t's ciphertexts ``X`` [tokens, features, ld] into slot ``slots[t]`` (int32 [tokens]),
+    rounded.  A slot outside the cache is skipped; of two tokens that name the same slot the later
+    one stays."""
+    X, ld, L = _want_words("X", X, cache.lwe_len, cache.device, (None, cache.features))
+    n = X.shape[0]
+    slots = cache._slots(slots, n)
+    _apart("the cache", cache.data, X)
+    _launch("pnb_cache_write", cache.device, slots.data_ptr(), n, X.data_ptr(), cache.features, ld,
+            L, cache.data.data_ptr(), cache.slots, cache.bits)
+    return cache
+
+
+def cache_read(cache: CiphertextCache, slots: torch.Tensor, ld: int | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """The ciphertexts of ``slots`` (int32 [tokens]) as u64 words [tokens, features, ld] (ld: out's, or
+    the cache's ``lwe_len``).  Tokens whose slot is outside the cache are left as they were (not set
+    when ``out`` is made here), as are words behind ``lwe_len``."""
+    slots = cache._slots(slots)
+    n, ld = slots.shape[0], _pitch(cache, ld, out)
+    out = _want_out(out, (n, cache.features, ld), cache.device, cache.lwe_len, cache.data)
+    _launch("pnb_cache_read", cache.device, slots.data_ptr(), n, cache.data.data_ptr(), cache.slots,
+            cache.bits, cache.features, out.data_ptr(), ld, cache.lwe_len)
+    return out
+
+
+def pack_int4(q: torch.Tensor) -> torch.Tensor:
+    """Values 0..15 [M, K] as nibbles, two inputs to a byte (the first one low): uint8
+    [M, ceil(K / 2)].  Signed weights -8..7 are packed as ``pack_int4(w + 8)``."""
+    if q.dim() != 2 or q.is_floating_point():
+        raise ValueError(f"q must be integers [M, K], got {q.dtype} {tuple(q.shape)}")
+    if q.numel() and not (0 <= int(q.min()) and int(q.max()) <= 15):
+        raise ValueError("values outside 0..15 do not fit four bits")
+    q = torch.nn.functional.pad(q.to(torch.uint8), (0, q.shape[1] % 2))
+    return q[:, ::2] | q[:, 1::2] << 4
+
+
+class GroupWeights:
+    """A matrix [M, K] of 4-bit weights with a scale and a zero point per ``group`` inputs:
+    ``w[j, i] = scales[j, i // group] * (q[j, i] - zeros[j, i // group])``.  ``q`` is packed as
+    ``pack_int4`` does, uint8 [M, ceil(K / 2)]; ``scales`` int8 and ``zeros`` uint8 (their low four
+    bits; None: 8) are [M, ceil(K / group)]."""
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor, group: int, K: int,
+                 zeros: torch.Tensor | None = None):
+        if q.dim() != 2 or K < 1 or group < 1:
+            raise ValueError(f"q must be [M, ceil(K / 2)] with K and group >= 1, got "
+                             f"{tuple(q.shape)}, K={K}, group={group}")
+        M = q.shape[0]
+        self.M, self.K, self.group, self.device = M, K, group, q.device
+        shape = (M, -(-K // group))
+        self.q = _want("q", q, torch.uint8, (M, (K + 1) // 2), q.device)
+        self.scales = _want("scales", scales, torch.int8, shape, q.device)
+        self.zeros = None if zeros is None else _want("zeros", zeros, torch.uint8, shape, q.device)
+
+
+def group_contract(W: GroupWeights, bias: torch.Tensor | None, delta: int, X: torch.Tensor,
+                   lwe_len: int | None = None, transposed: bool = False,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``Y[b, j] = sum_i w[j, i] X[b, i] + bias[j] * delta`` (on the body) with 4-bit weights: ``X``
+    [batch, K, ld] -> [batch, M, ld].  ``transposed``: ``Y[b, i] = sum_j w[j, i] X[b, j]``, the
+    gradient with respect to the inputs, [batch, M, ld] -> [batch, K, ld] without a bias."""
+    device = W.device
+    n_in, n_out = (W.M, W.K) if transposed else (W.K, W.M)
+    X, ld, L = _want_words("X", X, lwe_len, device, (None, n_in))
+    batch = X.shape[0]
+    if transposed and bias is not None:
+        raise ValueError("a transposed product takes no bias")
+    b = None if bias is None else _want("bias", bias, torch.int64, (W.M,), device)
+    out = _want_out(out, (batch, n_out, ld), device, L, X)
+    ws = torch.empty(_group_bytes(n_in, n_out), dtype=torch.uint8, device=device)
+    _launch("pnb_group_contract", device, W.q.data_ptr(), W.scales.data_ptr(), _at(W.zeros),
+            W.group, _at(b), delta % (1 << 64), W.M, W.K, 1 if transposed else 0, X.data_ptr(), ld,
+            out.data_ptr(), ld, batch, L, ws.data_ptr(), ws.numel())
+    return out
+
+
+def group_contract_cached(W: GroupWeights, bias: torch.Tensor | None, delta: int,
+                          cache: CiphertextCache, slots: torch.Tensor, ld: int | None = None,
+                          out: torch.Tensor | None = None) -> torch.Tensor:
+    """``group_contract`` of the ciphertexts in ``slots`` (int32 [batch]) of a cache with K features,
+    read as they lie there: [batch, M, ld] (ld: out's, or the cache's ``lwe_len``).  Requests whose
+    slot is outside the cache are left as they were (not set when ``out`` is made here), as are words
+    behind ``lwe_len``."""
+    device = cache.device
+    if W.K != cache.features:
+        raise ValueError(f"the cache holds {cache.features} ciphertexts a token, the weights take "
+                         f"{W.K}")
+    if W.device != device:
+        raise ValueError(f"the weights are on {W.device}, expected {device}")
+    slots = cache._slots(slots)
+    batch, ld = slots.shape[0], _pitch(cache, ld, out)
+    b = None if bias is None else _want("bias", bias, torch.int64, (W.M,), device)
+    out = _want_out(out, (batch, W.M, ld), device, cache.lwe_len, cache.data)
+    ws = torch.empty(_group_bytes(W.K, W.M), dtype=torch.uint8, device=device)
+    _launch("pnb_group_contract_cached", device, W.q.data_ptr(), W.scales.data_ptr(), _at(W.zeros),
+            W.group, _at(b), delta % (1 << 64), W.M, W.K, slots.data_ptr(), cache.data.data_ptr(),
+            cache.slots, cache.bits, out.data_ptr(), ld, batch, cache.lwe_len, ws.data_ptr(),
+            ws.numel())
+    return out
+
+
+def _group_bytes(n_in: int, n_out: int) -> int:
+    """``pnb_group_contract_workspace_bytes``."""
+    return 2 * n_out * ((n_in + 15) & -16)
+
+
+def _pitch(cache: CiphertextCache, ld, out) -> int:
+    """The pitch of a result made from a cache: the caller's, its buffer's or ``lwe_len``."""
+    if out is not None and out.dim() == 3:
+        if ld is not None and ld != out.shape[2]:
+            raise ValueError(f"out has a pitch of {out.shape[2]} words, not {ld}")
+        ld = out.shape[2]
+    ld = cache.lwe_len if ld is None else ld
+    if ld < cache.lwe_len:
+        raise ValueError(f"ciphertexts of {cache.lwe_len} words do not fit a pitch of {ld}")
+    return ld
 
 
 def fft_negacyclic_mul(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:

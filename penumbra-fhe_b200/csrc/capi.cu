@@ -634,6 +634,123 @@ int pnb_adapter_contract(const int8_t* W_dev, const int64_t* bias_dev, uint64_t 
                           workspace_bytes, (cudaStream_t)stream);
 }
 
+static int check_cache(const char* fn, int tokens, int bits, const void* cache, int n_slots) {
+  if (tokens < 0 || tokens > PNB_MAX_CACHE_TOKENS || n_slots < 1) {
+    set_error("%s: bad shape tokens=%d (0..%d) cache_slots=%d", fn, tokens, PNB_MAX_CACHE_TOKENS,
+              n_slots);
+    return PNB_ERR_INVALID;
+  }
+  if (bits != 16 && bits != 24 && bits != 32) {
+    set_error("%s: words of %d bits (16, 24 or 32)", fn, bits);
+    return PNB_ERR_INVALID;
+  }
+  if ((uintptr_t)cache % 16) {
+    set_error("%s: cache at %p, not 16-byte aligned", fn, cache);
+    return PNB_ERR_INVALID;
+  }
+  return PNB_OK;
+}
+
+size_t pnb_cache_row_bytes(int lwe_len, int bits) {
+  if (lwe_len < 1 || lwe_len > PNB_MAX_REQUEST_WORDS || (bits != 16 && bits != 24 && bits != 32))
+    return 0;
+  return cache_row_bytes(lwe_len, bits);
+}
+
+int pnb_cache_write(const int32_t* slots_dev, int tokens, const uint64_t* X_dev, int features,
+                    int ldx, int lwe_len, void* cache_dev, int cache_slots, int bits,
+                    void* stream) {
+  int rc = check_cache("cache_write", tokens, bits, cache_dev, cache_slots);
+  if (!rc) rc = check_rows("cache_write", features, lwe_len, ldx, lwe_len);
+  if (rc) return rc;
+  if (tokens == 0) return PNB_OK;
+  if (!slots_dev || !X_dev || !cache_dev) {
+    set_error("cache_write: NULL buffer");
+    return PNB_ERR_INVALID;
+  }
+  rc = check_aligned("cache_write", {X_dev}, {slots_dev});
+  if (rc) return rc;
+  return cache_write(slots_dev, tokens, X_dev, features, ldx, lwe_len, cache_dev, cache_slots, bits,
+                     (cudaStream_t)stream);
+}
+
+int pnb_cache_read(const int32_t* slots_dev, int tokens, const void* cache_dev, int cache_slots,
+                   int bits, int features, uint64_t* out_dev, int ldo, int lwe_len, void* stream) {
+  int rc = check_cache("cache_read", tokens, bits, cache_dev, cache_slots);
+  if (!rc) rc = check_rows("cache_read", features, lwe_len, lwe_len, ldo);
+  if (rc) return rc;
+  if (tokens == 0) return PNB_OK;
+  if (!slots_dev || !cache_dev || !out_dev) {
+    set_error("cache_read: NULL buffer");
+    return PNB_ERR_INVALID;
+  }
+  rc = check_aligned("cache_read", {out_dev}, {slots_dev});
+  if (rc) return rc;
+  return cache_read(slots_dev, tokens, cache_dev, cache_slots, bits, features, out_dev, ldo,
+                    lwe_len, (cudaStream_t)stream);
+}
+
+static int check_group(const char* fn, int M, int K, bool transposed, int group, int batch) {
+  const int rc = transposed ? check_weights(fn, K, M) : check_weights(fn, M, K);
+  if (rc) return rc;
+  if (group < 1 || batch < 0) {
+    set_error("%s: bad shape group=%d batch=%d", fn, group, batch);
+    return PNB_ERR_INVALID;
+  }
+  return PNB_OK;
+}
+
+size_t pnb_group_contract_workspace_bytes(int M, int K, int transposed) {
+  if (M < 1 || K < 1) return 0;
+  return transposed ? group_workspace_bytes(M, K) : group_workspace_bytes(K, M);
+}
+
+int pnb_group_contract(const uint8_t* W_dev, const int8_t* scales_dev, const uint8_t* zeros_dev,
+                       int group, const int64_t* bias_dev, uint64_t delta, int M, int K,
+                       int transposed, const uint64_t* X_dev, int ldx, uint64_t* Y_dev, int ldy,
+                       int batch, int lwe_len, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  int rc = check_group("group_contract", M, K, transposed != 0, group, batch);
+  if (!rc) rc = check_rows("group_contract", 1, lwe_len, ldx, ldy);
+  if (rc) return rc;
+  if (transposed && bias_dev) {
+    set_error("group_contract: a transposed product takes no bias");
+    return PNB_ERR_INVALID;
+  }
+  if (batch == 0) return PNB_OK;
+  if (!W_dev || !scales_dev || !X_dev || !Y_dev) {
+    set_error("group_contract: NULL buffer");
+    return PNB_ERR_INVALID;
+  }
+  rc = check_aligned("group_contract", {bias_dev, X_dev, Y_dev}, {});
+  if (rc) return rc;
+  return group_contract(W_dev, scales_dev, zeros_dev, group, bias_dev, delta, M, K, transposed != 0,
+                        X_dev, ldx, Y_dev, ldy, batch, lwe_len, workspace, workspace_bytes,
+                        (cudaStream_t)stream);
+}
+
+int pnb_group_contract_cached(const uint8_t* W_dev, const int8_t* scales_dev,
+                              const uint8_t* zeros_dev, int group, const int64_t* bias_dev,
+                              uint64_t delta, int M, int K, const int32_t* slots_dev,
+                              const void* cache_dev, int cache_slots, int bits, uint64_t* Y_dev,
+                              int ldy, int batch, int lwe_len, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  int rc = check_group("group_contract_cached", M, K, false, group, batch);
+  if (!rc) rc = check_rows("group_contract_cached", 1, lwe_len, lwe_len, ldy);
+  if (!rc) rc = check_cache("group_contract_cached", 0, bits, cache_dev, cache_slots);
+  if (rc) return rc;
+  if (batch == 0) return PNB_OK;
+  if (!W_dev || !scales_dev || !slots_dev || !cache_dev || !Y_dev) {
+    set_error("group_contract_cached: NULL buffer");
+    return PNB_ERR_INVALID;
+  }
+  rc = check_aligned("group_contract_cached", {bias_dev, Y_dev}, {slots_dev});
+  if (rc) return rc;
+  return group_contract_cached(W_dev, scales_dev, zeros_dev, group, bias_dev, delta, M, K,
+                               slots_dev, cache_dev, cache_slots, bits, Y_dev, ldy, batch, lwe_len,
+                               workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
 int pnb_fft_negacyclic_mul(int device, int N, const int64_t* a_dev, const uint64_t* b_dev,
                            uint64_t* out_dev, int count, void* stream) {
   if (count < 0 || (count > 0 && (!a_dev || !b_dev || !out_dev))) {

@@ -91,6 +91,22 @@ int adapter_contract(const int8_t* W, const int64_t* bias, uint64_t delta, int b
                      int K, const int8_t* A, const int8_t* B, int adapters, int rank,
                      const int32_t* adapter, const uint64_t* X, int ldx, uint64_t* Y, int ldy,
                      int batch, int L, void* ws, size_t ws_bytes, cudaStream_t st);
+// Ciphertexts rounded to fewer bits in the slots of a cache (cache.cu); contractions with 4-bit weights
+// and group scales over rows and over a cache (group.cu).  Arguments are checked by the C ABI.
+size_t cache_row_bytes(int L, int bits);
+int cache_write(const int32_t* slots, int tokens, const uint64_t* X, int features, int ldx, int L,
+                void* cache, int n_slots, int bits, cudaStream_t st);
+int cache_read(const int32_t* slots, int tokens, const void* cache, int n_slots, int bits,
+               int features, uint64_t* out, int ldo, int L, cudaStream_t st);
+size_t group_workspace_bytes(int n_in, int n_out);
+int group_contract(const uint8_t* W, const int8_t* scales, const uint8_t* zeros, int group,
+                   const int64_t* bias, uint64_t delta, int M, int K, bool transposed,
+                   const uint64_t* X, int ldx, uint64_t* Y, int ldy, int batch, int L, void* ws,
+                   size_t ws_bytes, cudaStream_t st);
+int group_contract_cached(const uint8_t* W, const int8_t* scales, const uint8_t* zeros, int group,
+                          const int64_t* bias, uint64_t delta, int M, int K, const int32_t* slots,
+                          const void* cache, int n_slots, int bits, uint64_t* Y, int ldy,
+                          int batch, int L, void* ws, size_t ws_bytes, cudaStream_t st);
 int keyswitch_tc(const pnb_keys* K, const uint64_t* in, uint64_t* out, int count, void* digits,
                  cudaStream_t st, int in_ld = 0);
 size_t ks_tc_workspace_bytes(const pnb_params& p, int count);
