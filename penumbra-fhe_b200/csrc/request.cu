@@ -56,11 +56,9 @@
 #include <atomic>
 #include <type_traits>
 
-#include <cudaTypedefs.h>
-
 #include "pnb_internal.cuh"
 #include "pnb_keys.h"
-#include "tc_primitives.cuh"
+#include "tc_tiles.cuh"
 
 namespace pnb {
 
@@ -75,8 +73,6 @@ int rq_status_read_and_clear(int* out) {
   *out = v;
   return PNB_OK;
 }
-
-PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder();
 
 constexpr int RQ_BM = 128;      // output rows per tile
 constexpr int RQ_WK = 128;      // K per weight slot
@@ -224,18 +220,6 @@ struct RqLister {
   }
 };
 
-// A ring of slots: the current one and the parity of its use.
-struct RqRing {
-  int slot = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void advance(int slots) {
-    if (++slot == slots) {
-      slot = 0;
-      phase ^= 1u;
-    }
-  }
-};
-
 // Bounded wait that also gives up as soon as another role has flagged an abort.  A completed phase
 // is found by the plain test: 145 cycles against a suspending wait's 186, which the thread that
 // issues the MMAs pays at every slot.  The rest is out of line: the roles' loops
@@ -251,33 +235,6 @@ __device__ __noinline__ bool rq_wait_slow(uint32_t bar, uint32_t parity, volatil
 }
 __device__ __forceinline__ bool rq_wait(uint32_t bar, uint32_t parity, volatile int* abort_s) {
   return tc::mbar_test(bar, parity & 1u) || rq_wait_slow(bar, parity & 1u, abort_s);
-}
-
-// No load may still be landing when the block exits: the last use of each slot completes when it has
-// landed (bounded; immediate unless a wait ran out).  `bars` are the ring's full barriers.
-__device__ __forceinline__ void rq_drain(uint32_t bars, RqRing ring, bool wrapped, int slots) {
-  for (int i = 0; i < slots; ++i)
-    if (i < ring.slot)
-      (void)tc::mbar_wait(bars + 8u * i, ring.phase, RQ_WAIT_LIMIT);
-    else if (wrapped)
-      (void)tc::mbar_wait(bars + 8u * i, ring.phase ^ 1u, RQ_WAIT_LIMIT);
-}
-
-__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int m) {
-  return (uint64_t)__shfl_xor_sync(0xffffffffu, (unsigned long long)v, m);
-}
-
-// v + sum_b c[b] << 8b mod 2^64: the low four limb sums reach into the high word (one multiply-add
-// of 32 x 32 + 64 bits each), the high four only live there.
-__device__ __forceinline__ uint64_t add_limbs(uint64_t v, const uint32_t* c) {
-  int64_t s = (int64_t)v;
-#pragma unroll
-  for (int b = 0; b < 4; ++b)
-    asm("mad.wide.s32 %0, %1, %2, %0;" : "+l"(s) : "r"((int)c[b]), "r"(1 << (8 * b)));
-  uint32_t hi = (uint32_t)((uint64_t)s >> 32);
-#pragma unroll
-  for (int b = 0; b < 4; ++b) hi += c[4 + b] << (8 * b);
-  return ((uint64_t)hi << 32) | (uint32_t)s;
 }
 
 template <bool SHIFTED, bool ADAPT, bool SPLIT>
@@ -388,7 +345,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
   if (warp == 0) {
     // ---------------- X loads (one lane) ---------------------------------------------------------
     if (lane == 0) {
-      RqRing ring;
+      TileRing ring;
       bool wrapped = false;
       const int slots = SHIFTED ? a.raw_slots : a.x_slots;
       each(true, [&](const RqGroup& g) {
@@ -420,11 +377,11 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
         }
         return true;
       });
-      rq_drain(SHIFTED ? r_full : x_full, ring, wrapped, slots);
+      tile_drain(SHIFTED ? r_full : x_full, ring, wrapped, slots, RQ_WAIT_LIMIT);
     }
   } else if (warp == 1) {
     // ---------------- the lists (the warp) and weight loads (one lane) ---------------------------
-    RqRing br;
+    TileRing br;
     bool b_wrap = false, ok = true;
     int w_slot = 0;
     uint32_t w_par = 0, w_used = 0;  // a bit per slot
@@ -483,7 +440,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       for (int s = 0; s < a.w_slots; ++s)
         if ((w_used >> s) & 1u)
           (void)tc::mbar_wait(w_full + 8 * s, ((w_par >> s) ^ 1u) & 1u, RQ_WAIT_LIMIT);
-      if (ADAPT) rq_drain(b_full, br, b_wrap, RQ_B_SLOTS);
+      if (ADAPT) tile_drain(b_full, br, b_wrap, RQ_B_SLOTS, RQ_WAIT_LIMIT);
     }
   } else if (warp < S::MMA_WARP) {
     // ---------------- raw rows -> operand layout (shifted rows only) -----------------------------
@@ -497,7 +454,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
     constexpr int BATCH = 16;           // passes whose words are on their way together
     const int word = lane % S::WORDS, sub = lane / S::WORDS;
     const int box = word >> 4, ch = (word & 15) >> 1, half = word & 1;
-    RqRing xr, rr;
+    TileRing xr, rr;
     bool x_wrap = false;
     each(false, [&](const RqGroup& g) {
       const int w = g.w;
@@ -546,7 +503,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       }
       return true;
     });
-    if (ADAPT && cw == 0 && lane == 0) rq_drain(x_full, xr, x_wrap, a.x_slots);
+    if (ADAPT && cw == 0 && lane == 0) tile_drain(x_full, xr, x_wrap, a.x_slots, RQ_WAIT_LIMIT);
   } else if (warp < S::MMA_WARP + S::MMA_WARPS) {
     // ---------------- main products (one lane of each warp) --------------------------------------
     // Tiles alternate between two warps, each with an accumulator of its own: waiting for a slot,
@@ -566,7 +523,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       const int x_slots = a.x_slots, w_slots = a.w_slots;
       const bool keep_w = a.keep_w != 0;
       const int me = warp - S::MMA_WARP;
-      RqRing x;
+      TileRing x;
       int w_slot = 0;
       uint32_t w_par = 0;
       int tt = 0;  // tiles of this warp
@@ -657,7 +614,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
           return !own   ? skip(g.load, g.drop, true)
                  : kept ? tile(yes{}, yes{}, false, false, true, true)
                         : tile(no{}, yes{}, g.load, g.drop, true, true);
-        const RqRing x0 = x;
+        const TileRing x0 = x;
         const int m0 = own ? 0 : 1;
         for (int m = 0; m < m_n; ++m) {
           if (turns && ((m ^ m0) & 1)) {
@@ -686,7 +643,7 @@ __global__ void __launch_bounds__(RqShape<SHIFTED, ADAPT>::THREADS, 1)
       const uint64_t ad = tc::smem_desc_sw128(a_at(0), 16u, 1024u);
       const uint32_t x_hi = (uint32_t)(xd >> 32), a_hi = (uint32_t)(ad >> 32);
       const int steps = (a.K + RQ_KSTEP - 1) / RQ_KSTEP;
-      RqRing x, br;
+      TileRing x, br;
       int tt = 0;
       uint32_t t_par = 0;
       int pending = -1;  // the accumulator whose t and D are still to come
@@ -1014,45 +971,8 @@ static int rq_place(RqMatrix* (&m)[3], int8_t* ws, cudaStream_t st, bool& placed
   return PNB_OK;
 }
 
-// A tiled map of `rank` dimensions (strides of all but the first, in bytes).  No promotion to larger
-// L2 reads: rows at an odd pitch would bring their neighbours' lines again (880 -> 790 us for 256 x
-// 784->128 without it; even pitches show no difference).
-static int rq_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank,
-                  const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
-                  CUtensorMapSwizzle swizzle) {
-  auto fn = tmap_encoder();
-  if (!fn) {
-    set_error("cuTensorMapEncodeTiled is unavailable from the driver");
-    return PNB_ERR_CUDA;
-  }
-  const cuuint32_t one[3] = {1, 1, 1};
-  const CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, one,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r == CUDA_SUCCESS) return PNB_OK;
-  set_error("cuTensorMapEncodeTiled failed (%d): %llu x %llu, pitch %llu", (int)r,
-            (unsigned long long)dims[0], (unsigned long long)dims[1],
-            (unsigned long long)strides[0]);
-  return PNB_ERR_CUDA;
-}
-
-// The swizzle whose span is a box row of these bytes.
-static CUtensorMapSwizzle rq_swizzle(int bytes) {
-  return bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-         : bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                       : CU_TENSOR_MAP_SWIZZLE_32B;
-}
-
-// Byte matrix [rows][cols] at a pitch, in boxes of box_cols bytes (one swizzle span) x box_rows.
-static int rq_map_bytes(CUtensorMap* map, const void* p, uint64_t cols, uint64_t rows,
-                        uint64_t pitch, int box_cols, int box_rows) {
-  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
-  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
-  return rq_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, p, 2, dims, strides, box,
-                rq_swizzle(box_cols));
-}
 static int rq_map_weights(CUtensorMap* map, const RqMatrix& m, int box_cols, int box_rows) {
-  return rq_map_bytes(map, m.p, (uint64_t)m.pitch(), (uint64_t)m.rows, (uint64_t)m.pitch(), box_cols,
+  return tile_map_bytes(map, m.p, (uint64_t)m.pitch(), (uint64_t)m.rows, (uint64_t)m.pitch(), box_cols,
                       box_rows);
 }
 
@@ -1341,8 +1261,8 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
   if (rc) return rc;
   if (!shifted) {
     const uint64_t pitch = (uint64_t)ldx * 8;
-    rc = rq_map_bytes(&tm.X[0], X, pitch, (uint64_t)x_rows, pitch, 128, S::XK);
-    if (!rc) rc = rq_map_bytes(&tm.X[1], X, pitch, (uint64_t)x_rows, pitch, 128, RQ_KSTEP);
+    rc = tile_map_bytes(&tm.X[0], X, pitch, (uint64_t)x_rows, pitch, 128, S::XK);
+    if (!rc) rc = tile_map_bytes(&tm.X[1], X, pitch, (uint64_t)x_rows, pitch, 128, RQ_KSTEP);
     // writes end at word L (rounded down to 16 bytes) of row M of each ciphertext row
     const cuuint64_t dims[3] = {(cuuint64_t)std::max(2, a.L & ~1), (cuuint64_t)a.M,
                                 (cuuint64_t)a.rows};
@@ -1350,8 +1270,8 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
     const int words = a.out_split ? S::EW / 2 : S::EW;
     const cuuint32_t box[3] = {(cuuint32_t)words, 32, 1};
     if (!rc)
-      rc = rq_map(&tm.Y, CU_TENSOR_MAP_DATA_TYPE_UINT64, a.Y, 3, dims, strides, box,
-                  rq_swizzle(8 * words));
+      rc = tile_map(&tm.Y, CU_TENSOR_MAP_DATA_TYPE_UINT64, a.Y, 3, dims, strides, box,
+                  tile_swizzle(8 * words));
   } else {
     // rows p, p + 2, ..: from the 16-byte boundary at or before row p, at twice the pitch.  A row
     // off by one word has that word's 16 bytes inside its allocation (allocations start aligned).
@@ -1363,7 +1283,7 @@ static int rq_run(RqMatrix W, RqMatrix A, RqMatrix B, RqArgs a, const uint64_t* 
                                   (cuuint64_t)std::max<long long>(1, (x_rows + 1 - p) / 2)};
       const cuuint64_t strides[1] = {(cuuint64_t)ldx * 16};
       const cuuint32_t box[2] = {S::WORDS + 2, S::RAW_ROWS / 2};
-      rc = rq_map(&tm.X[p], CU_TENSOR_MAP_DATA_TYPE_UINT64, X + (second ? ldx : 0) - off, 2, dims,
+      rc = tile_map(&tm.X[p], CU_TENSOR_MAP_DATA_TYPE_UINT64, X + (second ? ldx : 0) - off, 2, dims,
                   strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
     }
   }
