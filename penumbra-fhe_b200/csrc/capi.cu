@@ -766,7 +766,7 @@ int pnb_device_status(int device, int* status_out) {
   if (!status_out) { set_error("status_out is NULL"); return PNB_ERR_INVALID; }
   DeviceGuard g(device);
   if (g.rc) return g.rc;
-  int a = 0, b = 0, c = 0, d = 0;
+  int a = 0, b = 0, c = 0, d = 0, e = 0;
   int rc = tc_status_read_and_clear(&a);
   if (rc) return rc;
   rc = br_status_read_and_clear(&b);
@@ -775,7 +775,9 @@ int pnb_device_status(int device, int* status_out) {
   if (rc) return rc;
   rc = rq_status_read_and_clear(&d);
   if (rc) return rc;
-  *status_out = a ? a : (b ? 16 + b : (c ? 32 + c : (d ? 48 + d : 0)));
+  rc = gc_status_read_and_clear(&e);
+  if (rc) return rc;
+  *status_out = a ? a : (b ? 16 + b : (c ? 32 + c : (d ? 48 + d : (e ? 64 + e : 0))));
   return PNB_OK;
 }
 

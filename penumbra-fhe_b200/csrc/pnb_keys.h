@@ -118,4 +118,5 @@ int br_status_read_and_clear(int* out);
 int br8_status_read_and_clear(int* out);
 int ct_status_read_and_clear(int* out);
 int rq_status_read_and_clear(int* out);
+int gc_status_read_and_clear(int* out);
 }  // namespace pnb
