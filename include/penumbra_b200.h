@@ -306,6 +306,7 @@ size_t pnb_adapter_contract_workspace_bytes(const int8_t* W_dev, int M, int K,
  * 2^(64-bits) * sqrt((D / 2 + 1) / 12): 2^35.2, 2^43.2 and 2^51.2 for D = 2048.  No reference
  * counterpart (it holds SignedRadixCiphertext in full, runtime/src/ops/mod.rs:58). */
 #define PNB_MAX_CACHE_TOKENS 65536
+#define PNB_MAX_GROUP_INPUTS 61440 /* of one output: K, or M transposed */
 size_t pnb_cache_row_bytes(int lwe_len, int bits);
 /* Token t's ciphertexts X [tokens][features][ldx] into slot slots[t].  Tokens whose slot is outside
  * [0, cache_slots) are skipped; of two tokens that name the same slot the later one stays. */
@@ -323,7 +324,7 @@ int pnb_cache_read(const int32_t* slots_dev, int tokens, const void* cache_dev, 
  * uint8 (their low four bits) [M][ceil(K/group)]; zeros may be NULL: 8 everywhere.  So |w| <= 1920.
  * X [batch][K][ldx], Y [batch][M][ldy].  transposed = 1: Y[b][i] = sum_j w[j][i] X[b][j] with X
  * [batch][M][ldx], Y [batch][K][ldy] and no bias, the gradient with respect to the inputs.  At most
- * 65536 inputs and PNB_MAX_REQUEST_ROWS outputs.  The workspace (16-byte aligned,
+ * PNB_MAX_GROUP_INPUTS inputs and PNB_MAX_REQUEST_ROWS outputs.  The workspace (16-byte aligned,
  * pnb_group_contract_workspace_bytes, one per call in flight) holds the weights as bytes; when it is
  * NULL, memory is allocated on `stream`.
  * Replaces: the scalar_mul / add loops of Linear::eval (runtime/src/ops/linear.rs:52-75). */

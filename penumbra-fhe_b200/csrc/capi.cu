@@ -691,8 +691,12 @@ int pnb_cache_read(const int32_t* slots_dev, int tokens, const void* cache_dev, 
 }
 
 static int check_group(const char* fn, int M, int K, bool transposed, int group, int batch) {
-  const int rc = transposed ? check_weights(fn, K, M) : check_weights(fn, M, K);
-  if (rc) return rc;
+  const int n_in = transposed ? M : K, n_out = transposed ? K : M;
+  if (n_in < 1 || n_in > PNB_MAX_GROUP_INPUTS || n_out < 1 || n_out > PNB_MAX_REQUEST_ROWS) {
+    set_error("%s: bad weights M=%d K=%d (%d inputs, at most %d; %d outputs, at most %d)", fn, M, K,
+              n_in, PNB_MAX_GROUP_INPUTS, n_out, PNB_MAX_REQUEST_ROWS);
+    return PNB_ERR_INVALID;
+  }
   if (group < 1 || batch < 0) {
     set_error("%s: bad shape group=%d batch=%d", fn, group, batch);
     return PNB_ERR_INVALID;

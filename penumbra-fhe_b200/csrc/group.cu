@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(GF_THREADS) group_few_kernel(const __grid_cons
 }
 
 // ---- weights as bytes ---------------------------------------------------------------------------
-// Two rows of signed bytes per output, w = 256 hi + lo: row 2j holds the lo of output j, row 2j + 1 its
-// hi.  Rows are padded by zeros to a multiple of 16 bytes.  A thread makes 16 bytes of both.
+// Two matrices of signed bytes, w = lo + 256 hi: lo [n_out][pitch], then hi; rows are padded by zeros
+// to a multiple of 16 bytes.  A thread makes 16 bytes of both.
 constexpr int GX_THREADS = 128;
 
 __global__ void __launch_bounds__(GX_THREADS)
@@ -125,9 +125,9 @@ __global__ void __launch_bounds__(GX_THREADS)
     lo.b[i] = (int8_t)v;
     hi.b[i] = (int8_t)((v - lo.b[i]) >> 8);
   }
-  uint4* out = reinterpret_cast<uint4*>(to + (size_t)2 * o * pitch + i0);
-  out[0] = lo.v;
-  out[pitch / 16] = hi.v;
+  int8_t* out = to + (size_t)o * pitch + i0;
+  *reinterpret_cast<uint4*>(out) = lo.v;
+  *reinterpret_cast<uint4*>(out + (size_t)n_out * pitch) = hi.v;
 }
 
 // ---- tensor cores -------------------------------------------------------------------------------
@@ -143,36 +143,40 @@ int gc_status_read_and_clear(int* out) {
   return PNB_OK;
 }
 
-constexpr int GC_BM = 128;       // weight rows per tile: 64 outputs
-constexpr int GC_OUT = GC_BM / 2;
+constexpr int GC_BM = 128;       // outputs per tile, one per TMEM lane
 constexpr int GC_WK = 128;       // inputs per weight slot
-constexpr int GC_XK = 64;        // inputs per X slot
 constexpr int GC_KSTEP = 32;     // inputs per MMA
-constexpr int GC_W_SLOT = GC_BM * GC_WK;  // 16 KB
-constexpr int GC_X_SLOT = GC_XK * 256;    // 16 KB
-constexpr int GC_EPI_WARPS = 8;  // two per TMEM lane quarter
+constexpr int GC_W_HALF = GC_BM * GC_WK, GC_W_SLOT = 2 * GC_W_HALF;  // 16 KB of lo, 16 KB of hi
+constexpr int GC_X_SLOT = 16 * 1024;
 constexpr int GC_COPY_WARPS = 4;
-constexpr int GC_PART = 16;      // words staged at a time: rows of 128 bytes
-constexpr int GC_STAGE = 16 * GC_PART * 8;  // of one warp: its 16 outputs
-constexpr int GC_MAX_W = 12, GC_MAX_X = 12, GC_MAX_RAW = 16;
-constexpr int GC_RAW_ROWS = 32, GC_RAW_PITCH = 256 + 16, GC_RAW_SLOT = GC_RAW_ROWS * GC_RAW_PITCH;
+constexpr int GC_EPI_WARPS = 16;  // two groups of two per TMEM lane quarter
+constexpr int GC_PART = 8;        // words staged at a time: rows of 64 bytes
+constexpr int GC_STAGE = 32 * GC_PART * 8;  // of one warp
+constexpr int GC_MAX_W = 6, GC_MAX_X = 12, GC_MAX_RAW = 16;
 constexpr int GC_BARS = 2 * (GC_MAX_W + GC_MAX_X + GC_MAX_RAW) + 4;
 constexpr int GC_BAR_BYTES = (8 * GC_BARS + 8 + 127) / 128 * 128;
 constexpr int GC_SMEM = 227 * 1024;
 constexpr uint32_t GC_WAIT_LIMIT = 1u << 24;
 
-template <int BYTES, bool SHIFTED>
+// BYTES of an X word; STAGES accumulators.
+template <int BYTES, bool SHIFTED, int STAGES>
 struct GcShape {
-  // words of X per tile: 256 bytes (192 of the 256 that are loaded where words have three)
-  static constexpr int WORDS = BYTES == 8 ? 32 : BYTES == 2 ? 128 : 64;
-  static constexpr int BN = WORDS * BYTES;
+  static constexpr int LOAD = STAGES == 1 ? 256 : 128;   // bytes of an X row per tile,
+  static constexpr int BN = BYTES == 3 ? LOAD / 4 * 3 : LOAD;  // of which these are whole words
+  static constexpr int WORDS = BN / BYTES;
+  static constexpr int BOXES = LOAD / 128;               // swizzle spans
+  static constexpr int XK = GC_X_SLOT / LOAD;            // inputs per X slot
+  static constexpr int RAW_ROWS = XK / 2;                // inputs per raw slot, half of each parity
+  static constexpr int RAW_PITCH = LOAD + 16;            // one word of shift, to 16 bytes
+  static constexpr int RAW_SLOT = RAW_ROWS * RAW_PITCH;
   static constexpr int COPY = SHIFTED ? GC_COPY_WARPS : 0;
   static constexpr int MMA_WARP = 2 + COPY;  // warp 0 loads X, warp 1 the weights
-  static constexpr int EPI_WARP = MMA_WARP + 1;
+  static constexpr int EPI_WARP = MMA_WARP + 2;
   static constexpr int THREADS = 32 * (EPI_WARP + GC_EPI_WARPS);
-  static constexpr int EW = WORDS / 2;       // words per epilogue warp
-  static constexpr int CW = BYTES == 8 ? 4 : BYTES == 2 ? 16 : 8;  // of which it fetches at a time
+  static constexpr int EW = WORDS / (STAGES == 1 ? 4 : 2);  // words per epilogue warp,
+  static constexpr int CW = (BYTES == 8 ? 4 : BYTES == 2 ? 16 : 8) / (SHIFTED ? 2 : 1);  // at a time
   static constexpr int COLS = CW * BYTES;
+  static constexpr int HI_AT = STAGES == 1 ? 256 : 128;  // columns from lo's sums to hi's
 };
 
 struct GcMaps {
@@ -183,8 +187,8 @@ struct GcMaps {
 struct GcArgs {
   GroupArgs g;
   int off0, off1;    // words by which rows 0, 2, .. / 1, 3, .. start past 16-byte alignment
-  int n_tiles, m_tiles;
-  long long total;   // tiles: outputs fastest, then words, then requests
+  int n_tiles, m_tiles;            // tiles: outputs fastest, then words, then requests
+  int step_m, step_n, step_b;      // one grid of them
   int keep_w;        // a block's tiles all have the same outputs, whose weights stay
   int w_slots, x_slots, raw_slots;
   int x_at, raw_at, out_at, bars_at;  // shared-memory offsets; weights at 0
@@ -198,22 +202,27 @@ struct GcTile {
 template <bool CACHED>
 struct GcWalk {
   const GcArgs& a;
-  long long t;
-  int slot = 0;
-  __device__ __forceinline__ explicit GcWalk(const GcArgs& args) : a(args), t(blockIdx.x) {
-    if (CACHED && t < a.total) slot = __ldg(a.g.slots + t / a.m_tiles / a.n_tiles);
+  int b, nt, m, slot = 0;
+  __device__ __forceinline__ explicit GcWalk(const GcArgs& args) : a(args) {
+    const unsigned u = blockIdx.x / (unsigned)a.m_tiles;
+    m = (int)(blockIdx.x - u * a.m_tiles);
+    b = (int)(u / (unsigned)a.n_tiles);
+    nt = (int)(u - (unsigned)b * a.n_tiles);
+    if (CACHED && b < a.g.batch) slot = __ldg(a.g.slots + b);
   }
   // the next tile that has something to do; false behind the last
   __device__ __forceinline__ bool next(GcTile& tile) {
-    while (t < a.total) {
-      const long long u = t / a.m_tiles, b = u / a.n_tiles;
-      tile.m = (int)(t - u * a.m_tiles);
-      tile.nt = (int)(u - b * a.n_tiles);
-      tile.b = (int)b;
-      tile.src = CACHED ? slot : (int)b;
-      t += gridDim.x;
+    while (b < a.g.batch) {
+      tile = {b, nt, m, CACHED ? slot : b};
+      m += a.step_m;
+      const int carry_m = m >= a.m_tiles;
+      m -= carry_m ? a.m_tiles : 0;
+      nt += a.step_n + carry_m;
+      const int carry_n = nt >= a.n_tiles;
+      nt -= carry_n ? a.n_tiles : 0;
+      b += a.step_b + carry_n;
       if (!CACHED) return true;
-      if (t < a.total) slot = __ldg(a.g.slots + t / a.m_tiles / a.n_tiles);
+      if (b < a.g.batch) slot = __ldg(a.g.slots + b);
       if (tile.src >= 0 && tile.src < a.g.n_slots) return true;
     }
     return false;
@@ -238,6 +247,8 @@ template <int COLS>
 __device__ __forceinline__ void gc_tmem_ld(uint32_t at, uint32_t (&r)[COLS]) {
   if constexpr (COLS == 32) {
     tc::tmem_ld_32x32_nowait(at, r);
+  } else if constexpr (COLS == 16) {
+    tc::tmem_ld_32x32_x16(at, r);
   } else {
     static_assert(COLS == 24, "16 and 8 columns");
     tc::tmem_ld_32x32_x16(at, *reinterpret_cast<uint32_t(*)[16]>(&r[0]));
@@ -245,29 +256,29 @@ __device__ __forceinline__ void gc_tmem_ld(uint32_t at, uint32_t (&r)[COLS]) {
   }
 }
 
-// The word that the limb sums c stand for, mod 2^64; of a cache's word its high half, the low one is zero.
+// The word that its limbs' sums by lo and by hi stand for, sum_p (lo[p] + hi[p-1]) << 8p mod 2^64: the
+// sums of two stay below 2^31 for up to 61922 inputs ((128 + 7) * 255 each).  Of a cache's word these are
+// the top limbs, and its low half is zero.
 template <int BYTES>
-__device__ __forceinline__ uint64_t gc_word(const uint32_t* c) {
-  if constexpr (BYTES == 8) {
-    return add_limbs(0, c);
-  } else {
-    uint32_t v = c[0];
+__device__ __forceinline__ uint64_t gc_word(const uint32_t* lo, const uint32_t* hi) {
+  uint32_t t[BYTES];
+  t[0] = lo[0];
 #pragma unroll
-    for (int b = 1; b < BYTES; ++b) v += c[b] << (8 * b);
+  for (int p = 1; p < BYTES; ++p) t[p] = lo[p] + hi[p - 1];
+  if constexpr (BYTES == 8) {
+    return add_limbs(0, t);
+  } else {
+    uint32_t v = t[0];
+#pragma unroll
+    for (int p = 1; p < BYTES; ++p) v += t[p] << (8 * p);
     return (uint64_t)(v << (32 - 8 * BYTES)) << 32;
   }
 }
 
-template <int BYTES>
-__device__ __forceinline__ uint64_t gc_other_lane(uint64_t v) {
-  if (BYTES == 8) return shfl_xor_u64(v, 1);
-  return (uint64_t)__shfl_xor_sync(0xffffffffu, (uint32_t)(v >> 32), 1) << 32;
-}
-
-template <int BYTES, bool SHIFTED>
-__global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
+template <int BYTES, bool SHIFTED, int STAGES>
+__global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, STAGES>::THREADS, 1)
     group_kernel(const __grid_constant__ GcMaps tm, const __grid_constant__ GcArgs a) {
-  using S = GcShape<BYTES, SHIFTED>;
+  using S = GcShape<BYTES, SHIFTED, STAGES>;
   constexpr bool CACHED = BYTES != 8;
   extern __shared__ __align__(1024) unsigned char gc_raw[];  // the swizzles want 1024-byte boundaries
   const uint32_t base = tc::smem_u32(gc_raw);
@@ -277,7 +288,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
   }
   auto w_at = [&](int s) { return base + (uint32_t)(s * GC_W_SLOT); };
   auto x_at = [&](int s) { return base + (uint32_t)(a.x_at + s * GC_X_SLOT); };
-  auto raw_at = [&](int s) { return base + (uint32_t)(a.raw_at + s * GC_RAW_SLOT); };
+  auto raw_at = [&](int s) { return base + (uint32_t)(a.raw_at + s * S::RAW_SLOT); };
   const uint32_t bars = base + (uint32_t)a.bars_at;
   const uint32_t w_full = bars, w_empty = w_full + 8 * GC_MAX_W;
   const uint32_t x_full = w_empty + 8 * GC_MAX_W, x_empty = x_full + 8 * GC_MAX_X;
@@ -290,19 +301,19 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.w_slots; ++s) {
       tc::mbar_init(w_full + 8 * s, 1);
-      tc::mbar_init(w_empty + 8 * s, 1);
+      tc::mbar_init(w_empty + 8 * s, 2);
     }
     for (int s = 0; s < a.x_slots; ++s) {
       tc::mbar_init(x_full + 8 * s, SHIFTED ? S::COPY : 1);
-      tc::mbar_init(x_empty + 8 * s, 1);
+      tc::mbar_init(x_empty + 8 * s, 2);
     }
     for (int s = 0; s < a.raw_slots; ++s) {
       tc::mbar_init(r_full + 8 * s, 1);
       tc::mbar_init(r_empty + 8 * s, 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      tc::mbar_init(acc_full + 8 * s, 1);
-      tc::mbar_init(acc_empty + 8 * s, GC_EPI_WARPS);
+    for (int s = 0; s < STAGES; ++s) {
+      tc::mbar_init(acc_full + 8 * s, 2);
+      tc::mbar_init(acc_empty + 8 * s, GC_EPI_WARPS / STAGES);
     }
     *abort_s = 0;
     tc::fence_mbar_init();
@@ -317,7 +328,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
   tc::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gc_raw + (holder - base));
 
-  const int kx_n = (a.g.n_in + GC_XK - 1) / GC_XK;  // X slots of one tile
+  const int kx_n = (a.g.n_in + S::XK - 1) / S::XK;  // X slots of one tile
   const int kb_n = (a.g.n_in + GC_WK - 1) / GC_WK;  // weight slots
   GcTile tile;
 
@@ -330,22 +341,23 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
       const int slots = SHIFTED ? a.raw_slots : a.x_slots;
       GcWalk<CACHED> walk(a);
       while (ok && walk.next(tile)) {
-        for (int k = 0; k < a.g.n_in; k += SHIFTED ? GC_RAW_ROWS : GC_XK) {
+        for (int k = 0; k < a.g.n_in; k += SHIFTED ? S::RAW_ROWS : S::XK) {
           const int s = ring.slot;
           const uint32_t full = (SHIFTED ? r_full : x_full) + 8 * s;
           ok = gc_wait((SHIFTED ? r_empty : x_empty) + 8 * s, ring.phase ^ 1u, abort_s);
           if (!ok) break;
           if (SHIFTED) {
             const int row = tile.src * a.g.n_in + k;
-            tc::mbar_expect_tx(full, GC_RAW_SLOT);  // the rows of either parity, in order
+            tc::mbar_expect_tx(full, S::RAW_SLOT);  // the rows of either parity, in order
             tc::tma_load_2d(raw_at(s), &tm.X[row & 1], tile.nt * S::WORDS, row >> 1, full);
-            tc::tma_load_2d(raw_at(s) + GC_RAW_SLOT / 2, &tm.X[(row + 1) & 1], tile.nt * S::WORDS,
+            tc::tma_load_2d(raw_at(s) + S::RAW_SLOT / 2, &tm.X[(row + 1) & 1], tile.nt * S::WORDS,
                             (row + 1) >> 1, full);
           } else {
             tc::mbar_expect_tx(full, GC_X_SLOT);  // rows past the last input read as zeros
-            tc::tma_load_3d(x_at(s), &tm.X[0], tile.nt * S::BN, k, tile.src, full);
-            tc::tma_load_3d(x_at(s) + GC_X_SLOT / 2, &tm.X[0], tile.nt * S::BN + 128, k, tile.src,
-                            full);
+#pragma unroll
+            for (int b = 0; b < S::BOXES; ++b)
+              tc::tma_load_3d(x_at(s) + b * (S::XK * 128), &tm.X[0], tile.nt * S::BN + b * 128, k,
+                              tile.src, full);
           }
           ring.advance(slots);
           wrapped |= ring.slot == 0;
@@ -366,7 +378,10 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
           ok = gc_wait(w_empty + 8 * s, ring.phase ^ 1u, abort_s);
           if (!ok) break;
           tc::mbar_expect_tx(w_full + 8 * s, GC_W_SLOT);
-          tc::tma_load_2d(w_at(s), &tm.W, k * GC_WK, tile.m * GC_BM, w_full + 8 * s);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            tc::tma_load_3d(w_at(s) + h * GC_W_HALF, &tm.W, k * GC_WK, tile.m * GC_BM, h,
+                            w_full + 8 * s);
           ring.advance(a.w_slots);
           wrapped |= ring.slot == 0;
         }
@@ -380,8 +395,10 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
     // X slot's turn and answers it, also where it copies nothing: a parity tells only neighbouring
     // turns apart.
     const int cw = warp - 2;
-    constexpr int BATCH = 16;  // rows whose words are on their way together
-    const int box = lane >> 4, ch = (lane & 15) >> 1, half = lane & 1;
+    constexpr int PER = SHIFTED ? 32 / S::WORDS : 1;  // rows per pass of a warp
+    constexpr int BATCH = 16;           // passes whose words are on their way together
+    const int word = lane % S::WORDS, sub = lane / S::WORDS;
+    const int box = word >> 4, ch = (word & 15) >> 1, half = word & 1;
     TileRing xr, rr;
     bool ok = true;
     GcWalk<CACHED> walk(a);
@@ -391,28 +408,28 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
       for (int kx = 0; ok && kx < kx_n; ++kx) {
         ok = gc_wait(x_empty + 8 * xr.slot, xr.phase ^ 1u, abort_s);
         if (!ok) break;
-        const int raws = min(2, (a.g.n_in - kx * GC_XK + GC_RAW_ROWS - 1) / GC_RAW_ROWS);
+        const int raws = min(2, (a.g.n_in - kx * S::XK + S::RAW_ROWS - 1) / S::RAW_ROWS);
         for (int i = 0; i < raws; ++i) {
           if ((rr.slot & 3) == cw) {
             ok = gc_wait(r_full + 8 * rr.slot, rr.phase, abort_s);
             if (!ok) break;
             // row r of the slot: its parity's half, r / 2; one word further where it is shifted
-            const unsigned char* from = gc_raw + (raw_at(rr.slot) - base) + lane * 8;
-            unsigned char* to = gc_raw + (x_at(xr.slot) - base) + box * (GC_XK * 128) +
-                                i * (GC_RAW_ROWS * 128) + half * 8;
+            const unsigned char* from = gc_raw + (raw_at(rr.slot) - base) + word * 8;
+            unsigned char* to = gc_raw + (x_at(xr.slot) - base) + box * (S::XK * 128) +
+                                i * (S::RAW_ROWS * 128) + half * 8;
 #pragma unroll
-            for (int r0 = 0; r0 < GC_RAW_ROWS; r0 += BATCH) {
+            for (int b = 0; b < S::RAW_ROWS / PER; b += BATCH) {
               uint64_t v[BATCH];
 #pragma unroll
               for (int j = 0; j < BATCH; ++j) {
-                const int r = r0 + j;
+                const int r = (b + j) * PER + sub;
                 v[j] = *reinterpret_cast<const uint64_t*>(
-                    from + (r & 1 ? GC_RAW_SLOT / 2 + off_o * 8 : off_e * 8) +
-                    (r >> 1) * GC_RAW_PITCH);
+                    from + (r & 1 ? S::RAW_SLOT / 2 + off_o * 8 : off_e * 8) +
+                    (r >> 1) * S::RAW_PITCH);
               }
 #pragma unroll
               for (int j = 0; j < BATCH; ++j) {
-                const int r = r0 + j;
+                const int r = (b + j) * PER + sub;
                 *reinterpret_cast<uint64_t*>(to + r * 128 + ((ch ^ (r & 7)) << 4)) = v[j];
               }
             }
@@ -427,12 +444,14 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
         xr.advance(a.x_slots);
       }
     }
-  } else if (warp == S::MMA_WARP) {
-    // ---------------- products (one lane) --------------------------------------------------------
+  } else if (warp < S::EPI_WARP) {
+    // ---------------- products: one warp's lane by lo, the other's by hi -------------------------
     if (lane == 0) {
       constexpr uint32_t IDESC = tc::idesc_i8(GC_BM, S::BN, true, false, false, true);
-      const uint64_t wd = tc::smem_desc_sw128(w_at(0), 16u, 1024u);
-      const uint64_t xd = tc::smem_desc_sw128(x_at(0), GC_XK * 128u, 1024u);
+      constexpr int STEPS = S::XK / GC_KSTEP, PER_W = GC_WK / S::XK;
+      const int hi = warp - S::MMA_WARP;
+      const uint64_t wd = tc::smem_desc_sw128(w_at(0) + hi * GC_W_HALF, 16u, 1024u);
+      const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
       const uint32_t w_hi = (uint32_t)(wd >> 32), x_hi = (uint32_t)(xd >> 32);
       const int steps = (a.g.n_in + GC_KSTEP - 1) / GC_KSTEP;
       TileRing x, w;
@@ -440,34 +459,38 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
       bool ok = true;
       GcWalk<CACHED> walk(a);
       while (ok && walk.next(tile)) {
-        const int buf = tt & 1;
-        const uint32_t d = tmem + (uint32_t)(buf * 256);
-        ok = gc_wait(acc_empty + 8 * buf, (uint32_t)(tt >> 1) ^ 1u, abort_s);
+        const int buf = STAGES == 1 ? 0 : tt & 1;
+        const uint32_t d = tmem + (uint32_t)(buf * 256 + hi * S::HI_AT);
+        ok = gc_wait(acc_empty + 8 * buf, (uint32_t)(tt / STAGES) ^ 1u, abort_s);
         if (!ok) break;
         tc::tc_fence_after();
         const bool load = !a.keep_w || tt == 0;
         if (a.keep_w) w = TileRing{};
         uint32_t acc = 0;
-        for (int left = steps, kx = 0; left > 0; left -= GC_XK / GC_KSTEP, ++kx) {
-          if ((kx & 1) == 0 && load) {
+        for (int left = steps; ok && left > 0;) {  // one weight slot
+          if (load) {
             ok = gc_wait(w_full + 8 * w.slot, w.phase, abort_s);
             if (!ok) break;
           }
-          ok = gc_wait(x_full + 8 * x.slot, x.phase, abort_s);
-          if (!ok) break;
-          const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (GC_X_SLOT / 16));
-          const uint32_t w_lo = (uint32_t)wd + (uint32_t)(w.slot * (GC_W_SLOT / 16)) + 4u * (kx & 1);
+          const uint32_t w_lo = (uint32_t)wd + (uint32_t)(w.slot * (GC_W_SLOT / 16));
 #pragma unroll
-          for (int k = 0; k < GC_XK / GC_KSTEP; ++k)
-            if (k < left)
-              tc::mma_i8_lo(d, w_lo + 2 * k, w_hi, x_lo + 256 * k, x_hi, IDESC, k ? 1u : acc);
-          acc = 1;
-          tc::mma_commit(x_empty + 8 * x.slot);
-          x.advance(a.x_slots);
-          if ((kx & 1) || left <= GC_XK / GC_KSTEP) {
-            if (!a.keep_w) tc::mma_commit(w_empty + 8 * w.slot);
-            w.advance(a.w_slots);
+          for (int h = 0; h < PER_W; ++h) {
+            if (left <= 0) break;
+            ok = gc_wait(x_full + 8 * x.slot, x.phase, abort_s);
+            if (!ok) break;
+            const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (GC_X_SLOT / 16));
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+              if (k < left)
+                tc::mma_i8_lo(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
+                              k ? 1u : acc);
+            acc = 1;
+            left -= STEPS;
+            tc::mma_commit(x_empty + 8 * x.slot);
+            x.advance(a.x_slots);
           }
+          if (!a.keep_w) tc::mma_commit(w_empty + 8 * w.slot);
+          w.advance(a.w_slots);
         }
         if (!ok) break;
         tc::mma_commit(acc_full + 8 * buf);
@@ -476,98 +499,101 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
     }
   } else {
     // ---------------- epilogue -------------------------------------------------------------------
-    // Warp w reads TMEM lane quarter w % 4 and half eh of the tile's words.  An even lane has an output's
-    // lo sums and the odd lane beside it the hi sums: of every two words each lane completes one, with
-    // the other lane's share of it.  Words are staged in shared memory, 16 outputs x 16 words at a time with
-    // the 16-byte chunks XORed by the row, and leave by TMA, or as row segments by plain stores.
+    // Warp w reads TMEM lane quarter w % 4: 32 outputs, one per lane.  With two accumulators each group
+    // of eight warps has one of them, and a warp half of its words; with one, a warp has a quarter.
+    // Words are staged in shared memory, 32 outputs x 8 words at a time with the 16-byte chunks XORed by
+    // the row, and leave by TMA, or as row segments by plain stores.
     const int e_w = warp - S::EPI_WARP;
-    const int q = warp & 3, eh = e_w >> 2;
-    const bool odd = lane & 1;
+    const int q = warp & 3, group = e_w >> 3, share = STAGES == 1 ? e_w >> 2 : (e_w >> 2) & 1;
     const uint32_t out_at = base + (uint32_t)(a.out_at + e_w * GC_STAGE);
     unsigned char* out = gc_raw + (out_at - base);
-    const int row = lane >> 1;  // of the warp's 16 outputs
-    unsigned char* out_row = out + row * 128 + odd * 8;
+    unsigned char* out_row = out + lane * 64;
+    const int out_x = (lane >> 1) & 3;
     int tt = 0;
-    bool ok = true;
     GcWalk<CACHED> walk(a);
     while (walk.next(tile)) {
-      const int buf = tt & 1;
-      ok = gc_wait(acc_full + 8 * buf, (uint32_t)(tt >> 1), abort_s);
-      if (!ok) break;
-      tc::tc_fence_after();
+      const int buf = STAGES == 1 ? 0 : tt & 1;
+      const uint32_t turn = (uint32_t)(tt / STAGES);
       ++tt;
-      const uint32_t c_tmem = tmem + (uint32_t)(buf * 256 + eh * (S::BN / 2)) +
+      if (STAGES == 2 && buf != group) continue;
+      const int row0 = tile.m * GC_BM + q * 32, col0 = tile.nt * S::WORDS + share * S::EW;
+      // the body among this warp's words
+      const int body = a.g.L - 1 - col0;
+      const bool live = row0 + lane < a.g.n_out;
+      uint64_t bias = 0;
+      if (a.g.bias && body >= 0 && body < S::EW && live)
+        bias = (uint64_t)__ldg(a.g.bias + row0 + lane) * a.g.delta;
+      if (!gc_wait(acc_full + 8 * buf, turn, abort_s)) break;
+      tc::tc_fence_after();
+      const uint32_t c_tmem = tmem + (uint32_t)(buf * 256 + share * S::EW * BYTES) +
                               ((uint32_t)(q * 32) << 16);
-      const int row0 = tile.m * GC_OUT + q * 16, col0 = tile.nt * S::WORDS + eh * S::EW;
-      if (row0 >= a.g.n_out || col0 >= a.g.L) {  // nothing of this warp's share is kept
+      if (row0 >= a.g.n_out || body < 0) {  // nothing of this warp's share is kept
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(acc_empty + 8 * buf);
         continue;
       }
-      const int body = a.g.L - 1 - col0;  // the body among this warp's words
-      const bool live = row0 + row < a.g.n_out;
-      uint64_t bias = 0;
-      if (a.g.bias && body < S::EW && live)
-        bias = (uint64_t)__ldg(a.g.bias + row0 + row) * a.g.delta;
-      constexpr int CHUNKS = S::EW / S::CW, PER_PART = GC_PART / S::CW;
-      uint32_t c[2][S::COLS];
-      gc_tmem_ld<S::COLS>(c_tmem, c[0]);
 #pragma unroll
-      for (int i = 0; i < CHUNKS; ++i) {
-        tc::tmem_ld_wait_pin(c[i & 1]);
-        if (i + 1 < CHUNKS) {
-          gc_tmem_ld<S::COLS>(c_tmem + (uint32_t)((i + 1) * S::COLS), c[(i + 1) & 1]);
-        } else {
+      for (int i = 0; i < S::EW / S::CW; ++i) {
+        uint32_t lo[S::COLS], hi[S::COLS];
+        gc_tmem_ld<S::COLS>(c_tmem + (uint32_t)(i * S::COLS), lo);
+        gc_tmem_ld<S::COLS>(c_tmem + (uint32_t)(S::HI_AT + i * S::COLS), hi);
+        tc::tmem_ld_wait_pin(lo);
+        tc::tmem_ld_wait_pin(hi);
+        if (i + 1 == S::EW / S::CW) {
           tc::tc_fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(acc_empty + 8 * buf);
         }
-        const int w0 = i * S::CW / GC_PART * GC_PART;  // the part's first word
-        if (i % PER_PART == 0 && !a.plain_out) {  // what was staged before has left
-          if (lane == 0) tc::tma_store_wait_read();
-          __syncwarp();
-        }
 #pragma unroll
-        for (int u = 0; u < S::CW; u += 2) {
-          uint64_t v0 = gc_word<BYTES>(c[i & 1] + u * BYTES);
-          uint64_t v1 = gc_word<BYTES>(c[i & 1] + (u + 1) * BYTES);
-          if (odd) {
-            v0 <<= 8;
-            v1 <<= 8;
+        for (int u0 = 0; u0 < S::CW; u0 += GC_PART) {
+          const int first = i * S::CW + u0;           // of this warp's words
+          const int part = first / GC_PART * GC_PART;  // the first word staged with it
+          constexpr int N = S::CW < GC_PART ? S::CW : GC_PART;
+          uint64_t y[N];
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+            y[u] = gc_word<BYTES>(lo + (u0 + u) * BYTES, hi + (u0 + u) * BYTES);
+          if (first == part && !a.plain_out) {  // what was staged before has left
+            if (lane == 0) tc::tma_store_wait_read();
+            __syncwarp();
           }
-          const uint64_t keep = odd ? v1 : v0, give = odd ? v0 : v1;
-          uint64_t y = keep + gc_other_lane<BYTES>(give);
-          const int word = i * S::CW + u;
-          if (body - word == (odd ? 1 : 0)) {
-            y += bias;
+#pragma unroll
+          for (int u = 0; u < N; u += 2)
+            *reinterpret_cast<ulonglong2*>(
+                out_row + ((((first - part + u) >> 1) ^ out_x) << 4)) =
+                make_ulonglong2(y[u], y[u + 1]);
+          if (first + N != part + GC_PART) continue;
+          if (body >= part && body < part + GC_PART) {
+            uint64_t* p = reinterpret_cast<uint64_t*>(
+                out_row + ((((body - part) >> 1) ^ out_x) << 4) + ((body - part) & 1) * 8);
+            *p += bias;
             // tiled stores end on 16-byte boundaries, so the last word of an odd count goes alone
             if (!a.plain_out && (a.g.L & 1) && live)
-              a.g.Y[((size_t)tile.b * a.g.n_out + row0 + row) * a.g.ldy + a.g.L - 1] = y;
+              a.g.Y[((size_t)tile.b * a.g.n_out + row0 + lane) * a.g.ldy + a.g.L - 1] = *p;
           }
-          const int chunk = (word - w0) >> 1;
-          *reinterpret_cast<uint64_t*>(out_row + ((chunk ^ (row & 7)) << 4)) = y;
-        }
-        if ((i + 1) % PER_PART != 0) continue;
-        if (!a.plain_out) {
-          tc::fence_async_smem();
-          __syncwarp();
-          if (lane == 0 && col0 + w0 < (a.g.L & ~1))
-            tc::tma_store_3d(&tm.Y, col0 + w0, row0, tile.b, out_at);
-        } else {
-          __syncwarp();
-          const int wd = lane & 15, sub = lane >> 4;
-          uint64_t* y = a.g.Y + ((size_t)tile.b * a.g.n_out + row0 + sub) * a.g.ldy + col0 + w0 + wd;
-          const int left = col0 + w0 + wd < a.g.L ? a.g.n_out - row0 - sub : 0;
-          uint64_t v[8];
+          if (!a.plain_out) {
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && col0 + part < (a.g.L & ~1))
+              tc::tma_store_3d(&tm.Y, col0 + part, row0, tile.b, out_at);
+          } else {
+            __syncwarp();
+            const int wd = lane & 7, sub = lane >> 3;  // four rows per instruction
+            uint64_t* to = a.g.Y + ((size_t)tile.b * a.g.n_out + row0 + sub) * a.g.ldy + col0 + part + wd;
+            const int left = col0 + part + wd < a.g.L ? a.g.n_out - row0 - sub : 0;
+            uint64_t v[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            v[j] = *reinterpret_cast<const uint64_t*>(
-                out + (2 * j + sub) * 128 + (((wd >> 1) ^ ((2 * j + sub) & 7)) << 4) + (wd & 1) * 8);
+            for (int j = 0; j < 8; ++j) {
+              const int r = 4 * j + sub;
+              v[j] = *reinterpret_cast<const uint64_t*>(
+                  out + r * 64 + (((wd >> 1) ^ ((r >> 1) & 3)) << 4) + (wd & 1) * 8);
+            }
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (2 * j < left) y[(size_t)(2 * j) * a.g.ldy] = v[j];
-          __syncwarp();
+            for (int j = 0; j < 8; ++j)
+              if (4 * j < left) to[(size_t)(4 * j) * a.g.ldy] = v[j];
+            __syncwarp();
+          }
         }
       }
     }
@@ -583,24 +609,30 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED>::THREADS, 1)
 
 // ---- launch -------------------------------------------------------------------------------------
 // How one block's shared memory is shared out.  Weights stay when they leave X four slots (shifted rows:
-// three, and 40 KB of raw ones) and the grid is a whole number of times the tiles of outputs without
+// three, and 36 KB of raw ones) and the grid is a whole number of times the tiles of outputs without
 // losing more than a sixteenth of the machine.
-template <bool SHIFTED>
+template <int BYTES, bool SHIFTED, int STAGES>
 static unsigned gc_plan(GcArgs& a, int sms) {
+  using S = GcShape<BYTES, SHIFTED, STAGES>;
+  a.n_tiles = (a.g.L + S::WORDS - 1) / S::WORDS;
   const int kb = (a.g.n_in + GC_WK - 1) / GC_WK;
   int room = GC_SMEM - GC_BAR_BYTES - GC_EPI_WARPS * GC_STAGE;
-  const int raw_min = SHIFTED ? 40 * 1024 / GC_RAW_SLOT * GC_RAW_SLOT : 0;
   const int x_min = SHIFTED ? 3 : 4;
-  const int w_most = std::min(GC_MAX_W, (room - raw_min - x_min * GC_X_SLOT) / GC_W_SLOT);
-  unsigned grid = (unsigned)std::min<long long>(a.total, sms);
+  const int w_most =
+      std::min(GC_MAX_W, (room - (SHIFTED ? 4 * S::RAW_SLOT : 0) - x_min * GC_X_SLOT) / GC_W_SLOT);
+  const long long total = (long long)a.g.batch * a.n_tiles * a.m_tiles;
+  unsigned grid = (unsigned)std::min<long long>(total, sms);
   const unsigned whole = grid / a.m_tiles * a.m_tiles;
   a.keep_w = kb <= w_most && whole && 16 * (grid - whole) <= grid;
   if (a.keep_w) grid = whole;
-  a.w_slots = a.keep_w ? kb : 4;
+  a.w_slots = a.keep_w ? kb : SHIFTED ? 2 : 3;
+  a.step_m = (int)(grid % a.m_tiles);
+  a.step_n = (int)(grid / a.m_tiles % a.n_tiles);
+  a.step_b = (int)(grid / a.m_tiles / a.n_tiles);
   room -= a.w_slots * GC_W_SLOT;
   if (SHIFTED) {
     a.x_slots = x_min;
-    a.raw_slots = std::min(GC_MAX_RAW, (room - a.x_slots * GC_X_SLOT) / GC_RAW_SLOT & ~3);
+    a.raw_slots = std::min(GC_MAX_RAW, (room - a.x_slots * GC_X_SLOT) / S::RAW_SLOT & ~3);
   } else {
     a.x_slots = std::min(GC_MAX_X, room / GC_X_SLOT);
     a.raw_slots = 0;
@@ -608,24 +640,50 @@ static unsigned gc_plan(GcArgs& a, int sms) {
   a.x_at = a.w_slots * GC_W_SLOT;
   a.out_at = a.x_at + a.x_slots * GC_X_SLOT;
   a.raw_at = a.out_at + GC_EPI_WARPS * GC_STAGE;
-  a.bars_at = a.raw_at + a.raw_slots * GC_RAW_SLOT;
+  a.bars_at = a.raw_at + a.raw_slots * S::RAW_SLOT;
   return grid;
 }
 
-template <int BYTES, bool SHIFTED>
-static int gc_launch(const GcMaps& tm, GcArgs& a, cudaStream_t st) {
-  using S = GcShape<BYTES, SHIFTED>;
+template <int BYTES, bool SHIFTED, int STAGES>
+static int gc_launch(GcMaps& tm, GcArgs& a, cudaStream_t st) {
+  using S = GcShape<BYTES, SHIFTED, STAGES>;
   static std::atomic<int> sm_count[64];  // per device, once the kernel's shared-memory limit is raised
+  auto kernel = group_kernel<BYTES, SHIFTED, STAGES>;
   int dev = 0;
   PNB_CUDA(cudaGetDevice(&dev));
   int sms = dev < 64 ? sm_count[dev].load(std::memory_order_acquire) : 0;
   if (sms == 0) {
     PNB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    PNB_CUDA(cudaFuncSetAttribute(group_kernel<BYTES, SHIFTED>,
-                                  cudaFuncAttributeMaxDynamicSharedMemorySize, GC_SMEM));
+    PNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GC_SMEM));
     if (dev < 64) sm_count[dev].store(sms, std::memory_order_release);
   }
-  const unsigned grid = gc_plan<SHIFTED>(a, sms);
+  const unsigned grid = gc_plan<BYTES, SHIFTED, STAGES>(a, sms);
+  const GroupArgs& g = a.g;
+  int rc = PNB_OK;
+  if (!SHIFTED) {
+    const cuuint64_t dims[3] = {(cuuint64_t)g.L * BYTES, (cuuint64_t)g.n_in,
+                                (cuuint64_t)(g.slots ? g.n_slots : g.batch)};
+    const cuuint64_t strides[2] = {g.x_row, g.x_row * g.n_in};
+    const cuuint32_t box[3] = {128, (cuuint32_t)S::XK, 1};
+    rc = tile_map(&tm.X[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, g.X, 3, dims, strides, box,
+                  CU_TENSOR_MAP_SWIZZLE_128B);
+  } else {
+    // rows p, p + 2, ..: from the 16-byte boundary at or before row p, at twice the pitch.  A row
+    // off by one word has that word's 16 bytes inside its allocation (allocations start aligned).
+    const long long x_rows = (long long)g.batch * g.n_in;
+    for (int p = 0; p < 2 && !rc; ++p) {
+      // (a single row has no row 1: both maps are its own, and the second meets zero weights)
+      const bool second = p && x_rows > 1;
+      const int off = second ? a.off1 : a.off0;
+      const cuuint64_t dims[2] = {(cuuint64_t)g.L + off,
+                                  (cuuint64_t)std::max<long long>(1, (x_rows + 1 - p) / 2)};
+      const cuuint64_t strides[1] = {g.x_row * 2};
+      const cuuint32_t box[2] = {S::RAW_PITCH / 8, S::RAW_ROWS / 2};
+      rc = tile_map(&tm.X[p], CU_TENSOR_MAP_DATA_TYPE_UINT64, g.X + (second ? g.x_row : 0) - 8 * off,
+                    2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+    }
+  }
+  if (rc) return rc;
   cudaLaunchAttribute attr;  // its set-up and its first loads of X run beside the weights' kernel
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -636,8 +694,16 @@ static int gc_launch(const GcMaps& tm, GcArgs& a, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  PNB_CUDA(cudaLaunchKernelEx(&cfg, group_kernel<BYTES, SHIFTED>, tm, a));
+  PNB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tm, a));
   return PNB_OK;
+}
+
+constexpr int GC_LONG = 384;  // inputs from which one wide accumulator is faster than two
+
+template <int BYTES, bool SHIFTED>
+static int gc_stages(GcMaps& tm, GcArgs& a, cudaStream_t st) {
+  return a.g.n_in >= GC_LONG ? gc_launch<BYTES, SHIFTED, 1>(tm, a, st)
+                             : gc_launch<BYTES, SHIFTED, 2>(tm, a, st);
 }
 
 static int gc_run(const GroupArgs& g, int bits, int8_t* ws, cudaStream_t st) {
@@ -645,72 +711,44 @@ static int gc_run(const GroupArgs& g, int bits, int8_t* ws, cudaStream_t st) {
   const int bytes = bits / 8;
   GcArgs a{};
   a.g = g;
-  const int words = bytes == 8 ? 32 : bytes == 2 ? 128 : 64;
-  a.n_tiles = (g.L + words - 1) / words;
-  a.m_tiles = (g.n_out + GC_OUT - 1) / GC_OUT;
-  a.total = (long long)g.batch * a.n_tiles * a.m_tiles;
-  const long long x_rows = (long long)(g.slots ? g.n_slots : g.batch) * g.n_in;
-  if (bytes == 8 && x_rows > 0x7fffffffLL - GC_BM) {  // (TMA coordinates are 32-bit)
-    set_error("%s: %lld ciphertexts exceed a 32-bit index", name, x_rows);
+  a.m_tiles = (g.n_out + GC_BM - 1) / GC_BM;
+  a.off0 = bytes == 8 ? (int)((uintptr_t)g.X / 8 & 1) : 0;
+  a.off1 = bytes == 8 ? (int)(((uintptr_t)g.X + g.x_row) / 8 & 1) : 0;
+  const bool shifted = a.off0 || a.off1;
+  if (shifted && (long long)g.batch * g.n_in > 0x7fffffffLL - GC_WK) {
+    set_error("%s: %lld ciphertexts exceed a 32-bit index", name, (long long)g.batch * g.n_in);
     return PNB_ERR_INVALID;
   }
-  const uintptr_t xw = (uintptr_t)g.X / 8;
-  const int ldx = (int)(g.x_row / 8);  // (words)
-  a.off0 = bytes == 8 ? (int)(xw & 1) : 0;
-  a.off1 = bytes == 8 ? (int)((xw + (uintptr_t)ldx) & 1) : 0;
-  const bool shifted = a.off0 || a.off1;
   a.plain_out = g.ldy % 2 != 0 || ((uintptr_t)g.Y % 16) != 0;
   const int pitch = (g.n_in + 15) & ~15;
-  const long long chunks = (long long)g.n_out * (pitch / 16);
-  if ((chunks + GX_THREADS - 1) / GX_THREADS > 0x7fffffffLL) {
+  const long long blocks = ((long long)g.n_out * (pitch / 16) + GX_THREADS - 1) / GX_THREADS;
+  if (blocks > 0x7fffffffLL) {
     set_error("%s: %d x %d weights exceed one launch", name, g.n_out, g.n_in);
     return PNB_ERR_INVALID;
   }
   GcMaps tm{};
-  int rc = tile_map_bytes(&tm.W, ws, (uint64_t)pitch, 2 * (uint64_t)g.n_out, (uint64_t)pitch, GC_WK,
-                          GC_BM);
-  if (rc) return rc;
-  if (!shifted) {
-    const cuuint64_t dims[3] = {(cuuint64_t)g.L * bytes, (cuuint64_t)g.n_in,
-                                (cuuint64_t)(g.slots ? g.n_slots : g.batch)};
-    const cuuint64_t strides[2] = {g.x_row, g.x_row * g.n_in};
-    const cuuint32_t box[3] = {128, GC_XK, 1};
-    rc = tile_map(&tm.X[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, g.X, 3, dims, strides, box,
-                  CU_TENSOR_MAP_SWIZZLE_128B);
-  } else {
-    // rows p, p + 2, ..: from the 16-byte boundary at or before row p, at twice the pitch.  A row
-    // off by one word has that word's 16 bytes inside its allocation (allocations start aligned).
-    for (int p = 0; p < 2 && !rc; ++p) {
-      // (a single row has no row 1: both maps are its own, and the second meets zero weights)
-      const bool second = p && x_rows > 1;
-      const int off = second ? a.off1 : a.off0;
-      const cuuint64_t dims[2] = {(cuuint64_t)g.L + off,
-                                  (cuuint64_t)std::max<long long>(1, (x_rows + 1 - p) / 2)};
-      const cuuint64_t strides[1] = {g.x_row * 2};
-      const cuuint32_t box[2] = {GC_RAW_PITCH / 8, GC_RAW_ROWS / 2};
-      rc = tile_map(&tm.X[p], CU_TENSOR_MAP_DATA_TYPE_UINT64,
-                    reinterpret_cast<const uint64_t*>(g.X) + (second ? ldx : 0) - off, 2, dims,
-                    strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
-    }
-  }
+  const cuuint64_t w_dims[3] = {(cuuint64_t)pitch, (cuuint64_t)g.n_out, 2};
+  const cuuint64_t w_strides[2] = {(cuuint64_t)pitch, (cuuint64_t)pitch * g.n_out};
+  const cuuint32_t w_box[3] = {GC_WK, GC_BM, 1};
+  int rc = tile_map(&tm.W, CU_TENSOR_MAP_DATA_TYPE_UINT8, ws, 3, w_dims, w_strides, w_box,
+                    CU_TENSOR_MAP_SWIZZLE_128B);
   if (!rc && !a.plain_out) {
     // writes end at word L (rounded down to 16 bytes) of the last output of each request
     const cuuint64_t dims[3] = {(cuuint64_t)std::max(2, g.L & ~1), (cuuint64_t)g.n_out,
                                 (cuuint64_t)g.batch};
     const cuuint64_t strides[2] = {(cuuint64_t)g.ldy * 8, (cuuint64_t)g.ldy * 8 * g.n_out};
-    const cuuint32_t box[3] = {GC_PART, 16, 1};
+    const cuuint32_t box[3] = {GC_PART, 32, 1};
     rc = tile_map(&tm.Y, CU_TENSOR_MAP_DATA_TYPE_UINT64, g.Y, 3, dims, strides, box,
-                  CU_TENSOR_MAP_SWIZZLE_128B);
+                  CU_TENSOR_MAP_SWIZZLE_64B);
   }
   if (rc) return rc;
-  group_expand_kernel<<<(unsigned)((chunks + GX_THREADS - 1) / GX_THREADS), GX_THREADS, 0, st>>>(
-      g.w, g.n_in, g.n_out, pitch, ws);
+  group_expand_kernel<<<(unsigned)blocks, GX_THREADS, 0, st>>>(g.w, g.n_in, g.n_out, pitch, ws);
   PNB_CHECK_LAUNCH("group_expand_kernel");
   switch (bytes) {
-    case 8: return shifted ? gc_launch<8, true>(tm, a, st) : gc_launch<8, false>(tm, a, st);
-    case 4: return gc_launch<4, false>(tm, a, st);
-    case 3: return gc_launch<3, false>(tm, a, st);
-    default: return gc_launch<2, false>(tm, a, st);
+    case 8: return shifted ? gc_stages<8, true>(tm, a, st) : gc_stages<8, false>(tm, a, st);
+    case 4: return gc_stages<4, false>(tm, a, st);
+    case 3: return gc_stages<3, false>(tm, a, st);
+    default: return gc_stages<2, false>(tm, a, st);
   }
 }
 

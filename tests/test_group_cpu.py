@@ -48,8 +48,8 @@ def test_read_refuses(pnb, change, text):
 
 @pytest.mark.parametrize("change,text", [
     ({3: 0}, b"group=0"), ({6: 0}, b"M=0"), ({6: 524161}, b"M=524161"), ({7: 0}, b"K=0"),
-    ({7: 65537}, b"K=65537"), ({8: 1, 4: NUL, 6: 65537}, b"K=65537"),
-    ({8: 1, 4: NUL, 7: 524161}, b"M=524161"), ({8: 1}, b"no bias"), ({10: 9}, b"at pitches 9"),
+    ({7: 61441}, b"K=61441"), ({8: 1, 4: NUL, 6: 61441}, b"M=61441"),
+    ({8: 1, 4: NUL, 7: 524161}, b"K=524161"), ({8: 1}, b"no bias"), ({10: 9}, b"at pitches 9"),
     ({12: 9}, b"and 9"), ({13: -1}, b"batch=-1"), ({14: 0}, b" 0 words"), ({0: NUL}, b"NULL"),
     ({1: NUL}, b"NULL"), ({9: NUL}, b"NULL"), ({11: NUL}, b"NULL"), ({9: ODD4}, b"64-bit words"),
     ({11: ODD4}, b"64-bit words"), ({4: ODD4}, b"64-bit words"),
@@ -60,7 +60,7 @@ def test_group_contract_refuses(pnb, change, text):
 
 
 @pytest.mark.parametrize("change,text", [
-    ({3: -2}, b"group=-2"), ({6: 0}, b"M=0"), ({6: 524161}, b"M=524161"), ({7: 65537}, b"K=65537"),
+    ({3: -2}, b"group=-2"), ({6: 0}, b"M=0"), ({6: 524161}, b"M=524161"), ({7: 61441}, b"K=61441"),
     ({10: 0}, b"cache_slots=0"), ({11: 12}, b"12 bits"), ({13: 9}, b"and 9"),
     ({14: -1}, b"batch=-1"), ({15: 0}, b" 0 words"), ({0: NUL}, b"NULL"), ({1: NUL}, b"NULL"),
     ({8: NUL}, b"NULL"), ({9: NUL}, b"NULL"), ({12: NUL}, b"NULL"), ({9: ODD8}, b"16-byte"),
