@@ -947,10 +947,11 @@ def group_contract(W: GroupWeights, bias: torch.Tensor | None, delta: int, X: to
         raise ValueError("a transposed product takes no bias")
     b = None if bias is None else _want("bias", bias, torch.int64, (W.M,), device)
     out = _want_out(out, (batch, n_out, ld), device, L, X)
-    ws = torch.empty(_group_bytes(n_in, n_out), dtype=torch.uint8, device=device)
+    need = _group_bytes(n_in, n_out)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch("pnb_group_contract", device, W.q.data_ptr(), W.scales.data_ptr(), _at(W.zeros),
             W.group, _at(b), delta % (1 << 64), W.M, W.K, 1 if transposed else 0, X.data_ptr(), ld,
-            out.data_ptr(), ld, batch, L, ws.data_ptr(), ws.numel())
+            out.data_ptr(), ld, batch, L, _at(ws), need)
     return out
 
 
@@ -971,16 +972,18 @@ def group_contract_cached(W: GroupWeights, bias: torch.Tensor | None, delta: int
     batch, ld = slots.shape[0], _pitch(cache, ld, out)
     b = None if bias is None else _want("bias", bias, torch.int64, (W.M,), device)
     out = _want_out(out, (batch, W.M, ld), device, cache.lwe_len, cache.data)
-    ws = torch.empty(_group_bytes(W.K, W.M), dtype=torch.uint8, device=device)
+    need = _group_bytes(W.K, W.M)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch("pnb_group_contract_cached", device, W.q.data_ptr(), W.scales.data_ptr(), _at(W.zeros),
             W.group, _at(b), delta % (1 << 64), W.M, W.K, slots.data_ptr(), cache.data.data_ptr(),
-            cache.slots, cache.bits, out.data_ptr(), ld, batch, cache.lwe_len, ws.data_ptr(),
-            ws.numel())
+            cache.slots, cache.bits, out.data_ptr(), ld, batch, cache.lwe_len, _at(ws), need)
     return out
 
 
 def _group_bytes(n_in: int, n_out: int) -> int:
-    """``pnb_group_contract_workspace_bytes``."""
+    """``pnb_group_contract_workspace_bytes``: none where the weights stay in shared memory."""
+    if n_in <= 896 and n_out <= 37 * 128 or n_in * n_out <= 256:
+        return 0
     return 2 * n_out * ((n_in + 15) & -16)
 
 

@@ -25,6 +25,46 @@ struct GroupWeights {
     const size_t g = (size_t)j * groups + i / group;
     return __ldg(scales + g) * (v - (zeros ? __ldg(zeros + g) & 15 : 8));
   }
+  // The weights of output o from 16 inputs on (in), as pairs of signed bytes w = lo + 256 hi; zeros
+  // past the last input.
+  __device__ __forceinline__ void bytes(int o, int in, int n_in, uint4& lo_out, uint4& hi_out) const {
+    union { int8_t b[16]; uint4 v; } lo, hi;
+    lo.v = hi.v = make_uint4(0, 0, 0, 0);
+    auto put = [&](int t, int w) {
+      lo.b[t] = (int8_t)w;
+      hi.b[t] = (int8_t)((w - lo.b[t]) >> 8);
+    };
+    if (transposed) {
+#pragma unroll
+      for (int t = 0; t < 16; ++t)
+        if (in + t < n_in) put(t, at(in + t, o));
+    } else {
+      const uint8_t* p = q + (size_t)o * ((K + 1) / 2) + in / 2;  // (in is a multiple of 16)
+      uint8_t v[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] = in + 2 * t < n_in ? __ldg(p + t) : 0;
+      size_t g = (size_t)o * groups + in / group;
+      int left = group - in % group, scale = 0, zero = 8;
+      auto fetch = [&] {
+        scale = __ldg(scales + g);
+        if (zeros) zero = __ldg(zeros + g) & 15;
+      };
+      if (in < n_in) fetch();
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        if (in + t >= n_in) break;
+        if (left == 0) {
+          ++g;
+          left = group;
+          fetch();
+        }
+        --left;
+        put(t, scale * ((v[t / 2] >> (4 * (t & 1)) & 15) - zero));
+      }
+    }
+    lo_out = lo.v;
+    hi_out = hi.v;
+  }
 };
 
 struct GroupArgs {
@@ -104,8 +144,9 @@ __global__ void __launch_bounds__(GF_THREADS) group_few_kernel(const __grid_cons
 }
 
 // ---- weights as bytes ---------------------------------------------------------------------------
-// Two matrices of signed bytes, w = lo + 256 hi: lo [n_out][pitch], then hi; rows are padded by zeros
-// to a multiple of 16 bytes.  A thread makes 16 bytes of both.
+// For calls whose weights do not stay in shared memory: two matrices of signed bytes, w = lo + 256 hi, lo
+// [n_out][pitch], then hi, rows padded by zeros to a multiple of 16 bytes.  A thread makes 16 bytes of
+// both.
 constexpr int GX_THREADS = 128;
 
 __global__ void __launch_bounds__(GX_THREADS)
@@ -117,17 +158,10 @@ __global__ void __launch_bounds__(GX_THREADS)
   const long long t = (long long)blockIdx.x * GX_THREADS + threadIdx.x;
   if (t >= (long long)chunks * n_out) return;
   const int o = (int)(w.transposed ? t % n_out : t / chunks);
-  const int i0 = (int)(w.transposed ? t / n_out : t % chunks) * 16;
-  union { int8_t b[16]; uint4 v; } lo, hi;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int v = i0 + i >= n_in ? 0 : w.transposed ? w.at(i0 + i, o) : w.at(o, i0 + i);
-    lo.b[i] = (int8_t)v;
-    hi.b[i] = (int8_t)((v - lo.b[i]) >> 8);
-  }
-  int8_t* out = to + (size_t)o * pitch + i0;
-  *reinterpret_cast<uint4*>(out) = lo.v;
-  *reinterpret_cast<uint4*>(out + (size_t)n_out * pitch) = hi.v;
+  const int in = (int)(w.transposed ? t / n_out : t % chunks) * 16;
+  int8_t* out = to + (size_t)o * pitch + in;
+  w.bytes(o, in, n_in, *reinterpret_cast<uint4*>(out),
+          *reinterpret_cast<uint4*>(out + (size_t)n_out * pitch));
 }
 
 // ---- tensor cores -------------------------------------------------------------------------------
@@ -143,40 +177,51 @@ int gc_status_read_and_clear(int* out) {
   return PNB_OK;
 }
 
-constexpr int GC_BM = 128;       // outputs per tile, one per TMEM lane
+constexpr int GC_BM = 128;       // outputs per tile
 constexpr int GC_WK = 128;       // inputs per weight slot
 constexpr int GC_KSTEP = 32;     // inputs per MMA
-constexpr int GC_W_HALF = GC_BM * GC_WK, GC_W_SLOT = 2 * GC_W_HALF;  // 16 KB of lo, 16 KB of hi
+constexpr int GC_W_HALF = 128 * GC_WK;  // 16 KB: 128 rows of weights
 constexpr int GC_X_SLOT = 16 * 1024;
 constexpr int GC_COPY_WARPS = 4;
 constexpr int GC_EPI_WARPS = 16;  // two groups of two per TMEM lane quarter
-constexpr int GC_PART = 8;        // words staged at a time: rows of 64 bytes
-constexpr int GC_STAGE = 32 * GC_PART * 8;  // of one warp
-constexpr int GC_MAX_W = 6, GC_MAX_X = 12, GC_MAX_RAW = 16;
+constexpr int GC_STAGE = 2048;    // staged results of one warp
+constexpr int GC_MAX_W = 8, GC_MAX_X = 12, GC_MAX_RAW = 16;
 constexpr int GC_BARS = 2 * (GC_MAX_W + GC_MAX_X + GC_MAX_RAW) + 4;
 constexpr int GC_BAR_BYTES = (8 * GC_BARS + 8 + 127) / 128 * 128;
 constexpr int GC_SMEM = 227 * 1024;
 constexpr uint32_t GC_WAIT_LIMIT = 1u << 24;
 
-// BYTES of an X word; STAGES accumulators.
-template <int BYTES, bool SHIFTED, int STAGES>
+// LONG: one block, weights stream, one accumulator of 256 columns for lo and one for hi.
+// SHORT: one block, weights stay, two accumulators of 128 columns for each.
+// PAIR: two blocks share a tile, weights stay, two accumulators of 256 columns; every second row of the
+//   weights is a hi, in one block those of the first 64 outputs, in the other of the last.
+enum GcMode { LONG, SHORT, PAIR };
+
+// BYTES of an X word.
+template <int BYTES, bool SHIFTED, GcMode MODE>
 struct GcShape {
-  static constexpr int LOAD = STAGES == 1 ? 256 : 128;   // bytes of an X row per tile,
+  static constexpr int STAGES = MODE == LONG ? 1 : 2;
+  static constexpr int LOAD = MODE == LONG ? 256 : 128;  // bytes of an X row that one block loads,
   static constexpr int BN = BYTES == 3 ? LOAD / 4 * 3 : LOAD;  // of which these are whole words
   static constexpr int WORDS = BN / BYTES;
+  static constexpr int TILE = MODE == PAIR ? 2 * WORDS : WORDS;  // words per tile
   static constexpr int BOXES = LOAD / 128;               // swizzle spans
   static constexpr int XK = GC_X_SLOT / LOAD;            // inputs per X slot
+  static constexpr int W_SLOT = (MODE == PAIR ? 1 : 2) * GC_W_HALF;  // 128 rows; 128 of lo, 128 of hi
   static constexpr int RAW_ROWS = XK / 2;                // inputs per raw slot, half of each parity
   static constexpr int RAW_PITCH = LOAD + 16;            // one word of shift, to 16 bytes
   static constexpr int RAW_SLOT = RAW_ROWS * RAW_PITCH;
   static constexpr int COPY = SHIFTED ? GC_COPY_WARPS : 0;
   static constexpr int MMA_WARP = 2 + COPY;  // warp 0 loads X, warp 1 the weights
-  static constexpr int EPI_WARP = MMA_WARP + 2;
+  static constexpr int ISSUERS = MODE == PAIR ? 1 : 2;   // warps that issue MMAs: by lo, by hi
+  static constexpr int EPI_WARP = MMA_WARP + ISSUERS;
   static constexpr int THREADS = 32 * (EPI_WARP + GC_EPI_WARPS);
-  static constexpr int EW = WORDS / (STAGES == 1 ? 4 : 2);  // words per epilogue warp,
-  static constexpr int CW = (BYTES == 8 ? 4 : BYTES == 2 ? 16 : 8) / (SHIFTED ? 2 : 1);  // at a time
-  static constexpr int COLS = CW * BYTES;
-  static constexpr int HI_AT = STAGES == 1 ? 256 : 128;  // columns from lo's sums to hi's
+  static constexpr int EW = TILE / (MODE == LONG ? 4 : 2);  // words per epilogue warp,
+  static constexpr int CW = (BYTES == 8 ? 4 : BYTES == 2 ? 16 : 8) / (SHIFTED ? 2 : 1);  // as many
+  static constexpr int COLS = CW * BYTES;                // columns of two loads at a time
+  static constexpr int HI_AT = MODE == LONG ? 256 : 128;    // columns from lo's sums to hi's
+  static constexpr int ROWS = MODE == PAIR ? 16 : 32;    // outputs of a warp
+  static constexpr int PART = GC_STAGE / 8 / ROWS;       // words of each staged at a time
 };
 
 struct GcMaps {
@@ -187,60 +232,60 @@ struct GcMaps {
 struct GcArgs {
   GroupArgs g;
   int off0, off1;    // words by which rows 0, 2, .. / 1, 3, .. start past 16-byte alignment
-  int n_tiles, m_tiles;            // tiles: outputs fastest, then words, then requests
-  int step_m, step_n, step_b;      // one grid of them
-  int keep_w;        // a block's tiles all have the same outputs, whose weights stay
+  int n_tiles, m_tiles;         // tiles: outputs fastest, then words, then requests
+  int step_m, step_n, step_b;   // one grid of them
   int w_slots, x_slots, raw_slots;
   int x_at, raw_at, out_at, bars_at;  // shared-memory offsets; weights at 0
   int plain_out;     // results leave by plain stores
 };
 
-// A block's tiles, one grid apart.  The next one's slot is on its way while one is worked on.
-struct GcTile {
-  int b, nt, m, src;
-};
+// The tiles of a block (or pair), one grid apart.  The next one's slot is on its way while one is
+// worked on.
 template <bool CACHED>
 struct GcWalk {
   const GcArgs& a;
-  int b, nt, m, slot = 0;
-  __device__ __forceinline__ explicit GcWalk(const GcArgs& args) : a(args) {
-    const unsigned u = blockIdx.x / (unsigned)a.m_tiles;
-    m = (int)(blockIdx.x - u * a.m_tiles);
-    b = (int)(u / (unsigned)a.n_tiles);
-    nt = (int)(u - (unsigned)b * a.n_tiles);
-    if (CACHED && b < a.g.batch) slot = __ldg(a.g.slots + b);
+  int b, nt, m, src, next_b, next_n, next_m, slot = 0;
+  __device__ __forceinline__ GcWalk(const GcArgs& args, unsigned first) : a(args) {
+    const unsigned u = first / (unsigned)a.m_tiles;
+    next_m = (int)(first - u * a.m_tiles);
+    next_b = (int)(u / (unsigned)a.n_tiles);
+    next_n = (int)(u - (unsigned)next_b * a.n_tiles);
+    if (CACHED && next_b < a.g.batch) slot = __ldg(a.g.slots + next_b);
   }
-  // the next tile that has something to do; false behind the last
-  __device__ __forceinline__ bool next(GcTile& tile) {
-    while (b < a.g.batch) {
-      tile = {b, nt, m, CACHED ? slot : b};
-      m += a.step_m;
-      const int carry_m = m >= a.m_tiles;
-      m -= carry_m ? a.m_tiles : 0;
-      nt += a.step_n + carry_m;
-      const int carry_n = nt >= a.n_tiles;
-      nt -= carry_n ? a.n_tiles : 0;
-      b += a.step_b + carry_n;
-      if (!CACHED) return true;
-      if (b < a.g.batch) slot = __ldg(a.g.slots + b);
-      if (tile.src >= 0 && tile.src < a.g.n_slots) return true;
-    }
-    return false;
+  // src: the place of the request's ciphertexts, or the number of slots where it has none
+  __device__ __forceinline__ bool next() {
+    if (next_b >= a.g.batch) return false;
+    b = next_b, nt = next_n, m = next_m;
+    src = !CACHED ? b : slot >= 0 && slot < a.g.n_slots ? slot : a.g.n_slots;
+    next_m += a.step_m;
+    const int carry_m = next_m >= a.m_tiles;
+    next_m -= carry_m ? a.m_tiles : 0;
+    next_n += a.step_n + carry_m;
+    const int carry_n = next_n >= a.n_tiles;
+    next_n -= carry_n ? a.n_tiles : 0;
+    next_b += a.step_b + carry_n;
+    if (CACHED && next_b < a.g.batch) slot = __ldg(a.g.slots + next_b);
+    return true;
   }
 };
 
 // Bounded wait that also gives up as soon as another role has flagged an abort.
+template <bool CLUSTER>
 __device__ __noinline__ bool gc_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_s) {
   for (uint32_t it = 0; it < GC_WAIT_LIMIT; it += 1024) {
-    if (tc::mbar_wait(bar, parity, 1024)) return true;
+    if (CLUSTER ? tc::mbar_wait_cluster(bar, parity, 1024) : tc::mbar_wait(bar, parity, 1024))
+      return true;
     if (*abort_s) return false;
   }
   *abort_s = 1;
   atomicExch(&g_gc_status, 1);
   return false;
 }
+// CLUSTER: for barriers on which the other block arrives too.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool gc_wait(uint32_t bar, uint32_t parity, volatile int* abort_s) {
-  return tc::mbar_test(bar, parity & 1u) || gc_wait_slow(bar, parity & 1u, abort_s);
+  return (CLUSTER ? tc::mbar_test_cluster(bar, parity & 1u) : tc::mbar_test(bar, parity & 1u)) ||
+         gc_wait_slow<CLUSTER>(bar, parity & 1u, abort_s);
 }
 
 template <int COLS>
@@ -256,37 +301,49 @@ __device__ __forceinline__ void gc_tmem_ld(uint32_t at, uint32_t (&r)[COLS]) {
   }
 }
 
-// The word that its limbs' sums by lo and by hi stand for, sum_p (lo[p] + hi[p-1]) << 8p mod 2^64: the
-// sums of two stay below 2^31 for up to 61922 inputs ((128 + 7) * 255 each).  Of a cache's word these are
-// the top limbs, and its low half is zero.
+// sum_p t[p] << 8p: a word mod 2^64, or the high half of one from a cache, whose low half is zero.
 template <int BYTES>
-__device__ __forceinline__ uint64_t gc_word(const uint32_t* lo, const uint32_t* hi) {
-  uint32_t t[BYTES];
-  t[0] = lo[0];
-#pragma unroll
-  for (int p = 1; p < BYTES; ++p) t[p] = lo[p] + hi[p - 1];
+__device__ __forceinline__ auto gc_limbs(const uint32_t* t) {
   if constexpr (BYTES == 8) {
     return add_limbs(0, t);
   } else {
     uint32_t v = t[0];
 #pragma unroll
     for (int p = 1; p < BYTES; ++p) v += t[p] << (8 * p);
-    return (uint64_t)(v << (32 - 8 * BYTES)) << 32;
+    return v << (32 - 8 * BYTES);
   }
 }
+// The word of limb sums by lo and by hi, sum_p (lo[p] + hi[p-1]) << 8p.  Sums of two stay below 2^31 for
+// up to 61922 inputs ((128 + 8) * 255 each).
+template <int BYTES>
+__device__ __forceinline__ auto gc_word(const uint32_t* lo, const uint32_t* hi) {
+  uint32_t t[BYTES];
+  t[0] = lo[0];
+#pragma unroll
+  for (int p = 1; p < BYTES; ++p) t[p] = lo[p] + hi[p - 1];
+  return gc_limbs<BYTES>(t);
+}
+__device__ __forceinline__ uint64_t gc_whole(uint64_t v) { return v; }
+__device__ __forceinline__ uint64_t gc_whole(uint32_t v) { return (uint64_t)v << 32; }
+__device__ __forceinline__ uint64_t gc_other_lane(uint64_t v) { return shfl_xor_u64(v, 1); }
+__device__ __forceinline__ uint32_t gc_other_lane(uint32_t v) {
+  return __shfl_xor_sync(0xffffffffu, v, 1);
+}
 
-template <int BYTES, bool SHIFTED, int STAGES>
-__global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, STAGES>::THREADS, 1)
+template <int BYTES, bool SHIFTED, GcMode MODE>
+__global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     group_kernel(const __grid_constant__ GcMaps tm, const __grid_constant__ GcArgs a) {
-  using S = GcShape<BYTES, SHIFTED, STAGES>;
+  using S = GcShape<BYTES, SHIFTED, MODE>;
   constexpr bool CACHED = BYTES != 8;
+  constexpr bool TWO = MODE == PAIR;
+  constexpr int STAGES = S::STAGES;
   extern __shared__ __align__(1024) unsigned char gc_raw[];  // the swizzles want 1024-byte boundaries
   const uint32_t base = tc::smem_u32(gc_raw);
   if (base & 1023u) {
     if (threadIdx.x == 0) atomicExch(&g_gc_status, 1);
     return;
   }
-  auto w_at = [&](int s) { return base + (uint32_t)(s * GC_W_SLOT); };
+  auto w_at = [&](int s) { return base + (uint32_t)(s * S::W_SLOT); };
   auto x_at = [&](int s) { return base + (uint32_t)(a.x_at + s * GC_X_SLOT); };
   auto raw_at = [&](int s) { return base + (uint32_t)(a.raw_at + s * S::RAW_SLOT); };
   const uint32_t bars = base + (uint32_t)a.bars_at;
@@ -297,40 +354,64 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, STAGES>::THREADS, 1)
   const uint32_t holder = bars + 8 * GC_BARS;
   volatile int* abort_s = reinterpret_cast<volatile int*>(gc_raw + (holder + 4 - base));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Of a pair the first block issues the MMAs of both; it is told of both blocks' slots.
+  const int rank = TWO ? (int)(blockIdx.x & 1u) : 0;
+  const unsigned first = TWO ? blockIdx.x >> 1 : blockIdx.x, grid = TWO ? gridDim.x >> 1 : gridDim.x;
+  auto leads = [&](uint32_t bar) { return TWO ? tc::cluster_address(bar, 0) : bar; };
+  auto arrive = [&](uint32_t bar) {  // on the first block's
+    if (TWO)
+      tc::mbar_arrive_cluster(leads(bar));
+    else
+      tc::mbar_arrive(bar);
+  };
+  auto commit = [&](uint32_t bar) {
+    if (TWO)
+      tc::mma_commit_pair(bar);  // on both blocks'
+    else
+      tc::mma_commit(bar);
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.w_slots; ++s) {
-      tc::mbar_init(w_full + 8 * s, 1);
-      tc::mbar_init(w_empty + 8 * s, 2);
+      tc::mbar_init(w_full + 8 * s, MODE == LONG ? 1 : (1 + TWO) * GC_EPI_WARPS);
+      tc::mbar_init(w_empty + 8 * s, S::ISSUERS);
     }
     for (int s = 0; s < a.x_slots; ++s) {
-      tc::mbar_init(x_full + 8 * s, SHIFTED ? S::COPY : 1);
-      tc::mbar_init(x_empty + 8 * s, 2);
+      tc::mbar_init(x_full + 8 * s, SHIFTED ? (1 + TWO) * S::COPY : 1);
+      tc::mbar_init(x_empty + 8 * s, S::ISSUERS);
     }
     for (int s = 0; s < a.raw_slots; ++s) {
       tc::mbar_init(r_full + 8 * s, 1);
       tc::mbar_init(r_empty + 8 * s, 1);
     }
     for (int s = 0; s < STAGES; ++s) {
-      tc::mbar_init(acc_full + 8 * s, 2);
-      tc::mbar_init(acc_empty + 8 * s, GC_EPI_WARPS / STAGES);
+      tc::mbar_init(acc_full + 8 * s, S::ISSUERS);
+      tc::mbar_init(acc_empty + 8 * s, (1 + TWO) * GC_EPI_WARPS / STAGES);
     }
     *abort_s = 0;
     tc::fence_mbar_init();
-    tc::prefetch_tmap(&tm.W);
+    if (MODE == LONG) tc::prefetch_tmap(&tm.W);
     tc::prefetch_tmap(&tm.X[0]);
     if (SHIFTED) tc::prefetch_tmap(&tm.X[1]);
     if (!a.plain_out) tc::prefetch_tmap(&tm.Y);
   }
-  if (warp == S::MMA_WARP) tc::tmem_alloc(holder, 512);
+  if (warp == S::MMA_WARP) {
+    if (TWO)
+      tc::tmem_alloc_pair(holder, 512);
+    else
+      tc::tmem_alloc(holder, 512);
+  }
   tc::tc_fence_before();
-  __syncthreads();
+  if (TWO)
+    tc::cluster_sync();
+  else
+    __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gc_raw + (holder - base));
 
   const int kx_n = (a.g.n_in + S::XK - 1) / S::XK;  // X slots of one tile
   const int kb_n = (a.g.n_in + GC_WK - 1) / GC_WK;  // weight slots
-  GcTile tile;
+  const long long tiles = ((long long)a.g.batch * a.n_tiles * a.m_tiles - first + grid - 1) / grid;
 
   if (warp == 0) {
     // ---------------- X loads (one lane) ---------------------------------------------------------
@@ -339,53 +420,59 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, STAGES>::THREADS, 1)
       TileRing ring;
       bool wrapped = false, ok = true;
       const int slots = SHIFTED ? a.raw_slots : a.x_slots;
-      GcWalk<CACHED> walk(a);
-      while (ok && walk.next(tile)) {
+      GcWalk<CACHED> walk(a, first);
+      while (ok && walk.next()) {
+        const int word = walk.nt * S::TILE + rank * S::WORDS;
         for (int k = 0; k < a.g.n_in; k += SHIFTED ? S::RAW_ROWS : S::XK) {
           const int s = ring.slot;
           const uint32_t full = (SHIFTED ? r_full : x_full) + 8 * s;
-          ok = gc_wait((SHIFTED ? r_empty : x_empty) + 8 * s, ring.phase ^ 1u, abort_s);
+          ok = gc_wait<TWO>((SHIFTED ? r_empty : x_empty) + 8 * s, ring.phase ^ 1u, abort_s);
           if (!ok) break;
           if (SHIFTED) {
-            const int row = tile.src * a.g.n_in + k;
+            const int row = walk.src * a.g.n_in + k;
             tc::mbar_expect_tx(full, S::RAW_SLOT);  // the rows of either parity, in order
-            tc::tma_load_2d(raw_at(s), &tm.X[row & 1], tile.nt * S::WORDS, row >> 1, full);
-            tc::tma_load_2d(raw_at(s) + S::RAW_SLOT / 2, &tm.X[(row + 1) & 1], tile.nt * S::WORDS,
-                            (row + 1) >> 1, full);
+            tc::tma_load_2d(raw_at(s), &tm.X[row & 1], word, row >> 1, full);
+            tc::tma_load_2d(raw_at(s) + S::RAW_SLOT / 2, &tm.X[(row + 1) & 1], word, (row + 1) >> 1,
+                            full);
           } else {
-            tc::mbar_expect_tx(full, GC_X_SLOT);  // rows past the last input read as zeros
+            // rows past the last input, and requests without a place, read as zeros
+            if (rank == 0) tc::mbar_expect_tx(full, (1 + TWO) * GC_X_SLOT);
 #pragma unroll
-            for (int b = 0; b < S::BOXES; ++b)
-              tc::tma_load_3d(x_at(s) + b * (S::XK * 128), &tm.X[0], tile.nt * S::BN + b * 128, k,
-                              tile.src, full);
+            for (int b = 0; b < S::BOXES; ++b) {
+              if (TWO)
+                tc::tma_load_3d_pair(x_at(s), &tm.X[0], word * BYTES, k, walk.src, leads(full));
+              else
+                tc::tma_load_3d(x_at(s) + b * (S::XK * 128), &tm.X[0], word * BYTES + b * 128, k,
+                                walk.src, full);
+            }
           }
           ring.advance(slots);
           wrapped |= ring.slot == 0;
         }
       }
-      tile_drain(SHIFTED ? r_full : x_full, ring, wrapped, slots, GC_WAIT_LIMIT);
+      if (SHIFTED || rank == 0)
+        tile_drain(SHIFTED ? r_full : x_full, ring, wrapped, slots, GC_WAIT_LIMIT);
     }
   } else if (warp == 1) {
     // ---------------- weight loads (one lane) ----------------------------------------------------
-    if (lane == 0) {
+    if (MODE == LONG && lane == 0) {
       asm volatile("griddepcontrol.wait;" ::: "memory");  // the weights' kernel is done
       TileRing ring;
       bool wrapped = false, ok = true;
-      GcWalk<CACHED> walk(a);
-      while (ok && walk.next(tile)) {
+      GcWalk<false> walk(a, first);
+      while (ok && walk.next()) {
         for (int k = 0; k < kb_n; ++k) {
           const int s = ring.slot;
           ok = gc_wait(w_empty + 8 * s, ring.phase ^ 1u, abort_s);
           if (!ok) break;
-          tc::mbar_expect_tx(w_full + 8 * s, GC_W_SLOT);
+          tc::mbar_expect_tx(w_full + 8 * s, S::W_SLOT);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            tc::tma_load_3d(w_at(s) + h * GC_W_HALF, &tm.W, k * GC_WK, tile.m * GC_BM, h,
+            tc::tma_load_3d(w_at(s) + h * GC_W_HALF, &tm.W, k * GC_WK, walk.m * GC_BM, h,
                             w_full + 8 * s);
           ring.advance(a.w_slots);
           wrapped |= ring.slot == 0;
         }
-        if (a.keep_w) break;
       }
       tile_drain(w_full, ring, wrapped, a.w_slots, GC_WAIT_LIMIT);
     }
@@ -396,17 +483,17 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, STAGES>::THREADS, 1)
     // turns apart.
     const int cw = warp - 2;
     constexpr int PER = SHIFTED ? 32 / S::WORDS : 1;  // rows per pass of a warp
-    constexpr int BATCH = 16;           // passes whose words are on their way together
+    constexpr int BATCH = 16;                         // passes whose words are on their way together
     const int word = lane % S::WORDS, sub = lane / S::WORDS;
     const int box = word >> 4, ch = (word & 15) >> 1, half = word & 1;
     TileRing xr, rr;
     bool ok = true;
-    GcWalk<CACHED> walk(a);
-    while (ok && walk.next(tile)) {
-      const int parity = tile.src * a.g.n_in & 1;  // of the tile's first row
+    GcWalk<CACHED> walk(a, first);
+    while (ok && walk.next()) {
+      const int parity = walk.src * a.g.n_in & 1;  // of the tile's first row
       const int off_e = parity ? a.off1 : a.off0, off_o = parity ? a.off0 : a.off1;
       for (int kx = 0; ok && kx < kx_n; ++kx) {
-        ok = gc_wait(x_empty + 8 * xr.slot, xr.phase ^ 1u, abort_s);
+        ok = gc_wait<TWO>(x_empty + 8 * xr.slot, xr.phase ^ 1u, abort_s);
         if (!ok) break;
         const int raws = min(2, (a.g.n_in - kx * S::XK + S::RAW_ROWS - 1) / S::RAW_ROWS);
         for (int i = 0; i < raws; ++i) {
@@ -440,14 +527,14 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, STAGES>::THREADS, 1)
           rr.advance(a.raw_slots);
         }
         if (!ok) break;
-        if (lane == 0) tc::mbar_arrive(x_full + 8 * xr.slot);
+        if (lane == 0) arrive(x_full + 8 * xr.slot);
         xr.advance(a.x_slots);
       }
     }
   } else if (warp < S::EPI_WARP) {
-    // ---------------- products: one warp's lane by lo, the other's by hi -------------------------
-    if (lane == 0) {
-      constexpr uint32_t IDESC = tc::idesc_i8(GC_BM, S::BN, true, false, false, true);
+    // ---------------- products (one lane): one warp by lo, another by hi, or of a pair all ----------
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t IDESC = tc::idesc_i8(TWO ? 256 : 128, (1 + TWO) * S::BN, true, false, false, true);
       constexpr int STEPS = S::XK / GC_KSTEP, PER_W = GC_WK / S::XK;
       const int hi = warp - S::MMA_WARP;
       const uint64_t wd = tc::smem_desc_sw128(w_at(0) + hi * GC_W_HALF, 16u, 1024u);
@@ -455,143 +542,191 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, STAGES>::THREADS, 1)
       const uint32_t w_hi = (uint32_t)(wd >> 32), x_hi = (uint32_t)(xd >> 32);
       const int steps = (a.g.n_in + GC_KSTEP - 1) / GC_KSTEP;
       TileRing x, w;
-      int tt = 0;
-      bool ok = true;
-      GcWalk<CACHED> walk(a);
-      while (ok && walk.next(tile)) {
-        const int buf = STAGES == 1 ? 0 : tt & 1;
+      bool ok = MODE == LONG || gc_wait<TWO>(w_full, 0, abort_s);
+      tc::tc_fence_after();
+      for (long long t = 0; ok && t < tiles; ++t) {
+        const int buf = STAGES == 1 ? 0 : (int)t & 1;
         const uint32_t d = tmem + (uint32_t)(buf * 256 + hi * S::HI_AT);
-        ok = gc_wait(acc_empty + 8 * buf, (uint32_t)(tt / STAGES) ^ 1u, abort_s);
+        ok = gc_wait<TWO>(acc_empty + 8 * buf, (uint32_t)(t / STAGES) ^ 1u, abort_s);
         if (!ok) break;
         tc::tc_fence_after();
-        const bool load = !a.keep_w || tt == 0;
-        if (a.keep_w) w = TileRing{};
         uint32_t acc = 0;
+        if (MODE != LONG) w.slot = 0;
         for (int left = steps; ok && left > 0;) {  // one weight slot
-          if (load) {
+          if (MODE == LONG) {
             ok = gc_wait(w_full + 8 * w.slot, w.phase, abort_s);
             if (!ok) break;
           }
-          const uint32_t w_lo = (uint32_t)wd + (uint32_t)(w.slot * (GC_W_SLOT / 16));
+          const uint32_t w_lo = (uint32_t)wd + (uint32_t)(w.slot * (S::W_SLOT / 16));
 #pragma unroll
           for (int h = 0; h < PER_W; ++h) {
             if (left <= 0) break;
-            ok = gc_wait(x_full + 8 * x.slot, x.phase, abort_s);
+            ok = gc_wait<TWO>(x_full + 8 * x.slot, x.phase, abort_s);
             if (!ok) break;
             const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (GC_X_SLOT / 16));
 #pragma unroll
             for (int k = 0; k < STEPS; ++k)
-              if (k < left)
-                tc::mma_i8_lo(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
-                              k ? 1u : acc);
+              if (k < left) {
+                if (TWO)
+                  tc::mma_i8_lo_pair(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
+                                     k ? 1u : acc);
+                else
+                  tc::mma_i8_lo(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
+                                k ? 1u : acc);
+              }
             acc = 1;
             left -= STEPS;
-            tc::mma_commit(x_empty + 8 * x.slot);
+            commit(x_empty + 8 * x.slot);
             x.advance(a.x_slots);
           }
-          if (!a.keep_w) tc::mma_commit(w_empty + 8 * w.slot);
-          w.advance(a.w_slots);
+          if (MODE == LONG) {
+            commit(w_empty + 8 * w.slot);
+            w.advance(a.w_slots);
+          } else {
+            ++w.slot;
+          }
         }
         if (!ok) break;
-        tc::mma_commit(acc_full + 8 * buf);
-        ++tt;
+        commit(acc_full + 8 * buf);
       }
     }
   } else {
-    // ---------------- epilogue -------------------------------------------------------------------
-    // Warp w reads TMEM lane quarter w % 4: 32 outputs, one per lane.  With two accumulators each group
-    // of eight warps has one of them, and a warp half of its words; with one, a warp has a quarter.
-    // Words are staged in shared memory, 32 outputs x 8 words at a time with the 16-byte chunks XORed by
-    // the row, and leave by TMA, or as row segments by plain stores.
+    // ---------------- weights that stay, then the epilogue ---------------------------------------
     const int e_w = warp - S::EPI_WARP;
+    if (MODE != LONG) {
+      // 16 bytes of lo and of hi per thread and turn, of one output and 16 inputs, into the K-major operand
+      // layout: its lo in row r and its hi in the row of the same number or, of a pair, the next row
+      const int m0 = (int)(first % (unsigned)a.m_tiles) * GC_BM + rank * 64;
+      constexpr int OUTS = TWO ? 64 : 128;
+      const int chunks = kb_n * (GC_WK / 16);
+      for (int i = threadIdx.x - 32 * S::EPI_WARP; i < OUTS * chunks; i += 32 * GC_EPI_WARPS) {
+        const int o = i % OUTS, c = i / OUTS;
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        if (m0 + o < a.g.n_out) a.g.w.bytes(m0 + o, 16 * c, a.g.n_in, lo, hi);
+        const int r_lo = TWO ? 2 * o : o, r_hi = TWO ? 2 * o + 1 : o;
+        unsigned char* to = gc_raw + (c >> 3) * S::W_SLOT;
+        *reinterpret_cast<uint4*>(to + r_lo * 128 + (((c & 7) ^ (r_lo & 7)) << 4)) = lo;
+        *reinterpret_cast<uint4*>(to + (TWO ? 0 : GC_W_HALF) + r_hi * 128 +
+                                  (((c & 7) ^ (r_hi & 7)) << 4)) = hi;
+      }
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive(w_full);
+    }
+    // Warp w reads TMEM lane quarter w % 4.  With two accumulators each group of eight warps has one of
+    // them, and a warp half of its words; with one, a warp has a quarter.  A lane holds the sums of one
+    // output, or of a pair an even lane those by lo and the odd lane beside it those by hi: of every two
+    // words each then completes one, with the other's share of it.  Words are staged in shared memory
+    // with the 16-byte chunks XORed by the row, and leave by TMA, or as row segments by plain stores.
     const int q = warp & 3, group = e_w >> 3, share = STAGES == 1 ? e_w >> 2 : (e_w >> 2) & 1;
     const uint32_t out_at = base + (uint32_t)(a.out_at + e_w * GC_STAGE);
     unsigned char* out = gc_raw + (out_at - base);
-    unsigned char* out_row = out + lane * 64;
-    const int out_x = (lane >> 1) & 3;
+    constexpr int PITCH = S::PART * 8;  // 64 or 128 bytes
+    auto xored = [](int r) { return TWO ? r & 7 : (r >> 1) & 3; };
+    const int row = TWO ? lane >> 1 : lane, odd = TWO ? lane & 1 : 0;
+    unsigned char* out_row = out + row * PITCH;
+    const int out_x = xored(row);
     int tt = 0;
-    GcWalk<CACHED> walk(a);
-    while (walk.next(tile)) {
+    GcWalk<CACHED> walk(a, first);
+    while (walk.next()) {
       const int buf = STAGES == 1 ? 0 : tt & 1;
       const uint32_t turn = (uint32_t)(tt / STAGES);
       ++tt;
       if (STAGES == 2 && buf != group) continue;
-      const int row0 = tile.m * GC_BM + q * 32, col0 = tile.nt * S::WORDS + share * S::EW;
-      // the body among this warp's words
-      const int body = a.g.L - 1 - col0;
-      const bool live = row0 + lane < a.g.n_out;
+      const int row0 = walk.m * GC_BM + rank * 64 + q * S::ROWS, col0 = walk.nt * S::TILE + share * S::EW;
+      const int body = a.g.L - 1 - col0;  // the body among this warp's words
+      const bool live = row0 + row < a.g.n_out;
       uint64_t bias = 0;
       if (a.g.bias && body >= 0 && body < S::EW && live)
-        bias = (uint64_t)__ldg(a.g.bias + row0 + lane) * a.g.delta;
+        bias = (uint64_t)__ldg(a.g.bias + row0 + row) * a.g.delta;
       if (!gc_wait(acc_full + 8 * buf, turn, abort_s)) break;
       tc::tc_fence_after();
       const uint32_t c_tmem = tmem + (uint32_t)(buf * 256 + share * S::EW * BYTES) +
                               ((uint32_t)(q * 32) << 16);
-      if (row0 >= a.g.n_out || body < 0) {  // nothing of this warp's share is kept
+      // nothing of this warp's share is kept
+      if (row0 >= a.g.n_out || body < 0 || (CACHED && walk.src == a.g.n_slots)) {
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(acc_empty + 8 * buf);
+        if (lane == 0) arrive(acc_empty + 8 * buf);
         continue;
       }
+      constexpr int FETCH = TWO ? 2 * S::CW : S::CW;  // words of one turn
 #pragma unroll
-      for (int i = 0; i < S::EW / S::CW; ++i) {
-        uint32_t lo[S::COLS], hi[S::COLS];
-        gc_tmem_ld<S::COLS>(c_tmem + (uint32_t)(i * S::COLS), lo);
-        gc_tmem_ld<S::COLS>(c_tmem + (uint32_t)(S::HI_AT + i * S::COLS), hi);
-        tc::tmem_ld_wait_pin(lo);
-        tc::tmem_ld_wait_pin(hi);
-        if (i + 1 == S::EW / S::CW) {
+      for (int i = 0; i < S::EW / FETCH; ++i) {
+        // lo's sums and hi's, or of a pair the sums of two runs of words
+        uint32_t c0[S::COLS], c1[S::COLS];
+        gc_tmem_ld<S::COLS>(c_tmem + (uint32_t)(i * FETCH * BYTES), c0);
+        gc_tmem_ld<S::COLS>(
+            c_tmem + (uint32_t)(TWO ? i * FETCH * BYTES + S::COLS : S::HI_AT + i * S::COLS), c1);
+        tc::tmem_ld_wait_pin(c0);
+        tc::tmem_ld_wait_pin(c1);
+        if (i + 1 == S::EW / FETCH) {
           tc::tc_fence_before();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(acc_empty + 8 * buf);
+          if (lane == 0) arrive(acc_empty + 8 * buf);
         }
+        constexpr int N = FETCH < S::PART ? FETCH : S::PART;
 #pragma unroll
-        for (int u0 = 0; u0 < S::CW; u0 += GC_PART) {
-          const int first = i * S::CW + u0;           // of this warp's words
-          const int part = first / GC_PART * GC_PART;  // the first word staged with it
-          constexpr int N = S::CW < GC_PART ? S::CW : GC_PART;
-          uint64_t y[N];
+        for (int u0 = 0; u0 < FETCH; u0 += N) {
+          const int first_w = i * FETCH + u0;               // of this warp's words
+          const int part = first_w / S::PART * S::PART;     // the first word staged with it
+          uint64_t y[N];                                    // of a pair every other one: this lane's
+          if constexpr (TWO) {
 #pragma unroll
-          for (int u = 0; u < N; ++u)
-            y[u] = gc_word<BYTES>(lo + (u0 + u) * BYTES, hi + (u0 + u) * BYTES);
-          if (first == part && !a.plain_out) {  // what was staged before has left
+            for (int u = 0; u < N; u += 2) {
+              auto at = [&](int w) { return w < S::CW ? c0 + w * BYTES : c1 + (w - S::CW) * BYTES; };
+              const auto v0 = gc_limbs<BYTES>(at(u0 + u)) << (8 * odd);
+              const auto v1 = gc_limbs<BYTES>(at(u0 + u + 1)) << (8 * odd);
+              y[u] = gc_whole((odd ? v1 : v0) + gc_other_lane(odd ? v0 : v1));
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+              y[u] = gc_whole(gc_word<BYTES>(c0 + (u0 + u) * BYTES, c1 + (u0 + u) * BYTES));
+          }
+          if (first_w == part && !a.plain_out) {  // what was staged before has left
             if (lane == 0) tc::tma_store_wait_read();
             __syncwarp();
           }
 #pragma unroll
-          for (int u = 0; u < N; u += 2)
-            *reinterpret_cast<ulonglong2*>(
-                out_row + ((((first - part + u) >> 1) ^ out_x) << 4)) =
-                make_ulonglong2(y[u], y[u + 1]);
-          if (first + N != part + GC_PART) continue;
-          if (body >= part && body < part + GC_PART) {
+          for (int u = 0; u < N; u += 2) {
+            unsigned char* to = out_row + ((((first_w - part + u) >> 1) ^ out_x) << 4);
+            if constexpr (TWO)
+              *reinterpret_cast<uint64_t*>(to + 8 * odd) = y[u];
+            else
+              *reinterpret_cast<ulonglong2*>(to) = make_ulonglong2(y[u], y[u + 1]);
+          }
+          if (first_w + N != part + S::PART) continue;
+          if (body >= part && body < part + S::PART && (!TWO || ((body - part) & 1) == odd)) {
             uint64_t* p = reinterpret_cast<uint64_t*>(
                 out_row + ((((body - part) >> 1) ^ out_x) << 4) + ((body - part) & 1) * 8);
             *p += bias;
             // tiled stores end on 16-byte boundaries, so the last word of an odd count goes alone
             if (!a.plain_out && (a.g.L & 1) && live)
-              a.g.Y[((size_t)tile.b * a.g.n_out + row0 + lane) * a.g.ldy + a.g.L - 1] = *p;
+              a.g.Y[((size_t)walk.b * a.g.n_out + row0 + row) * a.g.ldy + a.g.L - 1] = *p;
           }
           if (!a.plain_out) {
             tc::fence_async_smem();
             __syncwarp();
             if (lane == 0 && col0 + part < (a.g.L & ~1))
-              tc::tma_store_3d(&tm.Y, col0 + part, row0, tile.b, out_at);
+              tc::tma_store_3d(&tm.Y, col0 + part, row0, walk.b, out_at);
           } else {
             __syncwarp();
-            const int wd = lane & 7, sub = lane >> 3;  // four rows per instruction
-            uint64_t* to = a.g.Y + ((size_t)tile.b * a.g.n_out + row0 + sub) * a.g.ldy + col0 + part + wd;
+            constexpr int PER = 32 / S::PART;  // rows per instruction
+            const int wd = lane % S::PART, sub = lane / S::PART;
+            uint64_t* to =
+                a.g.Y + ((size_t)walk.b * a.g.n_out + row0 + sub) * a.g.ldy + col0 + part + wd;
             const int left = col0 + part + wd < a.g.L ? a.g.n_out - row0 - sub : 0;
             uint64_t v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const int r = 4 * j + sub;
+              const int r = PER * j + sub;
               v[j] = *reinterpret_cast<const uint64_t*>(
-                  out + r * 64 + (((wd >> 1) ^ ((r >> 1) & 3)) << 4) + (wd & 1) * 8);
+                  out + r * PITCH + (((wd >> 1) ^ xored(r)) << 4) + (wd & 1) * 8);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              if (4 * j < left) to[(size_t)(4 * j) * a.g.ldy] = v[j];
+              if (PER * j < left) to[(size_t)(PER * j) * a.g.ldy] = v[j];
             __syncwarp();
           }
         }
@@ -600,55 +735,66 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, STAGES>::THREADS, 1)
     if (!a.plain_out && lane == 0) tc::tma_store_wait();
   }
   tc::tc_fence_before();
-  __syncthreads();
+  if (TWO)
+    tc::cluster_sync();  // the other block's MMAs read this one's memory, and it arrives on its barriers
+  else
+    __syncthreads();
   if (warp == S::MMA_WARP) {
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem, 512);
+    if (TWO)
+      tc::tmem_dealloc_pair(tmem, 512);
+    else
+      tc::tmem_dealloc(tmem, 512);
   }
 }
 
 // ---- launch -------------------------------------------------------------------------------------
-// How one block's shared memory is shared out.  Weights stay when they leave X four slots (shifted rows:
-// three, and 36 KB of raw ones) and the grid is a whole number of times the tiles of outputs without
-// losing more than a sixteenth of the machine.
-template <int BYTES, bool SHIFTED, int STAGES>
+// Which way a call goes, by the layer's size alone (the caller's workspace depends on it).
+constexpr int GC_SHORT = 256;    // most inputs for SHORT,
+constexpr int GC_STAYS = 896;    // and for PAIR, whose weights leave X five slots
+constexpr int GC_MOST_TILES = 37;  // of outputs: a quarter of the machine
+static GcMode gc_mode(int n_in, int n_out) {
+  if (n_in > GC_STAYS || n_out > GC_MOST_TILES * GC_BM) return LONG;
+  return n_in <= GC_SHORT ? SHORT : PAIR;
+}
+
+// The grid, and how one block's shared memory is shared out.
+template <int BYTES, bool SHIFTED, GcMode MODE>
 static unsigned gc_plan(GcArgs& a, int sms) {
-  using S = GcShape<BYTES, SHIFTED, STAGES>;
-  a.n_tiles = (a.g.L + S::WORDS - 1) / S::WORDS;
-  const int kb = (a.g.n_in + GC_WK - 1) / GC_WK;
-  int room = GC_SMEM - GC_BAR_BYTES - GC_EPI_WARPS * GC_STAGE;
-  const int x_min = SHIFTED ? 3 : 4;
-  const int w_most =
-      std::min(GC_MAX_W, (room - (SHIFTED ? 4 * S::RAW_SLOT : 0) - x_min * GC_X_SLOT) / GC_W_SLOT);
-  const long long total = (long long)a.g.batch * a.n_tiles * a.m_tiles;
-  unsigned grid = (unsigned)std::min<long long>(total, sms);
-  const unsigned whole = grid / a.m_tiles * a.m_tiles;
-  a.keep_w = kb <= w_most && whole && 16 * (grid - whole) <= grid;
-  if (a.keep_w) grid = whole;
-  a.w_slots = a.keep_w ? kb : SHIFTED ? 2 : 3;
+  using S = GcShape<BYTES, SHIFTED, MODE>;
+  a.n_tiles = (a.g.L + S::TILE - 1) / S::TILE;
+  const int per = MODE == PAIR ? 2 : 1;
+  unsigned grid =
+      (unsigned)std::min<long long>((long long)a.g.batch * a.n_tiles * a.m_tiles, sms / per);
+  if (MODE != LONG) grid = grid / a.m_tiles * a.m_tiles;  // a block's tiles have the same outputs
   a.step_m = (int)(grid % a.m_tiles);
   a.step_n = (int)(grid / a.m_tiles % a.n_tiles);
   a.step_b = (int)(grid / a.m_tiles / a.n_tiles);
-  room -= a.w_slots * GC_W_SLOT;
+  int room = GC_SMEM - GC_BAR_BYTES - GC_EPI_WARPS * GC_STAGE;
+  a.w_slots = MODE != LONG ? (a.g.n_in + GC_WK - 1) / GC_WK : SHIFTED ? 2 : 3;
+  room -= a.w_slots * S::W_SLOT;
   if (SHIFTED) {
-    a.x_slots = x_min;
+    a.x_slots = 3;
+    if (room - 3 * GC_X_SLOT < GC_COPY_WARPS * S::RAW_SLOT) a.x_slots = 2;
     a.raw_slots = std::min(GC_MAX_RAW, (room - a.x_slots * GC_X_SLOT) / S::RAW_SLOT & ~3);
   } else {
     a.x_slots = std::min(GC_MAX_X, room / GC_X_SLOT);
     a.raw_slots = 0;
   }
-  a.x_at = a.w_slots * GC_W_SLOT;
+  a.x_at = a.w_slots * S::W_SLOT;
   a.out_at = a.x_at + a.x_slots * GC_X_SLOT;
   a.raw_at = a.out_at + GC_EPI_WARPS * GC_STAGE;
   a.bars_at = a.raw_at + a.raw_slots * S::RAW_SLOT;
-  return grid;
+  return grid * per;
 }
 
-template <int BYTES, bool SHIFTED, int STAGES>
-static int gc_launch(GcMaps& tm, GcArgs& a, cudaStream_t st) {
-  using S = GcShape<BYTES, SHIFTED, STAGES>;
+template <int BYTES, bool SHIFTED, GcMode MODE>
+static int gc_launch(GcArgs& a, int8_t* ws, cudaStream_t st) {
+  using S = GcShape<BYTES, SHIFTED, MODE>;
+  const GroupArgs& g = a.g;
+  const char* name = g.slots ? "group_contract_cached" : "group_contract";
   static std::atomic<int> sm_count[64];  // per device, once the kernel's shared-memory limit is raised
-  auto kernel = group_kernel<BYTES, SHIFTED, STAGES>;
+  auto kernel = group_kernel<BYTES, SHIFTED, MODE>;
   int dev = 0;
   PNB_CUDA(cudaGetDevice(&dev));
   int sms = dev < 64 ? sm_count[dev].load(std::memory_order_acquire) : 0;
@@ -657,8 +803,13 @@ static int gc_launch(GcMaps& tm, GcArgs& a, cudaStream_t st) {
     PNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GC_SMEM));
     if (dev < 64) sm_count[dev].store(sms, std::memory_order_release);
   }
-  const unsigned grid = gc_plan<BYTES, SHIFTED, STAGES>(a, sms);
-  const GroupArgs& g = a.g;
+  a.m_tiles = (g.n_out + GC_BM - 1) / GC_BM;
+  const unsigned grid = gc_plan<BYTES, SHIFTED, MODE>(a, sms);
+  if (grid == 0 || a.x_slots < 2 || (SHIFTED && a.raw_slots < GC_COPY_WARPS)) {
+    set_error("%s: no plan for %d inputs and %d outputs", name, g.n_in, g.n_out);
+    return PNB_ERR_INVALID;
+  }
+  GcMaps tm{};
   int rc = PNB_OK;
   if (!SHIFTED) {
     const cuuint64_t dims[3] = {(cuuint64_t)g.L * BYTES, (cuuint64_t)g.n_in,
@@ -671,6 +822,10 @@ static int gc_launch(GcMaps& tm, GcArgs& a, cudaStream_t st) {
     // rows p, p + 2, ..: from the 16-byte boundary at or before row p, at twice the pitch.  A row
     // off by one word has that word's 16 bytes inside its allocation (allocations start aligned).
     const long long x_rows = (long long)g.batch * g.n_in;
+    if (x_rows > 0x7fffffffLL - GC_WK) {  // coordinates are 32-bit
+      set_error("%s: %lld ciphertexts exceed a 32-bit index", name, x_rows);
+      return PNB_ERR_INVALID;
+    }
     for (int p = 0; p < 2 && !rc; ++p) {
       // (a single row has no row 1: both maps are its own, and the second meets zero weights)
       const bool second = p && x_rows > 1;
@@ -683,76 +838,76 @@ static int gc_launch(GcMaps& tm, GcArgs& a, cudaStream_t st) {
                     2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
     }
   }
+  if (!rc && !a.plain_out) {
+    // writes end at word L (rounded down to 16 bytes) of the last output of each request
+    const cuuint64_t dims[3] = {(cuuint64_t)std::max(2, g.L & ~1), (cuuint64_t)g.n_out,
+                                (cuuint64_t)g.batch};
+    const cuuint64_t strides[2] = {(cuuint64_t)g.ldy * 8, (cuuint64_t)g.ldy * 8 * g.n_out};
+    const cuuint32_t box[3] = {S::PART, S::ROWS, 1};
+    rc = tile_map(&tm.Y, CU_TENSOR_MAP_DATA_TYPE_UINT64, g.Y, 3, dims, strides, box,
+                  tile_swizzle(8 * S::PART));
+  }
   if (rc) return rc;
-  cudaLaunchAttribute attr;  // its set-up and its first loads of X run beside the weights' kernel
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr{};
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = (size_t)(a.bars_at + GC_BAR_BYTES);
   cfg.stream = st;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = MODE == SHORT ? 0 : 1;
+  if (MODE == PAIR) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {2, 1, 1};
+  }
+  if (MODE == LONG) {
+    const int pitch = (g.n_in + 15) & ~15;
+    const long long blocks = ((long long)g.n_out * (pitch / 16) + GX_THREADS - 1) / GX_THREADS;
+    if (blocks > 0x7fffffffLL) {
+      set_error("%s: %d x %d weights exceed one launch", name, g.n_out, g.n_in);
+      return PNB_ERR_INVALID;
+    }
+    const cuuint64_t dims[3] = {(cuuint64_t)pitch, (cuuint64_t)g.n_out, 2};
+    const cuuint64_t strides[2] = {(cuuint64_t)pitch, (cuuint64_t)pitch * g.n_out};
+    const cuuint32_t box[3] = {GC_WK, GC_BM, 1};
+    rc = tile_map(&tm.W, CU_TENSOR_MAP_DATA_TYPE_UINT8, ws, 3, dims, strides, box,
+                  CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    group_expand_kernel<<<(unsigned)blocks, GX_THREADS, 0, st>>>(g.w, g.n_in, g.n_out, pitch, ws);
+    PNB_CHECK_LAUNCH("group_expand_kernel");
+    // this kernel's set-up and its first loads of X run beside that one
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+  }
   PNB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tm, a));
   return PNB_OK;
 }
 
-constexpr int GC_LONG = 384;  // inputs from which one wide accumulator is faster than two
-
 template <int BYTES, bool SHIFTED>
-static int gc_stages(GcMaps& tm, GcArgs& a, cudaStream_t st) {
-  return a.g.n_in >= GC_LONG ? gc_launch<BYTES, SHIFTED, 1>(tm, a, st)
-                             : gc_launch<BYTES, SHIFTED, 2>(tm, a, st);
+static int gc_run(GcArgs& a, int8_t* ws, cudaStream_t st) {
+  switch (gc_mode(a.g.n_in, a.g.n_out)) {
+    case LONG: return gc_launch<BYTES, SHIFTED, LONG>(a, ws, st);
+    case SHORT: return gc_launch<BYTES, SHIFTED, SHORT>(a, ws, st);
+    default: return gc_launch<BYTES, SHIFTED, PAIR>(a, ws, st);
+  }
 }
 
 static int gc_run(const GroupArgs& g, int bits, int8_t* ws, cudaStream_t st) {
-  const char* name = g.slots ? "group_contract_cached" : "group_contract";
-  const int bytes = bits / 8;
   GcArgs a{};
   a.g = g;
-  a.m_tiles = (g.n_out + GC_BM - 1) / GC_BM;
-  a.off0 = bytes == 8 ? (int)((uintptr_t)g.X / 8 & 1) : 0;
-  a.off1 = bytes == 8 ? (int)(((uintptr_t)g.X + g.x_row) / 8 & 1) : 0;
-  const bool shifted = a.off0 || a.off1;
-  if (shifted && (long long)g.batch * g.n_in > 0x7fffffffLL - GC_WK) {
-    set_error("%s: %lld ciphertexts exceed a 32-bit index", name, (long long)g.batch * g.n_in);
-    return PNB_ERR_INVALID;
-  }
   a.plain_out = g.ldy % 2 != 0 || ((uintptr_t)g.Y % 16) != 0;
-  const int pitch = (g.n_in + 15) & ~15;
-  const long long blocks = ((long long)g.n_out * (pitch / 16) + GX_THREADS - 1) / GX_THREADS;
-  if (blocks > 0x7fffffffLL) {
-    set_error("%s: %d x %d weights exceed one launch", name, g.n_out, g.n_in);
-    return PNB_ERR_INVALID;
+  if (bits == 64) {
+    a.off0 = (int)((uintptr_t)g.X / 8 & 1);
+    a.off1 = (int)(((uintptr_t)g.X + g.x_row) / 8 & 1);
+    return a.off0 || a.off1 ? gc_run<8, true>(a, ws, st) : gc_run<8, false>(a, ws, st);
   }
-  GcMaps tm{};
-  const cuuint64_t w_dims[3] = {(cuuint64_t)pitch, (cuuint64_t)g.n_out, 2};
-  const cuuint64_t w_strides[2] = {(cuuint64_t)pitch, (cuuint64_t)pitch * g.n_out};
-  const cuuint32_t w_box[3] = {GC_WK, GC_BM, 1};
-  int rc = tile_map(&tm.W, CU_TENSOR_MAP_DATA_TYPE_UINT8, ws, 3, w_dims, w_strides, w_box,
-                    CU_TENSOR_MAP_SWIZZLE_128B);
-  if (!rc && !a.plain_out) {
-    // writes end at word L (rounded down to 16 bytes) of the last output of each request
-    const cuuint64_t dims[3] = {(cuuint64_t)std::max(2, g.L & ~1), (cuuint64_t)g.n_out,
-                                (cuuint64_t)g.batch};
-    const cuuint64_t strides[2] = {(cuuint64_t)g.ldy * 8, (cuuint64_t)g.ldy * 8 * g.n_out};
-    const cuuint32_t box[3] = {GC_PART, 32, 1};
-    rc = tile_map(&tm.Y, CU_TENSOR_MAP_DATA_TYPE_UINT64, g.Y, 3, dims, strides, box,
-                  CU_TENSOR_MAP_SWIZZLE_64B);
-  }
-  if (rc) return rc;
-  group_expand_kernel<<<(unsigned)blocks, GX_THREADS, 0, st>>>(g.w, g.n_in, g.n_out, pitch, ws);
-  PNB_CHECK_LAUNCH("group_expand_kernel");
-  switch (bytes) {
-    case 8: return shifted ? gc_stages<8, true>(tm, a, st) : gc_stages<8, false>(tm, a, st);
-    case 4: return gc_stages<4, false>(tm, a, st);
-    case 3: return gc_stages<3, false>(tm, a, st);
-    default: return gc_stages<2, false>(tm, a, st);
-  }
+  return bits == 32 ? gc_run<4, false>(a, ws, st)
+         : bits == 24 ? gc_run<3, false>(a, ws, st)
+                      : gc_run<2, false>(a, ws, st);
 }
 
 size_t group_workspace_bytes(int n_in, int n_out) {
+  if ((long long)n_in * n_out <= GF_MOST || gc_mode(n_in, n_out) != LONG) return 0;
   return (size_t)2 * n_out * (((size_t)n_in + 15) & ~(size_t)15);
 }
 
@@ -773,14 +928,14 @@ static int few_run(const GroupArgs& a, int bits, cudaStream_t st) {
 
 static int group_run(const GroupArgs& a, int bits, void* ws, size_t ws_bytes, cudaStream_t st) {
   const size_t need = group_workspace_bytes(a.n_in, a.n_out);
-  if (ws && (ws_bytes < need || ((uintptr_t)ws % 16) != 0)) {
+  if (need && ws && (ws_bytes < need || ((uintptr_t)ws % 16) != 0)) {
     set_error("%s: workspace of %zu bytes at %p, %zu bytes 16-byte aligned are needed",
               a.slots ? "group_contract_cached" : "group_contract", ws_bytes, ws, need);
     return PNB_ERR_INVALID;
   }
   if ((long long)a.n_in * a.n_out <= GF_MOST) return few_run(a, bits, st);
   int8_t* own = nullptr;
-  if (!ws) PNB_CUDA(cudaMallocAsync((void**)&own, need, st));
+  if (need && !ws) PNB_CUDA(cudaMallocAsync((void**)&own, need, st));
   int rc = gc_run(a, bits, own ? own : (int8_t*)ws, st);
   if (own) {
     const cudaError_t e = cudaFreeAsync(own, st);

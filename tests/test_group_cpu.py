@@ -53,7 +53,7 @@ def test_read_refuses(pnb, change, text):
     ({12: 9}, b"and 9"), ({13: -1}, b"batch=-1"), ({14: 0}, b" 0 words"), ({0: NUL}, b"NULL"),
     ({1: NUL}, b"NULL"), ({9: NUL}, b"NULL"), ({11: NUL}, b"NULL"), ({9: ODD4}, b"64-bit words"),
     ({11: ODD4}, b"64-bit words"), ({4: ODD4}, b"64-bit words"),
-    ({15: P, 16: 95}, b"95 bytes"), ({15: ODD8, 16: 96}, b"16-byte"),
+    ({7: 1000, 15: P, 16: 6047}, b"6047 bytes"), ({7: 1000, 15: ODD8, 16: 6048}, b"16-byte"),
 ])
 def test_group_contract_refuses(pnb, change, text):
     _refused(pnb, "pnb_group_contract", GROUP, change, text)
@@ -65,7 +65,7 @@ def test_group_contract_refuses(pnb, change, text):
     ({14: -1}, b"batch=-1"), ({15: 0}, b" 0 words"), ({0: NUL}, b"NULL"), ({1: NUL}, b"NULL"),
     ({8: NUL}, b"NULL"), ({9: NUL}, b"NULL"), ({12: NUL}, b"NULL"), ({9: ODD8}, b"16-byte"),
     ({8: ODD2}, b"32-bit integers"), ({12: ODD4}, b"64-bit words"), ({4: ODD4}, b"64-bit words"),
-    ({16: P, 17: 95}, b"95 bytes"), ({16: ODD8, 17: 96}, b"16-byte"),
+    ({7: 1000, 16: P, 17: 6047}, b"6047 bytes"), ({7: 1000, 16: ODD8, 17: 6048}, b"16-byte"),
 ])
 def test_group_contract_cached_refuses(pnb, change, text):
     _refused(pnb, "pnb_group_contract_cached", CACHED, change, text)
@@ -95,7 +95,8 @@ def test_row_bytes_of_nothing(pnb):
     assert pnb.lib().pnb_cache_row_bytes(10, 48) == 0
 
 
-@pytest.mark.parametrize("M,K", [(1, 1), (3, 5), (10, 128), (128, 784), (33, 17), (16, 16)])
+@pytest.mark.parametrize("M,K", [(1, 1), (3, 5), (10, 128), (128, 784), (33, 17), (16, 16),
+                                 (896, 897), (4736, 100), (4737, 100), (1, 61440)])
 def test_binding_and_library_agree_on_workspaces(pnb, M, K):
     L = pnb.lib()
     assert L.pnb_group_contract_workspace_bytes(M, K, 0) == pnb._group_bytes(K, M)
