@@ -14,6 +14,8 @@
 
 namespace pnb {
 
+constexpr uint32_t GROUP_BIAS = 2048;  // above every |w|
+
 struct GroupWeights {
   const uint8_t* q;      // [M][ceil(K / 2)], low nibble first
   const int8_t* scales;  // [M][groups]
@@ -25,45 +27,88 @@ struct GroupWeights {
     const size_t g = (size_t)j * groups + i / group;
     return __ldg(scales + g) * (v - (zeros ? __ldg(zeros + g) & 15 : 8));
   }
-  // The weights of output o from 16 inputs on (in), as pairs of signed bytes w = lo + 256 hi; zeros
-  // past the last input.
-  __device__ __forceinline__ void bytes(int o, int in, int n_in, uint4& lo_out, uint4& hi_out) const {
-    union { int8_t b[16]; uint4 v; } lo, hi;
-    lo.v = hi.v = make_uint4(0, 0, 0, 0);
-    auto put = [&](int t, int w) {
-      lo.b[t] = (int8_t)w;
-      hi.b[t] = (int8_t)((w - lo.b[t]) >> 8);
-    };
+  // The weights of output o for the 16 inputs from `in` (a multiple of 16) on as signed bytes, w = lo +
+  // 256 hi, four to a word; zeros past the last input.
+  //
+  // Eight weights at a time: two nibbles in the halves of a word, times the scale and plus 2048 - scale *
+  // zero in both halves, give u = w + 2048 > 0 twice without a borrow between them.  The low byte of u is
+  // that of w, and hi = ((u + 128) >> 8) - 8.
+  __device__ __forceinline__ void bytes(int o, int in, int n_in, uint32_t (&lo)[4],
+                                        uint32_t (&hi)[4]) const {
+    const int n = min(16, n_in - in);
+    const int pitch = (K + 1) / 2;
+    uint32_t u[8];  // the u of inputs 8 h + k in the low half of u[4 h + k], of 8 h + k + 4 in its high one
     if (transposed) {
-#pragma unroll
-      for (int t = 0; t < 16; ++t)
-        if (in + t < n_in) put(t, at(in + t, o));
-    } else {
-      const uint8_t* p = q + (size_t)o * ((K + 1) / 2) + in / 2;  // (in is a multiple of 16)
-      uint8_t v[8];
-#pragma unroll
-      for (int t = 0; t < 8; ++t) v[t] = in + 2 * t < n_in ? __ldg(p + t) : 0;
-      size_t g = (size_t)o * groups + in / group;
-      int left = group - in % group, scale = 0, zero = 8;
-      auto fetch = [&] {
-        scale = __ldg(scales + g);
-        if (zeros) zero = __ldg(zeros + g) & 15;
-      };
-      if (in < n_in) fetch();
+      const uint8_t* qp = q + (size_t)in * pitch + o / 2;
+      const size_t g = (size_t)in * groups + o / group;
+      uint32_t v[16];
 #pragma unroll
       for (int t = 0; t < 16; ++t) {
-        if (in + t >= n_in) break;
-        if (left == 0) {
-          ++g;
-          left = group;
-          fetch();
+        v[t] = GROUP_BIAS;
+        if (t < n) {
+          const int nib = __ldg(qp + (size_t)t * pitch) >> (4 * (o & 1)) & 15;
+          const int zero = zeros ? __ldg(zeros + g + (size_t)t * groups) & 15 : 8;
+          v[t] += (uint32_t)(__ldg(scales + g + (size_t)t * groups) * (nib - zero));
         }
-        --left;
-        put(t, scale * ((v[t / 2] >> (4 * (t & 1)) & 15) - zero));
+      }
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        u[t] = v[t / 4 * 8 + t % 4] | v[t / 4 * 8 + t % 4 + 4] << 16;
+    } else {
+      const uint8_t* qp = q + (size_t)o * pitch + in / 2;
+      size_t g = (size_t)o * groups + in / group;
+      int left = group - in % group;  // inputs of the first group
+      uint32_t v[2] = {0, 0};
+      if (n == 16 && ((uintptr_t)q & 3) == 0 && (pitch & 3) == 0) {
+        v[0] = __ldg(reinterpret_cast<const uint32_t*>(qp));
+        v[1] = __ldg(reinterpret_cast<const uint32_t*>(qp) + 1);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          if (2 * t < n) v[t / 4] |= (uint32_t)__ldg(qp + t) << (8 * (t % 4));
+      }
+      if (left >= n && n == 16) {
+        const int scale = __ldg(scales + g), zero = zeros ? __ldg(zeros + g) & 15 : 8;
+        const uint32_t more = (uint32_t)((int)GROUP_BIAS - scale * zero) * 0x10001u;
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          u[t] = (v[t / 4] >> (4 * (t % 4)) & 0x000f000fu) * (uint32_t)scale + more;
+      } else {
+        int scale = 0, zero = 0;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) u[t] = GROUP_BIAS * 0x10001u;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+          if (t < n) {
+            if (t == 0 || left == 0) {
+              if (t != 0) {
+                ++g;
+                left = group;
+              }
+              scale = __ldg(scales + g);
+              zero = zeros ? __ldg(zeros + g) & 15 : 8;
+            }
+            --left;
+            const int w = scale * ((int)(v[t / 8] >> (4 * (t % 8)) & 15) - zero);
+            u[t / 8 * 4 + t % 4] += (uint32_t)w << (t & 4 ? 16 : 0);
+          }
+        }
       }
     }
-    lo_out = lo.v;
-    hi_out = hi.v;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t* x = u + 4 * h;
+      const uint32_t l01 = __byte_perm(x[0], x[1], 0x6240), l23 = __byte_perm(x[2], x[3], 0x6240);
+      lo[2 * h] = __byte_perm(l01, l23, 0x5410);
+      lo[2 * h + 1] = __byte_perm(l01, l23, 0x7632);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] += 0x00800080u;
+      const uint32_t h01 = __byte_perm(x[0], x[1], 0x7351), h23 = __byte_perm(x[2], x[3], 0x7351);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)  // each byte less 8
+        hi[2 * h + k] = ((__byte_perm(h01, h23, k ? 0x7632 : 0x5410) | 0x80808080u) - 0x08080808u) ^
+                        0x80808080u;
+    }
   }
 };
 
@@ -82,7 +127,6 @@ struct GroupArgs {
 // One thread per word, 16 outputs at a time, weights in shared memory as w + 2048 >= 0, so that a product
 // is one 32 x 32 + 64 and one 32 x 32 + 32 bit multiply-add and sum w x = sum (w + 2048) x - 2048 sum x.
 constexpr int GF_THREADS = 256, GF_OUT = 16, GF_IN = 64;
-constexpr uint32_t GF_BIAS = 2048;
 constexpr long long GF_MOST = 256;  // weights that go this way
 
 // A word of X, of 8 bytes or the top 2, 3 or 4 of them.
@@ -111,7 +155,7 @@ __global__ void __launch_bounds__(GF_THREADS) group_few_kernel(const __grid_cons
       for (int i = threadIdx.x; i < n * GF_OUT; i += GF_THREADS) {
         const int k = i / GF_OUT, j = j0 + i % GF_OUT;
         const int w = j >= a.n_out ? 0 : a.w.transposed ? a.w.at(k0 + k, j) : a.w.at(j, k0 + k);
-        w_s[k][i % GF_OUT] = GF_BIAS + (uint32_t)w;
+        w_s[k][i % GF_OUT] = GROUP_BIAS + (uint32_t)w;
       }
       __syncthreads();
       if (c >= a.L) continue;
@@ -136,7 +180,7 @@ __global__ void __launch_bounds__(GF_THREADS) group_few_kernel(const __grid_cons
 #pragma unroll
     for (int u = 0; u < GF_OUT; ++u) {
       if (j0 + u >= a.n_out) break;
-      uint64_t v = acc[u] - GF_BIAS * sum;
+      uint64_t v = acc[u] - GROUP_BIAS * sum;
       if (a.bias && c == a.L - 1) v += (uint64_t)__ldg(a.bias + j0 + u) * a.delta;
       y[(size_t)u * a.ldy] = v;
     }
@@ -160,8 +204,10 @@ __global__ void __launch_bounds__(GX_THREADS)
   const int o = (int)(w.transposed ? t % n_out : t / chunks);
   const int in = (int)(w.transposed ? t / n_out : t % chunks) * 16;
   int8_t* out = to + (size_t)o * pitch + in;
-  w.bytes(o, in, n_in, *reinterpret_cast<uint4*>(out),
-          *reinterpret_cast<uint4*>(out + (size_t)n_out * pitch));
+  uint32_t lo[4], hi[4];
+  w.bytes(o, in, n_in, lo, hi);
+  *reinterpret_cast<uint4*>(out) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  *reinterpret_cast<uint4*>(out + (size_t)n_out * pitch) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
 }
 
 // ---- tensor cores -------------------------------------------------------------------------------
@@ -353,7 +399,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
   const uint32_t acc_full = r_empty + 8 * GC_MAX_RAW, acc_empty = acc_full + 16;
   const uint32_t holder = bars + 8 * GC_BARS;
   volatile int* abort_s = reinterpret_cast<volatile int*>(gc_raw + (holder + 4 - base));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // Of a pair the first block issues the MMAs of both; it is told of both blocks' slots.
   const int rank = TWO ? (int)(blockIdx.x & 1u) : 0;
   const unsigned first = TWO ? blockIdx.x >> 1 : blockIdx.x, grid = TWO ? gridDim.x >> 1 : gridDim.x;
@@ -532,18 +578,20 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
       }
     }
   } else if (warp < S::EPI_WARP) {
-    // ---------------- products (one lane): one warp by lo, another by hi, or of a pair all ----------
-    if (lane == 0 && rank == 0) {
+    // ---------------- products: one warp by lo, another by hi, or of a pair one for both -----------
+    // The whole warp goes through the loop and one lane issues: what every lane knows stays in uniform
+    // registers, which the MMAs take their operands from.
+    if (rank == 0) {
       constexpr uint32_t IDESC = tc::idesc_i8(TWO ? 256 : 128, (1 + TWO) * S::BN, true, false, false, true);
       constexpr int STEPS = S::XK / GC_KSTEP, PER_W = GC_WK / S::XK;
+      const bool one = tc::elect_one();
       const int hi = warp - S::MMA_WARP;
       const uint64_t wd = tc::smem_desc_sw128(w_at(0) + hi * GC_W_HALF, 16u, 1024u);
       const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
       const uint32_t w_hi = (uint32_t)(wd >> 32), x_hi = (uint32_t)(xd >> 32);
       const int steps = (a.g.n_in + GC_KSTEP - 1) / GC_KSTEP;
       TileRing x, w;
-      bool ok = MODE == LONG || gc_wait<TWO>(w_full, 0, abort_s);
-      tc::tc_fence_after();
+      bool ok = true;
       for (long long t = 0; ok && t < tiles; ++t) {
         const int buf = STAGES == 1 ? 0 : (int)t & 1;
         const uint32_t d = tmem + (uint32_t)(buf * 256 + hi * S::HI_AT);
@@ -553,8 +601,8 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
         uint32_t acc = 0;
         if (MODE != LONG) w.slot = 0;
         for (int left = steps; ok && left > 0;) {  // one weight slot
-          if (MODE == LONG) {
-            ok = gc_wait(w_full + 8 * w.slot, w.phase, abort_s);
+          if (MODE == LONG || t == 0) {
+            ok = gc_wait<TWO>(w_full + 8 * w.slot, w.phase, abort_s);
             if (!ok) break;
           }
           const uint32_t w_lo = (uint32_t)wd + (uint32_t)(w.slot * (S::W_SLOT / 16));
@@ -564,30 +612,32 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
             ok = gc_wait<TWO>(x_full + 8 * x.slot, x.phase, abort_s);
             if (!ok) break;
             const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (GC_X_SLOT / 16));
+            if (one) {
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-              if (k < left) {
-                if (TWO)
-                  tc::mma_i8_lo_pair(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
-                                     k ? 1u : acc);
-                else
-                  tc::mma_i8_lo(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
-                                k ? 1u : acc);
-              }
+              for (int k = 0; k < STEPS; ++k)
+                if (k < left) {
+                  if (TWO)
+                    tc::mma_i8_lo_pair(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
+                                       k ? 1u : acc);
+                  else
+                    tc::mma_i8_lo(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
+                                  k ? 1u : acc);
+                }
+              commit(x_empty + 8 * x.slot);
+            }
             acc = 1;
             left -= STEPS;
-            commit(x_empty + 8 * x.slot);
             x.advance(a.x_slots);
           }
           if (MODE == LONG) {
-            commit(w_empty + 8 * w.slot);
+            if (one) commit(w_empty + 8 * w.slot);
             w.advance(a.w_slots);
           } else {
             ++w.slot;
           }
         }
         if (!ok) break;
-        commit(acc_full + 8 * buf);
+        if (one) commit(acc_full + 8 * buf);
       }
     }
   } else {
@@ -595,23 +645,28 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     const int e_w = warp - S::EPI_WARP;
     if (MODE != LONG) {
       // 16 bytes of lo and of hi per thread and turn, of one output and 16 inputs, into the K-major operand
-      // layout: its lo in row r and its hi in the row of the same number or, of a pair, the next row
+      // layout: its lo in row r and its hi in the row of the same number or, of a pair, the next row.  The
+      // MMAs of a slot's inputs may start when it is full.
       const int m0 = (int)(first % (unsigned)a.m_tiles) * GC_BM + rank * 64;
-      constexpr int OUTS = TWO ? 64 : 128;
-      const int chunks = kb_n * (GC_WK / 16);
-      for (int i = threadIdx.x - 32 * S::EPI_WARP; i < OUTS * chunks; i += 32 * GC_EPI_WARPS) {
-        const int o = i % OUTS, c = i / OUTS;
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        if (m0 + o < a.g.n_out) a.g.w.bytes(m0 + o, 16 * c, a.g.n_in, lo, hi);
-        const int r_lo = TWO ? 2 * o : o, r_hi = TWO ? 2 * o + 1 : o;
-        unsigned char* to = gc_raw + (c >> 3) * S::W_SLOT;
-        *reinterpret_cast<uint4*>(to + r_lo * 128 + (((c & 7) ^ (r_lo & 7)) << 4)) = lo;
-        *reinterpret_cast<uint4*>(to + (TWO ? 0 : GC_W_HALF) + r_hi * 128 +
-                                  (((c & 7) ^ (r_hi & 7)) << 4)) = hi;
+      constexpr int OUTS = TWO ? 64 : 128, SLOT = OUTS * (GC_WK / 16);  // turns of one slot
+      for (int s = 0; s < kb_n; ++s) {
+#pragma unroll
+        for (int i = 0; i < SLOT; i += 32 * GC_EPI_WARPS) {
+          const int t = i + (int)threadIdx.x - 32 * S::EPI_WARP, o = t % OUTS, c = t / OUTS;
+          uint32_t lo[4] = {}, hi[4] = {};
+          if (m0 + o < a.g.n_out && s * GC_WK + 16 * c < a.g.n_in)
+            a.g.w.bytes(m0 + o, s * GC_WK + 16 * c, a.g.n_in, lo, hi);
+          const int r_lo = TWO ? 2 * o : o, r_hi = TWO ? 2 * o + 1 : o;
+          unsigned char* to = gc_raw + s * S::W_SLOT;
+          *reinterpret_cast<uint4*>(to + r_lo * 128 + ((c ^ (r_lo & 7)) << 4)) =
+              make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(to + (TWO ? 0 : GC_W_HALF) + r_hi * 128 + ((c ^ (r_hi & 7)) << 4)) =
+              make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        }
+        tc::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) arrive(w_full + 8 * s);
       }
-      tc::fence_async_smem();
-      __syncwarp();
-      if (lane == 0) arrive(w_full);
     }
     // Warp w reads TMEM lane quarter w % 4.  With two accumulators each group of eight warps has one of
     // them, and a warp half of its words; with one, a warp has a quarter.  A lane holds the sums of one
