@@ -27,73 +27,53 @@ struct GroupWeights {
     const size_t g = (size_t)j * groups + i / group;
     return __ldg(scales + g) * (v - (zeros ? __ldg(zeros + g) & 15 : 8));
   }
-  // The weights of output o for the 16 inputs from `in` (a multiple of 16) on as signed bytes, w = lo +
-  // 256 hi, four to a word; zeros past the last input.
+  // The weights of output o for the 16 inputs from `in` (a multiple of 16, below n_in) on as signed
+  // bytes, w = lo + 256 hi, four to a word; zeros past the last input.
   //
   // Eight weights at a time: two nibbles in the halves of a word, times the scale and plus 2048 - scale *
   // zero in both halves, give u = w + 2048 > 0 twice without a borrow between them.  The low byte of u is
   // that of w, and hi = ((u + 128) >> 8) - 8.
   __device__ __forceinline__ void bytes(int o, int in, int n_in, uint32_t (&lo)[4],
                                         uint32_t (&hi)[4]) const {
-    const int n = min(16, n_in - in);
-    const int pitch = (K + 1) / 2;
     uint32_t u[8];  // the u of inputs 8 h + k in the low half of u[4 h + k], of 8 h + k + 4 in its high one
-    if (transposed) {
-      const uint8_t* qp = q + (size_t)in * pitch + o / 2;
-      const size_t g = (size_t)in * groups + o / group;
-      uint32_t v[16];
+    const int pitch = (K + 1) / 2;
+    if (!transposed && in + 16 <= n_in && in % group + 16 <= group) {  // one scale
+      const uint8_t* p = q + (size_t)o * pitch + in / 2;
+      uint32_t v[2] = {0, 0};
+      if (((uintptr_t)q & 3) == 0 && (pitch & 3) == 0) {
+        v[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        v[1] = __ldg(reinterpret_cast<const uint32_t*>(p) + 1);
+      } else {
 #pragma unroll
-      for (int t = 0; t < 16; ++t) {
-        v[t] = GROUP_BIAS;
-        if (t < n) {
-          const int nib = __ldg(qp + (size_t)t * pitch) >> (4 * (o & 1)) & 15;
-          const int zero = zeros ? __ldg(zeros + g + (size_t)t * groups) & 15 : 8;
-          v[t] += (uint32_t)(__ldg(scales + g + (size_t)t * groups) * (nib - zero));
-        }
+        for (int t = 0; t < 8; ++t) v[t / 4] |= (uint32_t)__ldg(p + t) << (8 * (t % 4));
       }
+      const size_t g = (size_t)o * groups + in / group;
+      const int scale = __ldg(scales + g), zero = zeros ? __ldg(zeros + g) & 15 : 8;
+      const uint32_t more = (uint32_t)((int)GROUP_BIAS - scale * zero) * 0x10001u;
 #pragma unroll
       for (int t = 0; t < 8; ++t)
-        u[t] = v[t / 4 * 8 + t % 4] | v[t / 4 * 8 + t % 4 + 4] << 16;
+        u[t] = (v[t / 4] >> (4 * (t % 4)) & 0x000f000fu) * (uint32_t)scale + more;
     } else {
-      const uint8_t* qp = q + (size_t)o * pitch + in / 2;
-      size_t g = (size_t)o * groups + in / group;
-      int left = group - in % group;  // inputs of the first group
-      uint32_t v[2] = {0, 0};
-      if (n == 16 && ((uintptr_t)q & 3) == 0 && (pitch & 3) == 0) {
-        v[0] = __ldg(reinterpret_cast<const uint32_t*>(qp));
-        v[1] = __ldg(reinterpret_cast<const uint32_t*>(qp) + 1);
-      } else {
+      // all loads on their way together
+      const int n = min(16, n_in - in);
+      int w[16], scale[16], zero[16];
+      const uint8_t* p = transposed ? q + (size_t)in * pitch + o / 2 : q + (size_t)o * pitch + in / 2;
+      const size_t g0 = transposed ? (size_t)in * groups + o / group : (size_t)o * groups;
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
-          if (2 * t < n) v[t / 4] |= (uint32_t)__ldg(qp + t) << (8 * (t % 4));
+      for (int t = 0; t < 16; ++t) {
+        const size_t row = t < n ? t : 0;
+        const size_t g = transposed ? g0 + row * groups : g0 + (in + (int)row) / group;
+        w[t] = __ldg(p + (transposed ? row * pitch : row / 2));
+        scale[t] = __ldg(scales + g);
+        zero[t] = zeros ? __ldg(zeros + g) : 8;
       }
-      if (left >= n && n == 16) {
-        const int scale = __ldg(scales + g), zero = zeros ? __ldg(zeros + g) & 15 : 8;
-        const uint32_t more = (uint32_t)((int)GROUP_BIAS - scale * zero) * 0x10001u;
 #pragma unroll
-        for (int t = 0; t < 8; ++t)
-          u[t] = (v[t / 4] >> (4 * (t % 4)) & 0x000f000fu) * (uint32_t)scale + more;
-      } else {
-        int scale = 0, zero = 0;
+      for (int t = 0; t < 16; ++t)
+        w[t] = t < n ? scale[t] * ((w[t] >> (4 * ((transposed ? o : t) & 1)) & 15) - (zero[t] & 15)) : 0;
 #pragma unroll
-        for (int t = 0; t < 8; ++t) u[t] = GROUP_BIAS * 0x10001u;
-#pragma unroll
-        for (int t = 0; t < 16; ++t) {
-          if (t < n) {
-            if (t == 0 || left == 0) {
-              if (t != 0) {
-                ++g;
-                left = group;
-              }
-              scale = __ldg(scales + g);
-              zero = zeros ? __ldg(zeros + g) & 15 : 8;
-            }
-            --left;
-            const int w = scale * ((int)(v[t / 8] >> (4 * (t % 8)) & 15) - zero);
-            u[t / 8 * 4 + t % 4] += (uint32_t)w << (t & 4 ? 16 : 0);
-          }
-        }
-      }
+      for (int t = 0; t < 8; ++t)
+        u[t] = (uint32_t)(w[t / 4 * 8 + t % 4] + (int)GROUP_BIAS) |
+               (uint32_t)(w[t / 4 * 8 + t % 4 + 4] + (int)GROUP_BIAS) << 16;
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -188,7 +168,7 @@ __global__ void __launch_bounds__(GF_THREADS) group_few_kernel(const __grid_cons
 }
 
 // ---- weights as bytes ---------------------------------------------------------------------------
-// For calls whose weights do not stay in shared memory: two matrices of signed bytes, w = lo + 256 hi, lo
+// Two matrices of signed bytes, w = lo + 256 hi, lo
 // [n_out][pitch], then hi, rows padded by zeros to a multiple of 16 bytes.  A thread makes 16 bytes of
 // both.
 constexpr int GX_THREADS = 128;
@@ -230,7 +210,10 @@ constexpr int GC_W_HALF = 128 * GC_WK;  // 16 KB: 128 rows of weights
 constexpr int GC_X_SLOT = 16 * 1024;
 constexpr int GC_COPY_WARPS = 4;
 constexpr int GC_EPI_WARPS = 16;  // two groups of two per TMEM lane quarter
-constexpr int GC_STAGE = 2048;    // staged results of one warp
+// Which way a call goes, by the layer's size alone (the caller's workspace depends on it).
+constexpr int GC_SHORT = 384;      // most inputs for SHORT,
+constexpr int GC_STAYS = 896;      // and for PAIR, whose weights leave X six slots
+constexpr int GC_MOST_TILES = 37;  // of outputs: a quarter of the machine
 constexpr int GC_MAX_W = 8, GC_MAX_X = 12, GC_MAX_RAW = 16;
 constexpr int GC_BARS = 2 * (GC_MAX_W + GC_MAX_X + GC_MAX_RAW) + 4;
 constexpr int GC_BAR_BYTES = (8 * GC_BARS + 8 + 127) / 128 * 128;
@@ -267,7 +250,8 @@ struct GcShape {
   static constexpr int COLS = CW * BYTES;                // columns of two loads at a time
   static constexpr int HI_AT = MODE == LONG ? 256 : 128;    // columns from lo's sums to hi's
   static constexpr int ROWS = MODE == PAIR ? 16 : 32;    // outputs of a warp
-  static constexpr int PART = GC_STAGE / 8 / ROWS;       // words of each staged at a time
+  static constexpr int PART = 8;                         // words of each staged at a time
+  static constexpr int STAGE = ROWS * PART * 8;          // of one warp
 };
 
 struct GcMaps {
@@ -283,6 +267,7 @@ struct GcArgs {
   int w_slots, x_slots, raw_slots;
   int x_at, raw_at, out_at, bars_at;  // shared-memory offsets; weights at 0
   int plain_out;     // results leave by plain stores
+  int in_place;      // SHORT: the weights are expanded by every block for itself
 };
 
 // The tiles of a block (or pair), one grid apart.  The next one's slot is on its way while one is
@@ -419,7 +404,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.w_slots; ++s) {
-      tc::mbar_init(w_full + 8 * s, MODE == LONG ? 1 : (1 + TWO) * GC_EPI_WARPS);
+      tc::mbar_init(w_full + 8 * s, MODE == SHORT && a.in_place ? GC_EPI_WARPS : 1);
       tc::mbar_init(w_empty + 8 * s, S::ISSUERS);
     }
     for (int s = 0; s < a.x_slots; ++s) {
@@ -436,7 +421,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     }
     *abort_s = 0;
     tc::fence_mbar_init();
-    if (MODE == LONG) tc::prefetch_tmap(&tm.W);
+    if (!a.in_place) tc::prefetch_tmap(&tm.W);
     tc::prefetch_tmap(&tm.X[0]);
     if (SHIFTED) tc::prefetch_tmap(&tm.X[1]);
     if (!a.plain_out) tc::prefetch_tmap(&tm.Y);
@@ -461,7 +446,10 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
 
   if (warp == 0) {
     // ---------------- X loads (one lane) ---------------------------------------------------------
-    // X was there before the weights' kernel began, so it need not be waited for.
+    // (X was there before the weights' kernel began, so it need not be waited for.)
+    // Loads of X fill the memory's queues, so those of weights that are expanded here go first.
+    if (MODE == SHORT && a.in_place)
+      asm volatile("barrier.cta.sync 1, %0;" ::"n"(32 * GC_EPI_WARPS + 32) : "memory");
     if (lane == 0) {
       TileRing ring;
       bool wrapped = false, ok = true;
@@ -501,7 +489,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     }
   } else if (warp == 1) {
     // ---------------- weight loads (one lane) ----------------------------------------------------
-    if (MODE == LONG && lane == 0) {
+    if (lane == 0 && !a.in_place) {
       asm volatile("griddepcontrol.wait;" ::: "memory");  // the weights' kernel is done
       TileRing ring;
       bool wrapped = false, ok = true;
@@ -511,16 +499,21 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
           const int s = ring.slot;
           ok = gc_wait(w_empty + 8 * s, ring.phase ^ 1u, abort_s);
           if (!ok) break;
-          tc::mbar_expect_tx(w_full + 8 * s, S::W_SLOT);
+          if (rank == 0) tc::mbar_expect_tx(w_full + 8 * s, (1 + TWO) * S::W_SLOT);
+          if (TWO)  // rows of lo and of hi in turn
+            tc::tma_load_3d_pair(w_at(s), &tm.W, k * GC_WK, 0, walk.m * GC_BM + rank * 64,
+                                 leads(w_full + 8 * s));
+          else
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            tc::tma_load_3d(w_at(s) + h * GC_W_HALF, &tm.W, k * GC_WK, walk.m * GC_BM, h,
-                            w_full + 8 * s);
+            for (int h = 0; h < 2; ++h)
+              tc::tma_load_3d(w_at(s) + h * GC_W_HALF, &tm.W, k * GC_WK, walk.m * GC_BM, h,
+                              w_full + 8 * s);
           ring.advance(a.w_slots);
           wrapped |= ring.slot == 0;
         }
+        if (MODE != LONG) break;  // they stay
       }
-      tile_drain(w_full, ring, wrapped, a.w_slots, GC_WAIT_LIMIT);
+      if (rank == 0) tile_drain(w_full, ring, wrapped, a.w_slots, GC_WAIT_LIMIT);
     }
   } else if (SHIFTED && warp < S::MMA_WARP) {
     // ---------------- raw rows -> operand layout (shifted rows only) -----------------------------
@@ -643,30 +636,23 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
   } else {
     // ---------------- weights that stay, then the epilogue ---------------------------------------
     const int e_w = warp - S::EPI_WARP;
-    if (MODE != LONG) {
+    if (MODE == SHORT && a.in_place) {
       // 16 bytes of lo and of hi per thread and turn, of one output and 16 inputs, into the K-major operand
-      // layout: its lo in row r and its hi in the row of the same number or, of a pair, the next row.  The
-      // MMAs of a slot's inputs may start when it is full.
-      const int m0 = (int)(first % (unsigned)a.m_tiles) * GC_BM + rank * 64;
-      constexpr int OUTS = TWO ? 64 : 128, SLOT = OUTS * (GC_WK / 16);  // turns of one slot
-      for (int s = 0; s < kb_n; ++s) {
-#pragma unroll
-        for (int i = 0; i < SLOT; i += 32 * GC_EPI_WARPS) {
-          const int t = i + (int)threadIdx.x - 32 * S::EPI_WARP, o = t % OUTS, c = t / OUTS;
-          uint32_t lo[4] = {}, hi[4] = {};
-          if (m0 + o < a.g.n_out && s * GC_WK + 16 * c < a.g.n_in)
-            a.g.w.bytes(m0 + o, s * GC_WK + 16 * c, a.g.n_in, lo, hi);
-          const int r_lo = TWO ? 2 * o : o, r_hi = TWO ? 2 * o + 1 : o;
-          unsigned char* to = gc_raw + s * S::W_SLOT;
-          *reinterpret_cast<uint4*>(to + r_lo * 128 + ((c ^ (r_lo & 7)) << 4)) =
-              make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          *reinterpret_cast<uint4*>(to + (TWO ? 0 : GC_W_HALF) + r_hi * 128 + ((c ^ (r_hi & 7)) << 4)) =
-              make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        }
-        tc::fence_async_smem();
-        __syncwarp();
-        if (lane == 0) arrive(w_full + 8 * s);
+      // layout
+      const int m0 = (int)(first % (unsigned)a.m_tiles) * GC_BM;
+#pragma unroll 1
+      for (int i = (int)threadIdx.x - 32 * S::EPI_WARP; i < GC_BM * GC_WK / 16; i += 32 * GC_EPI_WARPS) {
+        const int o = i % GC_BM, c = i / GC_BM;
+        uint32_t lo[4] = {}, hi[4] = {};
+        if (m0 + o < a.g.n_out && 16 * c < a.g.n_in) a.g.w.bytes(m0 + o, 16 * c, a.g.n_in, lo, hi);
+        unsigned char* to = gc_raw + o * 128 + ((c ^ (o & 7)) << 4);
+        *reinterpret_cast<uint4*>(to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint4*>(to + GC_W_HALF) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       }
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(w_full);
+      asm volatile("barrier.cta.arrive 1, %0;" ::"n"(32 * GC_EPI_WARPS + 32) : "memory");
     }
     // Warp w reads TMEM lane quarter w % 4.  With two accumulators each group of eight warps has one of
     // them, and a warp half of its words; with one, a warp has a quarter.  A lane holds the sums of one
@@ -674,10 +660,10 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     // words each then completes one, with the other's share of it.  Words are staged in shared memory
     // with the 16-byte chunks XORed by the row, and leave by TMA, or as row segments by plain stores.
     const int q = warp & 3, group = e_w >> 3, share = STAGES == 1 ? e_w >> 2 : (e_w >> 2) & 1;
-    const uint32_t out_at = base + (uint32_t)(a.out_at + e_w * GC_STAGE);
+    const uint32_t out_at = base + (uint32_t)(a.out_at + e_w * S::STAGE);
     unsigned char* out = gc_raw + (out_at - base);
-    constexpr int PITCH = S::PART * 8;  // 64 or 128 bytes
-    auto xored = [](int r) { return TWO ? r & 7 : (r >> 1) & 3; };
+    constexpr int PITCH = S::PART * 8;
+    auto xored = [](int r) { return (r >> 1) & 3; };
     const int row = TWO ? lane >> 1 : lane, odd = TWO ? lane & 1 : 0;
     unsigned char* out_row = out + row * PITCH;
     const int out_x = xored(row);
@@ -772,15 +758,16 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
             uint64_t* to =
                 a.g.Y + ((size_t)walk.b * a.g.n_out + row0 + sub) * a.g.ldy + col0 + part + wd;
             const int left = col0 + part + wd < a.g.L ? a.g.n_out - row0 - sub : 0;
-            uint64_t v[8];
+            constexpr int TIMES = S::ROWS / PER;
+            uint64_t v[TIMES];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < TIMES; ++j) {
               const int r = PER * j + sub;
               v[j] = *reinterpret_cast<const uint64_t*>(
                   out + r * PITCH + (((wd >> 1) ^ xored(r)) << 4) + (wd & 1) * 8);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < TIMES; ++j)
               if (PER * j < left) to[(size_t)(PER * j) * a.g.ldy] = v[j];
             __syncwarp();
           }
@@ -804,13 +791,13 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
 }
 
 // ---- launch -------------------------------------------------------------------------------------
-// Which way a call goes, by the layer's size alone (the caller's workspace depends on it).
-constexpr int GC_SHORT = 256;    // most inputs for SHORT,
-constexpr int GC_STAYS = 896;    // and for PAIR, whose weights leave X five slots
-constexpr int GC_MOST_TILES = 37;  // of outputs: a quarter of the machine
 static GcMode gc_mode(int n_in, int n_out) {
   if (n_in > GC_STAYS || n_out > GC_MOST_TILES * GC_BM) return LONG;
   return n_in <= GC_SHORT ? SHORT : PAIR;
+}
+// One slot of weights is expanded by every block for itself, which saves a launch; more by a kernel before.
+static bool gc_in_place(int n_in, int n_out) {
+  return n_in <= GC_WK && gc_mode(n_in, n_out) == SHORT;
 }
 
 // The grid, and how one block's shared memory is shared out.
@@ -825,7 +812,7 @@ static unsigned gc_plan(GcArgs& a, int sms) {
   a.step_m = (int)(grid % a.m_tiles);
   a.step_n = (int)(grid / a.m_tiles % a.n_tiles);
   a.step_b = (int)(grid / a.m_tiles / a.n_tiles);
-  int room = GC_SMEM - GC_BAR_BYTES - GC_EPI_WARPS * GC_STAGE;
+  int room = GC_SMEM - GC_BAR_BYTES - GC_EPI_WARPS * S::STAGE;
   a.w_slots = MODE != LONG ? (a.g.n_in + GC_WK - 1) / GC_WK : SHIFTED ? 2 : 3;
   room -= a.w_slots * S::W_SLOT;
   if (SHIFTED) {
@@ -838,7 +825,7 @@ static unsigned gc_plan(GcArgs& a, int sms) {
   }
   a.x_at = a.w_slots * S::W_SLOT;
   a.out_at = a.x_at + a.x_slots * GC_X_SLOT;
-  a.raw_at = a.out_at + GC_EPI_WARPS * GC_STAGE;
+  a.raw_at = a.out_at + GC_EPI_WARPS * S::STAGE;
   a.bars_at = a.raw_at + a.raw_slots * S::RAW_SLOT;
   return grid * per;
 }
@@ -903,36 +890,44 @@ static int gc_launch(GcArgs& a, int8_t* ws, cudaStream_t st) {
                   tile_swizzle(8 * S::PART));
   }
   if (rc) return rc;
-  cudaLaunchAttribute attr{};
+  cudaLaunchAttribute attrs[2]{};
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = (size_t)(a.bars_at + GC_BAR_BYTES);
   cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = MODE == SHORT ? 0 : 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = 0;
   if (MODE == PAIR) {
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {2, 1, 1};
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim = {2, 1, 1};
+    cfg.numAttrs = 1;
   }
-  if (MODE == LONG) {
+  if (!a.in_place) {
     const int pitch = (g.n_in + 15) & ~15;
     const long long blocks = ((long long)g.n_out * (pitch / 16) + GX_THREADS - 1) / GX_THREADS;
     if (blocks > 0x7fffffffLL) {
       set_error("%s: %d x %d weights exceed one launch", name, g.n_out, g.n_in);
       return PNB_ERR_INVALID;
     }
-    const cuuint64_t dims[3] = {(cuuint64_t)pitch, (cuuint64_t)g.n_out, 2};
-    const cuuint64_t strides[2] = {(cuuint64_t)pitch, (cuuint64_t)pitch * g.n_out};
-    const cuuint32_t box[3] = {GC_WK, GC_BM, 1};
+    const cuuint64_t all = (cuuint64_t)pitch * g.n_out;
+    cuuint64_t dims[3] = {(cuuint64_t)pitch, (cuuint64_t)g.n_out, 2};
+    cuuint64_t strides[2] = {(cuuint64_t)pitch, all};
+    cuuint32_t box[3] = {GC_WK, GC_BM, 1};
+    if (MODE == PAIR) {
+      std::swap(dims[1], dims[2]);
+      std::swap(strides[0], strides[1]);
+      box[1] = 2;
+      box[2] = GC_BM / 2;
+    }
     rc = tile_map(&tm.W, CU_TENSOR_MAP_DATA_TYPE_UINT8, ws, 3, dims, strides, box,
                   CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     group_expand_kernel<<<(unsigned)blocks, GX_THREADS, 0, st>>>(g.w, g.n_in, g.n_out, pitch, ws);
     PNB_CHECK_LAUNCH("group_expand_kernel");
     // this kernel's set-up and its first loads of X run beside that one
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
   PNB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tm, a));
   return PNB_OK;
@@ -950,6 +945,7 @@ static int gc_run(GcArgs& a, int8_t* ws, cudaStream_t st) {
 static int gc_run(const GroupArgs& g, int bits, int8_t* ws, cudaStream_t st) {
   GcArgs a{};
   a.g = g;
+  a.in_place = gc_in_place(g.n_in, g.n_out);
   a.plain_out = g.ldy % 2 != 0 || ((uintptr_t)g.Y % 16) != 0;
   if (bits == 64) {
     a.off0 = (int)((uintptr_t)g.X / 8 & 1);
@@ -962,7 +958,7 @@ static int gc_run(const GroupArgs& g, int bits, int8_t* ws, cudaStream_t st) {
 }
 
 size_t group_workspace_bytes(int n_in, int n_out) {
-  if ((long long)n_in * n_out <= GF_MOST || gc_mode(n_in, n_out) != LONG) return 0;
+  if ((long long)n_in * n_out <= GF_MOST || gc_in_place(n_in, n_out)) return 0;
   return (size_t)2 * n_out * (((size_t)n_in + 15) & ~(size_t)15);
 }
 
