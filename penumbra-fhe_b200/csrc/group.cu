@@ -312,7 +312,7 @@ __device__ __noinline__ bool gc_wait_slow(uint32_t bar, uint32_t parity, volatil
   atomicExch(&g_gc_status, 1);
   return false;
 }
-// CLUSTER: for barriers on which the other block arrives too.
+// CLUSTER: for what the other block's threads have written.
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool gc_wait(uint32_t bar, uint32_t parity, volatile int* abort_s) {
   return (CLUSTER ? tc::mbar_test_cluster(bar, parity & 1u) : tc::mbar_test(bar, parity & 1u)) ||
@@ -389,9 +389,9 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
   const int rank = TWO ? (int)(blockIdx.x & 1u) : 0;
   const unsigned first = TWO ? blockIdx.x >> 1 : blockIdx.x, grid = TWO ? gridDim.x >> 1 : gridDim.x;
   auto leads = [&](uint32_t bar) { return TWO ? tc::cluster_address(bar, 0) : bar; };
-  auto arrive = [&](uint32_t bar) {  // on the first block's
+  auto drained = [&](uint32_t bar) {  // the first block's: a warp's loads from tensor memory are done
     if (TWO)
-      tc::mbar_arrive_cluster(leads(bar));
+      tc::mbar_arrive_cluster_relaxed(leads(bar));
     else
       tc::mbar_arrive(bar);
   };
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
         for (int k = 0; k < a.g.n_in; k += SHIFTED ? S::RAW_ROWS : S::XK) {
           const int s = ring.slot;
           const uint32_t full = (SHIFTED ? r_full : x_full) + 8 * s;
-          ok = gc_wait<TWO>((SHIFTED ? r_empty : x_empty) + 8 * s, ring.phase ^ 1u, abort_s);
+          ok = gc_wait((SHIFTED ? r_empty : x_empty) + 8 * s, ring.phase ^ 1u, abort_s);
           if (!ok) break;
           if (SHIFTED) {
             const int row = walk.src * a.g.n_in + k;
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
       const int parity = walk.src * a.g.n_in & 1;  // of the tile's first row
       const int off_e = parity ? a.off1 : a.off0, off_o = parity ? a.off0 : a.off1;
       for (int kx = 0; ok && kx < kx_n; ++kx) {
-        ok = gc_wait<TWO>(x_empty + 8 * xr.slot, xr.phase ^ 1u, abort_s);
+        ok = gc_wait(x_empty + 8 * xr.slot, xr.phase ^ 1u, abort_s);
         if (!ok) break;
         const int raws = min(2, (a.g.n_in - kx * S::XK + S::RAW_ROWS - 1) / S::RAW_ROWS);
         for (int i = 0; i < raws; ++i) {
@@ -566,7 +566,12 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
           rr.advance(a.raw_slots);
         }
         if (!ok) break;
-        if (lane == 0) arrive(x_full + 8 * xr.slot);
+        if (lane == 0) {
+          if (TWO)
+            tc::mbar_arrive_cluster(leads(x_full + 8 * xr.slot));
+          else
+            tc::mbar_arrive(x_full + 8 * xr.slot);
+        }
         xr.advance(a.x_slots);
       }
     }
@@ -588,21 +593,21 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
       for (long long t = 0; ok && t < tiles; ++t) {
         const int buf = STAGES == 1 ? 0 : (int)t & 1;
         const uint32_t d = tmem + (uint32_t)(buf * 256 + hi * S::HI_AT);
-        ok = gc_wait<TWO>(acc_empty + 8 * buf, (uint32_t)(t / STAGES) ^ 1u, abort_s);
+        ok = gc_wait(acc_empty + 8 * buf, (uint32_t)(t / STAGES) ^ 1u, abort_s);
         if (!ok) break;
         tc::tc_fence_after();
         uint32_t acc = 0;
         if (MODE != LONG) w.slot = 0;
         for (int left = steps; ok && left > 0;) {  // one weight slot
           if (MODE == LONG || t == 0) {
-            ok = gc_wait<TWO>(w_full + 8 * w.slot, w.phase, abort_s);
+            ok = gc_wait(w_full + 8 * w.slot, w.phase, abort_s);
             if (!ok) break;
           }
           const uint32_t w_lo = (uint32_t)wd + (uint32_t)(w.slot * (S::W_SLOT / 16));
 #pragma unroll
           for (int h = 0; h < PER_W; ++h) {
             if (left <= 0) break;
-            ok = gc_wait<TWO>(x_full + 8 * x.slot, x.phase, abort_s);
+            ok = gc_wait<TWO && SHIFTED>(x_full + 8 * x.slot, x.phase, abort_s);
             if (!ok) break;
             const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (GC_X_SLOT / 16));
             if (one) {
@@ -688,7 +693,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
       if (row0 >= a.g.n_out || body < 0 || (CACHED && walk.src == a.g.n_slots)) {
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive(acc_empty + 8 * buf);
+        if (lane == 0) drained(acc_empty + 8 * buf);
         continue;
       }
       constexpr int FETCH = TWO ? 2 * S::CW : S::CW;  // words of one turn
@@ -704,7 +709,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
         if (i + 1 == S::EW / FETCH) {
           tc::tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive(acc_empty + 8 * buf);
+          if (lane == 0) drained(acc_empty + 8 * buf);
         }
         constexpr int N = FETCH < S::PART ? FETCH : S::PART;
 #pragma unroll
