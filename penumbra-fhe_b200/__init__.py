@@ -657,16 +657,19 @@ def _want(name: str, t, dtype, shape, device) -> torch.Tensor:
 
 def _want_words(name: str, X, lwe_len, device, shape):
     """Ciphertext rows [*, *, ld], contiguous, their pitch and the words used of each."""
-    if X.dtype is not torch.int64 and X.dtype is not torch.uint64:
-        raise TypeError(f"expected a 64-bit tensor, got {X.dtype}")
-    if X.dim() != 3 or not X.is_cuda:
+    dtype, got = X.dtype, X.shape
+    if dtype is not torch.int64 and dtype is not torch.uint64:
+        raise TypeError(f"expected a 64-bit tensor, got {dtype}")
+    if len(got) != 3 or not X.is_cuda:
         raise ValueError(f"{name} must be a 3-dimensional CUDA tensor of ciphertext rows, got "
-                         f"{tuple(X.shape)} on {X.device}")
-    ld = X.shape[2]
+                         f"{tuple(got)} on {X.device}")
+    n, features, ld = got
     lwe_len = ld if lwe_len is None else lwe_len
     if not 1 <= lwe_len <= ld:
         raise ValueError(f"lwe_len {lwe_len} does not fit rows of {ld} words")
-    return _want(name, X, X.dtype, shape + (ld,), device), ld, lwe_len
+    if features == shape[1] and (shape[0] is None or shape[0] == n) and X.device == device:
+        return X if X.is_contiguous() else X.contiguous(), ld, lwe_len
+    return _want(name, X, dtype, shape + (ld,), device), ld, lwe_len
 
 
 def _want_out(out, shape, device, lwe_len: int, X: torch.Tensor) -> torch.Tensor:
@@ -881,12 +884,13 @@ def cache_write(cache: CiphertextCache, X: torch.Tensor, slots: torch.Tensor) ->
     """Token t's ciphertexts ``X`` [tokens, features, ld] into slot ``slots[t]`` (int32 [tokens]),
     rounded.  A slot outside the cache is skipped; of two tokens that name the same slot the later
     one stays."""
-    X, ld, L = _want_words("X", X, cache.lwe_len, cache.device, (None, cache.features))
+    device = cache.device
+    X, ld, L = _want_words("X", X, cache.lwe_len, device, (None, cache.features))
     n = X.shape[0]
     slots = cache._slots(slots, n)
     _apart("the cache", cache.data, X)
-    _launch("pnb_cache_write", cache.device, slots.data_ptr(), n, X.data_ptr(), cache.features, ld,
-            L, cache.data.data_ptr(), cache.slots, cache.bits)
+    _launch("pnb_cache_write", device, slots.data_ptr(), n, X.data_ptr(), cache.features, ld, L,
+            cache.data.data_ptr(), cache.slots, cache.bits)
     return cache
 
 
@@ -931,6 +935,7 @@ class GroupWeights:
         self.q = _want("q", q, torch.uint8, (M, (K + 1) // 2), q.device)
         self.scales = _want("scales", scales, torch.int8, shape, q.device)
         self.zeros = None if zeros is None else _want("zeros", zeros, torch.uint8, shape, q.device)
+        self._bytes = (_group_bytes(K, M), _group_bytes(M, K))  # workspaces, forward and transposed
 
 
 def group_contract(W: GroupWeights, bias: torch.Tensor | None, delta: int, X: torch.Tensor,
@@ -940,6 +945,7 @@ def group_contract(W: GroupWeights, bias: torch.Tensor | None, delta: int, X: to
     [batch, K, ld] -> [batch, M, ld].  ``transposed``: ``Y[b, i] = sum_j w[j, i] X[b, j]``, the
     gradient with respect to the inputs, [batch, M, ld] -> [batch, K, ld] without a bias."""
     device = W.device
+    transposed = bool(transposed)
     n_in, n_out = (W.M, W.K) if transposed else (W.K, W.M)
     X, ld, L = _want_words("X", X, lwe_len, device, (None, n_in))
     batch = X.shape[0]
@@ -947,8 +953,8 @@ def group_contract(W: GroupWeights, bias: torch.Tensor | None, delta: int, X: to
         raise ValueError("a transposed product takes no bias")
     b = None if bias is None else _want("bias", bias, torch.int64, (W.M,), device)
     out = _want_out(out, (batch, n_out, ld), device, L, X)
-    need = _group_bytes(n_in, n_out)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    need = W._bytes[transposed]
+    ws = W.q.new_empty(need) if need else None
     _launch("pnb_group_contract", device, W.q.data_ptr(), W.scales.data_ptr(), _at(W.zeros),
             W.group, _at(b), delta % (1 << 64), W.M, W.K, 1 if transposed else 0, X.data_ptr(), ld,
             out.data_ptr(), ld, batch, L, _at(ws), need)
@@ -972,8 +978,8 @@ def group_contract_cached(W: GroupWeights, bias: torch.Tensor | None, delta: int
     batch, ld = slots.shape[0], _pitch(cache, ld, out)
     b = None if bias is None else _want("bias", bias, torch.int64, (W.M,), device)
     out = _want_out(out, (batch, W.M, ld), device, cache.lwe_len, cache.data)
-    need = _group_bytes(W.K, W.M)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    need = W._bytes[0]
+    ws = W.q.new_empty(need) if need else None
     _launch("pnb_group_contract_cached", device, W.q.data_ptr(), W.scales.data_ptr(), _at(W.zeros),
             W.group, _at(b), delta % (1 << 64), W.M, W.K, slots.data_ptr(), cache.data.data_ptr(),
             cache.slots, cache.bits, out.data_ptr(), ld, batch, cache.lwe_len, _at(ws), need)

@@ -18,10 +18,13 @@
 
 namespace pnb {
 
-constexpr int CH_THREADS = 256;
-constexpr int CH_AHEAD = 8;   // words of a thread on their way together
-constexpr int CH_RUN = CH_THREADS * CH_AHEAD;
-constexpr int CH_TOKENS = 8;  // most tokens of a block
+constexpr int CH_WARPS = 8, CH_BLOCKS = 5;
+constexpr int CH_AHEAD = 4;    // pairs of words of a thread on their way together
+constexpr int CH_PIECE = 512;  // words of a row that a warp takes at a time
+// Most pieces of a block.  Writing, a block looks for later tokens of its slot first, which more pieces
+// share (512 x 128 ciphertexts in 24 bits: 259 us with 8, 249 with 32, 265 with 128); reading, fewer are
+// better (from 32 bits: 251, 264, 281).
+constexpr int CH_PIECES_WRITE = 32, CH_PIECES_READ = 8;
 
 struct CacheArgs {
   const int32_t* slots;  // [tokens]
@@ -29,105 +32,136 @@ struct CacheArgs {
   uint64_t* out;         // read: the tokens' rows
   unsigned char* cache;
   int tokens, n_slots, features, L, ld;
-  int per_block;         // tokens
+  int row_pieces, block_pieces;
   size_t row_bytes;
-  int per_row;           // words of a row, rounded up to 4
-  uint32_t magic;        // u / per_row = umulhi(u, magic) >> shift for u < 2^21
-  int shift;
 };
 
-// A block takes the same run of words of a few tokens.  One word per thread and step, so that a warp's
-// 64-bit words are 256 consecutive bytes at any pitch.
-// Words of three bytes go through registers of four: lane k < 3 of every four holds bytes 4k .. 4k+3 of
-// their twelve, which is its own word without its first k bytes and the next lane's first k + 1.
+// A block takes some pieces of one token's rows, a warp one at a time: a piece lies in one row, so nothing
+// of its addresses but a constant step changes on the way (with runs that go on from row to row, whose
+// lanes each find their own row, the instructions bound these kernels).  Lanes take neighbouring pairs of
+// words, 16 aligned bytes at a time: where the row starts off by one word, the words before and of an even
+// column, and the lane before or behind has the other half of a pair.
+//
+// Words of three bytes go in groups of eight: lane k of the group's four has b_k, its pair's six bytes, and
+// for k < 3 moves eight of the 24 bytes, s_k = b_k >> 16k | b_(k+1) << (48 - 16k).
 template <int BYTES, bool WRITE>
-__global__ void __launch_bounds__(CH_THREADS, 4) cache_kernel(const __grid_constant__ CacheArgs a) {
-  constexpr int BITS = 8 * BYTES;
-  __shared__ int slot_s[CH_TOKENS];  // of the block's tokens, -1 for those to leave out
-  const long long units = (long long)a.features * a.per_row;
-  const long long first = (long long)blockIdx.x * CH_RUN;
-  const long long f0 = first / a.per_row;
-  const int u0 = (int)(first - f0 * a.per_row) + (int)threadIdx.x;
-  const int left = (int)min((long long)CH_RUN, units - first) - (int)threadIdx.x;
-  const int sub = threadIdx.x & 3;
-  size_t word[CH_AHEAD], cell[CH_AHEAD];  // where it is among a token's words, and among its bytes
-  bool live[CH_AHEAD];
-#pragma unroll
-  for (int j = 0; j < CH_AHEAD; ++j) {
-    const int u = u0 + j * CH_THREADS;
-    const int f = (int)(__umulhi((uint32_t)u, a.magic) >> a.shift);
-    const int col = u - f * a.per_row;
-    live[j] = j * CH_THREADS < left && col < a.L;
-    word[j] = (size_t)(f0 + f) * a.ld + col;
-    cell[j] = (size_t)(f0 + f) * a.row_bytes;
-    // of four words of three bytes the first three lanes move four bytes each, up to the last word's
-    if (BYTES != 3)
-      cell[j] += (size_t)col * BYTES;
-    else if (sub < 3 && j * CH_THREADS < left && 4 * (col / 4 * 3 + sub) < 3 * a.L)
-      cell[j] += 4 * (size_t)(col / 4 * 3 + sub);
-    else
-      cell[j] = ~(size_t)0;
-  }
-  for (int t0 = blockIdx.y * a.per_block; t0 < a.tokens; t0 += gridDim.y * a.per_block) {
-    const int n = min(a.per_block, a.tokens - t0);
-    __syncthreads();
-    if ((int)threadIdx.x < n) {
-      const int s = __ldg(a.slots + t0 + threadIdx.x);
-      slot_s[threadIdx.x] = s >= 0 && s < a.n_slots ? s : -1;
-    }
-    __syncthreads();
+__global__ void __launch_bounds__(32 * CH_WARPS, CH_BLOCKS)
+    cache_kernel(const __grid_constant__ CacheArgs a) {
+  using word = unsigned long long;
+  constexpr int STEP = 64;  // words of a warp's turn
+  constexpr int UP = 32 - 8 * BYTES;
+  constexpr uint32_t HALF = BYTES == 4 ? 0u : 1u << (31 - 8 * BYTES);  // in the high half of a word
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 3;
+  const long long pieces = (long long)a.features * a.row_pieces;
+  const long long first = (long long)blockIdx.x * a.block_pieces;
+  const int n = (int)min((long long)a.block_pieces, pieces - first);
+  for (int t = blockIdx.y; t < a.tokens; t += gridDim.y) {
+    const int slot = __ldg(a.slots + t);
     if (WRITE) {  // of two tokens that name the same slot the later one stays
-      unsigned again = 0;
-      for (int i = t0 + 1 + (int)threadIdx.x; i < a.tokens; i += CH_THREADS) {
-        const int s = __ldg(a.slots + i);
-        for (int k = 0; k < n; ++k) again |= t0 + k < i && slot_s[k] == s ? 1u << k : 0u;
-      }
-      __syncthreads();
-      for (int k = 0; k < n; ++k)
-        if (again >> k & 1u) slot_s[k] = -1;
-      __syncthreads();
+      bool skip = slot < 0 || slot >= a.n_slots;
+      for (int i = t + 1 + (int)threadIdx.x; i < a.tokens; i += 32 * CH_WARPS)
+        skip |= __ldg(a.slots + i) == slot;
+      if (__syncthreads_or(skip)) continue;
+    } else if (slot < 0 || slot >= a.n_slots) {
+      continue;
     }
-    for (int k = 0; k < n; ++k) {
-      const int slot = slot_s[k];
-      if (slot < 0) continue;
-      unsigned char* cells = a.cache + (size_t)slot * a.features * a.row_bytes;
-      const size_t x0 = (size_t)(t0 + k) * a.features * a.ld;
-      if (WRITE) {
-        uint64_t x[CH_AHEAD];
+#pragma unroll 1
+    for (int p = warp; p < n; p += CH_WARPS) {
+      const long long f = (first + p) / a.row_pieces;
+      const int c0 = (int)(first + p - f * a.row_pieces) * CH_PIECE, c1 = min(a.L, c0 + CH_PIECE);
+      word* row = reinterpret_cast<word*>(WRITE ? const_cast<uint64_t*>(a.in) : a.out) +
+                  ((size_t)t * a.features + f) * a.ld;
+      unsigned char* cell = a.cache + ((size_t)slot * a.features + f) * a.row_bytes;
+      const bool off = (uintptr_t)row & 8;  // (the same in all lanes)
+      // the bytes of column c's pair, or of the eight that this lane moves of its group
+      auto at = [&](int c) { return cell + (BYTES == 3 ? c / 8 * 24 + 8 * sub : c * BYTES); };
+      auto moves = [&](int c) { return BYTES == 3 ? sub < 3 && c / 8 * 24 + 8 * sub < 3 * c1 : c < c1; };
+      for (int c = c0 + 2 * lane; c - 2 * lane < c1; c += CH_AHEAD * STEP) {
+        if (WRITE) {
+          ulonglong2 x[CH_AHEAD];
 #pragma unroll
-        for (int j = 0; j < CH_AHEAD; ++j) x[j] = live[j] ? __ldcs(reinterpret_cast<const unsigned long long*>(a.in + x0 + word[j])) : 0;
-#pragma unroll
-        for (int j = 0; j < CH_AHEAD; ++j) {
-          const uint32_t q = (uint32_t)((x[j] + (1ull << (63 - BITS))) >> (64 - BITS));
-          if (BYTES == 4) {
-            if (live[j]) *reinterpret_cast<uint32_t*>(cells + cell[j]) = q;
-          } else if (BYTES == 2) {
-            if (live[j]) *reinterpret_cast<uint16_t*>(cells + cell[j]) = (uint16_t)q;
-          } else {
-            const uint32_t next = __shfl_down_sync(0xffffffffu, q, 1);
-            if (cell[j] != ~(size_t)0)
-              *reinterpret_cast<uint32_t*>(cells + cell[j]) = q >> (8 * sub) | next << (24 - 8 * sub);
+          for (int j = 0; j < CH_AHEAD; ++j) {
+            const int cj = c + j * STEP;
+            x[j] = make_ulonglong2(0, 0);
+            if (off) {
+              if (cj < c1) x[j] = __ldcs(reinterpret_cast<const ulonglong2*>(row + cj - 1));
+            } else if (cj + 1 < c1) {
+              x[j] = __ldcs(reinterpret_cast<const ulonglong2*>(row + cj));
+            } else if (cj < c1) {
+              x[j].x = __ldcs(row + cj);
+            }
           }
-        }
-      } else {
-        uint32_t q[CH_AHEAD];
+          if (off) {
+            word more[CH_AHEAD];  // where the lane behind has not got it
 #pragma unroll
-        for (int j = 0; j < CH_AHEAD; ++j) {
-          if (BYTES == 3)
-            q[j] = cell[j] != ~(size_t)0 ? __ldcs(reinterpret_cast<const uint32_t*>(cells + cell[j])) : 0;
-          else if (BYTES == 4)
-            q[j] = live[j] ? __ldcs(reinterpret_cast<const uint32_t*>(cells + cell[j])) : 0;
-          else
-            q[j] = live[j] ? __ldcs(reinterpret_cast<const uint16_t*>(cells + cell[j])) : 0;
-        }
+            for (int j = 0; j < CH_AHEAD; ++j) {
+              const int cj = c + j * STEP;
+              more[j] = (lane == 31 || cj + 2 >= c1) && cj + 1 < c1 ? __ldcs(row + cj + 1) : 0;
+            }
 #pragma unroll
-        for (int j = 0; j < CH_AHEAD; ++j) {
-          if (BYTES == 3) {  // word k: the last k bytes of the lane before, then its own first 3 - k
-            const uint32_t before = __shfl_up_sync(0xffffffffu, q[j], 1);
-            q[j] = sub == 0 ? q[j] : before >> (32 - 8 * sub) | q[j] << (8 * sub);
+            for (int j = 0; j < CH_AHEAD; ++j) {
+              const word behind = __shfl_down_sync(0xffffffffu, x[j].x, 1);
+              x[j] = make_ulonglong2(
+                  x[j].y, lane == 31 || c + j * STEP + 2 >= c1 ? more[j] : behind);
+            }
           }
-          if (live[j]) __stcs(reinterpret_cast<unsigned long long*>(a.out + x0 + word[j]),
-                               (unsigned long long)q[j] << (64 - BITS));
+#pragma unroll
+          for (int j = 0; j < CH_AHEAD; ++j) {
+            const int cj = c + j * STEP;
+            auto rounded = [](word v) {
+              const uint32_t hi = (uint32_t)(v >> 32);
+              return BYTES == 4 ? hi + ((uint32_t)v >> 31) : (hi + HALF) >> UP;
+            };
+            const uint32_t q0 = rounded(x[j].x), q1 = rounded(x[j].y);
+            if constexpr (BYTES == 3) {
+              const word b = q0 | (word)q1 << 24;
+              const word next = __shfl_down_sync(0xffffffffu, b, 1);
+              if (moves(cj))
+                *reinterpret_cast<word*>(at(cj)) = b >> (16 * sub) | next << (48 - 16 * sub);
+            } else if (moves(cj)) {  // (a second word behind the last goes to the row's padding)
+              if constexpr (BYTES == 4)
+                *reinterpret_cast<uint2*>(at(cj)) = make_uint2(q0, q1);
+              else
+                *reinterpret_cast<uint32_t*>(at(cj)) = q0 | q1 << 16;
+            }
+          }
+        } else {
+          word v[CH_AHEAD];
+#pragma unroll
+          for (int j = 0; j < CH_AHEAD; ++j) {
+            v[j] = 0;
+            if (moves(c + j * STEP)) {
+              if constexpr (BYTES == 2)
+                v[j] = __ldcs(reinterpret_cast<const uint32_t*>(at(c + j * STEP)));
+              else
+                v[j] = __ldcs(reinterpret_cast<const word*>(at(c + j * STEP)));
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < CH_AHEAD; ++j) {
+            const int cj = c + j * STEP;
+            if constexpr (BYTES == 3) {
+              const word before = __shfl_up_sync(0xffffffffu, v[j], 1);
+              if (sub) v[j] = before >> (64 - 16 * sub) | v[j] << (16 * sub);
+            }
+            const uint32_t h0 = (uint32_t)v[j] << UP, h1 = (uint32_t)(v[j] >> (8 * BYTES)) << UP;
+            const word y0 = (word)h0 << 32, y1 = (word)h1 << 32;
+            if (off) {
+              const uint32_t before = __shfl_up_sync(0xffffffffu, h1, 1);
+              if (cj < c1) {
+                if (lane)
+                  __stcs(reinterpret_cast<ulonglong2*>(row + cj - 1),
+                         make_ulonglong2((word)before << 32, y0));
+                else
+                  __stcs(row + cj, y0);
+                if ((lane == 31 || cj + 2 >= c1) && cj + 1 < c1) __stcs(row + cj + 1, y1);
+              }
+            } else if (cj + 1 < c1) {
+              __stcs(reinterpret_cast<ulonglong2*>(row + cj), make_ulonglong2(y0, y1));
+            } else if (cj < c1) {
+              __stcs(row + cj, y0);
+            }
+          }
         }
       }
     }
@@ -139,28 +173,25 @@ size_t cache_row_bytes(int L, int bits) { return ((size_t)L * (bits / 8) + 15) /
 template <bool WRITE>
 static int cache_launch(CacheArgs a, int bits, cudaStream_t st) {
   a.row_bytes = cache_row_bytes(a.L, bits);
-  a.per_row = (a.L + 3) & ~3;
-  // ceil(2^(32 + shift) / per_row) with 2^shift >= per_row / 2: exact for u < 2^21 (at most
-  // PNB_MAX_REQUEST_WORDS into a row, and a run)
-  a.shift = 0;
-  while ((2 << a.shift) < a.per_row) ++a.shift;
-  a.magic = (uint32_t)((((uint64_t)1 << (32 + a.shift)) + a.per_row - 1) / a.per_row);
-  const long long runs = ((long long)a.features * a.per_row + CH_RUN - 1) / CH_RUN;
-  if (runs > 0x7fffffffLL) {
+  a.row_pieces = (a.L + CH_PIECE - 1) / CH_PIECE;
+  const long long pieces = (long long)a.features * a.row_pieces;
+  // more pieces to a block where that leaves every multiprocessor its blocks
+  const long long most = WRITE ? CH_PIECES_WRITE : CH_PIECES_READ;
+  a.block_pieces = (int)std::max<long long>(
+      CH_WARPS, std::min(most, pieces * a.tokens / (2 * CH_BLOCKS * 148)));
+  const long long blocks = (pieces + a.block_pieces - 1) / a.block_pieces;
+  if (blocks > 0x7fffffffLL) {
     set_error("%s: tokens of %d ciphertexts of %d words exceed one launch",
               WRITE ? "cache_write" : "cache_read", a.features, a.L);
     return PNB_ERR_INVALID;
   }
-  // several tokens to a block where that leaves every multiprocessor its blocks
-  a.per_block = (int)std::max<long long>(1, std::min<long long>(CH_TOKENS, runs * a.tokens / 1184));
-  const dim3 grid((unsigned)runs,
-                  (unsigned)std::min(65535, (a.tokens + a.per_block - 1) / a.per_block));
+  const dim3 grid((unsigned)blocks, (unsigned)std::min(65535, a.tokens));
   if (bits == 16)
-    cache_kernel<2, WRITE><<<grid, CH_THREADS, 0, st>>>(a);
+    cache_kernel<2, WRITE><<<grid, 32 * CH_WARPS, 0, st>>>(a);
   else if (bits == 24)
-    cache_kernel<3, WRITE><<<grid, CH_THREADS, 0, st>>>(a);
+    cache_kernel<3, WRITE><<<grid, 32 * CH_WARPS, 0, st>>>(a);
   else
-    cache_kernel<4, WRITE><<<grid, CH_THREADS, 0, st>>>(a);
+    cache_kernel<4, WRITE><<<grid, 32 * CH_WARPS, 0, st>>>(a);
   PNB_CHECK_LAUNCH("cache_kernel");
   return PNB_OK;
 }
