@@ -256,7 +256,7 @@ struct GcShape {
 
 struct GcMaps {
   CUtensorMap W, Y;
-  CUtensorMap X[2];  // shifted: rows 0, 2, .. and 1, 3, ..; else X[0]
+  CUtensorMap X[2];  // boxes of one slot's and of one MMA's rows; shifted: rows 0, 2, .. and 1, 3, ..
 };
 
 struct GcArgs {
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     tc::fence_mbar_init();
     if (!a.in_place) tc::prefetch_tmap(&tm.W);
     tc::prefetch_tmap(&tm.X[0]);
-    if (SHIFTED) tc::prefetch_tmap(&tm.X[1]);
+    tc::prefetch_tmap(&tm.X[1]);
     if (!a.plain_out) tc::prefetch_tmap(&tm.Y);
   }
   if (warp == S::MMA_WARP) {
@@ -469,16 +469,21 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
             tc::tma_load_2d(raw_at(s) + S::RAW_SLOT / 2, &tm.X[(row + 1) & 1], word, (row + 1) >> 1,
                             full);
           } else {
-            // rows past the last input, and requests without a place, read as zeros
-            if (rank == 0) tc::mbar_expect_tx(full, (1 + TWO) * GC_X_SLOT);
+            // The last slot gets whole MMAs' rows only: a load takes its time also for rows past the last
+            // input, which read as zeros (as do requests without a place).
+            const int rows = min(S::XK, (a.g.n_in - k + GC_KSTEP - 1) / GC_KSTEP * GC_KSTEP);
+            const int box = rows == S::XK ? S::XK : GC_KSTEP;
+            const CUtensorMap* map = rows == S::XK ? &tm.X[0] : &tm.X[1];
+            if (rank == 0) tc::mbar_expect_tx(full, (uint32_t)((1 + TWO) * rows * S::LOAD));
+            for (int r = 0; r < rows; r += box)
 #pragma unroll
-            for (int b = 0; b < S::BOXES; ++b) {
-              if (TWO)
-                tc::tma_load_3d_pair(x_at(s), &tm.X[0], word * BYTES, k, walk.src, leads(full));
-              else
-                tc::tma_load_3d(x_at(s) + b * (S::XK * 128), &tm.X[0], word * BYTES + b * 128, k,
-                                walk.src, full);
-            }
+              for (int b = 0; b < S::BOXES; ++b) {
+                const uint32_t to = x_at(s) + (uint32_t)((b * S::XK + r) * 128);
+                if (TWO)
+                  tc::tma_load_3d_pair(to, map, word * BYTES, k + r, walk.src, leads(full));
+                else
+                  tc::tma_load_3d(to, map, word * BYTES + b * 128, k + r, walk.src, full);
+              }
           }
           ring.advance(slots);
           wrapped |= ring.slot == 0;
@@ -568,7 +573,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
         if (!ok) break;
         if (lane == 0) {
           if (TWO)
-            tc::mbar_arrive_cluster(leads(x_full + 8 * xr.slot));
+            tc::mbar_arrive_cluster_relaxed(leads(x_full + 8 * xr.slot));
           else
             tc::mbar_arrive(x_full + 8 * xr.slot);
         }
@@ -862,9 +867,11 @@ static int gc_launch(GcArgs& a, int8_t* ws, cudaStream_t st) {
     const cuuint64_t dims[3] = {(cuuint64_t)g.L * BYTES, (cuuint64_t)g.n_in,
                                 (cuuint64_t)(g.slots ? g.n_slots : g.batch)};
     const cuuint64_t strides[2] = {g.x_row, g.x_row * g.n_in};
-    const cuuint32_t box[3] = {128, (cuuint32_t)S::XK, 1};
-    rc = tile_map(&tm.X[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, g.X, 3, dims, strides, box,
-                  CU_TENSOR_MAP_SWIZZLE_128B);
+    for (int i = 0; i < 2 && !rc; ++i) {
+      const cuuint32_t box[3] = {128, (cuuint32_t)(i ? GC_KSTEP : S::XK), 1};
+      rc = tile_map(&tm.X[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, g.X, 3, dims, strides, box,
+                    CU_TENSOR_MAP_SWIZZLE_128B);
+    }
   } else {
     // rows p, p + 2, ..: from the 16-byte boundary at or before row p, at twice the pitch.  A row
     // off by one word has that word's 16 bytes inside its allocation (allocations start aligned).
