@@ -107,7 +107,11 @@ struct GroupArgs {
 // One thread per word, 16 outputs at a time, weights in shared memory as w + 2048 >= 0, so that a product
 // is one 32 x 32 + 64 and one 32 x 32 + 32 bit multiply-add and sum w x = sum (w + 2048) x - 2048 sum x.
 constexpr int GF_THREADS = 256, GF_OUT = 16, GF_IN = 64;
-constexpr long long GF_MOST = 256;  // weights that go this way
+constexpr long long GF_MOST = 384;  // weights, outputs padded to 16, that go this way
+
+static bool gf_few(int n_in, int n_out) {
+  return (long long)n_in * ((n_out + GF_OUT - 1) / GF_OUT * GF_OUT) <= GF_MOST;
+}
 
 // A word of X, of 8 bytes or the top 2, 3 or 4 of them.
 template <int BYTES>
@@ -950,7 +954,8 @@ static int gc_run(GcArgs& a, int8_t* ws, cudaStream_t st) {
   switch (gc_mode(a.g.n_in, a.g.n_out)) {
     case LONG: return gc_launch<BYTES, SHIFTED, LONG>(a, ws, st);
     case SHORT: return gc_launch<BYTES, SHIFTED, SHORT>(a, ws, st);
-    default: return gc_launch<BYTES, SHIFTED, PAIR>(a, ws, st);
+    // (copying shifted rows costs a pair more than it saves: 64 x 784->128 301 us, LONG 238)
+    default: return gc_launch<BYTES, SHIFTED, SHIFTED ? LONG : PAIR>(a, ws, st);
   }
 }
 
@@ -970,7 +975,7 @@ static int gc_run(const GroupArgs& g, int bits, int8_t* ws, cudaStream_t st) {
 }
 
 size_t group_workspace_bytes(int n_in, int n_out) {
-  if ((long long)n_in * n_out <= GF_MOST || gc_in_place(n_in, n_out)) return 0;
+  if (gf_few(n_in, n_out) || gc_in_place(n_in, n_out)) return 0;
   return (size_t)2 * n_out * (((size_t)n_in + 15) & ~(size_t)15);
 }
 
@@ -996,7 +1001,7 @@ static int group_run(const GroupArgs& a, int bits, void* ws, size_t ws_bytes, cu
               a.slots ? "group_contract_cached" : "group_contract", ws_bytes, ws, need);
     return PNB_ERR_INVALID;
   }
-  if ((long long)a.n_in * a.n_out <= GF_MOST) return few_run(a, bits, st);
+  if (gf_few(a.n_in, a.n_out)) return few_run(a, bits, st);
   int8_t* own = nullptr;
   if (need && !ws) PNB_CUDA(cudaMallocAsync((void**)&own, need, st));
   int rc = gc_run(a, bits, own ? own : (int8_t*)ws, st);
