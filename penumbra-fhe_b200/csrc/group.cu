@@ -267,38 +267,41 @@ struct GcArgs {
   GroupArgs g;
   int off0, off1;    // words by which rows 0, 2, .. / 1, 3, .. start past 16-byte alignment
   int n_tiles, m_tiles;         // tiles: outputs fastest, then words, then requests
-  int step_m, step_n, step_b;   // one grid of them
   int w_slots, x_slots, raw_slots;
   int x_at, raw_at, out_at, bars_at;  // shared-memory offsets; weights at 0
   int plain_out;     // results leave by plain stores
   int in_place;      // SHORT: the weights are expanded by every block for itself
 };
 
-// The tiles of a block (or pair), one grid apart.  The next one's slot is on its way while one is
-// worked on.
+// Every stride-th tile from `first` on.  The next one's slot is on its way while one is worked on.
 template <bool CACHED>
 struct GcWalk {
   const GcArgs& a;
   int b, nt, m, src, next_b, next_n, next_m, slot = 0;
-  __device__ __forceinline__ GcWalk(const GcArgs& args, unsigned first) : a(args) {
-    const unsigned u = first / (unsigned)a.m_tiles;
-    next_m = (int)(first - u * a.m_tiles);
-    next_b = (int)(u / (unsigned)a.n_tiles);
-    next_n = (int)(u - (unsigned)next_b * a.n_tiles);
+  int step_m, step_n, step_b;
+  __device__ __forceinline__ GcWalk(const GcArgs& args, unsigned first, unsigned stride) : a(args) {
+    split(first, next_m, next_n, next_b);
+    split(stride, step_m, step_n, step_b);
     if (CACHED && next_b < a.g.batch) slot = __ldg(a.g.slots + next_b);
+  }
+  __device__ __forceinline__ void split(unsigned t, int& m_of, int& n_of, int& b_of) const {
+    const unsigned u = t / (unsigned)a.m_tiles;
+    m_of = (int)(t - u * a.m_tiles);
+    b_of = (int)(u / (unsigned)a.n_tiles);
+    n_of = (int)(u - (unsigned)b_of * a.n_tiles);
   }
   // src: the place of the request's ciphertexts, or the number of slots where it has none
   __device__ __forceinline__ bool next() {
     if (next_b >= a.g.batch) return false;
     b = next_b, nt = next_n, m = next_m;
     src = !CACHED ? b : slot >= 0 && slot < a.g.n_slots ? slot : a.g.n_slots;
-    next_m += a.step_m;
+    next_m += step_m;
     const int carry_m = next_m >= a.m_tiles;
     next_m -= carry_m ? a.m_tiles : 0;
-    next_n += a.step_n + carry_m;
+    next_n += step_n + carry_m;
     const int carry_n = next_n >= a.n_tiles;
     next_n -= carry_n ? a.n_tiles : 0;
-    next_b += a.step_b + carry_n;
+    next_b += step_b + carry_n;
     if (CACHED && next_b < a.g.batch) slot = __ldg(a.g.slots + next_b);
     return true;
   }
@@ -336,10 +339,16 @@ __device__ __forceinline__ void gc_tmem_ld(uint32_t at, uint32_t (&r)[COLS]) {
   }
 }
 
-// sum_p t[p] << 8p: a word mod 2^64, or the high half of one from a cache, whose low half is zero.
-template <int BYTES>
+// sum_p t[p] << 8p: a word mod 2^64, or the high half of one from a cache, whose low half is zero.  NARROW:
+// t[p] + 256 t[p+1] stays below 2^31, so two multiply-adds of 64 bits do for the low four.
+template <int BYTES, bool NARROW = false>
 __device__ __forceinline__ auto gc_limbs(const uint32_t* t) {
-  if constexpr (BYTES == 8) {
+  if constexpr (BYTES == 8 && NARROW) {
+    const int t01 = (int)(t[0] + (t[1] << 8)), t23 = (int)(t[2] + (t[3] << 8));
+    const uint64_t s = (uint64_t)(t01 + (int64_t)t23 * 65536);
+    const uint32_t hi = (uint32_t)(s >> 32) + t[4] + (t[5] << 8) + (t[6] << 16) + (t[7] << 24);
+    return (uint64_t)hi << 32 | (uint32_t)s;
+  } else if constexpr (BYTES == 8) {
     return add_limbs(0, t);
   } else {
     uint32_t v = t[0];
@@ -350,13 +359,14 @@ __device__ __forceinline__ auto gc_limbs(const uint32_t* t) {
 }
 // The word of limb sums by lo and by hi, sum_p (lo[p] + hi[p-1]) << 8p.  Sums of two stay below 2^31 for
 // up to 61922 inputs ((128 + 8) * 255 each).
-template <int BYTES>
+constexpr int GC_NARROW = 240;  // inputs: 257 * (128 + 8) * 255 * 240 < 2^31
+template <int BYTES, bool NARROW>
 __device__ __forceinline__ auto gc_word(const uint32_t* lo, const uint32_t* hi) {
   uint32_t t[BYTES];
   t[0] = lo[0];
 #pragma unroll
   for (int p = 1; p < BYTES; ++p) t[p] = lo[p] + hi[p - 1];
-  return gc_limbs<BYTES>(t);
+  return gc_limbs<BYTES, NARROW>(t);
 }
 __device__ __forceinline__ uint64_t gc_whole(uint64_t v) { return v; }
 __device__ __forceinline__ uint64_t gc_whole(uint32_t v) { return (uint64_t)v << 32; }
@@ -458,7 +468,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
       TileRing ring;
       bool wrapped = false, ok = true;
       const int slots = SHIFTED ? a.raw_slots : a.x_slots;
-      GcWalk<CACHED> walk(a, first);
+      GcWalk<CACHED> walk(a, first, grid);
       while (ok && walk.next()) {
         const int word = walk.nt * S::TILE + rank * S::WORDS;
         for (int k = 0; k < a.g.n_in; k += SHIFTED ? S::RAW_ROWS : S::XK) {
@@ -502,7 +512,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
       asm volatile("griddepcontrol.wait;" ::: "memory");  // the weights' kernel is done
       TileRing ring;
       bool wrapped = false, ok = true;
-      GcWalk<false> walk(a, first);
+      GcWalk<false> walk(a, first, grid);
       while (ok && walk.next()) {
         for (int k = 0; k < kb_n; ++k) {
           const int s = ring.slot;
@@ -536,7 +546,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     const int box = word >> 4, ch = (word & 15) >> 1, half = word & 1;
     TileRing xr, rr;
     bool ok = true;
-    GcWalk<CACHED> walk(a, first);
+    GcWalk<CACHED> walk(a, first, grid);
     while (ok && walk.next()) {
       const int parity = walk.src * a.g.n_in & 1;  // of the tile's first row
       const int off_e = parity ? a.off1 : a.off0, off_o = parity ? a.off0 : a.off1;
@@ -679,21 +689,14 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     constexpr int PITCH = S::PART * 8;
     auto xored = [](int r) { return (r >> 1) & 3; };
     const int row = TWO ? lane >> 1 : lane, odd = TWO ? lane & 1 : 0;
-    unsigned char* out_row = out + row * PITCH;
-    const int out_x = xored(row);
-    int tt = 0;
-    GcWalk<CACHED> walk(a, first);
-    while (walk.next()) {
-      const int buf = STAGES == 1 ? 0 : tt & 1;
-      const uint32_t turn = (uint32_t)(tt / STAGES);
-      ++tt;
-      if (STAGES == 2 && buf != group) continue;
+    // chunk k of this lane's row, as XORed
+    auto chunk = [&](int k) { return out + ((row * PITCH | xored(row) << 4) ^ (k << 4)); };
+    const int buf = STAGES == 1 ? 0 : group;
+    uint32_t turn = 0;
+    GcWalk<CACHED> walk(a, STAGES == 1 ? first : first + group * grid, STAGES * grid);
+    for (; walk.next(); ++turn) {
       const int row0 = walk.m * GC_BM + rank * 64 + q * S::ROWS, col0 = walk.nt * S::TILE + share * S::EW;
       const int body = a.g.L - 1 - col0;  // the body among this warp's words
-      const bool live = row0 + row < a.g.n_out;
-      uint64_t bias = 0;
-      if (a.g.bias && body >= 0 && body < S::EW && live)
-        bias = (uint64_t)__ldg(a.g.bias + row0 + row) * a.g.delta;
       if (!gc_wait(acc_full + 8 * buf, turn, abort_s)) break;
       tc::tc_fence_after();
       const uint32_t c_tmem = tmem + (uint32_t)(buf * 256 + share * S::EW * BYTES) +
@@ -734,10 +737,14 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
               const auto v1 = gc_limbs<BYTES>(at(u0 + u + 1)) << (8 * odd);
               y[u] = gc_whole((odd ? v1 : v0) + gc_other_lane(odd ? v0 : v1));
             }
+          } else if (BYTES == 8 && MODE == SHORT && a.g.n_in <= GC_NARROW) {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+              y[u] = gc_whole(gc_word<BYTES, true>(c0 + (u0 + u) * BYTES, c1 + (u0 + u) * BYTES));
           } else {
 #pragma unroll
             for (int u = 0; u < N; ++u)
-              y[u] = gc_whole(gc_word<BYTES>(c0 + (u0 + u) * BYTES, c1 + (u0 + u) * BYTES));
+              y[u] = gc_whole(gc_word<BYTES, false>(c0 + (u0 + u) * BYTES, c1 + (u0 + u) * BYTES));
           }
           if (first_w == part && !a.plain_out) {  // what was staged before has left
             if (lane == 0) tc::tma_store_wait_read();
@@ -745,19 +752,19 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
           }
 #pragma unroll
           for (int u = 0; u < N; u += 2) {
-            unsigned char* to = out_row + ((((first_w - part + u) >> 1) ^ out_x) << 4);
+            unsigned char* to = chunk((first_w - part + u) >> 1);
             if constexpr (TWO)
               *reinterpret_cast<uint64_t*>(to + 8 * odd) = y[u];
             else
               *reinterpret_cast<ulonglong2*>(to) = make_ulonglong2(y[u], y[u + 1]);
           }
           if (first_w + N != part + S::PART) continue;
-          if (body >= part && body < part + S::PART && (!TWO || ((body - part) & 1) == odd)) {
-            uint64_t* p = reinterpret_cast<uint64_t*>(
-                out_row + ((((body - part) >> 1) ^ out_x) << 4) + ((body - part) & 1) * 8);
-            *p += bias;
+          if (body >= part && body < part + S::PART && (!TWO || ((body - part) & 1) == odd) &&
+              row0 + row < a.g.n_out) {
+            uint64_t* p = reinterpret_cast<uint64_t*>(chunk((body - part) >> 1) + ((body - part) & 1) * 8);
+            if (a.g.bias) *p += (uint64_t)__ldg(a.g.bias + row0 + row) * a.g.delta;
             // tiled stores end on 16-byte boundaries, so the last word of an odd count goes alone
-            if (!a.plain_out && (a.g.L & 1) && live)
+            if (!a.plain_out && (a.g.L & 1))
               a.g.Y[((size_t)walk.b * a.g.n_out + row0 + row) * a.g.ldy + a.g.L - 1] = *p;
           }
           if (!a.plain_out) {
@@ -823,9 +830,6 @@ static unsigned gc_plan(GcArgs& a, int sms) {
   unsigned grid =
       (unsigned)std::min<long long>((long long)a.g.batch * a.n_tiles * a.m_tiles, sms / per);
   if (MODE != LONG) grid = grid / a.m_tiles * a.m_tiles;  // a block's tiles have the same outputs
-  a.step_m = (int)(grid % a.m_tiles);
-  a.step_n = (int)(grid / a.m_tiles % a.n_tiles);
-  a.step_b = (int)(grid / a.m_tiles / a.n_tiles);
   int room = GC_SMEM - GC_BAR_BYTES - GC_EPI_WARPS * S::STAGE;
   a.w_slots = MODE != LONG ? (a.g.n_in + GC_WK - 1) / GC_WK : SHIFTED ? 2 : 3;
   room -= a.w_slots * S::W_SLOT;

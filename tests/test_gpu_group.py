@@ -230,7 +230,8 @@ def test_cached(pnb, oracle, B, K, M, group, L, ld, bits):
     assert pnb.device_status(0) == 0
 
 
-@pytest.mark.parametrize("K,M", [(784, 128), (100, 200), (61440, 70)])
+@pytest.mark.parametrize("K,M", [(784, 128), (100, 200), (240, 130), (241, 130), (384, 70),
+                                 (61440, 70)])
 @pytest.mark.parametrize("sign", [1, -1])
 def test_extreme_sums(pnb, K, M, sign):
     # every product as large as it can be: 128 * 15 times words of all ones
