@@ -308,22 +308,17 @@ struct GcWalk {
 };
 
 // Bounded wait that also gives up as soon as another role has flagged an abort.
-template <bool CLUSTER>
 __device__ __noinline__ bool gc_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_s) {
   for (uint32_t it = 0; it < GC_WAIT_LIMIT; it += 1024) {
-    if (CLUSTER ? tc::mbar_wait_cluster(bar, parity, 1024) : tc::mbar_wait(bar, parity, 1024))
-      return true;
+    if (tc::mbar_wait(bar, parity, 1024)) return true;
     if (*abort_s) return false;
   }
   *abort_s = 1;
   atomicExch(&g_gc_status, 1);
   return false;
 }
-// CLUSTER: for what the other block's threads have written.
-template <bool CLUSTER = false>
 __device__ __forceinline__ bool gc_wait(uint32_t bar, uint32_t parity, volatile int* abort_s) {
-  return (CLUSTER ? tc::mbar_test_cluster(bar, parity & 1u) : tc::mbar_test(bar, parity & 1u)) ||
-         gc_wait_slow<CLUSTER>(bar, parity & 1u, abort_s);
+  return tc::mbar_test(bar, parity & 1u) || gc_wait_slow(bar, parity & 1u, abort_s);
 }
 
 template <int COLS>
@@ -381,6 +376,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
   using S = GcShape<BYTES, SHIFTED, MODE>;
   constexpr bool CACHED = BYTES != 8;
   constexpr bool TWO = MODE == PAIR;
+  static_assert(!(TWO && SHIFTED), "the copying warps answer their own block's barriers");
   constexpr int STAGES = S::STAGES;
   extern __shared__ __align__(1024) unsigned char gc_raw[];  // the swizzles want 1024-byte boundaries
   const uint32_t base = tc::smem_u32(gc_raw);
@@ -405,7 +401,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
   auto leads = [&](uint32_t bar) { return TWO ? tc::cluster_address(bar, 0) : bar; };
   auto drained = [&](uint32_t bar) {  // the first block's: a warp's loads from tensor memory are done
     if (TWO)
-      tc::mbar_arrive_cluster_relaxed(leads(bar));
+      tc::mbar_arrive_cluster(leads(bar));
     else
       tc::mbar_arrive(bar);
   };
@@ -422,7 +418,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
       tc::mbar_init(w_empty + 8 * s, S::ISSUERS);
     }
     for (int s = 0; s < a.x_slots; ++s) {
-      tc::mbar_init(x_full + 8 * s, SHIFTED ? (1 + TWO) * S::COPY : 1);
+      tc::mbar_init(x_full + 8 * s, SHIFTED ? S::COPY : 1);
       tc::mbar_init(x_empty + 8 * s, S::ISSUERS);
     }
     for (int s = 0; s < a.raw_slots; ++s) {
@@ -503,8 +499,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
           wrapped |= ring.slot == 0;
         }
       }
-      if (SHIFTED || rank == 0)
-        tile_drain(SHIFTED ? r_full : x_full, ring, wrapped, slots, GC_WAIT_LIMIT);
+      if (rank == 0) tile_drain(SHIFTED ? r_full : x_full, ring, wrapped, slots, GC_WAIT_LIMIT);
     }
   } else if (warp == 1) {
     // ---------------- weight loads (one lane) ----------------------------------------------------
@@ -553,7 +548,8 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
       for (int kx = 0; ok && kx < kx_n; ++kx) {
         ok = gc_wait(x_empty + 8 * xr.slot, xr.phase ^ 1u, abort_s);
         if (!ok) break;
-        const int raws = min(2, (a.g.n_in - kx * S::XK + S::RAW_ROWS - 1) / S::RAW_ROWS);
+        const int raws =
+            min(S::XK, a.g.n_in - kx * S::XK + S::RAW_ROWS - 1) / S::RAW_ROWS;
         for (int i = 0; i < raws; ++i) {
           if ((rr.slot & 3) == cw) {
             ok = gc_wait(r_full + 8 * rr.slot, rr.phase, abort_s);
@@ -585,12 +581,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
           rr.advance(a.raw_slots);
         }
         if (!ok) break;
-        if (lane == 0) {
-          if (TWO)
-            tc::mbar_arrive_cluster_relaxed(leads(x_full + 8 * xr.slot));
-          else
-            tc::mbar_arrive(x_full + 8 * xr.slot);
-        }
+        if (lane == 0) tc::mbar_arrive(x_full + 8 * xr.slot);
         xr.advance(a.x_slots);
       }
     }
@@ -626,7 +617,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
 #pragma unroll
           for (int h = 0; h < PER_W; ++h) {
             if (left <= 0) break;
-            ok = gc_wait<TWO && SHIFTED>(x_full + 8 * x.slot, x.phase, abort_s);
+            ok = gc_wait(x_full + 8 * x.slot, x.phase, abort_s);
             if (!ok) break;
             const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (GC_X_SLOT / 16));
             if (one) {
@@ -835,7 +826,6 @@ static unsigned gc_plan(GcArgs& a, int sms) {
   room -= a.w_slots * S::W_SLOT;
   if (SHIFTED) {
     a.x_slots = 3;
-    if (room - 3 * GC_X_SLOT < GC_COPY_WARPS * S::RAW_SLOT) a.x_slots = 2;
     a.raw_slots = std::min(GC_MAX_RAW, (room - a.x_slots * GC_X_SLOT) / S::RAW_SLOT & ~3);
   } else {
     a.x_slots = std::min(GC_MAX_X, room / GC_X_SLOT);
