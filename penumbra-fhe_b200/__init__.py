@@ -987,8 +987,8 @@ def group_contract_cached(W: GroupWeights, bias: torch.Tensor | None, delta: int
 
 
 def _group_bytes(n_in: int, n_out: int) -> int:
-    """``pnb_group_contract_workspace_bytes``: none for few inputs."""
-    if n_in <= 128 and n_out <= 37 * 128 or n_in * ((n_out + 15) & -16) <= 384:
+    """``pnb_group_contract_workspace_bytes``: none for small layers."""
+    if n_in <= 128 and n_out <= 128 or n_in * ((n_out + 15) & -16) <= 384:
         return 0
     return 2 * n_out * ((n_in + 15) & -16)
 

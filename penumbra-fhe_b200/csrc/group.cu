@@ -225,7 +225,8 @@ constexpr int GC_SMEM = 227 * 1024;
 constexpr uint32_t GC_WAIT_LIMIT = 1u << 24;
 
 // LONG: one block, weights stream, one accumulator of 256 columns for lo and one for hi.
-// SHORT: one block, weights stay, two accumulators of 128 columns for each.
+// SHORT: one block, weights of some tiles of outputs stay, which take turns at a tile of X; two
+//   accumulators of 128 columns for each.
 // PAIR: two blocks share a tile, weights stay, two accumulators of 256 columns; every second row of the
 //   weights is a hi, in one block those of the first 64 outputs, in the other of the last.
 enum GcMode { LONG, SHORT, PAIR };
@@ -241,6 +242,7 @@ struct GcShape {
   static constexpr int BOXES = LOAD / 128;               // swizzle spans
   static constexpr int XK = GC_X_SLOT / LOAD;            // inputs per X slot
   static constexpr int W_SLOT = (MODE == PAIR ? 1 : 2) * GC_W_HALF;  // 128 rows; 128 of lo, 128 of hi
+  static constexpr int W_TAIL = 2 * 128 * GC_KSTEP;      // a last slot of 32 inputs (SHORT)
   static constexpr int RAW_ROWS = XK / 2;                // inputs per raw slot, half of each parity
   static constexpr int RAW_PITCH = LOAD + 16;            // one word of shift, to 16 bytes
   static constexpr int RAW_SLOT = RAW_ROWS * RAW_PITCH;
@@ -259,14 +261,17 @@ struct GcShape {
 };
 
 struct GcMaps {
-  CUtensorMap W, Y;
+  CUtensorMap W, W_tail, Y;
   CUtensorMap X[2];  // boxes of one slot's and of one MMA's rows; shifted: rows 0, 2, .. and 1, 3, ..
 };
 
 struct GcArgs {
   GroupArgs g;
   int off0, off1;    // words by which rows 0, 2, .. / 1, 3, .. start past 16-byte alignment
-  int n_tiles, m_tiles;         // tiles: outputs fastest, then words, then requests
+  int n_tiles, m_tiles;  // tiles: outputs fastest, then words, then requests
+  int m_group;           // SHORT: tiles of outputs of one block (of the last block's group fewer)
+  int w_tail;            // of the last weight slot 32 inputs are kept, not 128
+  int w_tile;            // bytes of the weights of one tile of outputs
   int w_slots, x_slots, raw_slots;
   int x_at, raw_at, out_at, bars_at;  // shared-memory offsets; weights at 0
   int plain_out;     // results leave by plain stores
@@ -279,14 +284,17 @@ struct GcWalk {
   const GcArgs& a;
   int b, nt, m, src, next_b, next_n, next_m, slot = 0;
   int step_m, step_n, step_b;
-  __device__ __forceinline__ GcWalk(const GcArgs& args, unsigned first, unsigned stride) : a(args) {
+  int m_tiles;
+  // (one_m: tiles of X)
+  __device__ __forceinline__ GcWalk(const GcArgs& args, unsigned first, unsigned stride, bool one_m)
+      : a(args), m_tiles(one_m ? 1 : args.m_tiles) {
     split(first, next_m, next_n, next_b);
     split(stride, step_m, step_n, step_b);
     if (CACHED && next_b < a.g.batch) slot = __ldg(a.g.slots + next_b);
   }
   __device__ __forceinline__ void split(unsigned t, int& m_of, int& n_of, int& b_of) const {
-    const unsigned u = t / (unsigned)a.m_tiles;
-    m_of = (int)(t - u * a.m_tiles);
+    const unsigned u = t / (unsigned)m_tiles;
+    m_of = (int)(t - u * m_tiles);
     b_of = (int)(u / (unsigned)a.n_tiles);
     n_of = (int)(u - (unsigned)b_of * a.n_tiles);
   }
@@ -296,8 +304,8 @@ struct GcWalk {
     b = next_b, nt = next_n, m = next_m;
     src = !CACHED ? b : slot >= 0 && slot < a.g.n_slots ? slot : a.g.n_slots;
     next_m += step_m;
-    const int carry_m = next_m >= a.m_tiles;
-    next_m -= carry_m ? a.m_tiles : 0;
+    const int carry_m = next_m >= m_tiles;
+    next_m -= carry_m ? m_tiles : 0;
     next_n += step_n + carry_m;
     const int carry_n = next_n >= a.n_tiles;
     next_n -= carry_n ? a.n_tiles : 0;
@@ -384,7 +392,8 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     if (threadIdx.x == 0) atomicExch(&g_gc_status, 1);
     return;
   }
-  auto w_at = [&](int s) { return base + (uint32_t)(s * S::W_SLOT); };
+  // slot s of the weights of the m-th tile of outputs that stay, or of the ring
+  auto w_at = [&](int m, int s) { return base + (uint32_t)(m * a.w_tile + s * S::W_SLOT); };
   auto x_at = [&](int s) { return base + (uint32_t)(a.x_at + s * GC_X_SLOT); };
   auto raw_at = [&](int s) { return base + (uint32_t)(a.raw_at + s * S::RAW_SLOT); };
   const uint32_t bars = base + (uint32_t)a.bars_at;
@@ -397,7 +406,18 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // Of a pair the first block issues the MMAs of both; it is told of both blocks' slots.
   const int rank = TWO ? (int)(blockIdx.x & 1u) : 0;
-  const unsigned first = TWO ? blockIdx.x >> 1 : blockIdx.x, grid = TWO ? gridDim.x >> 1 : gridDim.x;
+  unsigned first = TWO ? blockIdx.x >> 1 : blockIdx.x, grid = TWO ? gridDim.x >> 1 : gridDim.x;
+  int m_first = 0, m_n = 1;  // SHORT: the block's tiles of outputs
+  if (MODE == SHORT) {
+    // Of every m_tiles blocks in turn a group of outputs has as many as it has tiles, so that all groups
+    // go through X at the same pace, next to one another.
+    const unsigned round = blockIdx.x / (unsigned)a.m_tiles, r = blockIdx.x - round * a.m_tiles;
+    m_first = (int)r / a.m_group * a.m_group;
+    m_n = min(a.m_group, a.m_tiles - m_first);
+    first = round * m_n + (r - m_first);
+    grid = gridDim.x / (unsigned)a.m_tiles * m_n +
+           (unsigned)max(0, min(m_n, (int)(gridDim.x % (unsigned)a.m_tiles) - m_first));
+  }
   auto leads = [&](uint32_t bar) { return TWO ? tc::cluster_address(bar, 0) : bar; };
   auto drained = [&](uint32_t bar) {  // the first block's: a warp's loads from tensor memory are done
     if (TWO)
@@ -452,7 +472,8 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
 
   const int kx_n = (a.g.n_in + S::XK - 1) / S::XK;  // X slots of one tile
   const int kb_n = (a.g.n_in + GC_WK - 1) / GC_WK;  // weight slots
-  const long long tiles = ((long long)a.g.batch * a.n_tiles * a.m_tiles - first + grid - 1) / grid;
+  const long long x_tiles =
+      ((long long)a.g.batch * a.n_tiles * (MODE == SHORT ? 1 : a.m_tiles) - first + grid - 1) / grid;
 
   if (warp == 0) {
     // ---------------- X loads (one lane) ---------------------------------------------------------
@@ -464,7 +485,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
       TileRing ring;
       bool wrapped = false, ok = true;
       const int slots = SHIFTED ? a.raw_slots : a.x_slots;
-      GcWalk<CACHED> walk(a, first, grid);
+      GcWalk<CACHED> walk(a, first, grid, MODE == SHORT);
       while (ok && walk.next()) {
         const int word = walk.nt * S::TILE + rank * S::WORDS;
         for (int k = 0; k < a.g.n_in; k += SHIFTED ? S::RAW_ROWS : S::XK) {
@@ -505,29 +526,44 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     // ---------------- weight loads (one lane) ----------------------------------------------------
     if (lane == 0 && !a.in_place) {
       asm volatile("griddepcontrol.wait;" ::: "memory");  // the weights' kernel is done
-      TileRing ring;
-      bool wrapped = false, ok = true;
-      GcWalk<false> walk(a, first, grid);
-      while (ok && walk.next()) {
-        for (int k = 0; k < kb_n; ++k) {
-          const int s = ring.slot;
-          ok = gc_wait(w_empty + 8 * s, ring.phase ^ 1u, abort_s);
-          if (!ok) break;
-          if (rank == 0) tc::mbar_expect_tx(w_full + 8 * s, (1 + TWO) * S::W_SLOT);
-          if (TWO)  // rows of lo and of hi in turn
-            tc::tma_load_3d_pair(w_at(s), &tm.W, k * GC_WK, 0, walk.m * GC_BM + rank * 64,
-                                 leads(w_full + 8 * s));
-          else
+      if (MODE == LONG) {
+        TileRing ring;
+        bool wrapped = false, ok = true;
+        GcWalk<false> walk(a, first, grid, false);
+        while (ok && walk.next()) {
+          for (int k = 0; k < kb_n; ++k) {
+            const int s = ring.slot;
+            ok = gc_wait(w_empty + 8 * s, ring.phase ^ 1u, abort_s);
+            if (!ok) break;
+            tc::mbar_expect_tx(w_full + 8 * s, S::W_SLOT);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              tc::tma_load_3d(w_at(s) + h * GC_W_HALF, &tm.W, k * GC_WK, walk.m * GC_BM, h,
+              tc::tma_load_3d(w_at(0, s) + h * GC_W_HALF, &tm.W, k * GC_WK, walk.m * GC_BM, h,
                               w_full + 8 * s);
-          ring.advance(a.w_slots);
-          wrapped |= ring.slot == 0;
+            ring.advance(a.w_slots);
+            wrapped |= ring.slot == 0;
+          }
         }
-        if (MODE != LONG) break;  // they stay
+        tile_drain(w_full, ring, wrapped, a.w_slots, GC_WAIT_LIMIT);
+      } else {
+        const int m0 = TWO ? (int)(first % (unsigned)a.m_tiles) : m_first;
+        for (int m = 0; m < m_n; ++m)
+          for (int k = 0; k < kb_n; ++k) {
+            const int s = m * kb_n + k, row = (m0 + m) * GC_BM;
+            const bool tail = MODE == SHORT && a.w_tail && k + 1 == kb_n;
+            if (rank == 0)
+              tc::mbar_expect_tx(w_full + 8 * s, (uint32_t)((1 + TWO) * (tail ? S::W_TAIL : S::W_SLOT)));
+            if (TWO)  // rows of lo and of hi in turn
+              tc::tma_load_3d_pair(w_at(m, k), &tm.W, k * GC_WK, 0, row + rank * 64, leads(w_full + 8 * s));
+            else
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                tc::tma_load_3d(w_at(m, k) + h * (tail ? S::W_TAIL / 2 : GC_W_HALF),
+                                tail ? &tm.W_tail : &tm.W, k * GC_WK, row, h, w_full + 8 * s);
+          }
+        if (rank == 0)
+          for (int s = 0; s < m_n * kb_n; ++s) (void)tc::mbar_wait(w_full + 8 * s, 0, GC_WAIT_LIMIT);
       }
-      if (rank == 0) tile_drain(w_full, ring, wrapped, a.w_slots, GC_WAIT_LIMIT);
     }
   } else if (SHIFTED && warp < S::MMA_WARP) {
     // ---------------- raw rows -> operand layout (shifted rows only) -----------------------------
@@ -541,7 +577,7 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     const int box = word >> 4, ch = (word & 15) >> 1, half = word & 1;
     TileRing xr, rr;
     bool ok = true;
-    GcWalk<CACHED> walk(a, first, grid);
+    GcWalk<CACHED> walk(a, first, grid, MODE == SHORT);
     while (ok && walk.next()) {
       const int parity = walk.src * a.g.n_in & 1;  // of the tile's first row
       const int off_e = parity ? a.off1 : a.off0, off_o = parity ? a.off0 : a.off1;
@@ -594,58 +630,80 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
       constexpr int STEPS = S::XK / GC_KSTEP, PER_W = GC_WK / S::XK;
       const bool one = tc::elect_one();
       const int hi = warp - S::MMA_WARP;
-      const uint64_t wd = tc::smem_desc_sw128(w_at(0) + hi * GC_W_HALF, 16u, 1024u);
+      const uint64_t wd = tc::smem_desc_sw128(w_at(0, 0) + hi * GC_W_HALF, 16u, 1024u);
+      const uint64_t td = tc::smem_desc_sw32(w_at(0, kb_n - 1) + hi * (S::W_TAIL / 2), 16u, 256u);
       const uint64_t xd = tc::smem_desc_sw128(x_at(0), S::XK * 128u, 1024u);
       const uint32_t w_hi = (uint32_t)(wd >> 32), x_hi = (uint32_t)(xd >> 32);
+      const int tail = MODE == SHORT ? a.w_tail : 0;
       const int steps = (a.g.n_in + GC_KSTEP - 1) / GC_KSTEP;
       TileRing x, w;
       bool ok = true;
-      for (long long t = 0; ok && t < tiles; ++t) {
-        const int buf = STAGES == 1 ? 0 : (int)t & 1;
-        const uint32_t d = tmem + (uint32_t)(buf * 256 + hi * S::HI_AT);
-        ok = gc_wait(acc_empty + 8 * buf, (uint32_t)(t / STAGES) ^ 1u, abort_s);
-        if (!ok) break;
-        tc::tc_fence_after();
-        uint32_t acc = 0;
-        if (MODE != LONG) w.slot = 0;
-        for (int left = steps; ok && left > 0;) {  // one weight slot
-          if (MODE == LONG || t == 0) {
-            ok = gc_wait(w_full + 8 * w.slot, w.phase, abort_s);
-            if (!ok) break;
-          }
-          const uint32_t w_lo = (uint32_t)wd + (uint32_t)(w.slot * (S::W_SLOT / 16));
-#pragma unroll
-          for (int h = 0; h < PER_W; ++h) {
-            if (left <= 0) break;
-            ok = gc_wait(x_full + 8 * x.slot, x.phase, abort_s);
-            if (!ok) break;
-            const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (GC_X_SLOT / 16));
-            if (one) {
-#pragma unroll
-              for (int k = 0; k < STEPS; ++k)
-                if (k < left) {
-                  if (TWO)
-                    tc::mma_i8_lo_pair(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
-                                       k ? 1u : acc);
-                  else
-                    tc::mma_i8_lo(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
-                                  k ? 1u : acc);
-                }
-              commit(x_empty + 8 * x.slot);
+      int buf = 0;
+      uint32_t turn = 0;
+      for (long long t = 0; ok && t < x_tiles; ++t) {
+        const TileRing x0 = x;
+        for (int m = 0; ok && m < m_n; ++m) {  // tiles of outputs that take turns at these X slots
+          const uint32_t d = tmem + (uint32_t)(buf * 256 + hi * S::HI_AT);
+          ok = gc_wait(acc_empty + 8 * buf, turn ^ 1u, abort_s);
+          if (!ok) break;
+          tc::tc_fence_after();
+          uint32_t acc = 0;
+          x = x0;
+          if (MODE != LONG) w.slot = 0;
+          const uint32_t w_m = (uint32_t)(m * (a.w_tile / 16));
+          for (int left = steps - tail; ok && left > 0;) {  // one weight slot
+            if (MODE == LONG || t == 0) {
+              ok = gc_wait(w_full + 8 * (MODE == SHORT ? m * kb_n + w.slot : w.slot), w.phase, abort_s);
+              if (!ok) break;
             }
-            acc = 1;
-            left -= STEPS;
+            const uint32_t w_lo = (uint32_t)wd + w_m + (uint32_t)(w.slot * (S::W_SLOT / 16));
+#pragma unroll
+            for (int h = 0; h < PER_W; ++h) {
+              if (left <= 0) break;
+              if (m == 0) ok = gc_wait(x_full + 8 * x.slot, x.phase, abort_s);
+              if (!ok) break;
+              const uint32_t x_lo = (uint32_t)xd + (uint32_t)(x.slot * (GC_X_SLOT / 16));
+              if (one) {
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k)
+                  if (k < left) {
+                    if (TWO)
+                      tc::mma_i8_lo_pair(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi,
+                                         IDESC, k ? 1u : acc);
+                    else
+                      tc::mma_i8_lo(d, w_lo + 2 * (h * STEPS + k), w_hi, x_lo + 256 * k, x_hi, IDESC,
+                                    k ? 1u : acc);
+                  }
+                if (m + 1 == m_n) commit(x_empty + 8 * x.slot);
+              }
+              acc = 1;
+              left -= STEPS;
+              x.advance(a.x_slots);
+            }
+            if (MODE == LONG) {
+              if (one) commit(w_empty + 8 * w.slot);
+              w.advance(a.w_slots);
+            } else {
+              ++w.slot;
+            }
+          }
+          if (MODE == SHORT && tail && ok) {  // the last slot, of one MMA
+            if (t == 0) ok = gc_wait(w_full + 8 * (m * kb_n + kb_n - 1), 0, abort_s);
+            if (ok && m == 0) ok = gc_wait(x_full + 8 * x.slot, x.phase, abort_s);
+            if (ok && one) {
+              tc::mma_i8_lo(d, (uint32_t)td + w_m, (uint32_t)(td >> 32),
+                            (uint32_t)xd + (uint32_t)(x.slot * (GC_X_SLOT / 16)), x_hi, IDESC, acc);
+              if (m + 1 == m_n) commit(x_empty + 8 * x.slot);
+            }
             x.advance(a.x_slots);
           }
-          if (MODE == LONG) {
-            if (one) commit(w_empty + 8 * w.slot);
-            w.advance(a.w_slots);
-          } else {
-            ++w.slot;
+          if (!ok) break;
+          if (one) commit(acc_full + 8 * buf);
+          if (++buf == STAGES) {
+            buf = 0;
+            turn ^= 1u;
           }
         }
-        if (!ok) break;
-        if (one) commit(acc_full + 8 * buf);
       }
     }
   } else {
@@ -654,15 +712,17 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     if (MODE == SHORT && a.in_place) {
       // 16 bytes of lo and of hi per thread and turn, of one output and 16 inputs, into the K-major operand
       // layout
-      const int m0 = (int)(first % (unsigned)a.m_tiles) * GC_BM;
+      const int chunks = a.w_tail ? GC_KSTEP / 16 : GC_WK / 16;
 #pragma unroll 1
-      for (int i = (int)threadIdx.x - 32 * S::EPI_WARP; i < GC_BM * GC_WK / 16; i += 32 * GC_EPI_WARPS) {
+      for (int i = (int)threadIdx.x - 32 * S::EPI_WARP; i < GC_BM * chunks; i += 32 * GC_EPI_WARPS) {
         const int o = i % GC_BM, c = i / GC_BM;
         uint32_t lo[4] = {}, hi[4] = {};
-        if (m0 + o < a.g.n_out && 16 * c < a.g.n_in) a.g.w.bytes(m0 + o, 16 * c, a.g.n_in, lo, hi);
-        unsigned char* to = gc_raw + o * 128 + ((c ^ (o & 7)) << 4);
+        if (o < a.g.n_out && 16 * c < a.g.n_in) a.g.w.bytes(o, 16 * c, a.g.n_in, lo, hi);
+        unsigned char* to =
+            gc_raw + (a.w_tail ? o * 32 + ((c ^ (o >> 2 & 1)) << 4) : o * 128 + ((c ^ (o & 7)) << 4));
         *reinterpret_cast<uint4*>(to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        *reinterpret_cast<uint4*>(to + GC_W_HALF) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(to + (a.w_tail ? S::W_TAIL / 2 : GC_W_HALF)) =
+            make_uint4(hi[0], hi[1], hi[2], hi[3]);
       }
       tc::fence_async_smem();
       __syncwarp();
@@ -684,16 +744,28 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     auto chunk = [&](int k) { return out + ((row * PITCH | xored(row) << 4) ^ (k << 4)); };
     const int buf = STAGES == 1 ? 0 : group;
     uint32_t turn = 0;
-    GcWalk<CACHED> walk(a, STAGES == 1 ? first : first + group * grid, STAGES * grid);
-    for (; walk.next(); ++turn) {
-      const int row0 = walk.m * GC_BM + rank * 64 + q * S::ROWS, col0 = walk.nt * S::TILE + share * S::EW;
+    // A group's tiles: every second one, or where several tiles of outputs take turns at one of X
+    // every second turn.
+    const bool turns = MODE == SHORT && m_n > 1, apart = STAGES == 2 && !turns;
+    GcWalk<CACHED> walk(a, apart ? first + group * grid : first, apart ? 2 * grid : grid, MODE == SHORT);
+    int m = turns ? group : 0;
+    for (bool more = walk.next(); more; ++turn) {
+      const int row0 = (MODE == SHORT ? m_first + m : walk.m) * GC_BM + rank * 64 + q * S::ROWS, col0 = walk.nt * S::TILE + share * S::EW;
       const int body = a.g.L - 1 - col0;  // the body among this warp's words
+      const int b = walk.b, src = walk.src;
+      // the next one
+      if (turns && (m += 2) < m_n) {
+        more = true;
+      } else {
+        m = turns ? m - m_n : 0;
+        more = walk.next();
+      }
       if (!gc_wait(acc_full + 8 * buf, turn, abort_s)) break;
       tc::tc_fence_after();
       const uint32_t c_tmem = tmem + (uint32_t)(buf * 256 + share * S::EW * BYTES) +
                               ((uint32_t)(q * 32) << 16);
       // nothing of this warp's share is kept
-      if (row0 >= a.g.n_out || body < 0 || (CACHED && walk.src == a.g.n_slots)) {
+      if (row0 >= a.g.n_out || body < 0 || (CACHED && src == a.g.n_slots)) {
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) drained(acc_empty + 8 * buf);
@@ -756,19 +828,19 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
             if (a.g.bias) *p += (uint64_t)__ldg(a.g.bias + row0 + row) * a.g.delta;
             // tiled stores end on 16-byte boundaries, so the last word of an odd count goes alone
             if (!a.plain_out && (a.g.L & 1))
-              a.g.Y[((size_t)walk.b * a.g.n_out + row0 + row) * a.g.ldy + a.g.L - 1] = *p;
+              a.g.Y[((size_t)b * a.g.n_out + row0 + row) * a.g.ldy + a.g.L - 1] = *p;
           }
           if (!a.plain_out) {
             tc::fence_async_smem();
             __syncwarp();
             if (lane == 0 && col0 + part < (a.g.L & ~1))
-              tc::tma_store_3d(&tm.Y, col0 + part, row0, walk.b, out_at);
+              tc::tma_store_3d(&tm.Y, col0 + part, row0, b, out_at);
           } else {
             __syncwarp();
             constexpr int PER = 32 / S::PART;  // rows per instruction
             const int wd = lane % S::PART, sub = lane / S::PART;
             uint64_t* to =
-                a.g.Y + ((size_t)walk.b * a.g.n_out + row0 + sub) * a.g.ldy + col0 + part + wd;
+                a.g.Y + ((size_t)b * a.g.n_out + row0 + sub) * a.g.ldy + col0 + part + wd;
             const int left = col0 + part + wd < a.g.L ? a.g.n_out - row0 - sub : 0;
             constexpr int TIMES = S::ROWS / PER;
             uint64_t v[TIMES];
@@ -807,9 +879,10 @@ static GcMode gc_mode(int n_in, int n_out) {
   if (n_in > GC_STAYS || n_out > GC_MOST_TILES * GC_BM) return LONG;
   return n_in <= GC_SHORT ? SHORT : PAIR;
 }
-// One slot of weights is expanded by every block for itself, which saves a launch; more by a kernel before.
+// One slot of weights for one tile of outputs is expanded by every block for itself, which saves a launch;
+// more by a kernel before.
 static bool gc_in_place(int n_in, int n_out) {
-  return n_in <= GC_WK && gc_mode(n_in, n_out) == SHORT;
+  return n_in <= GC_WK && n_out <= GC_BM;
 }
 
 // The grid, and how one block's shared memory is shared out.
@@ -818,20 +891,40 @@ static unsigned gc_plan(GcArgs& a, int sms) {
   using S = GcShape<BYTES, SHIFTED, MODE>;
   a.n_tiles = (a.g.L + S::TILE - 1) / S::TILE;
   const int per = MODE == PAIR ? 2 : 1;
+  const int kb = (a.g.n_in + GC_WK - 1) / GC_WK, kx = (a.g.n_in + S::XK - 1) / S::XK;
   unsigned grid =
       (unsigned)std::min<long long>((long long)a.g.batch * a.n_tiles * a.m_tiles, sms / per);
-  if (MODE != LONG) grid = grid / a.m_tiles * a.m_tiles;  // a block's tiles have the same outputs
+  if (MODE == PAIR) grid = grid / a.m_tiles * a.m_tiles;  // a block's tiles have the same outputs
   int room = GC_SMEM - GC_BAR_BYTES - GC_EPI_WARPS * S::STAGE;
-  a.w_slots = MODE != LONG ? (a.g.n_in + GC_WK - 1) / GC_WK : SHIFTED ? 2 : 3;
-  room -= a.w_slots * S::W_SLOT;
+  a.w_slots = MODE == LONG ? SHIFTED ? 2 : 3 : kb;
+  a.m_group = 1;
+  a.w_tail = MODE == SHORT && a.g.n_in > (kb - 1) * GC_WK && a.g.n_in <= (kb - 1) * GC_WK + GC_KSTEP;
+  a.w_tile = a.w_slots * S::W_SLOT - (a.w_tail ? S::W_SLOT - S::W_TAIL : 0);
+  if (MODE == SHORT) {
+    // As many tiles of outputs as leave X its slots, in groups of about the same size, but no fewer
+    // blocks for it: every group reads X again, in time with the others at first (96 x 128->784, with
+    // seven groups: 460 MB for 201).
+    const int x_want = (SHIFTED ? std::max(3, kx + 1) : std::max(4, kx + 2)) * GC_X_SLOT +
+                       (SHIFTED ? GC_COPY_WARPS * S::RAW_SLOT : 0);
+    const long long x_tiles = (long long)a.g.batch * a.n_tiles;
+    int most = std::min({a.m_tiles, (room - x_want) / a.w_tile, GC_MAX_W / kb});
+    most = (int)std::max<long long>(1, std::min<long long>(most, x_tiles * a.m_tiles / (4 * sms)));
+    const int groups = (a.m_tiles + most - 1) / most;
+    a.m_group = (a.m_tiles + groups - 1) / groups;
+    grid = (unsigned)std::min<long long>(
+        sms, x_tiles * ((a.m_tiles + a.m_group - 1) / a.m_group));
+    if (grid < (unsigned)a.m_tiles) grid = 0;  // (a machine with fewer multiprocessors than that)
+    a.w_slots = a.m_group * kb;
+  }
+  room -= a.m_group * a.w_tile;
   if (SHIFTED) {
-    a.x_slots = 3;
+    a.x_slots = a.m_group > 1 ? std::max(3, kx + 1) : 3;
     a.raw_slots = std::min(GC_MAX_RAW, (room - a.x_slots * GC_X_SLOT) / S::RAW_SLOT & ~3);
   } else {
     a.x_slots = std::min(GC_MAX_X, room / GC_X_SLOT);
     a.raw_slots = 0;
   }
-  a.x_at = a.w_slots * S::W_SLOT;
+  a.x_at = a.m_group * a.w_tile;
   a.out_at = a.x_at + a.x_slots * GC_X_SLOT;
   a.raw_at = a.out_at + GC_EPI_WARPS * S::STAGE;
   a.bars_at = a.raw_at + a.raw_slots * S::RAW_SLOT;
@@ -932,6 +1025,10 @@ static int gc_launch(GcArgs& a, int8_t* ws, cudaStream_t st) {
     }
     rc = tile_map(&tm.W, CU_TENSOR_MAP_DATA_TYPE_UINT8, ws, 3, dims, strides, box,
                   CU_TENSOR_MAP_SWIZZLE_128B);
+    box[0] = GC_KSTEP;
+    if (!rc && a.w_tail)
+      rc = tile_map(&tm.W_tail, CU_TENSOR_MAP_DATA_TYPE_UINT8, ws, 3, dims, strides, box,
+                    CU_TENSOR_MAP_SWIZZLE_32B);
     if (rc) return rc;
     group_expand_kernel<<<(unsigned)blocks, GX_THREADS, 0, st>>>(g.w, g.n_in, g.n_out, pitch, ws);
     PNB_CHECK_LAUNCH("group_expand_kernel");

@@ -97,7 +97,8 @@ def test_row_bytes_of_nothing(pnb):
 
 @pytest.mark.parametrize("M,K", [(1, 1), (3, 5), (10, 128), (128, 784), (33, 17), (16, 16),
                                  (896, 897), (4736, 100), (4737, 100), (1, 61440),
-                                 (16, 24), (16, 25), (384, 1), (4737, 1)])
+                                 (16, 24), (16, 25), (384, 1), (4737, 1),
+                                 (128, 128), (129, 128), (128, 129)])
 def test_binding_and_library_agree_on_workspaces(pnb, M, K):
     L = pnb.lib()
     assert L.pnb_group_contract_workspace_bytes(M, K, 0) == pnb._group_bytes(K, M)
