@@ -269,7 +269,7 @@ struct GcArgs {
   GroupArgs g;
   int off0, off1;    // words by which rows 0, 2, .. / 1, 3, .. start past 16-byte alignment
   int n_tiles, m_tiles;  // tiles: outputs fastest, then words, then requests
-  int m_group;           // SHORT: tiles of outputs of one block (of the last block's group fewer)
+  int m_group;           // SHORT: tiles of outputs of one block, one or all
   int w_tail;            // of the last weight slot 32 inputs are kept, not 128
   int w_tile;            // bytes of the weights of one tile of outputs
   int w_slots, x_slots, raw_slots;
@@ -409,14 +409,15 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
   unsigned first = TWO ? blockIdx.x >> 1 : blockIdx.x, grid = TWO ? gridDim.x >> 1 : gridDim.x;
   int m_first = 0, m_n = 1;  // SHORT: the block's tiles of outputs
   if (MODE == SHORT) {
-    // Of every m_tiles blocks in turn a group of outputs has as many as it has tiles, so that all groups
-    // go through X at the same pace, next to one another.
-    const unsigned round = blockIdx.x / (unsigned)a.m_tiles, r = blockIdx.x - round * a.m_tiles;
-    m_first = (int)r / a.m_group * a.m_group;
-    m_n = min(a.m_group, a.m_tiles - m_first);
-    first = round * m_n + (r - m_first);
-    grid = gridDim.x / (unsigned)a.m_tiles * m_n +
-           (unsigned)max(0, min(m_n, (int)(gridDim.x % (unsigned)a.m_tiles) - m_first));
+    // All tiles of outputs, or one: then a run of neighbouring blocks has the same.
+    auto start = [&](int m) { return (unsigned)((long long)gridDim.x * m / a.m_tiles); };
+    if (a.m_group > 1) {
+      m_n = a.m_tiles;
+    } else {
+      while (blockIdx.x >= start(m_first + 1)) ++m_first;
+      first = blockIdx.x - start(m_first);
+      grid = start(m_first + 1) - start(m_first);
+    }
   }
   auto leads = [&](uint32_t bar) { return TWO ? tc::cluster_address(bar, 0) : bar; };
   auto drained = [&](uint32_t bar) {  // the first block's: a warp's loads from tensor memory are done
@@ -901,18 +902,14 @@ static unsigned gc_plan(GcArgs& a, int sms) {
   a.w_tail = MODE == SHORT && a.g.n_in > (kb - 1) * GC_WK && a.g.n_in <= (kb - 1) * GC_WK + GC_KSTEP;
   a.w_tile = a.w_slots * S::W_SLOT - (a.w_tail ? S::W_SLOT - S::W_TAIL : 0);
   if (MODE == SHORT) {
-    // As many tiles of outputs as leave X its slots, in groups of about the same size, but no fewer
-    // blocks for it: every group reads X again, in time with the others at first (96 x 128->784, with
-    // seven groups: 460 MB for 201).
+    // All tiles of outputs, if their weights leave X its slots and there are tiles of X for all blocks:
+    // it is then loaded (and at odd pitches copied) once.
     const int x_want = (SHIFTED ? std::max(3, kx + 1) : std::max(4, kx + 2)) * GC_X_SLOT +
                        (SHIFTED ? GC_COPY_WARPS * S::RAW_SLOT : 0);
     const long long x_tiles = (long long)a.g.batch * a.n_tiles;
-    int most = std::min({a.m_tiles, (room - x_want) / a.w_tile, GC_MAX_W / kb});
-    most = (int)std::max<long long>(1, std::min<long long>(most, x_tiles * a.m_tiles / (4 * sms)));
-    const int groups = (a.m_tiles + most - 1) / most;
-    a.m_group = (a.m_tiles + groups - 1) / groups;
-    grid = (unsigned)std::min<long long>(
-        sms, x_tiles * ((a.m_tiles + a.m_group - 1) / a.m_group));
+    if (a.m_tiles * a.w_tile <= room - x_want && a.m_tiles * kb <= GC_MAX_W && x_tiles >= 4 * sms)
+      a.m_group = a.m_tiles;
+    grid = (unsigned)std::min<long long>(sms, x_tiles * (a.m_tiles / a.m_group));
     if (grid < (unsigned)a.m_tiles) grid = 0;  // (a machine with fewer multiprocessors than that)
     a.w_slots = a.m_group * kb;
   }
