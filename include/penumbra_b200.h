@@ -325,8 +325,8 @@ int pnb_cache_read(const int32_t* slots_dev, int tokens, const void* cache_dev, 
  * X [batch][K][ldx], Y [batch][M][ldy].  transposed = 1: Y[b][i] = sum_j w[j][i] X[b][j] with X
  * [batch][M][ldx], Y [batch][K][ldy] and no bias, the gradient with respect to the inputs.  At most
  * PNB_MAX_GROUP_INPUTS inputs and PNB_MAX_REQUEST_ROWS outputs.  The workspace (16-byte aligned,
- * pnb_group_contract_workspace_bytes, one per call in flight) holds the weights as bytes; when it is
- * NULL, memory is allocated on `stream`.
+ * pnb_group_contract_workspace_bytes, 0 for small layers; one per call in flight) holds the weights
+ * as bytes; when it is NULL, memory is allocated on `stream`.
  * Replaces: the scalar_mul / add loops of Linear::eval (runtime/src/ops/linear.rs:52-75). */
 int pnb_group_contract(const uint8_t* W_dev, const int8_t* scales_dev, const uint8_t* zeros_dev,
                        int group, const int64_t* bias_dev, uint64_t delta, int M, int K,

@@ -6,6 +6,41 @@
 // mod 2^64 over LWE ciphertexts.  |w| <= 128 * 15 = 1920.  X comes as rows of u64 words, or as the
 // rounded words of a cache (cache.cu), whose limbs below the kept ones are zero.  The reference's
 // Linear holds one integer per weight (runtime/src/ops/linear.rs:52-75).
+//
+// On the tensor cores (calls of few products take plain multiply-adds, below).  A word is BYTES
+// little-endian byte limbs (8, or the 2 to 4 that a cache keeps), so the inputs of a request are a u8
+// matrix [n_in][BYTES L], which kind::i8 reads as an MN-major operand where it lies; a weight is two
+// signed bytes, w = lo + 256 hi, however small its group, and
+//     Y = sum_p (LO[p] + HI[p - 1]) << 8p,    LO[p] = sum_i lo_i x_i[p],  HI[p] = sum_i hi_i x_i[p].
+// (Products by the bare nibbles with a scale per group in the epilogue would need half of the MMAs and
+// read the accumulators once per group: 13 times at K = 784 in groups of 64, where this reads two.)
+//
+// The floor is HBM, X read once and Y written once, with the MMAs close behind: 256 requests 784->128
+// need 585 us for 3.83 GB at the measured copy bandwidth and 513 us for the products at twice the
+// measured bf16 rate (from a cache of 32 bits 333 and 257).  Then shared memory: an MMA of N columns reads
+// 4 KB of weights and 32 N bytes of X in N / 2 cycles, at N = 128 all of its 128 bytes a cycle.  And the
+// path from the end of a tile's MMAs to the next ones into the same accumulator (a commit, a wait, two
+// loads of columns, the limb sums, an arrival, a wait), about 2000 cycles.  So there are three forms:
+//
+//   LONG (over 896 inputs, over 4736 outputs, odd pitches over 384): tiles of 128 outputs x 32 words (of
+//     8 bytes), lo and hi in 256 columns each; weights stream from L2.
+//   SHORT (up to 384 inputs): tiles of 128 x 16, lo and hi in 128 columns each, twice, so that the
+//     epilogue of a tile runs beside the MMAs of the next; weights stay in shared memory.
+//   PAIR (between): a pair of blocks shares a tile of 128 x 32 by MMAs of M = 256 (cta_group::2), each with
+//     half of X and half of the weights, which stay.  Lo and hi are neighbouring rows, so that either block
+//     can finish its half of the outputs; the lanes exchange words, which makes the epilogue dearer.
+//
+// Sustained, us (rows of 2049 words):                      SHORT   PAIR   LONG   floor
+//     64 x 300->300                                          210    250    270      96
+//     64 x 400->128                                                 107    148      85
+//     64 x 784->128                                                 177    208     146
+//     32 x 512->512                                                 195    230      82
+//     61 x 130->200, odd pitch                                95           138      50
+//     64 x 784->128, odd pitch                                      301    238     146
+// Measured: 256 x 784->128 655 us at its best (0.89 of the copy's rate) and 790-880 under the power cap,
+// where the SM clock falls to about 1.2 GHz; from 32 bits 421-460.  96 x 128->784 transposed 430-460 (its
+// share of the floor, 219, is the lowest: the path above, 1000 cycles a tile).  45 x 257->384 from 24 bits
+// 96.  One request 784->128 9.2 us in a graph, 13.6 a call: the host's.
 #include <algorithm>
 #include <atomic>
 
@@ -107,7 +142,10 @@ struct GroupArgs {
 // One thread per word, 16 outputs at a time, weights in shared memory as w + 2048 >= 0, so that a product
 // is one 32 x 32 + 64 and one 32 x 32 + 32 bit multiply-add and sum w x = sum (w + 2048) x - 2048 sum x.
 constexpr int GF_THREADS = 256, GF_OUT = 16, GF_IN = 64;
-constexpr long long GF_MOST = 384;  // weights, outputs padded to 16, that go this way
+// Most weights, outputs padded to 16, that go this way.  256 requests of 2049-word rows take 137 us on the
+// tensor cores with 24->16 (161 at an odd pitch, 62 from 24 bits) and 75 (75, 64) here, with 10->4 136 and
+// 31; 64->10 takes 118 there and 166 here.
+constexpr long long GF_MOST = 384;
 
 static bool gf_few(int n_in, int n_out) {
   return (long long)n_in * ((n_out + GF_OUT - 1) / GF_OUT * GF_OUT) <= GF_MOST;
@@ -172,9 +210,9 @@ __global__ void __launch_bounds__(GF_THREADS) group_few_kernel(const __grid_cons
 }
 
 // ---- weights as bytes ---------------------------------------------------------------------------
-// Two matrices of signed bytes, w = lo + 256 hi, lo
-// [n_out][pitch], then hi, rows padded by zeros to a multiple of 16 bytes.  A thread makes 16 bytes of
-// both.
+// Two matrices of signed bytes, w = lo + 256 hi, lo [n_out][pitch], then hi, rows padded by zeros to a
+// multiple of 16 bytes.  A thread makes 16 bytes of both.  (Every block expanding for itself what stays in
+// its shared memory costs more, as the code runs once and cold: 784 inputs 9 us against 2.)
 constexpr int GX_THREADS = 128;
 
 __global__ void __launch_bounds__(GX_THREADS)
@@ -225,8 +263,8 @@ constexpr int GC_SMEM = 227 * 1024;
 constexpr uint32_t GC_WAIT_LIMIT = 1u << 24;
 
 // LONG: one block, weights stream, one accumulator of 256 columns for lo and one for hi.
-// SHORT: one block, weights of some tiles of outputs stay, which take turns at a tile of X; two
-//   accumulators of 128 columns for each.
+// SHORT: one block, the weights of one tile of outputs stay, or of all, which then take turns at a tile of
+//   X; two accumulators of 128 columns for each.
 // PAIR: two blocks share a tile, weights stay, two accumulators of 256 columns; every second row of the
 //   weights is a hi, in one block those of the first 64 outputs, in the other of the last.
 enum GcMode { LONG, SHORT, PAIR };
@@ -409,7 +447,9 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
   unsigned first = TWO ? blockIdx.x >> 1 : blockIdx.x, grid = TWO ? gridDim.x >> 1 : gridDim.x;
   int m_first = 0, m_n = 1;  // SHORT: the block's tiles of outputs
   if (MODE == SHORT) {
-    // All tiles of outputs, or one: then a run of neighbouring blocks has the same.
+    // All tiles of outputs, or one: then a run of neighbouring blocks has the same.  (Dealt out in turn,
+    // seven tiles of outputs of 96 x 128->784 take 770 us instead of 430 when a launch writes more than L2
+    // holds.)
     auto start = [&](int m) { return (unsigned)((long long)gridDim.x * m / a.m_tiles); };
     if (a.m_group > 1) {
       m_n = a.m_tiles;
@@ -751,7 +791,8 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
     GcWalk<CACHED> walk(a, apart ? first + group * grid : first, apart ? 2 * grid : grid, MODE == SHORT);
     int m = turns ? group : 0;
     for (bool more = walk.next(); more; ++turn) {
-      const int row0 = (MODE == SHORT ? m_first + m : walk.m) * GC_BM + rank * 64 + q * S::ROWS, col0 = walk.nt * S::TILE + share * S::EW;
+      const int row0 = (MODE == SHORT ? m_first + m : walk.m) * GC_BM + rank * 64 + q * S::ROWS;
+      const int col0 = walk.nt * S::TILE + share * S::EW;
       const int body = a.g.L - 1 - col0;  // the body among this warp's words
       const int b = walk.b, src = walk.src;
       // the next one
@@ -886,7 +927,9 @@ static bool gc_in_place(int n_in, int n_out) {
   return n_in <= GC_WK && n_out <= GC_BM;
 }
 
-// The grid, and how one block's shared memory is shared out.
+// The grid, and how one block's shared memory is shared out: weights, then X.  Slots of X in flight hide
+// memory's latency (64 x 784->128 in pairs: 256, 214 and 199 us with 3, 4 and 5 of them), so a warp
+// stages no more than 8 words of its outputs at a time.
 template <int BYTES, bool SHIFTED, GcMode MODE>
 static unsigned gc_plan(GcArgs& a, int sms) {
   using S = GcShape<BYTES, SHIFTED, MODE>;
@@ -903,7 +946,8 @@ static unsigned gc_plan(GcArgs& a, int sms) {
   a.w_tile = a.w_slots * S::W_SLOT - (a.w_tail ? S::W_SLOT - S::W_TAIL : 0);
   if (MODE == SHORT) {
     // All tiles of outputs, if their weights leave X its slots and there are tiles of X for all blocks:
-    // it is then loaded (and at odd pitches copied) once.
+    // it is then loaded (and at odd pitches copied) once.  61 x 130->200 88 -> 84 us, at an odd pitch 125
+    // -> 95; several of more, so that X is read by fewer groups, 430 -> 600 (96 x 128->784).
     const int x_want = (SHIFTED ? std::max(3, kx + 1) : std::max(4, kx + 2)) * GC_X_SLOT +
                        (SHIFTED ? GC_COPY_WARPS * S::RAW_SLOT : 0);
     const long long x_tiles = (long long)a.g.batch * a.n_tiles;
