@@ -171,6 +171,15 @@ SHAPES = [  # batch, K, M, group, L, ld
     (2, 130, 200, 32, 2049, 2049), (2, 130, 200, 32, 2049, 2050), (5, 128, 10, 48, 2049, 2050),
     (1, 784, 128, 128, 2049, 2050), (1, 784, 128, 784, 2049, 2049), (3, 257, 129, 17, 835, 836),
     (2, 257, 384, 48, 835, 835), (1, 1000, 40, 128, 8193, 8194), (1, 90, 70, 3, 8193, 8193),
+    # last weight slots of 32 inputs and of more; on both sides of each way of computing
+    (3, 32, 20, 32, 40, 41), (3, 160, 150, 16, 40, 42), (3, 161, 150, 16, 40, 40),
+    (2, 384, 130, 64, 35, 36), (2, 384, 130, 64, 35, 35), (2, 385, 130, 64, 35, 36),
+    (2, 385, 130, 64, 35, 35), (2, 896, 130, 896, 35, 36), (2, 897, 130, 16, 35, 36),
+    (2, 128, 128, 16, 35, 36), (2, 129, 128, 16, 35, 36), (2, 128, 129, 16, 35, 36),
+    (1, 24, 16, 8, 35, 36), (1, 25, 16, 8, 35, 36), (1, 100, 4800, 20, 20, 20),
+    # enough tiles of X for a block to have all tiles of outputs
+    (320, 130, 200, 32, 70, 71), (320, 130, 200, 32, 70, 72), (320, 30, 300, 7, 70, 70),
+    (320, 257, 140, 48, 66, 66),
     (7, 16, 10, 16, 2049, 2049), (70, 40, 24, 8, 100, 100), (2, 2100, 66, 64, 70, 70),
     (2, 2100, 300, 100, 70, 72), (300, 16, 4, 16, 33, 34), (2, 300, 1000, 64, 40, 40),
 ]
