@@ -78,7 +78,8 @@ class Weights:
 ROWS = [  # features, L, ld
     (1, 1, 1), (1, 1, 2), (3, 2, 2), (2, 3, 5), (5, 4, 4), (3, 5, 6), (7, 15, 15), (2, 16, 16),
     (3, 17, 18), (2, 835, 835), (3, 835, 836), (1, 2048, 2048), (3, 2049, 2049), (4, 2049, 2050),
-    (2, 2049, 2052), (2, 8193, 8193), (40, 33, 33), (513, 5, 5),
+    (2, 2049, 2052), (2, 8193, 8193), (40, 33, 33), (513, 5, 5), (1, 511, 511), (2, 512, 513),
+    (2, 513, 513), (1, 1 << 20, 1 << 20), (2, (1 << 20) - 1, (1 << 20) - 1),
 ]
 
 
@@ -180,6 +181,8 @@ SHAPES = [  # batch, K, M, group, L, ld
     # enough tiles of X for a block to have all tiles of outputs
     (320, 130, 200, 32, 70, 71), (320, 130, 200, 32, 70, 72), (320, 30, 300, 7, 70, 70),
     (320, 257, 140, 48, 66, 66),
+    # the longest ciphertexts
+    (1, 3, 2, 2, 1 << 20, 1 << 20), (1, 40, 20, 16, 1 << 20, (1 << 20) + 1),
     (7, 16, 10, 16, 2049, 2049), (70, 40, 24, 8, 100, 100), (2, 2100, 66, 64, 70, 70),
     (2, 2100, 300, 100, 70, 72), (300, 16, 4, 16, 33, 34), (2, 300, 1000, 64, 40, 40),
 ]
@@ -275,14 +278,15 @@ def test_gradient_is_the_transpose(pnb):
         assert np.array_equal(moved[0].view(np.int64), np.repeat(W.dense[:, i:i + 1], 9, 1))
 
 
+@pytest.mark.parametrize("K,M", [(70, 90), (200, 150), (500, 90)])
 @pytest.mark.parametrize("off_x,off_y,ldx,ldy", [
     (0, 0, 66, 66), (1, 0, 66, 66), (0, 1, 66, 66), (1, 1, 67, 67), (0, 0, 67, 66), (0, 0, 66, 67),
     (1, 0, 67, 70), (0, 1, 70, 65),
 ])
-def test_every_alignment_through_the_c_abi(pnb, oracle, off_x, off_y, ldx, ldy):
+def test_every_alignment_through_the_c_abi(pnb, oracle, off_x, off_y, ldx, ldy, K, M):
     import ctypes as C
     rng = np.random.default_rng(off_x + 2 * off_y + 4 * ldx + ldy)
-    B, K, M, L = 3, 70, 90, 65
+    B, L = 3, 65
     W = Weights(pnb, rng, M, K, 32)
     x = torch.zeros(B * K * ldx + 2, dtype=torch.int64, device="cuda")
     X = words(rng, B, K, ldx)
@@ -299,7 +303,7 @@ def test_every_alignment_through_the_c_abi(pnb, oracle, off_x, off_y, ldx, ldy):
     got = host(y)
     assert np.array_equal(got[off_y:off_y + want.size].reshape(want.shape), want)
     assert np.all(np.delete(got, np.s_[off_y:off_y + want.size]) == MARK)
-    # the same result without a workspace of the caller's, and at a cache's rows
+    # (without a workspace of the caller's) and over a cache
     cache = pnb.CiphertextCache(B, K, L, 32)
     slots = dev(np.arange(B, dtype=np.int32))
     pnb.cache_write(cache, dev(X), slots)
@@ -414,6 +418,35 @@ def test_two_host_threads(pnb, oracle):
     for i in range(2):
         want = oracle.contract(W[i].dense, None, 0, X[i])
         assert len(got[i]) == 20 and all(np.array_equal(host(y), want) for y in got[i])
+
+
+def test_weights_at_any_address_and_other_types_of_words(pnb, oracle):
+    import ctypes as C
+    rng = np.random.default_rng(12)
+    K, M, L = 160, 70, 40
+    W = Weights(pnb, rng, M, K, 32)
+    X = words(rng, 2, K, L)
+    want = oracle.contract(W.dense, None, 0, X)
+    # unsigned words, and inputs that are a view
+    x = dev(X)
+    assert np.array_equal(host(pnb.group_contract(W.own, None, 0, x.view(torch.uint64))), want)
+    wide = torch.zeros(2, 2 * K, L, dtype=torch.int64, device="cuda")
+    wide[:, ::2] = x
+    assert np.array_equal(host(pnb.group_contract(W.own, None, 0, wide[:, ::2])), want)
+    # packed weights, scales and zero points that start anywhere
+    for off in (1, 2, 3):
+        at = []
+        for t in (W.own.q, W.own.scales, W.own.zeros):
+            moved = torch.zeros(t.numel() + 4, dtype=t.dtype, device="cuda")
+            moved[off:off + t.numel()] = t.reshape(-1)
+            at.append(moved)
+        y = marked(2, M, L)
+        torch.cuda.synchronize()
+        assert pnb.lib().pnb_group_contract(
+            *(C.c_void_p(t.data_ptr() + off) for t in at), 32, None, 0, M, K, 0,
+            C.c_void_p(x.data_ptr()), L, C.c_void_p(y.data_ptr()), L, 2, L, None, 0, None) == 0
+        torch.cuda.synchronize()
+        assert np.array_equal(host(y), want)
 
 
 def test_refusals_on_the_device(pnb):
