@@ -9,7 +9,7 @@
 // The reference holds every ciphertext in full (SignedRadixCiphertext, runtime/src/ops/mod.rs:58).
 //
 // Both move each byte once, which HBM bounds: 512 tokens of 128 ciphertexts of 2049 words, one in twenty
-// unused, are written in 24 bits at an odd pitch in 250-260 us (floor 203; the look for later tokens of a
+// unused, are written in 24 bits at an odd pitch in 239-250 us (floor 203; the look for later tokens of a
 // slot is part of the rest) and read from 32 bits in 242 (floor 234).
 //
 // A row of the cache is L little-endian words of n / 8 bytes (n = 16, 24, 32), padded to a multiple of
@@ -24,10 +24,12 @@ namespace pnb {
 
 constexpr int CH_WARPS = 8, CH_BLOCKS = 5;
 constexpr int CH_AHEAD = 4;    // pairs of words of a thread on their way together
-constexpr int CH_PIECE = 512;  // words of a row that a warp takes at a time
+// Words of a row that a warp takes at a time: 512 x 128 ciphertexts written in 24 bits 239 us with 256, 249
+// with 512, read from 32 bits 262 and 251.
+constexpr int CH_PIECE_WRITE = 256, CH_PIECE_READ = 512;
 // Most pieces of a block.  Writing, a block looks for later tokens of its slot first, which more pieces
-// share (512 x 128 ciphertexts in 24 bits: 259 us with 8, 249 with 32, 265 with 128); reading, fewer are
-// better (from 32 bits: 251, 264, 281).
+// share (in 24 bits, pieces of 512: 259 us with 8, 249 with 32, 265 with 128); reading, fewer are better
+// (from 32 bits: 251, 264, 281).
 constexpr int CH_PIECES_WRITE = 32, CH_PIECES_READ = 8;
 
 struct CacheArgs {
@@ -53,6 +55,7 @@ __global__ void __launch_bounds__(32 * CH_WARPS, CH_BLOCKS)
     cache_kernel(const __grid_constant__ CacheArgs a) {
   using word = unsigned long long;
   constexpr int STEP = 64;  // words of a warp's turn
+  constexpr int PIECE = WRITE ? CH_PIECE_WRITE : CH_PIECE_READ;
   constexpr int UP = 32 - 8 * BYTES;
   constexpr uint32_t HALF = BYTES == 4 ? 0u : 1u << (31 - 8 * BYTES);  // in the high half of a word
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 3;
@@ -72,7 +75,7 @@ __global__ void __launch_bounds__(32 * CH_WARPS, CH_BLOCKS)
 #pragma unroll 1
     for (int p = warp; p < n; p += CH_WARPS) {
       const long long f = (first + p) / a.row_pieces;
-      const int c0 = (int)(first + p - f * a.row_pieces) * CH_PIECE, c1 = min(a.L, c0 + CH_PIECE);
+      const int c0 = (int)(first + p - f * a.row_pieces) * PIECE, c1 = min(a.L, c0 + PIECE);
       word* row = reinterpret_cast<word*>(WRITE ? const_cast<uint64_t*>(a.in) : a.out) +
                   ((size_t)t * a.features + f) * a.ld;
       unsigned char* cell = a.cache + ((size_t)slot * a.features + f) * a.row_bytes;
@@ -177,7 +180,8 @@ size_t cache_row_bytes(int L, int bits) { return ((size_t)L * (bits / 8) + 15) /
 template <bool WRITE>
 static int cache_launch(CacheArgs a, int bits, cudaStream_t st) {
   a.row_bytes = cache_row_bytes(a.L, bits);
-  a.row_pieces = (a.L + CH_PIECE - 1) / CH_PIECE;
+  constexpr int PIECE = WRITE ? CH_PIECE_WRITE : CH_PIECE_READ;
+  a.row_pieces = (a.L + PIECE - 1) / PIECE;
   const long long pieces = (long long)a.features * a.row_pieces;
   // more pieces to a block where that leaves every multiprocessor its blocks
   const long long most = WRITE ? CH_PIECES_WRITE : CH_PIECES_READ;

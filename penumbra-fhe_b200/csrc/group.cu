@@ -37,8 +37,8 @@
 //     32 x 512->512                                                 195    230      82
 //     61 x 130->200, odd pitch                                95           138      50
 //     64 x 784->128, odd pitch                                      301    238     146
-// Measured: 256 x 784->128 655 us at its best (0.89 of the copy's rate) and 790-880 under the power cap,
-// where the SM clock falls to about 1.2 GHz; from 32 bits 421-460.  96 x 128->784 transposed 430-460 (its
+// Measured: 256 x 784->128 655 us at its best (0.89 of the copy's rate) and 790-925 under the power cap,
+// where the SM clock falls to about 1.2 GHz; from 32 bits 421-486.  96 x 128->784 transposed 430-460 (its
 // share of the floor, 219, is the lowest: the path above, 1000 cycles a tile).  45 x 257->384 from 24 bits
 // 96.  One request 784->128 9.2 us in a graph, 13.6 a call: the host's.
 #include <algorithm>
