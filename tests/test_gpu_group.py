@@ -352,9 +352,10 @@ def test_layers_over_a_cache_decrypt(pnb):
     keys.free()
 
 
-def test_on_another_stream_and_captured(pnb, oracle):
+@pytest.mark.parametrize("K,M", [(150, 140), (500, 140), (90, 500), (1000, 60)])
+def test_on_another_stream_and_captured(pnb, oracle, K, M):
     rng = np.random.default_rng(6)
-    B, K, M, L = 3, 150, 140, 2049
+    B, L = 3, 2049
     W = Weights(pnb, rng, M, K, 32)
     X = words(rng, B, K, L)
     slots = dev(np.array([2, 0, 1], np.int32))
@@ -396,11 +397,12 @@ def test_on_another_stream_and_captured(pnb, oracle):
         check_all(X)
 
 
-def test_two_host_threads(pnb, oracle):
+@pytest.mark.parametrize("K", [100, 500, 1000])
+def test_two_host_threads(pnb, oracle, K):
     import threading
     rng = np.random.default_rng(7)
-    W = [Weights(pnb, rng, 130, 100, 32) for _ in range(2)]
-    X = [words(rng, 2, 100, 300) for _ in range(2)]
+    W = [Weights(pnb, rng, 130, K, 32) for _ in range(2)]
+    X = [words(rng, 2, K, 300) for _ in range(2)]
     got = [[], []]
 
     def work(i):
@@ -447,6 +449,28 @@ def test_weights_at_any_address_and_other_types_of_words(pnb, oracle):
             C.c_void_p(x.data_ptr()), L, C.c_void_p(y.data_ptr()), L, 2, L, None, 0, None) == 0
         torch.cuda.synchronize()
         assert np.array_equal(host(y), want)
+
+
+def test_calls_one_after_the_other_in_one_workspace(pnb, oracle):
+    # the second call's weights are laid out only when the first is done with its own
+    import ctypes as C
+    rng = np.random.default_rng(13)
+    K, M, L = 700, 100, 2049
+    W = [Weights(pnb, rng, M, K, 64) for _ in range(2)]
+    X = words(rng, 4, K, L)
+    x = dev(X)
+    ws = torch.empty(2 * M * ((K + 15) & -16), dtype=torch.uint8, device="cuda")
+    y = [marked(4, M, L) for _ in range(2)]
+    at = lambda t: C.c_void_p(t.data_ptr())
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for w, out in zip(W, y):
+            assert pnb.lib().pnb_group_contract(
+                at(w.own.q), at(w.own.scales), at(w.own.zeros), 64, None, 0, M, K, 0, at(x), L,
+                at(out), L, 4, L, at(ws), ws.numel(), None) == 0
+    torch.cuda.synchronize()
+    for w, out in zip(W, y):
+        assert np.array_equal(host(out), oracle.contract(w.dense, None, 0, X))
 
 
 def test_refusals_on_the_device(pnb):
