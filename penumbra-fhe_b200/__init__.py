@@ -637,6 +637,7 @@ def lwe_contract_gather_ld(W: torch.Tensor, bias: torch.Tensor | None, delta: in
 # These calls may be a few microseconds of GPU work, so their host side is kept short: plain checks,
 # addresses as integers, and the device switched only when it is another one.
 _MAX_WORDS = 1 << 20  # PNB_MAX_REQUEST_WORDS
+_MAX_INT = (1 << 31) - 1  # the library's sizes; ctypes would pass what is left of a longer one
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -667,6 +668,8 @@ def _want_words(name: str, X, lwe_len, device, shape):
     lwe_len = ld if lwe_len is None else lwe_len
     if not 1 <= lwe_len <= ld:
         raise ValueError(f"lwe_len {lwe_len} does not fit rows of {ld} words")
+    if (n | features | ld) > _MAX_INT:
+        raise ValueError(f"{name} has shape {tuple(got)}, sizes are below 2^31")
     if features == shape[1] and (shape[0] is None or shape[0] == n) and X.device == device:
         return X if X.is_contiguous() else X.contiguous(), ld, lwe_len
     return _want(name, X, dtype, shape + (ld,), device), ld, lwe_len
@@ -859,7 +862,8 @@ class CiphertextCache:
                  data: torch.Tensor | None = None):
         if bits not in (16, 24, 32):
             raise ValueError(f"words of {bits} bits, expected 16, 24 or 32")
-        if slots < 1 or features < 1 or not 1 <= lwe_len <= _MAX_WORDS:
+        if (not 1 <= slots <= _MAX_INT or not 1 <= features <= _MAX_INT or
+                not 1 <= lwe_len <= _MAX_WORDS):
             raise ValueError(f"a cache of {slots} tokens of {features} ciphertexts of {lwe_len} "
                              f"words (1..{_MAX_WORDS})")
         self.slots, self.features, self.lwe_len, self.bits = slots, features, lwe_len, bits
@@ -877,7 +881,10 @@ class CiphertextCache:
     def _slots(self, slots: torch.Tensor, n=None) -> torch.Tensor:
         if not self.data.is_cuda:
             raise ValueError(f"the cache must be a CUDA tensor, it is on {self.device}")
-        return _want("slots", slots, torch.int32, (n,), self.device)
+        slots = _want("slots", slots, torch.int32, (n,), self.device)
+        if slots.shape[0] > _MAX_INT:
+            raise ValueError(f"{slots.shape[0]} slots, sizes are below 2^31")
+        return slots
 
 
 def cache_write(cache: CiphertextCache, X: torch.Tensor, slots: torch.Tensor) -> CiphertextCache:
@@ -922,7 +929,7 @@ class GroupWeights:
     """A matrix [M, K] of 4-bit weights with a scale and a zero point per ``group`` inputs:
     ``w[j, i] = scales[j, i // group] * (q[j, i] - zeros[j, i // group])``.  ``q`` is packed as
     ``pack_int4`` does, uint8 [M, ceil(K / 2)]; ``scales`` int8 and ``zeros`` uint8 (their low four
-    bits; None: 8) are [M, ceil(K / group)]."""
+    bits; None: 8) are [M, ceil(K / group)].  A group past K is one group of K."""
 
     def __init__(self, q: torch.Tensor, scales: torch.Tensor, group: int, K: int,
                  zeros: torch.Tensor | None = None):
@@ -930,6 +937,9 @@ class GroupWeights:
             raise ValueError(f"q must be [M, ceil(K / 2)] with K and group >= 1, got "
                              f"{tuple(q.shape)}, K={K}, group={group}")
         M = q.shape[0]
+        if (M | K) > _MAX_INT:
+            raise ValueError(f"weights [{M}, {K}], sizes are below 2^31")
+        group = min(group, K)
         self.M, self.K, self.group, self.device = M, K, group, q.device
         shape = (M, -(-K // group))
         self.q = _want("q", q, torch.uint8, (M, (K + 1) // 2), q.device)
@@ -1000,7 +1010,7 @@ def _pitch(cache: CiphertextCache, ld, out) -> int:
             raise ValueError(f"out has a pitch of {out.shape[2]} words, not {ld}")
         ld = out.shape[2]
     ld = cache.lwe_len if ld is None else ld
-    if ld < cache.lwe_len:
+    if not cache.lwe_len <= ld <= _MAX_INT:
         raise ValueError(f"ciphertexts of {cache.lwe_len} words do not fit a pitch of {ld}")
     return ld
 

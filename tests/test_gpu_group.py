@@ -451,6 +451,18 @@ def test_weights_at_any_address_and_other_types_of_words(pnb, oracle):
         assert np.array_equal(host(y), want)
 
 
+@pytest.mark.parametrize("group", [41, (1 << 32) + 16, 1 << 40])
+def test_a_group_past_the_inputs_is_one_group(pnb, oracle, group):
+    rng = np.random.default_rng(14)
+    W = Weights(pnb, rng, 20, 40, 40)
+    wide = pnb.GroupWeights(W.own.q, W.own.scales, group, 40, W.own.zeros)
+    X, G = words(rng, 2, 40, 30), words(rng, 2, 20, 30)
+    assert np.array_equal(host(pnb.group_contract(wide, None, 0, dev(X))),
+                          oracle.contract(W.dense, None, 0, X))
+    assert np.array_equal(host(pnb.group_contract(wide, None, 0, dev(G), transposed=True)),
+                          oracle.contract(np.ascontiguousarray(W.dense.T), None, 0, G))
+
+
 def test_calls_one_after_the_other_in_one_workspace(pnb, oracle):
     # the second call's weights are laid out only when the first is done with its own
     import ctypes as C

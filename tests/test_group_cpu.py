@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -144,3 +145,33 @@ def test_binding_refuses(pnb):
         pnb.group_contract_cached(W, None, 0, pnb.CiphertextCache(2, 4, 10, device="cpu"), slots)
     with pytest.raises(TypeError, match="64-bit"):
         pnb.group_contract(W, None, 0, X.to(torch.int32))
+
+
+def test_sizes_past_32_bits_are_not_cut_short(pnb):
+    # ctypes passes the low 32 bits of a longer integer, which the library cannot tell from a size
+    long = 1 << 32
+    q = torch.zeros(3, 3, dtype=torch.uint8)
+    scales = torch.zeros(3, 1, dtype=torch.int8)
+    for group in (5, 6, long, long + 4):  # one group of all K
+        assert pnb.GroupWeights(q, scales, group, 5).group == 5
+    meta = dict(device="meta")
+    for M, K in ((1, long + 8), (1, 1 << 31), (long + 8, 1)):
+        shape = (M, (K + 1) // 2)
+        with pytest.raises(ValueError, match="below 2"):
+            pnb.GroupWeights(torch.empty(shape, dtype=torch.uint8, **meta),
+                             torch.empty(M, 1, dtype=torch.int8, **meta), K, K)
+    for size in ((long + 2, 1), (1 << 31, 1), (1, long + 2)):
+        with pytest.raises(ValueError, match="a cache of"):
+            pnb.CiphertextCache(*size, 1, **meta)
+    cache = pnb.CiphertextCache(2, 1, 3, device="cpu")
+    for ld in (long + 3, 1 << 31):
+        with pytest.raises(ValueError, match="do not fit a pitch"):
+            pnb._pitch(cache, ld, None)
+    for n, features, ld in ((long + 2, 1, 3), (2, long + 1, 3), (2, 1, long + 3), (2, 1, 1 << 31)):
+        X = SimpleNamespace(dtype=torch.int64, shape=(n, features, ld), is_cuda=True, device=None,
+                            is_contiguous=lambda: True)
+        with pytest.raises(ValueError, match="below 2"):
+            pnb._want_words("X", X, 3, None, (None, features))
+    held = SimpleNamespace(data=SimpleNamespace(is_cuda=True), device=torch.device("meta"))
+    with pytest.raises(ValueError, match="below 2"):
+        pnb.CiphertextCache._slots(held, torch.empty(long + 2, dtype=torch.int32, **meta))
