@@ -317,6 +317,11 @@ int pnb_cache_write(const int32_t* slots_dev, int tokens, const uint64_t* X_dev,
  * whose slot is outside [0, cache_slots) are left as they were. */
 int pnb_cache_read(const int32_t* slots_dev, int tokens, const void* cache_dev, int cache_slots,
                    int bits, int features, uint64_t* out_dev, int ldo, int lwe_len, void* stream);
+/* Sets row t of out [rows][words] to zero where index[t] is outside [0, limit): the rows that the
+ * calls here and above leave as they were (index: their slots, or a route's row_choice), in a buffer
+ * that holds something else, another client's ciphertexts perhaps. */
+int pnb_zero_skipped(const int32_t* index_dev, int rows, int limit, uint64_t* out_dev, size_t words,
+                     void* stream);
 /* A projection with 4-bit weights, a scale and a zero point per group of `group` inputs:
  *   w[j][i] = scales[j][i/group] * (q[j][i] - zeros[j][i/group]),
  *   Y[b][j] = sum_i w[j][i] X[b][i] (+ bias[j] * delta on the body).

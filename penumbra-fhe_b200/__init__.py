@@ -126,6 +126,8 @@ _SIGS = {
                                   C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "pnb_cache_read": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                  C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "pnb_zero_skipped": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_size_t,
+                                   C.c_void_p]),
     "pnb_group_contract": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
                                      C.c_uint64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int,
                                      C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p,
@@ -675,12 +677,19 @@ def _want_words(name: str, X, lwe_len, device, shape):
     return _want(name, X, dtype, shape + (ld,), device), ld, lwe_len
 
 
-def _want_out(out, shape, device, lwe_len: int, X: torch.Tensor) -> torch.Tensor:
+def _want_out(out, shape, device, lwe_len: int, X: torch.Tensor,
+              index: torch.Tensor | None = None, limit: int = 0) -> torch.Tensor:
     """The caller's buffer, checked and apart from the input ``X``, or a new one: zeros where the
-    call leaves words behind ``lwe_len``."""
+    call leaves words behind ``lwe_len`` or skips rows, those whose ``index`` is outside [0, limit).
+    (Such rows would otherwise hand out what the memory held, another client's ciphertexts perhaps.)"""
     if out is None:
-        make = torch.empty if shape[-1] == lwe_len else torch.zeros
-        return make(shape, dtype=torch.int64, device=device)
+        if shape[-1] != lwe_len:
+            return torch.zeros(shape, dtype=torch.int64, device=device)
+        out = torch.empty(shape, dtype=torch.int64, device=device)
+        if index is not None:
+            _launch("pnb_zero_skipped", device, index.data_ptr(), shape[0], limit, out.data_ptr(),
+                    shape[1] * shape[2])
+        return out
     if out.dtype is not torch.int64 and out.dtype is not torch.uint64:
         raise TypeError(f"expected a 64-bit tensor, got {out.dtype}")
     if out.shape != shape or out.device != device or not out.is_contiguous():
@@ -770,11 +779,11 @@ def expert_dispatch(route: ExpertRoute, X: torch.Tensor, lwe_len: int | None = N
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """The tokens' ciphertexts ``X`` [tokens, features, ld] in row order, each times its choice's
     weight (int32 [tokens, top_k], None = 1): [tokens*top_k, features, ld].  Rows without a choice
-    are left as they were (not set when ``out`` is made here), as are words behind ``lwe_len``."""
+    are left as they were (zeros when ``out`` is made here), as are words behind ``lwe_len``."""
     X, ld, L = _want_words("X", X, lwe_len, route.device, (route.tokens, None))
     F = X.shape[1]
     w = _route_weights(route, weights)
-    out = _want_out(out, (route.rows, F, ld), route.device, L, X)
+    out = _want_out(out, (route.rows, F, ld), route.device, L, X, route.row_choice, route.rows)
     _launch("pnb_expert_dispatch", route.device, route.choice_row.data_ptr(), route.tokens,
             route.top_k, _at(w), X.data_ptr(), F, ld, out.data_ptr(), ld, L)
     return out
@@ -802,7 +811,7 @@ def expert_contract(route: ExpertRoute, W: torch.Tensor, bias: torch.Tensor | No
     [experts, M] or None (times ``delta``, on the body).  ``X`` holds the tokens [tokens, K, ld]
     (no dispatch needed), or with ``sorted_rows`` the rows [tokens*top_k, K, ld] of an earlier
     call.  The result is [tokens*top_k, M, ld] in row order; rows without a choice are left as they
-    were (not set when ``out`` is made here), as are words behind ``lwe_len``."""
+    were (zeros when ``out`` is made here), as are words behind ``lwe_len``."""
     if W.dim() != 3:
         raise ValueError(f"W must be [experts, M, K], got {tuple(W.shape)}")
     device = route.device
@@ -811,7 +820,7 @@ def expert_contract(route: ExpertRoute, W: torch.Tensor, bias: torch.Tensor | No
                            (route.rows if sorted_rows else route.tokens, K))
     W = _want("W", W, torch.int8, (route.experts, M, K), device)
     b = None if bias is None else _want("bias", bias, torch.int64, (E, M), device)
-    out = _want_out(out, (route.rows, M, ld), device, L, X)
+    out = _want_out(out, (route.rows, M, ld), device, L, X, route.row_choice, route.rows)
     need = _padded(W, E * M, K)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _launch("pnb_expert_contract", device, route.row_choice.data_ptr(),
@@ -904,11 +913,12 @@ def cache_write(cache: CiphertextCache, X: torch.Tensor, slots: torch.Tensor) ->
 def cache_read(cache: CiphertextCache, slots: torch.Tensor, ld: int | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
     """The ciphertexts of ``slots`` (int32 [tokens]) as u64 words [tokens, features, ld] (ld: out's, or
-    the cache's ``lwe_len``).  Tokens whose slot is outside the cache are left as they were (not set
+    the cache's ``lwe_len``).  Tokens whose slot is outside the cache are left as they were (zeros
     when ``out`` is made here), as are words behind ``lwe_len``."""
     slots = cache._slots(slots)
     n, ld = slots.shape[0], _pitch(cache, ld, out)
-    out = _want_out(out, (n, cache.features, ld), cache.device, cache.lwe_len, cache.data)
+    out = _want_out(out, (n, cache.features, ld), cache.device, cache.lwe_len, cache.data,
+                    slots, cache.slots)
     _launch("pnb_cache_read", cache.device, slots.data_ptr(), n, cache.data.data_ptr(), cache.slots,
             cache.bits, cache.features, out.data_ptr(), ld, cache.lwe_len)
     return out
@@ -976,7 +986,7 @@ def group_contract_cached(W: GroupWeights, bias: torch.Tensor | None, delta: int
                           out: torch.Tensor | None = None) -> torch.Tensor:
     """``group_contract`` of the ciphertexts in ``slots`` (int32 [batch]) of a cache with K features,
     read as they lie there: [batch, M, ld] (ld: out's, or the cache's ``lwe_len``).  Requests whose
-    slot is outside the cache are left as they were (not set when ``out`` is made here), as are words
+    slot is outside the cache are left as they were (zeros when ``out`` is made here), as are words
     behind ``lwe_len``."""
     device = cache.device
     if W.K != cache.features:
@@ -987,7 +997,8 @@ def group_contract_cached(W: GroupWeights, bias: torch.Tensor | None, delta: int
     slots = cache._slots(slots)
     batch, ld = slots.shape[0], _pitch(cache, ld, out)
     b = None if bias is None else _want("bias", bias, torch.int64, (W.M,), device)
-    out = _want_out(out, (batch, W.M, ld), device, cache.lwe_len, cache.data)
+    out = _want_out(out, (batch, W.M, ld), device, cache.lwe_len, cache.data, slots,
+                    cache.slots)
     need = W._bytes[0]
     ws = W.q.new_empty(need) if need else None
     _launch("pnb_group_contract_cached", device, W.q.data_ptr(), W.scales.data_ptr(), _at(W.zeros),

@@ -220,4 +220,32 @@ int cache_read(const int32_t* slots, int tokens, const void* cache, int n_slots,
   return cache_launch<false>(a, bits, st);
 }
 
+// ---- rows without a place -----------------------------------------------------------------------
+// Rows whose index is outside [0, limit) become zero: the others' blocks only look.  Of 512 rows of 2 MB
+// none takes 4 us, 26 (54 MB) 29 and all 174, where filling the buffer before every call takes 157.
+constexpr int ZS_THREADS = 256;
+
+__global__ void __launch_bounds__(ZS_THREADS)
+    zero_skipped_kernel(const int32_t* index, int rows, int limit, unsigned long long* out,
+                        size_t words) {
+  for (int t = blockIdx.y; t < rows; t += gridDim.y) {
+    const int i = __ldg(index + t);
+    if (i >= 0 && i < limit) continue;
+    unsigned long long* row = out + (size_t)t * words;
+    for (size_t c = (size_t)blockIdx.x * ZS_THREADS + threadIdx.x; c < words;
+         c += (size_t)gridDim.x * ZS_THREADS)
+      row[c] = 0;
+  }
+}
+
+int zero_skipped(const int32_t* index, int rows, int limit, uint64_t* out, size_t words,
+                 cudaStream_t st) {
+  // blocks for every multiprocessor, of eight words a thread at least
+  const size_t most = std::max(1, 16 * 148 / rows), all = words / (8 * ZS_THREADS) + 1;
+  const dim3 grid((unsigned)std::min(most, all), (unsigned)std::min(65535, rows));
+  zero_skipped_kernel<<<grid, ZS_THREADS, 0, st>>>(index, rows, limit, (unsigned long long*)out, words);
+  PNB_CHECK_LAUNCH("zero_skipped_kernel");
+  return PNB_OK;
+}
+
 }  // namespace pnb

@@ -690,6 +690,22 @@ int pnb_cache_read(const int32_t* slots_dev, int tokens, const void* cache_dev, 
                     lwe_len, (cudaStream_t)stream);
 }
 
+int pnb_zero_skipped(const int32_t* index_dev, int rows, int limit, uint64_t* out_dev, size_t words,
+                     void* stream) {
+  if (rows < 0 || limit < 0) {
+    set_error("zero_skipped: bad shape rows=%d limit=%d", rows, limit);
+    return PNB_ERR_INVALID;
+  }
+  if (rows == 0 || words == 0) return PNB_OK;
+  if (!index_dev || !out_dev) {
+    set_error("zero_skipped: NULL buffer");
+    return PNB_ERR_INVALID;
+  }
+  const int rc = check_aligned("zero_skipped", {out_dev}, {index_dev});
+  if (rc) return rc;
+  return zero_skipped(index_dev, rows, limit, out_dev, words, (cudaStream_t)stream);
+}
+
 static int check_group(const char* fn, int M, int K, bool transposed, int group, int batch) {
   const int n_in = transposed ? M : K, n_out = transposed ? K : M;
   if (n_in < 1 || n_in > PNB_MAX_GROUP_INPUTS || n_out < 1 || n_out > PNB_MAX_REQUEST_ROWS) {

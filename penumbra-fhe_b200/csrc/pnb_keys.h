@@ -98,6 +98,9 @@ int cache_write(const int32_t* slots, int tokens, const uint64_t* X, int feature
                 void* cache, int n_slots, int bits, cudaStream_t st);
 int cache_read(const int32_t* slots, int tokens, const void* cache, int n_slots, int bits,
                int features, uint64_t* out, int ldo, int L, cudaStream_t st);
+// Rows whose index is outside [0, limit) to zero (cache.cu).
+int zero_skipped(const int32_t* index, int rows, int limit, uint64_t* out, size_t words,
+                 cudaStream_t st);
 size_t group_workspace_bytes(int n_in, int n_out);
 int group_contract(const uint8_t* W, const int8_t* scales, const uint8_t* zeros, int group,
                    const int64_t* bias, uint64_t delta, int M, int K, bool transposed,

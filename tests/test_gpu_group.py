@@ -136,6 +136,48 @@ def test_the_last_of_many_tokens_with_one_slot_stays(pnb):
         assert np.array_equal(cache.data.cpu().numpy()[:, :, :70 * bits // 8], want)
 
 
+@pytest.mark.parametrize("rows,words", [(1, 1), (1, 5_000_001), (3, 2047), (2368, 2048),
+                                        (3000, 2050), (70_000, 3)])
+def test_zero_skipped(pnb, rows, words):
+    rng = np.random.default_rng(rows + words)
+    index = rng.integers(-1, 7, rows).astype(np.int32)
+    index[0], index[-1] = -2147483648, 2147483647
+    out = marked(rows + 1, words)  # (the last row is nobody's)
+    i = dev(index)
+    torch.cuda.synchronize()
+    assert pnb.lib().pnb_zero_skipped(i.data_ptr(), rows, 5, out.data_ptr(), words, None) == 0
+    torch.cuda.synchronize()
+    want = marked(rows + 1, words)
+    want[:rows][(i < 0) | (i >= 5)] = 0
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("ld", [64, 65])
+def test_results_made_here_hold_zeros_where_a_token_is_skipped(pnb, ld):
+    rng = np.random.default_rng(15)
+    F, L = 8, 64
+    cache = pnb.CiphertextCache(4, F, L, 32)
+    cache.data.copy_(torch.tensor(rng.integers(0, 256, cache.data.shape, dtype=np.uint8)))
+    slots = dev(np.array([1, -1, 2, 9], np.int32))
+    W = Weights(pnb, rng, F, F, F)
+    route = pnb.expert_route(dev(np.array([[0], [-1], [1], [-1]], np.int32)), 2)
+    X = dev(words(rng, 4, F, ld))
+    We = torch.ones(2, F, F, dtype=torch.int8, device="cuda")
+    for skipped, call in [
+            ([1, 3], lambda **o: pnb.cache_read(cache, slots, ld=ld, **o)),
+            ([1, 3], lambda **o: pnb.group_contract_cached(W.own, None, 0, cache, slots, ld=ld, **o)),
+            ([2, 3], lambda **o: pnb.expert_dispatch(route, X, L, **o)),
+            ([2, 3], lambda **o: pnb.expert_contract(route, We, None, 0, X, L, **o))]:
+        want = marked(4, F, ld)
+        call(out=want)
+        assert bool((want[skipped] == MARK).all())
+        want[skipped] = 0
+        want[..., L:] = 0
+        used = marked(4, F, ld)  # memory that the next buffer of its size gets
+        del used
+        assert torch.equal(call(), want)
+
+
 def test_most_tokens(pnb):
     T = 65536
     X = torch.arange(T, device="cuda").view(T, 1, 1) << 40

@@ -72,8 +72,18 @@ def test_group_contract_cached_refuses(pnb, change, text):
     _refused(pnb, "pnb_group_contract_cached", CACHED, change, text)
 
 
+@pytest.mark.parametrize("change,text", [
+    ({1: -1}, b"rows=-1"), ({2: -1}, b"limit=-1"), ({0: NUL}, b"NULL"), ({3: NUL}, b"NULL"),
+    ({0: ODD2}, b"32-bit integers"), ({3: ODD4}, b"64-bit words"),
+])
+def test_zero_skipped_refuses(pnb, change, text):
+    _refused(pnb, "pnb_zero_skipped", [P, 4, 8, P, 10, NUL], change, text)
+
+
 def test_empty_batches_run_nothing(pnb):
     L = pnb.lib()
+    assert L.pnb_zero_skipped(NUL, 0, 8, NUL, 10, NUL) == 0
+    assert L.pnb_zero_skipped(NUL, 4, 8, NUL, 0, NUL) == 0
     assert L.pnb_cache_write(NUL, 0, NUL, 3, 10, 10, NUL, 8, 32, NUL) == 0
     assert L.pnb_cache_read(NUL, 0, NUL, 8, 32, 3, NUL, 10, 10, NUL) == 0
     assert L.pnb_group_contract(NUL, NUL, NUL, 16, NUL, 1, 3, 5, 0, NUL, 10, NUL, 10, 0, 10, NUL, 0,
