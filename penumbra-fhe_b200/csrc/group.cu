@@ -861,26 +861,32 @@ __global__ void __launch_bounds__(GcShape<BYTES, SHIFTED, MODE>::THREADS, 1)
 }
 
 // ---- launch -------------------------------------------------------------------------------------
+// Multiprocessors of the current device.
+static int gc_sms(int* sms) {
+  static std::atomic<int> count[64];
+  int dev = 0;
+  PNB_CUDA(cudaGetDevice(&dev));
+  *sms = dev < 64 ? count[dev].load(std::memory_order_relaxed) : 0;
+  if (*sms) return PNB_OK;
+  PNB_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64) count[dev].store(*sms, std::memory_order_relaxed);
+  return PNB_OK;
+}
+
 template <int BYTES, bool SHIFTED, GcMode MODE>
-static int gc_launch(GcArgs& a, int8_t* ws, cudaStream_t st) {
+static int gc_launch(GcArgs& a, int sms, int8_t* ws, cudaStream_t st) {
   using S = GcShape<BYTES, SHIFTED, MODE>;
   const GroupArgs& g = a.g;
   const char* name = g.slots ? "group_contract_cached" : "group_contract";
-  static std::atomic<int> sm_count[64];  // per device, once the kernel's shared-memory limit is raised
+  static std::atomic<bool> raised[64];  // per device: the kernel's shared-memory limit
   auto kernel = group_kernel<BYTES, SHIFTED, MODE>;
   int dev = 0;
   PNB_CUDA(cudaGetDevice(&dev));
-  int sms = dev < 64 ? sm_count[dev].load(std::memory_order_acquire) : 0;
-  if (sms == 0) {
-    PNB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  if (dev >= 64 || !raised[dev].load(std::memory_order_acquire)) {
     PNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GC_SMEM));
-    if (dev < 64) sm_count[dev].store(sms, std::memory_order_release);
+    if (dev < 64) raised[dev].store(true, std::memory_order_release);
   }
   const unsigned grid = gc_plan<BYTES, SHIFTED, MODE>(a, g.n_in, g.n_out, g.L, g.batch, sms);
-  if (grid == 0 || a.x_slots < 2 || (SHIFTED && a.raw_slots < GC_COPY_WARPS)) {
-    set_error("%s: no plan for %d inputs and %d outputs", name, g.n_in, g.n_out);
-    return PNB_ERR_INVALID;
-  }
   GcMaps tm{};
   int rc = PNB_OK;
   if (!SHIFTED) {
@@ -971,11 +977,13 @@ static int gc_launch(GcArgs& a, int8_t* ws, cudaStream_t st) {
 
 template <int BYTES, bool SHIFTED>
 static int gc_run(GcArgs& a, int8_t* ws, cudaStream_t st) {
-  switch (gc_mode(a.g.n_in, a.g.n_out)) {
-    case LONG: return gc_launch<BYTES, SHIFTED, LONG>(a, ws, st);
-    case SHORT: return gc_launch<BYTES, SHIFTED, SHORT>(a, ws, st);
-    // (copying shifted rows costs a pair more than it saves: 64 x 784->128 301 us, LONG 238)
-    default: return gc_launch<BYTES, SHIFTED, SHIFTED ? LONG : PAIR>(a, ws, st);
+  int sms = 0;
+  const int rc = gc_sms(&sms);
+  if (rc) return rc;
+  switch (gc_mode(a.g.n_in, a.g.n_out, SHIFTED, sms)) {
+    case LONG: return gc_launch<BYTES, SHIFTED, LONG>(a, sms, ws, st);
+    case SHORT: return gc_launch<BYTES, SHIFTED, SHORT>(a, sms, ws, st);
+    default: return gc_launch<BYTES, SHIFTED, SHIFTED ? LONG : PAIR>(a, sms, ws, st);
   }
 }
 

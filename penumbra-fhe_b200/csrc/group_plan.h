@@ -12,10 +12,10 @@ constexpr int GC_W_HALF = 128 * GC_WK;  // 16 KB: 128 rows of weights
 constexpr int GC_X_SLOT = 16 * 1024;
 constexpr int GC_COPY_WARPS = 4;
 constexpr int GC_EPI_WARPS = 16;  // two groups of two per TMEM lane quarter
-// Which way a call goes, by the layer's size alone (the caller's workspace depends on it).
+// Which way a call goes, by the layer's size.  (The caller's workspace is the same for all.)
 constexpr int GC_SHORT = 384;      // most inputs for SHORT,
 constexpr int GC_STAYS = 896;      // and for PAIR, whose weights leave X six slots
-constexpr int GC_MOST_TILES = 37;  // of outputs: a quarter of the machine
+constexpr int GC_MOST_TILES = 37;  // of outputs: a quarter of 148 multiprocessors
 constexpr int GC_MAX_W = 8, GC_MAX_X = 12, GC_MAX_RAW = 16;
 constexpr int GC_BARS = 2 * (GC_MAX_W + GC_MAX_X + GC_MAX_RAW) + 4;
 constexpr int GC_BAR_BYTES = (8 * GC_BARS + 8 + 127) / 128 * 128;
@@ -67,9 +67,12 @@ struct GcPlan {
   int x_at, raw_at, out_at, bars_at;  // shared-memory offsets; weights at 0
 };
 
-inline GcMode gc_mode(int n_in, int n_out) {
+inline GcMode gc_mode(int n_in, int n_out, bool shifted, int sms) {
   if (n_in > GC_STAYS || n_out > GC_MOST_TILES * GC_BM) return LONG;
-  return n_in <= GC_SHORT ? SHORT : PAIR;
+  const int m_tiles = (n_out + GC_BM - 1) / GC_BM;  // each wants a block or a pair of its own
+  if (n_in <= GC_SHORT) return m_tiles <= sms ? SHORT : LONG;
+  // (copying shifted rows costs a pair more than it saves: 64 x 784->128 301 us, LONG 238)
+  return !shifted && m_tiles <= sms / 2 ? PAIR : LONG;
 }
 // One slot of weights for one tile of outputs is expanded by every block for itself, which saves a launch;
 // more by a kernel before.
@@ -105,7 +108,6 @@ unsigned gc_plan(GcPlan& a, int n_in, int n_out, int L, int batch, int sms) {
     if (a.m_tiles * a.w_tile <= room - x_want && a.m_tiles * kb <= GC_MAX_W && x_tiles >= 4 * sms)
       a.m_group = a.m_tiles;
     grid = (unsigned)std::min<long long>(sms, x_tiles * (a.m_tiles / a.m_group));
-    if (grid < (unsigned)a.m_tiles) grid = 0;  // (a machine with fewer multiprocessors than that)
     a.w_slots = a.m_group * kb;
   }
   room -= a.m_group * a.w_tile;
