@@ -362,6 +362,103 @@ def test_every_alignment_through_the_c_abi(pnb, oracle, off_x, off_y, ldx, ldy, 
     assert np.all(np.delete(got, np.s_[off_y:off_y + want.size]) == MARK)
 
 
+# Pairs of blocks (385 to 896 inputs, an even pitch) with 5 to 40 tiles a pair: the second accumulator, its
+# hand-back across the blocks, and the inputs' slots from tile to tile.
+PAIRED = [(12, 500, 140), (9, 385, 300), (10, 896, 128), (5, 784, 1000)]
+
+
+@pytest.mark.parametrize("ldy", [2050, 2049])
+@pytest.mark.parametrize("B,K,M", PAIRED)
+def test_many_tiles_of_a_pair(pnb, oracle, B, K, M, ldy):
+    import ctypes as C
+    rng = np.random.default_rng(B + K + M)
+    L, ldx = 2049, 2050
+    W = Weights(pnb, rng, M, K, 64)
+    X = words(rng, B, K, ldx)
+    bias = rng.integers(-1000, 1000, M)
+    x, y, b = dev(X), marked(B, M, ldy), dev(bias)
+    at = lambda t: C.c_void_p(t.data_ptr())
+    torch.cuda.synchronize()
+    assert pnb.lib().pnb_group_contract(
+        at(W.own.q), at(W.own.scales), at(W.own.zeros), 64, at(b), 1 << 45, M, K, 0, at(x), ldx, at(y),
+        ldy, B, L, None, 0, None) == 0
+    torch.cuda.synchronize()
+    want = np.full((B, M, ldy), MARK, np.uint64)
+    want[:, :, :L] = oracle.contract(W.dense, bias, 1 << 45, np.ascontiguousarray(X[:, :, :L]))
+    assert np.array_equal(host(y), want)
+    # and transposed, from as many inputs
+    T = Weights(pnb, rng, K, M, 64)
+    check(pnb, oracle, T, X, L, ldx, rng, transposed=True)
+
+
+@pytest.mark.parametrize("bits", [16, 24, 32])
+@pytest.mark.parametrize("B,K,M", PAIRED)
+@pytest.mark.parametrize("ld", [2050, 2049])
+def test_many_tiles_of_a_pair_over_a_cache(pnb, oracle, B, K, M, bits, ld):
+    rng = np.random.default_rng(B + K + M + bits)
+    B, L = 3 * B, 2049
+    W = Weights(pnb, rng, M, K, 48)
+    cache = pnb.CiphertextCache(2 * B, K, L, bits)
+    cache.data.copy_(torch.randint(0, 256, cache.data.shape, dtype=torch.uint8,
+                                   generator=torch.Generator().manual_seed(bits)))
+    slots = rng.permutation(2 * B)[:B].astype(np.int32)
+    slots[1::4] = -1
+    slots[2::8] = 2 * B
+    bias = rng.integers(-1000, 1000, M)
+    got = marked(B, M, ld)
+    pnb.group_contract_cached(W.own, dev(bias), 3, cache, dev(slots), out=got)
+    used = np.flatnonzero((slots >= 0) & (slots < 2 * B))
+    x = as_words(cache.data[slots[used].astype(np.int64)].cpu().numpy(), L, bits)
+    want = np.full((B, M, ld), MARK, np.uint64)
+    want[used, :, :L] = oracle.contract(W.dense, bias, 3, x)
+    assert np.array_equal(host(got), want)
+    assert pnb.device_status(0) == 0
+
+
+def test_pairs_captured_and_in_one_workspace(pnb, oracle):
+    import ctypes as C
+    rng = np.random.default_rng(16)
+    B, K, M, L, ld = 6, 700, 140, 2049, 2050
+    W = [Weights(pnb, rng, M, K, 64) for _ in range(2)]
+    X = words(rng, B, K, ld)
+    x = dev(X)
+    y = [marked(B, M, ld) for _ in range(2)]
+    at = lambda t: C.c_void_p(t.data_ptr())
+
+    def wanted(X):
+        want = np.full((2, B, M, ld), MARK, np.uint64)
+        for i in range(2):
+            want[i, :, :, :L] = oracle.contract(W[i].dense, None, 0, np.ascontiguousarray(X[:, :, :L]))
+        return want
+
+    # one call after the other in one workspace
+    ws = torch.empty(2 * M * ((K + 15) & -16), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for w, out in zip(W, y):
+            assert pnb.lib().pnb_group_contract(
+                at(w.own.q), at(w.own.scales), at(w.own.zeros), 64, None, 0, M, K, 0, at(x), ld,
+                at(out), ld, B, L, at(ws), ws.numel(), None) == 0
+    torch.cuda.synchronize()
+    assert np.array_equal(np.stack([host(t) for t in y]), wanted(X))
+    # two graphs of a call each, replayed in turn with new inputs
+    graphs = []
+    for w, out in zip(W, y):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            pnb.group_contract(w.own, None, 0, x, L, out=out)
+    for _ in range(3):
+        X = words(rng, B, K, ld)
+        x.copy_(dev(X))
+        for t in y:
+            t.fill_(MARK)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(np.stack([host(t) for t in y]), wanted(X))
+    assert pnb.device_status(0) == 0
+
+
 # ---- together, as a server uses them ------------------------------------------------------------
 def test_layers_over_a_cache_decrypt(pnb):
     # two requests' encrypted inputs are kept in 32 bits, go through a 4-bit layer from the cache and
