@@ -10,7 +10,8 @@
 //
 // Both move each byte once, which HBM bounds: 512 tokens of 128 ciphertexts of 2049 words, one in twenty
 // unused, are written in 24 bits at an odd pitch in 239-250 us (floor 203; the look for later tokens of a
-// slot is part of the rest) and read from 32 bits in 242 (floor 234).
+// slot is part of the rest) and read from 32 bits in 242 (floor 234).  That look grows with the square of the
+// tokens: one ciphertext each of 4096 tokens takes 25 us (floor 14), of 16384 123 (56), of 65536 1481 (226).
 //
 // A row of the cache is L little-endian words of n / 8 bytes (n = 16, 24, 32), padded to a multiple of
 // 16 bytes: the bytes of a word are the limbs that the tensor-core contraction multiplies, so it
@@ -46,7 +47,8 @@ struct CacheArgs {
 // of its addresses but a constant step changes on the way (with runs that go on from row to row, whose
 // lanes each find their own row, the instructions bound these kernels).  Lanes take neighbouring pairs of
 // words, 16 aligned bytes at a time: where the row starts off by one word, the words before and of an even
-// column, and the lane before or behind has the other half of a pair.
+// column, and the lane before or behind has the other half of a pair.  (So the eight bytes before such a row
+// are read, inside the 16 that its first word is in, and dropped; they are never written.)
 //
 // Words of three bytes go in groups of eight: lane k of the group's four has b_k, its pair's six bytes, and
 // for k < 3 moves eight of the 24 bytes, s_k = b_k >> 16k | b_(k+1) << (48 - 16k).

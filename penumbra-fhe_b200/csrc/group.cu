@@ -22,25 +22,32 @@
 // path from the end of a tile's MMAs to the next ones into the same accumulator (a commit, a wait, two
 // loads of columns, the limb sums, an arrival, a wait), about 2000 cycles.  So there are three forms:
 //
-//   LONG (over 896 inputs, over 4736 outputs, odd pitches over 384): tiles of 128 outputs x 32 words (of
-//     8 bytes), lo and hi in 256 columns each; weights stream from L2.
+//   LONG (over 896 inputs, over 4736 outputs, odd pitches over 384, more tiles of outputs than the device
+//     has blocks or pairs for): tiles of 128 outputs x 32 words (of 8 bytes), lo and hi in 256 columns each;
+//     weights stream from L2.
 //   SHORT (up to 384 inputs): tiles of 128 x 16, lo and hi in 128 columns each, twice, so that the
 //     epilogue of a tile runs beside the MMAs of the next; weights stay in shared memory.
 //   PAIR (between): a pair of blocks shares a tile of 128 x 32 by MMAs of M = 256 (cta_group::2), each with
 //     half of X and half of the weights, which stay.  Lo and hi are neighbouring rows, so that either block
 //     can finish its half of the outputs; the lanes exchange words, which makes the epilogue dearer.
 //
-// Sustained, us (rows of 2049 words):                      SHORT   PAIR   LONG   floor
-//     64 x 300->300                                          210    250    270      96
-//     64 x 400->128                                                 107    148      85
-//     64 x 784->128                                                 177    208     146
-//     32 x 512->512                                                 195    230      82
-//     61 x 130->200, odd pitch                                95           138      50
-//     64 x 784->128, odd pitch                                      301    238     146
-// Measured: 256 x 784->128 655 us at its best (0.89 of the copy's rate) and 790-925 under the power cap,
-// where the SM clock falls to about 1.2 GHz; from 32 bits 421-486.  96 x 128->784 transposed 430-460 (its
-// share of the floor, 219, is the lowest: the path above, 1000 cycles a tile).  45 x 257->384 from 24 bits
-// 96.  One request 784->128 9.2 us in a graph, 13.6 a call: the host's.
+// Each form made to take the layers of the others, us, calls one after the other under the power cap (rows of
+// 2049 random words), and the floors by bytes and by MMAs:
+//                                                          SHORT   PAIR   LONG   bytes   MMAs
+//     64 x 300->300                                          241    258    286      96    115
+//     64 x 400->128                                                 128    175      85     65
+//     64 x 784->128                                                 216    255     146    128
+//     32 x 512->512                                                 238    263      82    167
+//     61 x 130->200                                           99    125    176      50     32
+//     61 x 130->200, odd pitch                               111           182      50     32
+//     64 x 784->128, odd pitch (a pair that copied: 301 where LONG took 238)
+//                                                                          272     146    128
+// Measured: 256 x 784->128 670 us as a call of its own (0.87 of the copy's rate), 790-925 one after the
+// other, where the power cap takes the SM clock to about 1.2 GHz; from 32 bits 370 and 420-486, from 16 250.
+// 96 x 128->784 transposed 414-472 (its share of the floor, 219, is the lowest of the batches: the path
+// above, 1000 cycles a tile).  45 x 257->384 from 24 bits 97-110.  One request 784->128 9.2 us in a graph,
+// 13.6 a call: the host's.
+// Layers of few outputs pay for 128 rows: 256 x 64->10 119 us (floor 47), 128->10 137 (89).
 #include <algorithm>
 #include <atomic>
 

@@ -71,7 +71,7 @@ inline GcMode gc_mode(int n_in, int n_out, bool shifted, int sms) {
   if (n_in > GC_STAYS || n_out > GC_MOST_TILES * GC_BM) return LONG;
   const int m_tiles = (n_out + GC_BM - 1) / GC_BM;  // each wants a block or a pair of its own
   if (n_in <= GC_SHORT) return m_tiles <= sms ? SHORT : LONG;
-  // (copying shifted rows costs a pair more than it saves: 64 x 784->128 301 us, LONG 238)
+  // (copying shifted rows costs a pair more than it saves: 64 x 784->128 301 us where LONG took 238)
   return !shifted && m_tiles <= sms / 2 ? PAIR : LONG;
 }
 // One slot of weights for one tile of outputs is expanded by every block for itself, which saves a launch;
@@ -92,7 +92,9 @@ unsigned gc_plan(GcPlan& a, int n_in, int n_out, int L, int batch, int sms) {
   const int kb = (n_in + GC_WK - 1) / GC_WK, kx = (n_in + S::XK - 1) / S::XK;
   unsigned grid =
       (unsigned)std::min<long long>((long long)batch * a.n_tiles * a.m_tiles, sms / per);
-  if (MODE == PAIR) grid = grid / a.m_tiles * a.m_tiles;  // a block's tiles have the same outputs
+  // A block's tiles have the same outputs.  (At some numbers of tiles pairs are left over: 16 x 512->3200
+  // takes 50 of 74 and 811 us, its MMAs 523.)
+  if (MODE == PAIR) grid = grid / a.m_tiles * a.m_tiles;
   int room = GC_SMEM - GC_BAR_BYTES - GC_EPI_WARPS * S::STAGE;
   a.w_slots = MODE == LONG ? SHIFTED ? 2 : 3 : kb;
   a.m_group = 1;
